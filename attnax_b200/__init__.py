@@ -26,7 +26,7 @@ from .ring import ring_attention, ring_attention_reference
 from .rope import (apply_rope, apply_rope_table, rope_cos_sin_from_positions, rope_cos_sin_table,
                    rope_inv_freq)
 from .score_mods import (additive_bias_mod, alibi_mod, alibi_slopes, causal_mod, document_mask_mod,
-                         mask_mod_to_score_mod, prefix_lm_mod, sliding_window_mod)
+                         mask_mod_to_score_mod, prefix_lm_mod, sink_window_mod, sliding_window_mod)
 
 __all__ = [
     "AttentionFn", "MaskMod", "ScoreMod", "PagedKVCache", "KVLayerCache", "init_kv_layer_cache",
@@ -38,5 +38,5 @@ __all__ = [
     "make_sliding_window_mask", "mask_mod_to_boolean_mask", "mask_mod_to_score_mod",
     "memory_efficient_attention", "paged_attention", "paged_attention_batched",
     "pallas_flash_attention", "prefix_lm_mod", "ring_attention", "ring_attention_reference",
-    "score_mods", "sliding_window_mod", "standard_attention",
+    "score_mods", "sink_window_mod", "sliding_window_mod", "standard_attention",
 ]

@@ -31,7 +31,7 @@ class AttnMask(C.Structure):
         ("doc_q_bstride", i64), ("doc_kv_bstride", i64),
         ("alibi_slopes", vp), ("bias", vp), ("bias_dtype", C.c_int),
         ("bias_strides", i64 * 4), ("bool_mask", vp), ("mask_strides", i64 * 4),
-        ("q_offset", i64), ("kv_offset", i64),
+        ("q_offset", i64), ("kv_offset", i64), ("num_sinks", i64),
     ]
 
 

@@ -3,7 +3,7 @@
 Selections (causal, window, prefix, document, MaskMods, ``mask=``) AND
 together and additive terms (ALiBi, bias) sum, so a left-to-right chain of
 built-in mods (attnax/kernels/_api.py:166-196) reduces to one static spec:
-a band ``lo <= q - kv <= hi``, an optional prefix-length vector, an optional
+a band ``lo <= q - kv <= hi`` whose upper end may spare the first keys (sinks), an optional prefix-length vector, an optional
 document-id vector, summed ALiBi slopes, one summed bias tensor and one
 boolean mask.  Callables that are not built-in mods raise
 ``NotImplementedError``: there is no fallback.
@@ -18,7 +18,7 @@ import torch
 from . import _lib
 from ._api import ComposedScoreMod, position_indices
 from .score_mods import (AdditiveBiasMod, AlibiMod, CausalMod, DocumentMaskMod, MaskModScoreMod,
-                         PrefixLMMod, SlidingWindowMod)
+                         PrefixLMMod, SinkWindowMod, SlidingWindowMod)
 
 BAND_INF = 1 << 62
 
@@ -65,6 +65,7 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
     keep = []
     lo, hi = -BAND_INF, BAND_INF
     has_band = False
+    sink = None
     prefix = doc = slopes = bias = bmask = None
     for p in flatten_mods(score_mod):
         if isinstance(p, CausalMod):
@@ -74,6 +75,11 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
             lo = max(lo, 0 if p.causal else -(w - 1))
             hi = min(hi, w - 1)
             has_band = True
+        elif isinstance(p, SinkWindowMod):
+            if sink is not None and (sink.window_size, sink.num_sinks) != (p.window_size, p.num_sinks):
+                raise NotImplementedError("two different sink_window_mod windows in one chain")
+            sink = p
+            lo, has_band = max(lo, 0), True
         elif isinstance(p, AlibiMod):
             if p.num_heads != heads_q:
                 raise ValueError(f"alibi_mod({p.num_heads}) used with {heads_q} query heads")
@@ -102,6 +108,13 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
         mk = torch.as_tensor(mask, device=device).to(torch.bool)
         bmask = mk if bmask is None else (bmask & mk)
 
+    if sink is not None:
+        if hi >= sink.window_size and hi != BAND_INF:
+            # (a plain window wider than the sinks' cuts the sinks off at a second distance)
+            raise NotImplementedError(f"{sink!r} composed with a wider sliding window")
+        # a plain window no wider than the sinks' own drops everything that the sinks add
+        if hi == BAND_INF:
+            hi, m.num_sinks = sink.window_size - 1, sink.num_sinks
     if has_band:
         m.has_band, m.band_lo, m.band_hi = 1, lo, hi
     if prefix is not None:
@@ -147,7 +160,11 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
 
 
 def band_of(score_mod):
-    """(lo, hi) of the causal/window selection of a mod chain, or None."""
+    """(lo, hi) of the causal/window selection of a mod chain, or None.
+
+    (lo, hi) bounds q - kv of every kept entry, so a sink window counts as
+    causal only: its sinks are kept at any distance.
+    """
     lo, hi, has = -BAND_INF, BAND_INF, False
     for p in flatten_mods(score_mod):
         if isinstance(p, CausalMod):
@@ -156,6 +173,8 @@ def band_of(score_mod):
             lo = max(lo, 0 if p.causal else -(p.window_size - 1))
             hi = min(hi, p.window_size - 1)
             has = True
+        elif isinstance(p, SinkWindowMod):
+            lo, has = max(lo, 0), True
     return (lo, hi) if has else None
 
 

@@ -4,6 +4,8 @@
 // ScoreMods (attnax/kernels/score_mods.py) and `mask=` argument:
 //   causal_mod          keep kv <= q                    (score_mods.py:100-102)
 //   sliding_window_mod  keep kv <= q and q - kv < W      (:139-141), or |q-kv| < W (:142)
+//   sink_window_mod     keep kv <= q and (q - kv < W or kv < num_sinks); no counterpart in
+//                       the reference (first tokens that stay visible to every later query)
 //   prefix_lm_mod       keep kv < prefix[b] or kv <= q   (:171-174)
 //   document_mask_mod   keep ids[b,q] == ids[b,kv]       (:195-209)
 //   alibi_mod           s - slope[h] * |q - kv|          (:76-79)
@@ -44,7 +46,9 @@ __host__ __device__ inline long long ll_max(long long a, long long b) { return a
 
 // Classifies the tile [q0,q1) x [k0,k1) of batch b (local positions).
 // doc_q_tiles/doc_kv_tiles hold (min,max) ids per kDocTile-row tile; when
-// they are null a document mask makes every tile partial.
+// they are null a document mask makes every tile partial.  SINK: the mask may
+// hold sinks (num_sinks); the instantiations without it never look.
+template <bool SINK = false>
 __host__ __device__ inline int tile_state(const attn_mask_t& m, const int2* doc_q_tiles,
                                           const int2* doc_kv_tiles, int nq_doc, int nk_doc, int b,
                                           int q0, int q1, int k0, int k1, int bn) {
@@ -54,8 +58,8 @@ __host__ __device__ inline int tile_state(const attn_mask_t& m, const int2* doc_
   const long long klo = m.kv_offset + k0, khi = m.kv_offset + k1 - 1;
   if (m.has_band) {
     const long long dmin = qlo - khi, dmax = qhi - klo;
-    if (dmax < m.band_lo || dmin > m.band_hi) return kSkip;
-    if (!(dmin >= m.band_lo && dmax <= m.band_hi)) st = kPartial;
+    if (dmax < m.band_lo || (dmin > m.band_hi && !(SINK && klo < m.num_sinks))) return kSkip;
+    if (!(dmin >= m.band_lo && (dmax <= m.band_hi || (SINK && khi < m.num_sinks)))) st = kPartial;
   }
   if (m.prefix_len) {
     const long long pref = m.prefix_len[b];
@@ -100,6 +104,19 @@ __host__ __device__ inline void band_tile_range(const attn_mask_t& m, int q0, in
   }
 }
 
+// kv tiles [0, n) of bn columns that hold a sink some row of [.., q1) may see:
+// the last such key is min(num_sinks - 1, q - band_lo) of the last row.
+__host__ __device__ inline int sink_tile_count(const attn_mask_t& m, int q1, int seq_kv, int bn) {
+  const long long last =
+      ll_min(ll_min(m.num_sinks - 1, m.q_offset + q1 - 1 - m.band_lo) - m.kv_offset, (long long)seq_kv - 1);
+  return last < 0 ? 0 : (int)(last / bn) + 1;
+}
+
+// Of `sink` such tiles, those in front of the band's tiles [j_lo, j_hi) (all, if the band is empty).
+__host__ __device__ inline int sink_tiles_before(int sink, int j_lo, int j_hi) {
+  return j_hi > j_lo && sink > j_lo ? j_lo : sink;
+}
+
 __device__ __forceinline__ float load_bias(const void* p, attn_dtype_t dt, long long idx) {
   if (dt == ATTN_F32) return __ldg(reinterpret_cast<const float*>(p) + idx);
   if (dt == ATTN_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[idx]);
@@ -119,7 +136,7 @@ __device__ __forceinline__ float mask_score(const attn_mask_t& m, float raw, flo
   bool keep = true;
   if (m.has_band) {
     const long long d = qg - kvg;
-    keep = keep && d >= m.band_lo && d <= m.band_hi;
+    keep = keep && d >= m.band_lo && (d <= m.band_hi || kvg < m.num_sinks);
   }
   if (m.prefix_len) keep = keep && (kvg < (long long)m.prefix_len[b] || kvg <= qg);
   if (m.doc_q)
@@ -254,6 +271,7 @@ struct RowCtx {
   int ncols;        // columns < ncols are inside the sequence
   int band_lo, band_hi;
   int pref_cols;    // prefix: columns c < pref_cols are kept regardless of d (see make_row_ctx)
+  int sink_cols;    // sinks: columns c < sink_cols are kept regardless of band_hi
   int doc_fixed;    // document id of this row
   const int32_t* doc_cols;  // document ids indexed by column
   const uint8_t* bmask;     // bool mask at column 0, column stride bmask_cs
@@ -292,6 +310,8 @@ __device__ __forceinline__ RowCtx make_row_ctx(const attn_mask_t& m, float sl2, 
   r.band = m.has_band != 0;
   r.band_lo = clamp_i32(m.has_band ? m.band_lo : -(1ll << 40));
   r.band_hi = clamp_i32(m.has_band ? m.band_hi : (1ll << 40));
+  // forward columns c < num_sinks - kg0; transposed: all or none
+  r.sink_cols = transposed ? (kg0 < m.num_sinks ? (1 << 30) : 0) : clamp_i32(m.num_sinks - kg0);
   r.prefix = m.prefix_len != nullptr;
   r.pref_cols = 0;
   if (r.prefix) {
@@ -335,7 +355,7 @@ __device__ __forceinline__ RowCtx make_row_ctx(const attn_mask_t& m, float sl2, 
 // Raw q.k scores -> log2-domain masked scores, for N register-resident
 // columns.  Each feature is its own branch-free unrolled loop so the common
 // (full-tile) path stays short.
-template <int N>
+template <int N, bool SINK = false>
 __device__ __forceinline__ void transform_row(float (&s)[N], const RowCtx& r, bool partial) {
   if (r.alibi) {
     const float fd0 = (float)r.d0, fstep = (float)r.dstep;
@@ -361,7 +381,7 @@ __device__ __forceinline__ void transform_row(float (&s)[N], const RowCtx& r, bo
 #pragma unroll
   for (int c = 0; c < N; ++c) {
     const int d = r.d0 + r.dstep * c;
-    bool keep = !r.band || (d >= r.band_lo && d <= r.band_hi);
+    bool keep = !r.band || (d >= r.band_lo && (d <= r.band_hi || (SINK && c < r.sink_cols)));
     if (r.prefix) keep = keep && (c < r.pref_cols || d >= 0);
     s[c] = c < r.ncols ? (keep ? s[c] : -FLT_MAX) : -INFINITY;
   }

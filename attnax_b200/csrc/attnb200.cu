@@ -126,6 +126,7 @@ static bool simt_dim_ok(int d) { return d == 8 || d == 16 || d == 32 || d == 64 
 
 static bool check_mask(const attn_mask_t& m, int B) {
   if (m.has_band && m.band_lo > m.band_hi) return false;
+  if (m.num_sinks < 0 || (m.num_sinks > 0 && !m.has_band)) return false;
   if ((m.doc_q == nullptr) != (m.doc_kv == nullptr)) return false;
   if (m.bias && m.bias_dtype != ATTN_F32 && m.bias_dtype != ATTN_BF16 && m.bias_dtype != ATTN_F16)
     return false;
@@ -262,18 +263,22 @@ static int launch_sm100_fwd2(const attn_fwd_params_t* p, float* lse, const int2*
   a.acc_row0 = acc ? acc->row0 : 0;
   a.acc_final_from = acc ? acc->final_from : 0;
   constexpr int smem = fwd2::Cfg<D>::SMEM;
-  auto kern = acc ? fwd2::flash_fwd2_kernel<D, BF16, true> : fwd2::flash_fwd2_kernel<D, BF16, false>;
-  static int attr_dev[2] = {-1, -1};
+  const bool sink = p->mask.num_sinks > 0;
+  if (acc && sink) return ATTN_ERR_UNSUPPORTED;  // (the ring's entry points take no sinks)
+  const int variant = acc ? 1 : sink ? 2 : 0;
+  auto kern = acc ? fwd2::flash_fwd2_kernel<D, BF16, true>
+                  : sink ? fwd2::flash_fwd2_kernel<D, BF16, false, true> : fwd2::flash_fwd2_kernel<D, BF16, false>;
+  static int attr_dev[3] = {-1, -1, -1};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (attr_dev[acc ? 1 : 0] != dev) {
+  if (attr_dev[variant] != dev) {
     // The in-kernel register split assumes this exact launch register count.
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs != fwd2::kLaunchRegs)
       return ATTN_ERR_UNSUPPORTED;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return ATTN_ERR_CUDA;
-    attr_dev[acc ? 1 : 0] = dev;
+    attr_dev[variant] = dev;
   }
   // With an order table, blockIdx.x walks (rank, head) with heads fastest.
   dim3 grid = order ? dim3(a.n_ctas * p->num_heads_q, 1, p->batch) : dim3(a.n_ctas, p->num_heads_q, p->batch);
@@ -305,14 +310,15 @@ static int launch_sm100_fwd(const attn_fwd_params_t* p, float* lse, const int2* 
   a.nq_doc = (p->seq_q + kDocTile - 1) / kDocTile;
   a.nk_doc = (p->seq_kv + kDocTile - 1) / kDocTile;
   constexpr int smem = fwd::Cfg<D>::SMEM;
-  auto kern = fwd::flash_fwd_kernel<D, BF16>;
-  static int attr_dev = -1;
+  const int sink = p->mask.num_sinks > 0;
+  auto kern = sink ? fwd::flash_fwd_kernel<D, BF16, true> : fwd::flash_fwd_kernel<D, BF16>;
+  static int attr_dev[2] = {-1, -1};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (attr_dev != dev) {
+  if (attr_dev[sink] != dev) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return ATTN_ERR_CUDA;
-    attr_dev = dev;
+    attr_dev[sink] = dev;
   }
   dim3 grid(a.nq_tiles, p->num_heads_q, p->batch);
   kern<<<grid, fwd::kThreads, smem, st>>>(tq, tk, tv, a);
@@ -557,20 +563,21 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
       !make_tmap(&v64, p->dtype, p->v, B, Hkv, Skv, D, p->v_strides, KT))
     return ATTN_ERR_INVALID;
   // With an order table, blockIdx.x walks (rank, kv head) with heads fastest.
+  const int sink = p->mask.num_sinks > 0;
   const dim3 grid_kv = a.kv_order ? dim3(a.n_kt * Hkv, 1, B) : dim3(a.n_kt, Hkv, B);
   if constexpr (D == 128) {
     if (bwd_fused_dq(p)) {
       // dQ accumulated in fp32 by the dK/dV kernel, then scaled and converted.
-      static int attr_dev_f = -1;
-      auto kf = dkdv_kernel<D, BF16, true>;
-      if (attr_dev_f < 0 && CfgKV<D, true>::DQW) {
+      static int attr_dev_f[2] = {-1, -1};
+      auto kf = sink ? dkdv_kernel<D, BF16, true, true> : dkdv_kernel<D, BF16, true>;
+      if (attr_dev_f[sink] < 0 && CfgKV<D, true>::DQW) {
         // The in-kernel setmaxnreg split draws on exactly LAUNCH_REGS registers per
         // thread: with any other launch count the growing warps could wait forever.
         cudaFuncAttributes fa;
         if (cudaFuncGetAttributes(&fa, kf) != cudaSuccess || fa.numRegs != CfgKV<D, true>::LAUNCH_REGS)
           return ATTN_ERR_UNSUPPORTED;
       }
-      if (!smem_attr_once(kf, CfgKV<D, true>::SMEM, &attr_dev_f)) return ATTN_ERR_CUDA;
+      if (!smem_attr_once(kf, CfgKV<D, true>::SMEM, &attr_dev_f[sink])) return ATTN_ERR_CUDA;
       // (dq_acc rows were zeroed by prep_rows_kernel; the transposed layout is cleared here)
       if (CfgKV<D, true>::RED &&
           cudaMemsetAsync(dq_acc, 0, (size_t)B * Hq * Sq_pad * D * sizeof(float), st) != cudaSuccess)
@@ -587,10 +594,11 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
       return launch_status(3);
     }
   }
-  static int attr_dev_kv = -1, attr_dev_q = -1;
-  auto kkv = dkdv_kernel<D, BF16, false>;
-  auto kq = dq_kernel<D, BF16>;
-  if (!smem_attr_once(kkv, CfgKV<D, false>::SMEM, &attr_dev_kv) || !smem_attr_once(kq, CfgQ<D>::SMEM, &attr_dev_q))
+  static int attr_dev_kv[2] = {-1, -1}, attr_dev_q[2] = {-1, -1};
+  auto kkv = sink ? dkdv_kernel<D, BF16, false, true> : dkdv_kernel<D, BF16, false>;
+  auto kq = sink ? dq_kernel<D, BF16, true> : dq_kernel<D, BF16>;
+  if (!smem_attr_once(kkv, CfgKV<D, false>::SMEM, &attr_dev_kv[sink]) ||
+      !smem_attr_once(kq, CfgQ<D>::SMEM, &attr_dev_q[sink]))
     return ATTN_ERR_CUDA;
   kkv<<<grid_kv, CfgKV<D, false>::THREADS, CfgKV<D, false>::SMEM, st>>>(q64, k128, v128, do64, a);
   kq<<<dim3((Sq + QROWS - 1) / QROWS, Hq, B), kThreads, CfgQ<D>::SMEM, st>>>(q128, k64, v64, do128, a);

@@ -140,6 +140,16 @@ __device__ __forceinline__ void band_q_range(const attn_mask_t& m, int k0, int k
   }
 }
 
+// q-tile index range of a kv tile at k0 that holds a sink: every row from band_lo behind its first key.
+__device__ __forceinline__ void sink_q_range(const attn_mask_t& m, int k0, int Sq, int* lo, int* hi) {
+  const long long r_lo = ll_max(m.kv_offset + k0 + m.band_lo - m.q_offset, 0);
+  *lo = *hi = 0;
+  if (r_lo < Sq) {
+    *lo = (int)(r_lo / QT);
+    *hi = (Sq + QT - 1) / QT;
+  }
+}
+
 // Launch order of dkdv_kernel's kv tiles under a document mask: per batch, kv
 // tile indices ranked by the q tiles they visit (band range intersected with
 // the document range kv_qr), largest first (earlier tiles first on ties), so
@@ -237,7 +247,8 @@ struct CfgKV {
   static_assert(SMEM <= 232448, "dkdv kernel shared memory");
 };
 
-template <int D, bool BF16, bool FQ>
+// SINK: the mask holds sinks; the kv tiles that hold them visit every q tile behind the band's too.
+template <int D, bool BF16, bool FQ, bool SINK = false>
 __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
     dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -311,6 +322,7 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
 
   int t_lo, t_hi;
   band_q_range(a.mask, k0, k1, a.Sq, &t_lo, &t_hi);
+  if (SINK && a.mask.kv_offset + k0 < a.mask.num_sinks) sink_q_range(a.mask, k0, a.Sq, &t_lo, &t_hi);
   if (a.doc_kv_qr) {
     static_assert(KROWS == kDocTile && kDocTile % QT == 0, "document tiles vs kv / q tiles");
     const int2 r = a.doc_kv_qr[(long long)b * a.nk_doc + kt];
@@ -321,7 +333,7 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
   const int iters = a.group * ntiles;  // (g, q tile) pairs, g outer
   auto state_of = [&](int qt) {
     const int q0 = qt * QT;
-    return tile_state(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, q0, min(q0 + QT, a.Sq), k0,
+    return tile_state<SINK>(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, q0, min(q0 + QT, a.Sq), k0,
                       k1, KROWS);
   };
   // Inside [t_lo, t_hi) only a prefix mask (or a document mask) can drop a
@@ -616,7 +628,8 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
         if (part_bits) {
           const long long dd = a.mask.q_offset + c0 - kg_row;  // q - kv at this thread's column 0
           uint32_t keep = k0 + r < a.Skv ? bit_range(0, (long long)a.Sq - c0 - 1) : 0u;
-          if (a.mask.has_band) keep &= bit_range(a.mask.band_lo - dd, a.mask.band_hi - dd);
+          if (a.mask.has_band)
+            keep &= bit_range(a.mask.band_lo - dd, SINK && kg_row < a.mask.num_sinks ? 31 : a.mask.band_hi - dd);
           if (a.mask.prefix_len && !row_in_prefix) keep &= bit_range(-dd, 31);  // kv < prefix, else kv <= q
           if (has_doc) {
             uint32_t same = 0u;
@@ -633,7 +646,7 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
         }
       } else {
         const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, k0 + r, c0, max(0, min(HC, a.Sq - c0)), true);
-        transform_row<HC>(sc, rc, st == kPartial || k0 + r >= a.Skv);
+        transform_row<HC, SINK>(sc, rc, st == kPartial || k0 + r >= a.Skv);
         const bool row_ok = k0 + r < a.Skv;
 #pragma unroll
         for (int c = 0; c < HC; c += 4) {
@@ -804,7 +817,7 @@ struct CfgQ {
   static constexpr uint32_t COL_S = 0, COL_DP = 128, COL_DQ = 256;
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool SINK = false>
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -865,8 +878,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     j_lo = max(j_lo, r.x * (kDocTile / KT));
     j_hi = max(j_lo, min(j_hi, r.y * (kDocTile / KT)));
   }
+  // SINK: the sinks' kv tiles in front of the band's run first; position t of [j_lo - n_sk, j_hi) is tile_at(t).
+  const int n_sk = SINK ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
+  auto tile_at = [&](int t) { return (SINK && t < j_lo) ? t - (j_lo - n_sk) : t; };
   auto state_of = [&](int j) {
-    return tile_state(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, q0, q1, j * KT,
+    return tile_state<SINK>(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, q0, q1, j * KT,
                       min((j + 1) * KT, a.Skv), KT);
   };
 
@@ -882,7 +898,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_4d(sb + C::OFF_DO + c * QROWS * 128, &tm_do, q_full, c * 64, q0, hq, b);
       }
       int i = 0;
-      for (int j = j_lo; j < j_hi; ++j) {
+      for (int t = j_lo - n_sk; t < j_hi; ++t) {
+        const int j = tile_at(t);
         if (state_of(j) == kSkip) continue;
         const int s = i % ST;
         if (!mbar_wait(st_free(s), ((i / ST) & 1) ^ 1, kStatusTimeoutLoad)) break;
@@ -918,7 +935,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       int i = 0;
-      for (int j = j_lo; ok && j < j_hi; ++j) {
+      for (int t = j_lo - n_sk; ok && t < j_hi; ++t) {
+        const int j = tile_at(t);
         if (state_of(j) == kSkip) continue;
         const int s = i % ST;
         ok = mbar_wait(st_full(s), (i / ST) & 1, kStatusTimeoutMma) &&
@@ -960,7 +978,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const unsigned long long step2 = f2_pack(8.f * slope_l2, 8.f * slope_l2);
     int i = 0;
     bool ok = true;
-    for (int j = j_lo; j < j_hi; ++j) {
+    for (int t = j_lo - n_sk; t < j_hi; ++t) {
+      const int j = tile_at(t);
       const int st = state_of(j);
       if (st == kSkip) continue;
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(i % NSB), (i / NSB) & 1, kStatusTimeoutSoftmax));
@@ -1003,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, q0 + r, c0, max(0, min(32, a.Skv - c0)), false);
-          transform_row<32>(sc, rc, st == kPartial);
+          transform_row<32, SINK>(sc, rc, st == kPartial);
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             const float p = ex2(sc[c] - lse2);

@@ -109,17 +109,22 @@ __device__ __forceinline__ float exp2_poly(float x) {
 // time.  dq0 = q - kv and kv0 = global kv at column 0; ncols columns lie inside
 // the sequence; doc_ids (or null) holds the tile's column document ids.  Out
 // of line, so the full-tile code around the call keeps its registers and
-// schedule.
+// schedule.  SINK: the first num_sinks - kv0 columns stay whatever band_hi says.
+template <bool SINK>
 __device__ __noinline__ void mask_boundary_row(uint32_t s_addr, long long dq0, long long kv0, int ncols, bool has_band,
                                                long long band_lo, long long band_hi, bool has_prefix, int pref,
-                                               const int* doc_ids, int doc_row) {
+                                               const int* doc_ids, int doc_row, long long num_sinks) {
 #pragma unroll 1
   for (int c = 0; c < BN / 32; ++c) {
     uint32_t raw[32];
     tmem_ld32(s_addr + c * 32, raw);
     const long long dc = dq0 - c * 32;  // q - kv at chunk column e is dc - e
     uint32_t keep = bit_range(0, (long long)ncols - c * 32 - 1);  // inside the sequence
-    if (has_band) keep &= bit_range(dc - band_hi, dc - band_lo);
+    if (has_band) {
+      uint32_t in = bit_range(dc - band_hi, dc - band_lo);
+      if (SINK) in |= bit_range(0, ll_min(num_sinks - (kv0 + c * 32) - 1, dc - band_lo));
+      keep &= in;
+    }
     if (has_prefix) keep &= bit_range(0, pref - (kv0 + c * 32) - 1) | bit_range(0, dc);
     if (doc_ids) {
       const int4* ids = reinterpret_cast<const int4*>(doc_ids + c * 32);
@@ -144,7 +149,9 @@ __device__ __noinline__ void mask_boundary_row(uint32_t s_addr, long long dq0, l
 
 // ACC: the ring variant that merges into a running result (Args::acc_o); a
 // separate instantiation so the plain forward's epilogue stays as it is.
-template <int D, bool BF16, bool ACC = false>
+// SINK: the mask holds sinks (num_sinks); their kv tiles in front of the
+// band's are visited last.
+template <int D, bool BF16, bool ACC = false, bool SINK = false>
 __global__ void __launch_bounds__(kThreads, 1)
     flash_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
@@ -221,22 +228,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int j_lo = act[1] ? min(jl[0], jl[1]) : jl[0];
   const int j_hi = act[1] ? max(jh[0], jh[1]) : jh[0];
+  // Sinks: query tile x sees sink keys in the kv tiles [0, sk[x]).
+  int sk[2] = {0, 0};
+  if (SINK)
+    for (int x = 0; x < 2; ++x) sk[x] = act[x] ? sink_tile_count(a.mask, q1[x], a.Skv, BN) : 0;
+  const int n_sk = SINK ? sink_tiles_before(max(sk[0], sk[1]), j_lo, j_hi) : 0;
+  const int n_band = j_hi - j_lo, n_tiles = n_band + n_sk;
   // kv tile visited at position t of the loop (all three roles use the same order).
-  auto kv_tile = [&](int t) { return ATTN_FWD2_REVERSE ? j_hi - 1 - t : j_lo + t; };
-  const int n_tiles = j_hi - j_lo;
+  auto kv_tile = [&](int t) {
+    if (SINK && t >= n_band) return n_tiles - 1 - t;
+    return ATTN_FWD2_REVERSE ? j_hi - 1 - t : j_lo + t;
+  };
   // State of kv tile j for the query tile (active, kv range [lo, hi), rows [r0, r1)).
-  auto state_at = [&](bool x_act, int lo, int hi, int r0, int r1, int j) {
-    if (!x_act || j < lo || j >= hi) return (int)kSkip;
-    return tile_state(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, r0, r1, j * BN,
+  auto state_at = [&](bool x_act, int lo, int hi, int r0, int r1, int j, int x_sk) {
+    if (!x_act || ((j < lo || j >= hi) && !(SINK && j < x_sk))) return (int)kSkip;
+    return tile_state<SINK>(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, r0, r1, j * BN,
                       min((j + 1) * BN, a.Skv), BN);
   };
   // x is a compile-time constant at every call (the arrays stay in registers).
-  auto state_of = [&](int x, int j) { return state_at(act[x], jl[x], jh[x], q0[x], q1[x], j); };
+  auto state_of = [&](int x, int j) { return state_at(act[x], jl[x], jh[x], q0[x], q1[x], j, sk[x]); };
   // Inside a tile's band range only a prefix or document mask can drop a kv
   // tile; otherwise the TMA and MMA warps need only the range test.
   const bool may_skip = a.mask.prefix_len != nullptr || a.mask.doc_q != nullptr;
   auto kept = [&](int x, int j) {
-    return may_skip ? state_of(x, j) != kSkip : (act[x] && j >= jl[x] && j < jh[x]);
+    return may_skip ? state_of(x, j) != kSkip : (act[x] && ((j >= jl[x] && j < jh[x]) || (SINK && j < sk[x])));
   };
 
   if (warp >= 8) {
@@ -355,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int my_q0 = x ? q0[1] : q0[0];
     const bool my_act = x ? act[1] : act[0];
     const int my_q1 = x ? q1[1] : q1[0], my_jl = x ? jl[1] : jl[0], my_jh = x ? jh[1] : jh[0];
+    const int my_sk = x ? sk[1] : sk[0];
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     float m_run = -FLT_MAX, l_run = 0.f;
     int i = 0;
@@ -384,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* doc_ids = reinterpret_cast<int*>(sp + C::OFF_DOC) + warp * BN;  // this warp's copy
     for (int t = 0; t < n_tiles; ++t) {
       const int j = kv_tile(t);
-      const int st = state_at(my_act, my_jl, my_jh, my_q0, my_q1, j);
+      const int st = state_at(my_act, my_jl, my_jh, my_q0, my_q1, j, my_sk);
       if (st == kSkip) continue;
       const int k0 = j * BN;
       const bool part = st == kPartial;
@@ -410,9 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int u = 0; u < BN / 32; ++u) doc_ids[u * 32 + lane] = cid[u];
           __syncwarp();
         }
-        mask_boundary_row(s_addr, qg_row - (a.mask.kv_offset + k0), a.mask.kv_offset + k0, a.Skv - k0,
+        mask_boundary_row<SINK>(s_addr, qg_row - (a.mask.kv_offset + k0), a.mask.kv_offset + k0, a.Skv - k0,
                           a.mask.has_band != 0, a.mask.band_lo, a.mask.band_hi, a.mask.prefix_len != nullptr, pref,
-                          has_doc ? doc_ids : nullptr, doc_row);
+                          has_doc ? doc_ids : nullptr, doc_row, a.mask.num_sinks);
       } else if (part) {
         // Boundary tile: mask/transform 32 columns at a time in TMEM so the
         // per-column mask state never competes with the 128 scores.
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; ++e) t[e] = __uint_as_float(raw[e]);
           const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, my_q0 + r, k0 + c * 32,
                                          max(0, min(32, a.Skv - (k0 + c * 32))), false);
-          transform_row<32>(t, rc, true);
+          transform_row<32, SINK>(t, rc, true);
 #pragma unroll
           for (int e = 0; e < 32; ++e) raw[e] = __float_as_uint(t[e]);
           tmem_st32(s_addr + c * 32, raw);

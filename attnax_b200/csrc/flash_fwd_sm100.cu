@@ -58,7 +58,8 @@ struct Args {
   int nq_doc, nk_doc;
 };
 
-template <int D, bool BF16>
+// SINK: the mask holds sinks; their tiles in front of the band's run first.
+template <int D, bool BF16, bool SINK = false>
 __global__ void __launch_bounds__(kThreads, 1)
     flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
@@ -118,8 +119,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     j_lo = max(j_lo, r.x);
     j_hi = max(j_lo, min(j_hi, r.y));
   }
+  const int n_sk = SINK ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, BN), j_lo, j_hi) : 0;
+  // kv tile at position t of [j_lo - n_sk, j_hi)
+  auto tile_at = [&](int t) { return (SINK && t < j_lo) ? t - (j_lo - n_sk) : t; };
   auto state_of = [&](int j) {
-    return tile_state(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, q0, q1, j * BN,
+    return tile_state<SINK>(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, q0, q1, j * BN,
                       min((j + 1) * BN, a.Skv), BN);
   };
 
@@ -133,7 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < C::KCH; ++c)
         tma_load_4d(sb + C::OFF_Q + c * BM * 128, &tm_q, q_full, c * 64, q0, hq, b);
       int i = 0;
-      for (int j = j_lo; j < j_hi; ++j) {
+      for (int t = j_lo - n_sk; t < j_hi; ++t) {
+        const int j = tile_at(t);
         if (state_of(j) == kSkip) continue;
         const int s = i % S;
         if (!mbar_wait(kv_empty(s), ((i / S) & 1) ^ 1, kStatusTimeoutLoad)) break;
@@ -171,7 +176,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       int i = 0;
-      for (int j = j_lo; ok && j < j_hi; ++j) {
+      for (int t = j_lo - n_sk; ok && t < j_hi; ++t) {
+        const int j = tile_at(t);
         if (state_of(j) == kSkip) continue;
         const int s = i % S;
         ok = mbar_wait(k_full(s), (i / S) & 1, kStatusTimeoutMma) &&
@@ -200,7 +206,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int i = 0;
     bool ok = true;
     uint8_t* P = sp + C::OFF_P;
-    for (int j = j_lo; j < j_hi; ++j) {
+    for (int t = j_lo - n_sk; t < j_hi; ++t) {
+      const int j = tile_at(t);
       const int st = state_of(j);
       if (st == kSkip) continue;
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(i & 1), (i >> 1) & 1, kStatusTimeoutSoftmax));
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       const int k0 = j * BN;
       const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, q0 + r, k0, min(BN, a.Skv - k0), false);
-      transform_row<BN>(s, rc, st == kPartial);
+      transform_row<BN, SINK>(s, rc, st == kPartial);
       float mx = m_run;
 #pragma unroll
       for (int c = 0; c < BN; ++c) mx = fmaxf(mx, s[c]);

@@ -67,9 +67,12 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const FwdArgs a) {
   float m = -FLT_MAX, l = 0.f;
   int j_lo, j_hi;
   band_tile_range(a.mask, q0, q1, a.Skv, KT, &j_lo, &j_hi);
-  for (int j = j_lo; j < j_hi; ++j) {
+  // the sinks' tiles in front of the band's run first
+  const int n_sk = a.mask.num_sinks > 0 ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
+  for (int t0 = j_lo - n_sk; t0 < j_hi; ++t0) {
+    const int j = t0 < j_lo ? t0 - (j_lo - n_sk) : t0;
     const int k0 = j * KT, k1 = min(k0 + KT, a.Skv);
-    const int st = tile_state(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
+    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
     if (st == kSkip) continue;
     __syncthreads();
     for (int x = tid; x < KT * D; x += kThreads) {
@@ -179,9 +182,12 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) 
   const float slope_l2 = a.mask.alibi_slopes ? a.mask.alibi_slopes[hq] * kLog2e : 0.f;
   int j_lo, j_hi;
   band_tile_range(a.mask, q0, q1, a.Skv, KT, &j_lo, &j_hi);
-  for (int j = j_lo; j < j_hi; ++j) {
+  // the sinks' tiles in front of the band's run first
+  const int n_sk = a.mask.num_sinks > 0 ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
+  for (int t0 = j_lo - n_sk; t0 < j_hi; ++t0) {
+    const int j = t0 < j_lo ? t0 - (j_lo - n_sk) : t0;
     const int k0 = j * KT, k1 = min(k0 + KT, a.Skv);
-    const int st = tile_state(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
+    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
     if (st == kSkip) continue;
     __syncthreads();
     for (int x = tid; x < KT * D; x += kThreads) {
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dkv_kernel(const BwdArgs a)
     const int nqt = (a.Sq + KT - 1) / KT;
     for (int i = 0; i < nqt; ++i) {
       const int q0 = i * KT, q1 = min(q0 + KT, a.Sq);
-      const int st = tile_state(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, L::RPB);
+      const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, L::RPB);
       if (st == kSkip) continue;
       __syncthreads();
       for (int x = tid; x < KT * D; x += kThreads) {

@@ -85,7 +85,8 @@ def fwd_raw(q, k, v, spec, *, want_lse=True, out=None, lse=None):
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.check(lib.attn_fwd(C.byref(p), C.c_void_p(_stream_ptr(q.device))), "attn_fwd")
+    with torch.cuda.device(q.device):
+        _lib.check(lib.attn_fwd(C.byref(p), C.c_void_p(_stream_ptr(q.device))), "attn_fwd")
     return out, lse
 
 
@@ -110,7 +111,8 @@ def bwd_raw(q, k, v, out, lse, dout, spec):
     nbytes = lib.attn_bwd_workspace_size(C.byref(p))
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
-    _lib.check(lib.attn_bwd(C.byref(p), C.c_void_p(_stream_ptr(q.device))), "attn_bwd")
+    with torch.cuda.device(q.device):
+        _lib.check(lib.attn_bwd(C.byref(p), C.c_void_p(_stream_ptr(q.device))), "attn_bwd")
     return dq, dk, dv
 
 

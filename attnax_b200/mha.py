@@ -20,7 +20,7 @@ from ._api import compose_score_mods
 from .flash import flash_attention
 from .kv_cache import KVLayerCache, update_kv_layer_cache
 from .rope import apply_rope_table, rope_cos_sin_table
-from .score_mods import sliding_window_mod
+from .score_mods import sink_window_mod, sliding_window_mod
 
 
 def _split_heads(x: torch.Tensor, heads: int) -> torch.Tensor:
@@ -32,6 +32,7 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
                    num_kv_heads: int, use_rope: bool = False, rope_base: float = 10000.0,
                    rope_max_positions: int = 4096, position_ids_q=None, position_ids_kv=None,
                    kv_cache: KVLayerCache | None = None, attention_window: int | None = None,
+                   attention_sinks: int = 0,
                    self_attention: bool = True, mask=None, score_mod=None, base_score_mod=None,
                    attention_fn=flash_attention, dropout_rate: float = 0.0, deterministic: bool = True):
     """``query (B, Sq, Hq*D)``, ``key``/``value (B, Skv, Hkv*D)`` -- the projected
@@ -42,8 +43,12 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     branch: no window and no cache.  ``base_score_mod`` is the mod the layer
     was built with, composed before the per-call ``score_mod``
     (attention.py:436).  ``attention_fn`` must accept K/V with fewer heads
-    than Q (every function of this package does).
+    than Q (every function of this package does).  ``attention_sinks`` keeps
+    the first tokens of the sequence visible beside ``attention_window`` (no
+    counterpart in the reference).
     """
+    if attention_sinks < 0 or (attention_sinks and attention_window is None):
+        raise ValueError("attention_sinks must not be negative and needs an attention_window")
     if kv_cache is not None and not self_attention:
         raise ValueError("kv_cache is only supported for self-attention (context must be None).")
     if num_heads % num_kv_heads:
@@ -71,12 +76,14 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     if attention_window is not None and self_attention:
         if past == 0:
             # the reference's boolean window mask (attention.py:417-431) is this band
-            mods = compose_score_mods(sliding_window_mod(attention_window), mods)
+            window = (sink_window_mod(attention_window, attention_sinks) if attention_sinks
+                      else sliding_window_mod(attention_window))
+            mods = compose_score_mods(window, mods)
         else:
             # query positions shifted by the cached length, as the reference does
             qi = torch.arange(seq_q, device=q.device)[:, None] + past
             ki = torch.arange(k.shape[2], device=q.device)[None, :]
-            win = ((ki <= qi) & (qi - ki < attention_window))[None, None]
+            win = ((ki <= qi) & ((qi - ki < attention_window) | (ki < attention_sinks)))[None, None]
             mask = win if mask is None else (torch.as_tensor(mask, device=q.device) & win)
 
     out = attention_fn(q, k, v, mask=mask, score_mod=mods, dropout_rng=None, dropout_rate=dropout_rate,

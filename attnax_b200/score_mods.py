@@ -80,6 +80,29 @@ class SlidingWindowMod(TaggedScoreMod):
         return f"sliding_window_mod({self.window_size}, causal={self.causal})"
 
 
+class SinkWindowMod(TaggedScoreMod):
+    """Causal window of ``window_size`` keys plus the first ``num_sinks`` keys.
+
+    Keep ``kv <= q and (q - kv < window_size or kv < num_sinks)``: the
+    sequence's first tokens stay visible to every later query, so the softmax
+    keeps the mass that it gathers on them when the window has moved on.  No
+    counterpart in the reference.
+    """
+
+    kind = "sink_window"
+
+    def __init__(self, window_size: int, num_sinks: int):
+        self.window_size = int(window_size)
+        self.num_sinks = int(num_sinks)
+
+    def __call__(self, scores, b_idx, h_idx, q_idx, kv_idx):
+        keep = (kv_idx <= q_idx) & ((q_idx - kv_idx < self.window_size) | (kv_idx < self.num_sinks))
+        return torch.where(keep, scores, _neg(scores))
+
+    def __repr__(self):
+        return f"sink_window_mod({self.window_size}, {self.num_sinks})"
+
+
 class AlibiMod(TaggedScoreMod):
     """``scores - slope[h] * |q - kv|`` (score_mods.py:48-81)."""
 
@@ -175,6 +198,15 @@ def sliding_window_mod(window_size: int, *, causal: bool = True) -> ScoreMod:
     if window_size <= 0:
         raise ValueError(f"window_size must be positive, got {window_size}")
     return SlidingWindowMod(window_size, causal)
+
+
+def sink_window_mod(window_size: int, num_sinks: int) -> ScoreMod:
+    """Causal sliding window whose first ``num_sinks`` tokens stay visible."""
+    if window_size <= 0:
+        raise ValueError(f"window_size must be positive, got {window_size}")
+    if num_sinks < 0:
+        raise ValueError(f"num_sinks must not be negative, got {num_sinks}")
+    return SinkWindowMod(window_size, num_sinks)
 
 
 def alibi_mod(num_heads: int) -> ScoreMod:

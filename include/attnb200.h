@@ -57,6 +57,7 @@ typedef enum { ATTN_F32 = 0, ATTN_BF16 = 1, ATTN_F16 = 2 } attn_dtype_t;
  * (attnax/kernels/_api.py:166-196) plus the boolean `mask=` argument.
  * Selections AND together; additive terms sum.  An entry is kept iff
  *   band_lo <= q - kv <= band_hi                        (has_band)
+ *     or band_lo <= q - kv and kv < num_sinks           (num_sinks > 0)
  *   and (kv < prefix_len[b] or kv <= q)                 (prefix_len)
  *   and doc_q[b, q] == doc_kv[b, kv]                    (doc_q, doc_kv)
  *   and bool_mask[b, h, q, kv] != 0                     (bool_mask)
@@ -78,6 +79,7 @@ typedef struct {
   const uint8_t* bool_mask;      /* broadcastable (b, h, q, kv) or NULL */
   int64_t mask_strides[4];
   int64_t q_offset, kv_offset;   /* global position of local row/col 0 */
+  int64_t num_sinks;             /* first keys that band_hi never drops; 0: none; > 0 needs has_band */
 } attn_mask_t;
 
 typedef struct {
