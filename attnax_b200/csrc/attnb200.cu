@@ -470,8 +470,29 @@ static bool bwd_fused_dq(const attn_bwd_params_t* p) { return ATTN_BWD_FUSED_DQ 
 
 struct BwdWorkspace {
   size_t lse2 = 0, dq_acc = 0, doc_q = 0, doc_kv = 0, doc_q_jr = 0, doc_kv_qr = 0, doc_kv_order = 0,
-         total = 0;  // delta at 0
+         sink_part = 0, total = 0;  // delta at 0
 };
+
+// How dkdv_kernel splits the rows behind the window of the kv tiles that hold
+// sinks: chunks of about the q tiles that a window's kv tile visits, not under
+// 32 (a CTA's start and its partial then cost under a few per cent), and at
+// most 64 chunks (the partials stay small next to dK and dV).
+struct SinkSplit {
+  int rows = 0, tiles = 0, chunks = 0, chunk_tiles = 1;
+};
+static SinkSplit sink_split(const attn_mask_t& m, int seq_q, int seq_kv) {
+  SinkSplit s;
+  const long long rows = ll_min(m.num_sinks - m.kv_offset, seq_kv);
+  if (m.num_sinks <= 0 || rows <= 0) return s;
+  s.rows = (int)rows;
+  s.tiles = (s.rows + bwd::KROWS - 1) / bwd::KROWS;
+  const int nq = (seq_q + bwd::QT - 1) / bwd::QT;
+  const int left = nq - bwd::sink_q_first(m, 0, seq_kv < bwd::KROWS ? seq_kv : bwd::KROWS, seq_q);
+  const long long band = ll_min((m.band_hi - m.band_lo) / bwd::QT, nq) + bwd::KROWS / bwd::QT + 1;
+  s.chunk_tiles = (int)ll_max(ll_max(band, 32), (left + 63) / 64);
+  s.chunks = left > 0 ? (left + s.chunk_tiles - 1) / s.chunk_tiles : 0;
+  return s;
+}
 
 // Document masks: dkdv_kernel runs its kv tiles longest first (doc_kv_order_kernel)
 // when the per-batch ranking fits one block.
@@ -502,6 +523,11 @@ static BwdWorkspace bwd_workspace_layout(const attn_bwd_params_t* p) {
       off += align256((size_t)p->batch * bwd_kv_tiles(p->seq_kv) * sizeof(int));
     }
   }
+  if (tc && p->mask.num_sinks > 0) {
+    const SinkSplit s = sink_split(p->mask, p->seq_q, p->seq_kv);
+    w.sink_part = off;
+    off += align256((size_t)(1 + s.chunks) * p->batch * p->num_heads_kv * s.rows * 2 * p->head_dim * sizeof(float));
+  }
   w.total = off;
   return w;
 }
@@ -524,7 +550,7 @@ static bool smem_attr_once(K kernel, int bytes, int* cached_dev) {
 
 template <int D, bool BF16>
 static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse2, float* dq_acc,
-                            const BwdDocTables& doc, cudaStream_t st) {
+                            float* sink_part, const BwdDocTables& doc, cudaStream_t st) {
   using namespace bwd;
   const int Sq_pad = bwd_seq_pad(p);
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -564,7 +590,16 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
     return ATTN_ERR_INVALID;
   // With an order table, blockIdx.x walks (rank, kv head) with heads fastest.
   const int sink = p->mask.num_sinks > 0;
-  const dim3 grid_kv = a.kv_order ? dim3(a.n_kt * Hkv, 1, B) : dim3(a.n_kt, Hkv, B);
+  const SinkSplit split = sink_split(p->mask, Sq, Skv);
+  a.sink_part = sink_part;
+  a.sink_rows = split.rows; a.sink_tiles = split.tiles;
+  a.sink_chunks = split.chunks; a.sink_chunk_tiles = split.chunk_tiles;
+  const int items = a.n_kt + split.tiles * split.chunks;
+  const dim3 grid_kv = a.kv_order ? dim3(items * Hkv, 1, B) : dim3(items, Hkv, B);
+  auto reduce_sinks = [&] {
+    if (split.rows > 0) sink_reduce_kernel<T, D><<<dim3(split.rows, Hkv, B), 2 * D, 0, st>>>(a);
+    return split.rows > 0 ? 1 : 0;
+  };
   if constexpr (D == 128) {
     if (bwd_fused_dq(p)) {
       // dQ accumulated in fp32 by the dK/dV kernel, then scaled and converted.
@@ -591,7 +626,7 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
         dq_convert_kernel<T><<<dim3((Sq + 7) / 8, Hq, B), 256, 0, st>>>(
             dq_acc, reinterpret_cast<T*>(p->dq), p->dq_strides[0], p->dq_strides[1], p->dq_strides[2], Hq, Sq,
             Sq_pad, D, p->softmax_scale);
-      return launch_status(3);
+      return launch_status(3 + reduce_sinks());
     }
   }
   static int attr_dev_kv[2] = {-1, -1}, attr_dev_q[2] = {-1, -1};
@@ -602,7 +637,7 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
     return ATTN_ERR_CUDA;
   kkv<<<grid_kv, CfgKV<D, false>::THREADS, CfgKV<D, false>::SMEM, st>>>(q64, k128, v128, do64, a);
   kq<<<dim3((Sq + QROWS - 1) / QROWS, Hq, B), kThreads, CfgQ<D>::SMEM, st>>>(q128, k64, v64, do128, a);
-  return launch_status(3);
+  return launch_status(3 + reduce_sinks());
 }
 
 }  // namespace attnb200
@@ -630,6 +665,7 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
   float* delta = reinterpret_cast<float*>(p->workspace);
   float* lse2 = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + wl.lse2);
   float* dq_acc = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + wl.dq_acc);
+  float* sink_part = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + wl.sink_part);
   const int grp = p->num_heads_q / p->num_heads_kv;
 
   simt::BwdArgs a;
@@ -668,11 +704,11 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
     }
     const bool bf = p->dtype == ATTN_BF16;
     if (p->head_dim == 128)
-      rc = bf ? launch_sm100_bwd<128, true>(p, delta, lse2, dq_acc, doc, st)
-              : launch_sm100_bwd<128, false>(p, delta, lse2, dq_acc, doc, st);
+      rc = bf ? launch_sm100_bwd<128, true>(p, delta, lse2, dq_acc, sink_part, doc, st)
+              : launch_sm100_bwd<128, false>(p, delta, lse2, dq_acc, sink_part, doc, st);
     else
-      rc = bf ? launch_sm100_bwd<64, true>(p, delta, lse2, dq_acc, doc, st)
-              : launch_sm100_bwd<64, false>(p, delta, lse2, dq_acc, doc, st);
+      rc = bf ? launch_sm100_bwd<64, true>(p, delta, lse2, dq_acc, sink_part, doc, st)
+              : launch_sm100_bwd<64, false>(p, delta, lse2, dq_acc, sink_part, doc, st);
     if (rc != ATTN_OK || !p->fix_masked_rows) return rc;
     auto fix = [&](auto tag) {
       using T = decltype(tag);

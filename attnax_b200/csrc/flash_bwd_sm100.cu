@@ -118,10 +118,18 @@ struct Args {
   // (or null); its grid is then (n_kt * Hkv, 1, B) with heads fastest.
   const int* kv_order;
   int n_kt;
+  // Sinks (dkdv_kernel<.., SINK>): the rows behind the window that a sink's kv
+  // tile sees are split into sink_chunks ranges of sink_chunk_tiles q tiles,
+  // each a CTA of its own (grid indices behind the n_kt kv tiles: kv tile
+  // slowest, chunk fastest).  The first sink_rows kv rows leave fp32 partials
+  // [1 + sink_chunks][B][Hkv][sink_rows][dV, dK][D]: slot 0 from the kv tile's
+  // window, slot 1 + c from chunk c; sink_reduce_kernel sums them.
+  float* sink_part;
+  int sink_rows, sink_tiles, sink_chunks, sink_chunk_tiles;
 };
 
 // q-tile index range [lo, hi) (tiles of QT) that the band allows for kv rows [k0, k1).
-__device__ __forceinline__ void band_q_range(const attn_mask_t& m, int k0, int k1, int Sq, int* lo, int* hi) {
+__host__ __device__ __forceinline__ void band_q_range(const attn_mask_t& m, int k0, int k1, int Sq, int* lo, int* hi) {
   const int nq = (Sq + QT - 1) / QT;
   *lo = 0;
   *hi = nq;
@@ -140,14 +148,14 @@ __device__ __forceinline__ void band_q_range(const attn_mask_t& m, int k0, int k
   }
 }
 
-// q-tile index range of a kv tile at k0 that holds a sink: every row from band_lo behind its first key.
-__device__ __forceinline__ void sink_q_range(const attn_mask_t& m, int k0, int Sq, int* lo, int* hi) {
+// First q tile behind the band's range of the kv tile [k0, k1), from where only its sinks are visible
+// (every row from band_lo behind a sink sees it).
+__host__ __device__ __forceinline__ int sink_q_first(const attn_mask_t& m, int k0, int k1, int Sq) {
+  int lo, hi;
+  band_q_range(m, k0, k1, Sq, &lo, &hi);
+  if (hi > lo) return hi;
   const long long r_lo = ll_max(m.kv_offset + k0 + m.band_lo - m.q_offset, 0);
-  *lo = *hi = 0;
-  if (r_lo < Sq) {
-    *lo = (int)(r_lo / QT);
-    *hi = (Sq + QT - 1) / QT;
-  }
+  return r_lo < Sq ? (int)(r_lo / QT) : (Sq + QT - 1) / QT;
 }
 
 // Launch order of dkdv_kernel's kv tiles under a document mask: per batch, kv
@@ -247,7 +255,11 @@ struct CfgKV {
   static_assert(SMEM <= 232448, "dkdv kernel shared memory");
 };
 
-// SINK: the mask holds sinks; the kv tiles that hold them visit every q tile behind the band's too.
+// SINK: the mask holds sinks.  Their kv tile is visible to every later row: as
+// one CTA it walked all q tiles alone (B2 Hq16 Hkv4 S16384 W512, 16 sinks: the
+// whole call 2.76 ms), so the rows behind its window are split over CTAs of
+// about the other kv tiles' length (Args::sink_chunks) that leave fp32 partials
+// of the sinks' dK/dV rows, summed in a fixed order.
 template <int D, bool BF16, bool FQ, bool SINK = false>
 __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
     dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -261,8 +273,13 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
   uint8_t* sp = smem_raw + (sb - raw_base);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z;
-  int kt, hkv;
-  if (a.kv_order) {
+  int kt, hkv, chunk = -1;  // chunk >= 0: q tiles behind the window of a kv tile that holds sinks
+  const int item = a.kv_order ? (int)blockIdx.x / a.Hkv : (int)blockIdx.x;
+  if (SINK && item >= a.n_kt) {
+    kt = (item - a.n_kt) / a.sink_chunks;
+    chunk = (item - a.n_kt) - kt * a.sink_chunks;
+    hkv = a.kv_order ? (int)blockIdx.x - item * a.Hkv : (int)blockIdx.y;
+  } else if (a.kv_order) {
     const int k = (int)blockIdx.x / a.Hkv;
     hkv = (int)blockIdx.x - k * a.Hkv;
     kt = a.kv_order[(long long)b * a.n_kt + k];
@@ -322,7 +339,11 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
 
   int t_lo, t_hi;
   band_q_range(a.mask, k0, k1, a.Sq, &t_lo, &t_hi);
-  if (SINK && a.mask.kv_offset + k0 < a.mask.num_sinks) sink_q_range(a.mask, k0, a.Sq, &t_lo, &t_hi);
+  if (SINK && chunk >= 0) {
+    const int nq = (a.Sq + QT - 1) / QT;
+    t_lo = min(nq, sink_q_first(a.mask, k0, k1, a.Sq) + chunk * a.sink_chunk_tiles);
+    t_hi = min(nq, t_lo + a.sink_chunk_tiles);
+  }
   if (a.doc_kv_qr) {
     static_assert(KROWS == kDocTile && kDocTile % QT == 0, "document tiles vs kv / q tiles");
     const int2 r = a.doc_kv_qr[(long long)b * a.nk_doc + kt];
@@ -698,6 +719,11 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
       const bool row_ok = k0 + r < a.Skv;
       T* dvr = reinterpret_cast<T*>(a.dv) + b * a.dv_s[0] + hkv * a.dv_s[1] + (long long)(k0 + r) * a.dv_s[2];
       T* dkr = reinterpret_cast<T*>(a.dk) + b * a.dk_s[0] + hkv * a.dk_s[1] + (long long)(k0 + r) * a.dk_s[2];
+      const bool sink_row = SINK && k0 + r < a.sink_rows;
+      float* part = nullptr;  // this row's fp32 partial (dV, dK)
+      if (sink_row)
+        part = a.sink_part +
+               ((((long long)(chunk + 1) * a.B + b) * a.Hkv + hkv) * a.sink_rows + k0 + r) * (2 * D);
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         T* dst = which ? dkr : dvr;
@@ -715,7 +741,13 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-          if (row_ok) {
+          if (sink_row) {
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<float4*>(part + which * D + c * 32 + v * 4) =
+                  make_float4(__uint_as_float(o[v * 4 + 0]) * mul, __uint_as_float(o[v * 4 + 1]) * mul,
+                              __uint_as_float(o[v * 4 + 2]) * mul, __uint_as_float(o[v * 4 + 3]) * mul);
+          } else if (row_ok && chunk < 0) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               uint4 w;
@@ -1079,6 +1111,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
+}
+
+// dK/dV rows of the sinks: sum of their partials over the slots, in slot order
+// (32-bit sums, rounded once).  One block per (sink row, kv head, batch).
+template <typename T, int D>
+__global__ void __launch_bounds__(2 * D) sink_reduce_kernel(const Args a) {
+  const int row = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z, e = threadIdx.x;
+  const long long slot = (long long)a.B * a.Hkv * a.sink_rows * (2 * D);
+  const float* p = a.sink_part + (((long long)b * a.Hkv + hkv) * a.sink_rows + row) * (2 * D) + e;
+  float acc = 0.f;
+#pragma unroll 4
+  for (int s = 0; s <= a.sink_chunks; ++s) acc += p[s * slot];
+  if (e < D)
+    reinterpret_cast<T*>(a.dv)[b * a.dv_s[0] + hkv * a.dv_s[1] + (long long)row * a.dv_s[2] + e] = from_f32<T>(acc);
+  else
+    reinterpret_cast<T*>(a.dk)[b * a.dk_s[0] + hkv * a.dk_s[1] + (long long)row * a.dk_s[2] + e - D] =
+        from_f32<T>(acc);
 }
 
 // dQ = scale * dq_acc^T (fused path with a [B][H][D][S_pad] accumulator):

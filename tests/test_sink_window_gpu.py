@@ -45,6 +45,8 @@ CASES = [
     (1, 2, 2, 100, 128, BF, 20, 3),        # one-tile forward
     (1, 2, 1, 127, 64, HF, 33, 2),
     (1, 2, 1, 1, 128, BF, 5, 2),           # one token
+    (1, 4, 1, 6001, 128, BF, 64, 4),       # the sinks' gradient split over several CTAs
+    (1, 2, 2, 6001, 64, HF, 30, 300),
     (2, 4, 2, 200, 64, F32, 33, 4),        # 32-bit path
     (1, 2, 1, 150, 32, BF, 17, 5),         # head dims of the CUDA-core path
     (1, 2, 1, 90, 8, F32, 7, 40),
