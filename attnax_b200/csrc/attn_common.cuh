@@ -104,6 +104,15 @@ __host__ __device__ inline void band_tile_range(const attn_mask_t& m, int q0, in
   }
 }
 
+// Of the band's kv tiles [j_lo, j_hi), those [lo, hi) that rows [q0, q1) keep whole.
+__host__ __device__ inline void full_tile_range(const attn_mask_t& m, int q0, int q1, int seq_kv, int bn, int j_lo,
+                                                int j_hi, int* lo, int* hi) {
+  const long long last = m.q_offset + q0 - m.band_lo - m.kv_offset;        // last column the first row keeps
+  const long long first = m.q_offset + q1 - 1 - m.band_hi - m.kv_offset;   // first column the last row keeps
+  *lo = first <= 0 ? j_lo : (int)ll_min(ll_max((first + bn - 1) / bn, j_lo), j_hi);
+  *hi = last < 0 ? *lo : (int)ll_max(ll_min(ll_min((last + 1) / bn, seq_kv / bn), j_hi), *lo);
+}
+
 // kv tiles [0, n) of bn columns that hold a sink some row of [.., q1) may see:
 // the last such key is min(num_sinks - 1, q - band_lo) of the last row.
 __host__ __device__ inline int sink_tile_count(const attn_mask_t& m, int q1, int seq_kv, int bn) {

@@ -475,12 +475,12 @@ struct BwdWorkspace {
 
 // How dkdv_kernel splits the rows behind the window of the kv tiles that hold
 // sinks: chunks of about the q tiles that a window's kv tile visits, not under
-// 32 (a CTA's start and its partial then cost under a few per cent), and at
-// most 64 chunks (the partials stay small next to dK and dV).
+// 32 (query head, q tile) pairs (a CTA's start and its partial then cost a few
+// per cent), and at most 64 chunks (the partials stay small next to dK and dV).
 struct SinkSplit {
   int rows = 0, tiles = 0, chunks = 0, chunk_tiles = 1;
 };
-static SinkSplit sink_split(const attn_mask_t& m, int seq_q, int seq_kv) {
+static SinkSplit sink_split(const attn_mask_t& m, int seq_q, int seq_kv, int group) {
   SinkSplit s;
   const long long rows = ll_min(m.num_sinks - m.kv_offset, seq_kv);
   if (m.num_sinks <= 0 || rows <= 0) return s;
@@ -489,7 +489,7 @@ static SinkSplit sink_split(const attn_mask_t& m, int seq_q, int seq_kv) {
   const int nq = (seq_q + bwd::QT - 1) / bwd::QT;
   const int left = nq - bwd::sink_q_first(m, 0, seq_kv < bwd::KROWS ? seq_kv : bwd::KROWS, seq_q);
   const long long band = ll_min((m.band_hi - m.band_lo) / bwd::QT, nq) + bwd::KROWS / bwd::QT + 1;
-  s.chunk_tiles = (int)ll_max(ll_max(band, 32), (left + 63) / 64);
+  s.chunk_tiles = (int)ll_max(ll_max(band, (31 + group) / group), (left + 63) / 64);
   s.chunks = left > 0 ? (left + s.chunk_tiles - 1) / s.chunk_tiles : 0;
   return s;
 }
@@ -524,7 +524,7 @@ static BwdWorkspace bwd_workspace_layout(const attn_bwd_params_t* p) {
     }
   }
   if (tc && p->mask.num_sinks > 0) {
-    const SinkSplit s = sink_split(p->mask, p->seq_q, p->seq_kv);
+    const SinkSplit s = sink_split(p->mask, p->seq_q, p->seq_kv, p->num_heads_q / p->num_heads_kv);
     w.sink_part = off;
     off += align256((size_t)(1 + s.chunks) * p->batch * p->num_heads_kv * s.rows * 2 * p->head_dim * sizeof(float));
   }
@@ -590,7 +590,7 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
     return ATTN_ERR_INVALID;
   // With an order table, blockIdx.x walks (rank, kv head) with heads fastest.
   const int sink = p->mask.num_sinks > 0;
-  const SinkSplit split = sink_split(p->mask, Sq, Skv);
+  const SinkSplit split = sink_split(p->mask, Sq, Skv, a.group);
   a.sink_part = sink_part;
   a.sink_rows = split.rows; a.sink_tiles = split.tiles;
   a.sink_chunks = split.chunks; a.sink_chunk_tiles = split.chunk_tiles;

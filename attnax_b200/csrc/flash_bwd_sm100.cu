@@ -120,8 +120,8 @@ struct Args {
   int n_kt;
   // Sinks (dkdv_kernel<.., SINK>): the rows behind the window that a sink's kv
   // tile sees are split into sink_chunks ranges of sink_chunk_tiles q tiles,
-  // each a CTA of its own (grid indices behind the n_kt kv tiles: kv tile
-  // slowest, chunk fastest).  The first sink_rows kv rows leave fp32 partials
+  // each a CTA of its own (grid indices in front of the n_kt kv tiles, since they may be
+  // the longest: kv tile slowest, chunk fastest).  The first sink_rows kv rows leave fp32 partials
   // [1 + sink_chunks][B][Hkv][sink_rows][dV, dK][D]: slot 0 from the kv tile's
   // window, slot 1 + c from chunk c; sink_reduce_kernel sums them.
   float* sink_part;
@@ -274,18 +274,22 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z;
   int kt, hkv, chunk = -1;  // chunk >= 0: q tiles behind the window of a kv tile that holds sinks
-  const int item = a.kv_order ? (int)blockIdx.x / a.Hkv : (int)blockIdx.x;
-  if (SINK && item >= a.n_kt) {
-    kt = (item - a.n_kt) / a.sink_chunks;
-    chunk = (item - a.n_kt) - kt * a.sink_chunks;
-    hkv = a.kv_order ? (int)blockIdx.x - item * a.Hkv : (int)blockIdx.y;
-  } else if (a.kv_order) {
+  const int n_split = SINK ? a.sink_tiles * a.sink_chunks : 0;
+  if (a.kv_order) {
     const int k = (int)blockIdx.x / a.Hkv;
     hkv = (int)blockIdx.x - k * a.Hkv;
-    kt = a.kv_order[(long long)b * a.n_kt + k];
-  } else {
-    kt = blockIdx.x;  // early kv tiles carry the most q tiles under causal bands
+    if (SINK && k < n_split) chunk = k;
+    else kt = a.kv_order[(long long)b * a.n_kt + k - n_split];
+  } else if (SINK && (int)blockIdx.x < n_split) {
+    chunk = blockIdx.x;
     hkv = blockIdx.y;
+  } else {
+    kt = (int)blockIdx.x - n_split;  // early kv tiles carry the most q tiles under causal bands
+    hkv = blockIdx.y;
+  }
+  if (SINK && chunk >= 0) {
+    kt = chunk / a.sink_chunks;
+    chunk -= kt * a.sink_chunks;
   }
   const int k0 = kt * KROWS, k1 = min(k0 + KROWS, a.Skv);
 

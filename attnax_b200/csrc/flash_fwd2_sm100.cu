@@ -239,14 +239,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (SINK && t >= n_band) return n_tiles - 1 - t;
     return ATTN_FWD2_REVERSE ? j_hi - 1 - t : j_lo + t;
   };
+  // Sinks: kv tiles [fl, fh) that query tile x keeps whole, so the loop over
+  // them compares two integers instead of redoing the 64-bit distances.
+  int fl[2] = {0, 0}, fh[2] = {0, 0};
+  if (SINK && !a.mask.prefix_len && !a.mask.doc_q && !a.mask.bias && !a.mask.bool_mask)
+    for (int x = 0; x < 2; ++x)
+      full_tile_range(a.mask, q0[x], q1[x], a.Skv, BN, jl[x], jh[x], &fl[x], &fh[x]);
   // State of kv tile j for the query tile (active, kv range [lo, hi), rows [r0, r1)).
-  auto state_at = [&](bool x_act, int lo, int hi, int r0, int r1, int j, int x_sk) {
+  auto state_at = [&](bool x_act, int lo, int hi, int r0, int r1, int j, int x_sk, int x_fl, int x_fh) {
+    if (SINK && j >= x_fl && j < x_fh) return (int)kFull;
     if (!x_act || ((j < lo || j >= hi) && !(SINK && j < x_sk))) return (int)kSkip;
     return tile_state<SINK>(a.mask, a.doc_q_tiles, a.doc_kv_tiles, a.nq_doc, a.nk_doc, b, r0, r1, j * BN,
                       min((j + 1) * BN, a.Skv), BN);
   };
   // x is a compile-time constant at every call (the arrays stay in registers).
-  auto state_of = [&](int x, int j) { return state_at(act[x], jl[x], jh[x], q0[x], q1[x], j, sk[x]); };
+  auto state_of = [&](int x, int j) { return state_at(act[x], jl[x], jh[x], q0[x], q1[x], j, sk[x], fl[x], fh[x]); };
   // Inside a tile's band range only a prefix or document mask can drop a kv
   // tile; otherwise the TMA and MMA warps need only the range test.
   const bool may_skip = a.mask.prefix_len != nullptr || a.mask.doc_q != nullptr;
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int my_q0 = x ? q0[1] : q0[0];
     const bool my_act = x ? act[1] : act[0];
     const int my_q1 = x ? q1[1] : q1[0], my_jl = x ? jl[1] : jl[0], my_jh = x ? jh[1] : jh[0];
-    const int my_sk = x ? sk[1] : sk[0];
+    const int my_sk = x ? sk[1] : sk[0], my_fl = x ? fl[1] : fl[0], my_fh = x ? fh[1] : fh[0];
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     float m_run = -FLT_MAX, l_run = 0.f;
     int i = 0;
@@ -400,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* doc_ids = reinterpret_cast<int*>(sp + C::OFF_DOC) + warp * BN;  // this warp's copy
     for (int t = 0; t < n_tiles; ++t) {
       const int j = kv_tile(t);
-      const int st = state_at(my_act, my_jl, my_jh, my_q0, my_q1, j, my_sk);
+      const int st = state_at(my_act, my_jl, my_jh, my_q0, my_q1, j, my_sk, my_fl, my_fh);
       if (st == kSkip) continue;
       const int k0 = j * BN;
       const bool part = st == kPartial;
