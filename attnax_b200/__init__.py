@@ -6,7 +6,9 @@ hand-written CUDA in ``libattnb200.so`` (C ABI: ``include/attnb200.h``):
 * ``flash_attention`` / ``pallas_flash_attention`` / ``memory_efficient_attention``
   / ``standard_attention`` — fused forward + backward with GQA/MQA and the
   built-in ScoreMods compiled into the kernel;
-* ``paged_attention`` / ``paged_attention_batched`` over ``PagedKVCache``;
+* ``paged_attention`` / ``paged_attention_batched`` over ``PagedKVCache``, and
+  ``paged_window_attention`` / ``paged_tree_attention`` for sliding windows with
+  sinks and trees of drafted tokens;
 * ``kv_cache_attention`` over the contiguous per-layer ``KVLayerCache``;
 * ``apply_rope`` (+ the reference's cos/sin table builders) for Q/K rotation;
 * ``ring_attention`` — sequence parallel over NCCL.
@@ -20,6 +22,7 @@ from .masking import (combine_masks, make_causal_mask, make_document_mask, make_
                       make_sliding_window_mask)
 from .paged import (PagedKVCache, allocate_blocks, append_kv, gather_kv, init_paged_kv_cache,
                     paged_attention, paged_attention_batched)
+from .paged_rows import paged_tree_attention, paged_window_attention
 from .kv_cache import (KVLayerCache, init_decoder_kv_caches, init_kv_layer_cache, kv_cache_attention,
                        update_kv_layer_cache)
 from .ring import ring_attention, ring_attention_reference
@@ -36,7 +39,8 @@ __all__ = [
     "compose_score_mods", "document_mask_mod", "flash_attention", "gather_kv",
     "init_paged_kv_cache", "make_causal_mask", "make_document_mask", "make_padding_mask",
     "make_sliding_window_mask", "mask_mod_to_boolean_mask", "mask_mod_to_score_mod",
-    "memory_efficient_attention", "paged_attention", "paged_attention_batched",
+    "memory_efficient_attention", "paged_attention", "paged_attention_batched", "paged_tree_attention",
+    "paged_window_attention",
     "pallas_flash_attention", "prefix_lm_mod", "ring_attention", "ring_attention_reference",
     "score_mods", "sink_window_mod", "sliding_window_mod", "standard_attention",
 ]

@@ -20,6 +20,8 @@ ATTN_F32, ATTN_BF16, ATTN_F16 = 0, 1, 2
 STATUS_TIMEOUTS = (0x101, 0x102, 0x103, 0x104)
 NOTICE_CONTEXT_OVERRUN = 0x201   # a paged decode met a length above max_context
 NOTICE_TABLE_OVERRUN = 0x202     # a paged decode met a length past its block-table row
+NOTICE_TREE_ORDER = 0x203        # a drafted token's parent was not in front of it
+NOTICE_PAGE_LIST = 0x204         # a page operator skipped an entry that it could not use
 
 i32, i64, f32, vp, szt = C.c_int32, C.c_int64, C.c_float, C.c_void_p, C.c_size_t
 
@@ -72,6 +74,13 @@ class PagedParams(C.Structure):
     ]
 
 
+class PagedTree(C.Structure):
+    _fields_ = [
+        ("draft_keys", vp), ("draft_values", vp), ("k_strides", i64 * 3), ("v_strides", i64 * 3),
+        ("parents", vp), ("tree_lengths", vp),
+    ]
+
+
 class RopeParams(C.Structure):
     _fields_ = [
         ("dtype", C.c_int), ("batch", i32), ("heads", i32), ("seq", i32), ("head_dim", i32),
@@ -112,6 +121,10 @@ SIGNATURES = {
     "attn_paged_decode_workspace_size": (szt, [C.POINTER(PagedParams)]),
     "attn_paged_decode": (C.c_int, [C.POINTER(PagedParams), vp]),
     "attn_paged_decode_static": (C.c_int, [C.POINTER(PagedParams), vp]),
+    "attn_paged_window_workspace_size": (szt, [C.POINTER(PagedParams), i64, i64]),
+    "attn_paged_window": (C.c_int, [C.POINTER(PagedParams), i64, i64, vp]),
+    "attn_paged_tree_workspace_size": (szt, [C.POINTER(PagedParams)]),
+    "attn_paged_tree": (C.c_int, [C.POINTER(PagedParams), C.POINTER(PagedTree), vp]),
     "attn_paged_gather": (C.c_int, [C.c_int, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, vp]),
     "attn_paged_append": (C.c_int, [C.c_int, vp, vp, i32, i32, i32, i32, vp, i32, i32, i32, vp, vp, vp, vp]),
     "attn_paged_physical_page": (i64, [i32, i32]),

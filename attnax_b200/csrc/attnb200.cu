@@ -1,5 +1,8 @@
-// C-ABI entry points (include/attnb200.h).  One translation unit: the kernel
-// sources are included here so every kernel shares the device status word.
+// C-ABI entry points (include/attnb200.h) of flash attention, the paged decode,
+// RoPE and the ring.  One translation unit: the kernel sources are included
+// here so every kernel of it shares the device status word.  The window and
+// tree attention over pages and the page operators are units of their own
+// (paged_rows.cu, pages.cu).
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
@@ -10,6 +13,8 @@
 
 #include "../../include/attnb200.h"
 #include "attn_common.cuh"
+#include "doc_tiles.cuh"
+#include "host_util.h"
 #include "flash_fwd_sm100.cu"
 #include "flash_fwd2_sm100.cu"
 #include "flash_simt.cu"
@@ -79,11 +84,7 @@ __global__ void masked_rows_dv_kernel(const T* dout, long long ds0, long long ds
 }
 
 // -------------------------------------------------------------- helpers ----
-static size_t dtype_size(attn_dtype_t t) { return t == ATTN_F32 ? 4 : 2; }
-
-static size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -99,8 +100,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // 4-D tiled map over a (B, H, S, D) tensor with element strides s[0..2] for
 // b, h, s; box = 64 features (one 128-byte swizzle row) x box_rows rows.
-static bool make_tmap(CUtensorMap* m, attn_dtype_t dt, const void* ptr, int B, int H, int S, int D,
-                      const int64_t* s, int box_rows) {
+bool make_tmap(CUtensorMap* m, attn_dtype_t dt, const void* ptr, int B, int H, int S, int D, const int64_t* s,
+               int box_rows) {
   auto enc = encode_fn();
   if (!enc) return false;
   const uint64_t es = dtype_size(dt);
@@ -137,7 +138,7 @@ static bool check_mask(const attn_mask_t& m, int B) {
 static std::atomic<unsigned long long> g_launches{0};
 
 // Counts `n` kernel launches and reports the launch error state.
-static int launch_status(int n = 1) {
+int launch_status(int n) {
   g_launches.fetch_add(n, std::memory_order_relaxed);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
@@ -370,6 +371,12 @@ int attn_device_status(int32_t* status) {
   const int zero = 0;
   if (cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) != cudaSuccess) return ATTN_ERR_CUDA;
   if (cudaMemcpyToSymbol(g_notice, &zero, sizeof(int)) != cudaSuccess) return ATTN_ERR_CUDA;
+  for (auto take : {&rows_take_status, &pages_take_status}) {
+    int v1 = 0, n1 = 0;
+    if (!take(&v1, &n1)) return ATTN_ERR_CUDA;
+    if (!v) v = v1;
+    if (!n) n = n1;
+  }
   if (status) *status = v ? v : n;
   return ATTN_OK;
 }
@@ -858,8 +865,8 @@ static PagedWs paged_ws_layout(const attn_paged_params_t* p) {
 
 // 3-D map over a pool [blocks*block_size tokens, heads_kv, head_dim]:
 // box = 64 features x 1 head x box_tokens tokens, 128B swizzle.
-static bool make_pool_tmap(CUtensorMap* m, attn_dtype_t dt, const void* pool, long long tokens,
-                           int heads_kv, int head_dim, int box_tokens) {
+bool make_pool_tmap(CUtensorMap* m, attn_dtype_t dt, const void* pool, long long tokens, int heads_kv, int head_dim,
+                    int box_tokens) {
   auto enc = encode_fn();
   if (!enc) return false;
   const uint64_t es = dtype_size(dt);

@@ -1,0 +1,33 @@
+// Host helpers shared by the library's translation units.
+#pragma once
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <cstddef>
+
+#include "../../include/attnb200.h"
+
+namespace attnb200 {
+
+inline size_t dtype_size(attn_dtype_t t) { return t == ATTN_F32 ? 4 : 2; }
+inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// cuTensorMapEncodeTiled of the running driver (null without one).
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+
+// Counts `n` kernel launches and reports the launch error state.
+int launch_status(int n = 1);
+
+// 4-D tiled map over a (B, H, S, D) tensor (see attnb200.cu).
+bool make_tmap(CUtensorMap* m, attn_dtype_t dt, const void* ptr, int B, int H, int S, int D, const int64_t* s,
+               int box_rows);
+// 3-D map over a page pool (see attnb200.cu).
+bool make_pool_tmap(CUtensorMap* m, attn_dtype_t dt, const void* pool, long long tokens, int heads_kv, int head_dim,
+                    int box_tokens);
+
+// Each translation unit has its own device status words (sm100.cuh); these
+// read and clear those of the others for attn_device_status.
+bool rows_take_status(int* status, int* notice);
+bool pages_take_status(int* status, int* notice);
+
+}  // namespace attnb200

@@ -18,6 +18,7 @@
 #include <cfloat>
 
 #include "attn_common.cuh"
+#include "mma_sm80.cuh"
 #include "sm100.cuh"
 
 namespace attnb200 {
@@ -347,35 +348,6 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------- tensor-core consumers ----
-// mma.sync m16n8k16 with fp32 accumulation; A row-major (16 x 16), B
-// column-major (16 x 8).  The decode is HBM-bound: the tensor core only
-// replaces ~1300 scalar FMA/convert instructions per 16-token page slice.
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-
 // Paged decode with tensor-core consumers (block_size a multiple of 16).
 // The TMA ring streams units of U tokens (16 or 32, dividing block_size) of
 // one kv head's slice, 128/U stages (64 KB) so every block size up to 256

@@ -1,0 +1,949 @@
+// Attention of several query rows per sequence over the paged KV cache:
+//   * window: the rows are the last T positions of the cache and see a causal
+//     sliding window plus the first tokens (sinks);
+//   * tree: the rows are T drafted tokens, they see the whole context and the
+//     drafted tokens on their own path (K/V of the drafts are not in the pages).
+// No counterpart in the reference, which decodes with every row seeing the
+// whole context (attnax/kernels/paged.py:17-84).
+//
+// Both are softmax(q k^T * scale | keep) v in one pass with a running maximum
+// and sum, split over the visible tokens and joined by their log-sum-exp.  The
+// rows of one kv head (its query heads x T) share every K/V read.  With up to
+// 64 rows the work is bound by HBM (4 * rows flops per byte of K/V); wider
+// trees approach the tensor cores' rate.
+//   rows_mma_kernel  up to 64 rows: warp-level MMA on a TMA ring of 16- or
+//                    32-token units, 1, 2 or 4 row tiles of 16 per CTA
+//   rows_tc_kernel   more rows: tcgen05 on 128-row x 128-token tiles gathered page by page by
+//                    TMA, two CTAs per SM
+//   rows_join_kernel joins the splits
+#include <cfloat>
+
+#include <atomic>
+
+#include "attn_common.cuh"
+#include "host_util.h"
+#include "mma_sm80.cuh"
+#include "sm100.cuh"
+
+namespace attnb200 {
+namespace rows {
+
+constexpr int kMaxTree = 1024;  // drafted tokens per sequence
+
+struct Args {
+  int N, Hq, Hkv, T, group, rows, row_groups;  // rows = group * T of one kv head
+  int BS, max_blocks, num_blocks;
+  long long window, sinks;
+  int unit;                      // tokens of a TMA box
+  int span_unit;                 // tokens of the units that splits count: `unit`, or the 128 of a tile
+  int max_splits, split_units;   // units per split
+  const void* q;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* parents;        // tree
+  const int32_t* tree_lens;      // tree, or null
+  float* part_o;    // [seq][Hkv * rows][max_splits][D], normalised
+  float* part_lse;  // [seq][Hkv * rows][max_splits], log2 domain
+  void* out;        // [seq][Hkv * rows][D]
+  float sl2;
+};
+
+// What one sequence's rows see, in units of U tokens: units [0, n_sink) of the
+// context, units [first, first + n_ctx) of the context, then n_draft units of
+// drafted tokens.  Window: tokens in [lo, len) or below min(sinks, lo).
+struct Span {
+  int len, drafts, lo, first, n_sink, n_ctx, n_draft, total;
+};
+
+template <bool TREE>
+__device__ __forceinline__ Span make_span(const Args& a, int seq, int U) {
+  Span s;
+  s.len = max(a.seq_lens[seq], 0);
+  s.drafts = 0;
+  s.lo = 0;
+  s.n_sink = 0;
+  if (TREE) {
+    s.drafts = a.tree_lens ? min(max(a.tree_lens[seq], 0), a.T) : a.T;
+  } else {
+    s.lo = (int)ll_max(0, (long long)s.len - a.T - a.window + 1);
+  }
+  s.first = s.lo / U;
+  if (!TREE) s.n_sink = min((int)((ll_min(a.sinks, s.lo) + U - 1) / U), s.first);
+  s.n_ctx = (s.len + U - 1) / U - s.first;
+  s.n_draft = (s.drafts + U - 1) / U;
+  s.total = s.n_sink + s.n_ctx + s.n_draft;
+  return s;
+}
+
+// First token of unit v; `draft` says of which source.
+__device__ __forceinline__ int unit_token(const Span& s, int v, int U, bool& draft) {
+  draft = v >= s.n_sink + s.n_ctx;
+  if (draft) return (v - s.n_sink - s.n_ctx) * U;
+  return (v < s.n_sink ? v : s.first + v - s.n_sink) * U;
+}
+
+// Whether any row sees context token c.
+template <bool TREE>
+__device__ __forceinline__ bool ctx_visible(const Args& a, const Span& s, int c) {
+  return c < s.len && (TREE || c >= s.lo || c < a.sinks);
+}
+
+__device__ __forceinline__ int page_of(const Args& a, int seq, int tok) {
+  int col = tok / a.BS;
+  if (col >= a.max_blocks) {
+    atomicCAS(&g_notice, 0, kNoticeTableOverrun);
+    col = a.max_blocks - 1;
+  }
+  return (int)paged_phys_page(a.block_table[(long long)seq * a.max_blocks + col], a.num_blocks);
+}
+
+// Parent of drafted token t: negative, or in front of t.
+__device__ __forceinline__ int parent_of(const int32_t* parents, int t) {
+  const int p = parents[t];
+  if (p >= t) {
+    atomicCAS(&g_notice, 0, kNoticeTreeOrder);
+    return -1;
+  }
+  return p;
+}
+
+// Splits this sequence really has (a length above max_context is cut to those planned).
+__device__ __forceinline__ int split_count(const Args& a, const Span& s) {
+  return min((s.total + a.split_units - 1) / a.split_units, a.max_splits);
+}
+
+// ---------------------------------------------------- up to 64 query rows --
+constexpr int NW = 4;  // consumer warps
+constexpr int kMmaThreads = (NW + 1) * 32;
+
+template <int D, int U>
+struct MmaCfg {
+  static constexpr int BOX = U * 128;            // U tokens x 64 features
+  static constexpr int SLICE = (D / 64) * BOX;   // K or V of a unit
+  static constexpr int STAGES = 65536 / (2 * SLICE);
+  static constexpr int MS = D + 4;               // padded row of the merge buffer
+  static constexpr int SMEM = 1024 + STAGES * 2 * SLICE + 2 * STAGES * 8;
+  static_assert(NW * 16 * (MS + 2) * 4 <= STAGES * 2 * SLICE, "the merge buffer fits the drained ring");
+};
+
+// RW row tiles of 16 per CTA, one per warp; the other NW / RW warps of a row
+// tile take every (NW / RW)-th unit and are merged at the end.  64 KB of
+// K/V in flight per CTA, three CTAs per SM.
+template <bool BF16, int D, int U, int RW, bool TREE>
+__global__ void __launch_bounds__(kMmaThreads, 3)
+    rows_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
+                    const __grid_constant__ Args a) {
+  using C = MmaCfg<D, U>;
+  constexpr int S = C::STAGES, TW = NW / RW;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const int hkv = blockIdx.x / a.row_groups, rg = blockIdx.x % a.row_groups;
+  const int split = blockIdx.y, seq = blockIdx.z;
+  const Span sp = make_span<TREE>(a, seq, U);
+  const int n_split = split_count(a, sp);
+  if (split >= n_split && split > 0) return;
+  if (split == 0 && threadIdx.x == 0 && sp.total > a.max_splits * a.split_units)
+    atomicCAS(&g_notice, 0, kNoticeContextOverrun);
+  const int v0 = split * a.split_units;
+  const int n = max(0, min(sp.total - v0, a.split_units));
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t sb = (raw_base + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sb - raw_base);
+  const uint32_t k_base = sb, v_base = sb + S * C::SLICE, bar0 = sb + 2 * S * C::SLICE;
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), RW);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  if (warp == NW) {
+    // Pages of 32 units at a time are looked up by the 32 lanes.
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      int row = 0;  // pool row (context) or token (draft) of this lane's unit
+      bool draft = false;
+      if (i0 + lane < n) {
+        const int tok = unit_token(sp, v0 + i0 + lane, U, draft);
+        row = draft ? tok : page_of(a, seq, tok) * a.BS + tok % a.BS;
+      }
+      bool ok = true;
+      for (int j = 0; j < min(32, n - i0); ++j) {
+        const int r = __shfl_sync(0xffffffffu, row, j), d = __shfl_sync(0xffffffffu, (int)draft, j);
+        const int s = (i0 + j) % S;
+        if (lane == 0 && ok) {
+          ok = mbar_wait(empty(s), (((i0 + j) / S) & 1) ^ 1, kStatusTimeoutLoad);
+          if (ok) {
+            mbar_expect_tx(full(s), 2 * C::SLICE);
+            for (int c = 0; c < D / 64; ++c) {
+              const uint32_t kd = k_base + s * C::SLICE + c * C::BOX, vd = v_base + s * C::SLICE + c * C::BOX;
+              if (TREE && d) {
+                tma_load_4d(kd, &tm_dk, full(s), c * 64, r, hkv, seq);
+                tma_load_4d(vd, &tm_dv, full(s), c * 64, r, hkv, seq);
+              } else {
+                tma_load_3d(kd, &tm_k, full(s), c * 64, hkv, r);
+                tma_load_3d(vd, &tm_v, full(s), c * 64, hkv, r);
+              }
+            }
+          }
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+    }
+    return;
+  }
+
+  const int rt = warp % RW, tw = warp / RW;  // row tile, share of the units
+  const int g = lane >> 2, tig = lane & 3;
+  const long long row0 = ((long long)seq * a.Hkv + hkv) * a.rows;  // rows of q / out before this kv head's
+  int pos[2];                          // window: position of the fragment rows; tree: drafted token
+  bool row_ok[2];
+  unsigned long long anc[2] = {0, 0};  // tree: drafted tokens on the row's path
+  uint32_t qf[D / 16][4];              // A fragments: [k-step][row g lo, row g + 8 lo, row g hi, row g + 8 hi]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = (rg * RW + rt) * 16 + g + 8 * h;
+    const int t = r % a.T;
+    row_ok[h] = r < a.rows && (!TREE || t < sp.drafts);
+    pos[h] = TREE ? t : sp.len - a.T + t;
+    const T* qr = reinterpret_cast<const T*>(a.q) + (row0 + r) * D;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      qf[kk][h] = row_ok[h] ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * tig) : 0u;
+      qf[kk][2 + h] = row_ok[h] ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * tig) : 0u;
+    }
+    if (TREE && row_ok[h] && v0 + n > sp.n_ctx)
+      for (int p = t; p >= 0; p = parent_of(a.parents + (long long)seq * a.T, p)) anc[h] |= 1ull << p;
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int x = 0; x < D / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+  float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
+  const int mi = lane >> 3, ri = lane & 7;  // ldmatrix: matrix and row of this lane
+  auto sw = [&](uint32_t base, int tok, int d) {  // swizzled [tok][d] of a unit's slice
+    return base + (d >> 6) * C::BOX + tok * 128 + ((((d & 63) >> 3) ^ (tok & 7)) << 4);
+  };
+  bool ok = true;
+  for (int i = tw; i < n; i += TW) {
+    const int s = i % S;
+    ok = __all_sync(0xffffffffu, mbar_wait(full(s), (i / S) & 1, kStatusTimeoutSoftmax));
+    if (!ok) break;
+    const uint32_t kst = k_base + s * C::SLICE, vst = v_base + s * C::SLICE;
+    bool draft;
+    const int tok0 = unit_token(sp, v0 + i, U, draft);
+    // Kept whole by every row: no masks, every V row finite by contract.
+    const bool whole = !draft && tok0 + U <= sp.len &&
+                       (TREE || (tok0 + U - 1 <= sp.len - a.T && (tok0 >= sp.len - a.window || tok0 + U <= a.sinks)));
+    bool zeroed = false;
+#pragma unroll
+    for (int g16 = 0; g16 < U; g16 += 16) {
+      const int tok_a = tok0 + g16;
+      if (!whole) {
+        // V rows that nothing sees -> 0: P is 0 there, but a slot never written may hold NaN.
+        // (Several row tiles write the same zeros.)
+        for (int x = lane; x < 16 * (D / 8); x += 32) {
+          const int r = x / (D / 8), u = x % (D / 8), tk = tok_a + r;
+          if (draft ? tk >= sp.drafts : !ctx_visible<TREE>(a, sp, tk))
+            *reinterpret_cast<uint4*>(smem + (sw(vst, g16 + r, u * 8) - sb)) = make_uint4(0, 0, 0, 0);
+        }
+        zeroed = true;
+        __syncwarp();
+      }
+      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t b[4];  // (tokens 0-7, d lo), (0-7, hi), (8-15, lo), (8-15, hi)
+        ldsm_x4(b, sw(kst, g16 + 8 * (mi >> 1) + ri, 16 * kk + 8 * (mi & 1)));
+        mma16816<BF16>(sc[0], qf[kk], b[0], b[1]);
+        mma16816<BF16>(sc[1], qf[kk], b[2], b[3]);
+      }
+      // column (x, e) is token tok_a + 8x + 2*tig + (e & 1); e < 2: row g, else row g + 8
+      if (!whole) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tk = tok_a + 8 * x + 2 * tig + (e & 1), h = e >> 1;
+            bool keep;
+            if (TREE) keep = draft ? (tk < sp.drafts && ((anc[h] >> (tk & 63)) & 1)) : tk < sp.len;
+            else keep = tk <= pos[h] && (pos[h] - tk < a.window || tk < a.sinks);
+            if (!keep) sc[x][e] = -INFINITY;
+          }
+      }
+      float alpha[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[h], mx * a.sl2);
+        alpha[h] = ex2(m[h] - m_new);
+        m[h] = m_new;
+      }
+      float pr[2][4];
+      float ps[2] = {0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pr[x][e] = ex2(fmaf(sc[x][e], a.sl2, -m[e >> 1]));
+          ps[e >> 1] += pr[x][e];
+        }
+      l[0] = l[0] * alpha[0] + ps[0];
+      l[1] = l[1] * alpha[1] + ps[1];
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          o[x][0] *= alpha[0]; o[x][1] *= alpha[0];
+          o[x][2] *= alpha[1]; o[x][3] *= alpha[1];
+        }
+      }
+      // P is rounded once to the cache's type, as the A operand of P V.
+      const uint32_t pa[4] = {pack2(pr[0][0], pr[0][1], BF16), pack2(pr[0][2], pr[0][3], BF16),
+                              pack2(pr[1][0], pr[1][1], BF16), pack2(pr[1][2], pr[1][3], BF16)};
+#pragma unroll
+      for (int np = 0; np < D / 16; ++np) {
+        uint32_t b[4];  // (tokens 0-7, d tile 2np), (8-15, 2np), (0-7, 2np+1), (8-15, 2np+1)
+        ldsm_x4_t(b, sw(vst, g16 + 8 * (mi & 1) + ri, 16 * np + 8 * (mi >> 1)));
+        mma16816<BF16>(o[2 * np], pa, b[0], b[1]);
+        mma16816<BF16>(o[2 * np + 1], pa, b[2], b[3]);
+      }
+    }
+    if (zeroed) fence_proxy_async_smem();  // generic writes before the next TMA into this stage
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty(s));
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (!row_ok[h]) l[h] = 0.f;
+  }
+  // ---- merge the warps of a row tile through the drained ring ----
+  named_bar_sync(1, NW * 32);
+  constexpr int MS = C::MS;
+  float* mo = reinterpret_cast<float*>(smem);  // [NW][16][MS]
+  float* ml = mo + NW * 16 * MS;               // [NW][16][2]
+#pragma unroll
+  for (int x = 0; x < D / 8; ++x) {
+    *reinterpret_cast<float2*>(mo + (warp * 16 + g) * MS + 8 * x + 2 * tig) = make_float2(o[x][0], o[x][1]);
+    *reinterpret_cast<float2*>(mo + (warp * 16 + g + 8) * MS + 8 * x + 2 * tig) = make_float2(o[x][2], o[x][3]);
+  }
+  if (tig == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      ml[(warp * 16 + g + 8 * h) * 2] = m[h];
+      ml[(warp * 16 + g + 8 * h) * 2 + 1] = l[h];
+    }
+  }
+  named_bar_sync(1, NW * 32);
+  if (!__all_sync(0xffffffffu, ok)) return;
+  for (int j = warp; j < RW * 16; j += NW) {
+    const int r = rg * RW * 16 + j;
+    if (r >= a.rows) continue;
+    const int t = j >> 4, jr = j & 15;  // row tile and row in it: warps t, t + RW, ...
+    float mx = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < TW; ++w) mx = fmaxf(mx, ml[((w * RW + t) * 16 + jr) * 2]);
+    float lt = 0.f, acc[D / 32];
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < TW; ++w) {
+      const int at = (w * RW + t) * 16 + jr;
+      const float lw = ml[at * 2 + 1];
+      const float f = lw > 0.f ? ex2(ml[at * 2] - mx) : 0.f;  // (a row without keys holds o of nothing)
+      lt += f * lw;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] += f > 0.f ? f * mo[at * MS + lane * (D / 32) + e] : 0.f;
+    }
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    if (n_split <= 1) {
+      T* orow = reinterpret_cast<T*>(a.out) + (row0 + r) * D + lane * (D / 32);
+#pragma unroll
+      for (int e = 0; e < D / 32; e += 2)
+        *reinterpret_cast<uint32_t*>(orow + e) = pack2(acc[e] * inv, acc[e + 1] * inv, BF16);
+    } else {
+      const long long at = (row0 + r) * a.max_splits + split;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) a.part_o[at * D + lane * (D / 32) + e] = acc[e] * inv;
+      if (lane == 0) a.part_lse[at] = lt > 0.f ? mx + lg2(lt) : -INFINITY;
+    }
+  }
+}
+
+// ----------------------------------------------- more than 64 query rows --
+// CTA = 128 rows of one kv head x a split of its 128-token tiles.  Warps 0-3
+// run the softmax (thread = row = TMEM lane), warp 4 gathers the tiles by TMA
+// (one box per page piece, a lane each), warp 5 issues the MMAs; warps 6-7 only
+// complete the warpgroup that hands its registers to the softmax warps.  TMEM:
+// S in [0, 128), P over its first 64 columns, O in [128, 128 + D).  One CTA's
+// chain S -> softmax -> P V is serial; the second CTA on the SM fills its gaps,
+// which is enough to stay on HBM at 128 rows (one tile per CTA and stage, 96 KB
+// of shared memory).
+constexpr int BM = 128, BN = 128;
+constexpr int kTcThreads = 256;
+// Register split (setmaxnreg) of a CTA launched at kTcRegs per thread.
+constexpr int kTcRegs = 128, kTcProducerRegs = 56, kTcSoftmaxRegs = 200;
+static_assert(128 * (kTcProducerRegs + kTcSoftmaxRegs) == kTcThreads * kTcRegs, "register split");
+
+template <int D>
+struct TcCfg {
+  static constexpr int KCH = D / 64;
+  static constexpr int STAGES = D == 64 ? 2 : 1;
+  static constexpr int Q_BYTES = KCH * BM * 128;
+  static constexpr int KV_BYTES = KCH * BN * 128;
+  static constexpr int OFF_K = Q_BYTES;
+  static constexpr int OFF_V = OFF_K + STAGES * KV_BYTES;
+  static constexpr int OFF_BAR = OFF_V + STAGES * KV_BYTES;
+  static constexpr int NBAR = 4 + 4 * STAGES;
+  static constexpr int OFF_TMEMPTR = OFF_BAR + NBAR * 8;
+  static constexpr int SMEM = OFF_TMEMPTR + 16 + 1024;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+  static constexpr uint32_t TMEM_COLS = 256, O_COL = 128;
+};
+
+// The tile that position i of the split visits: context tiles in order, drafted
+// tiles backwards, so that a row's walk up the tree goes on where it stopped.
+__device__ __forceinline__ int tile_at(const Span& s, int v0, int n, int i) {
+  const int ctx = s.n_sink + s.n_ctx, v = v0 + i;
+  return v < ctx ? v : max(v0, ctx) + (v0 + n - 1 - v);
+}
+
+template <bool BF16, int D, bool TREE>
+__global__ void __launch_bounds__(kTcThreads, 2)
+    rows_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_dk,
+                   const __grid_constant__ CUtensorMap tm_dv, const __grid_constant__ Args a) {
+  using C = TcCfg<D>;
+  constexpr int S = C::STAGES;
+  const int hkv = blockIdx.x / a.row_groups, rg = blockIdx.x % a.row_groups;
+  const int split = blockIdx.y, seq = blockIdx.z;
+  const Span sp = make_span<TREE>(a, seq, BN);
+  const int n_split = split_count(a, sp);
+  if (split >= n_split && split > 0) return;
+  if (split == 0 && threadIdx.x == 0 && sp.total > a.max_splits * a.split_units)
+    atomicCAS(&g_notice, 0, kNoticeContextOverrun);
+  const int v0 = split * a.split_units;
+  const int n = max(0, min(sp.total - v0, a.split_units));
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t sb = (raw_base + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sb - raw_base);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bar0 = sb + C::OFF_BAR;
+  const uint32_t q_full = bar0, s_full = bar0 + 8, p_full = bar0 + 16, o_done = bar0 + 24;
+  auto k_full = [&](int s) { return bar0 + 8u * (4 + s); };
+  auto v_full = [&](int s) { return bar0 + 8u * (4 + S + s); };
+  auto k_empty = [&](int s) { return bar0 + 8u * (4 + 2 * S + s); };
+  auto v_empty = [&](int s) { return bar0 + 8u * (4 + 3 * S + s); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEMPTR);
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 4);  // one arrival per softmax warp
+    mbar_init(o_done, 1);
+    for (int s = 0; s < S; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcProducerRegs));
+    if (warp == 4) {
+      if (n > 0 && lane == 0) {
+        mbar_expect_tx(q_full, C::Q_BYTES);
+        for (int c = 0; c < C::KCH; ++c)
+          tma_load_4d(sb + c * BM * 128, &tm_q, q_full, c * 64, rg * BM, hkv, seq);
+      }
+      const int ub = a.unit;  // tokens per box: a page, or the power of two that divides it
+      for (int i = 0; i < n; ++i) {
+        const int s = i % S;
+        bool draft;
+        const int tok0 = unit_token(sp, tile_at(sp, v0, n, i), BN, draft);
+        const int tok = tok0 + lane * ub;  // this lane's box
+        bool load = false;
+        int row = 0;
+        if (!draft && lane * ub < BN) {
+          load = tok < sp.len && (TREE || tok + ub > sp.lo || tok < a.sinks);
+          if (load) row = page_of(a, seq, tok) * a.BS + tok % a.BS;
+        }
+        const uint32_t bytes = draft ? (uint32_t)C::KV_BYTES
+                                     : __popc(__ballot_sync(0xffffffffu, load)) * (uint32_t)(ub * 128 * C::KCH);
+        bool ok = true;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {  // K, then V
+          const uint32_t bar = kv ? v_full(s) : k_full(s), free = kv ? v_empty(s) : k_empty(s);
+          const uint32_t dst = sb + (kv ? C::OFF_V : C::OFF_K) + s * C::KV_BYTES;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(free, ((i / S) & 1) ^ 1, kStatusTimeoutLoad));
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(bar, bytes);
+          __syncwarp();
+          if (TREE && draft) {
+            if (lane == 0)
+              for (int c = 0; c < C::KCH; ++c)
+                tma_load_4d(dst + c * BN * 128, kv ? &tm_dv : &tm_dk, bar, c * 64, tok0, hkv, seq);
+          } else if (load) {
+            for (int c = 0; c < C::KCH; ++c)
+              tma_load_3d(dst + c * BN * 128 + lane * ub * 128, kv ? &tm_v : &tm_k, bar, c * 64, hkv, row);
+          }
+        }
+        if (!ok) break;
+      }
+    } else if (warp == 5 && lane == 0 && n > 0) {
+      constexpr int FMT = BF16 ? 1 : 0;
+      constexpr uint32_t ID_S = idesc_f16(128, BN, FMT, 0, 0);
+      constexpr uint32_t ID_O = idesc_f16(128, D, FMT, 0, 1);
+      const uint64_t dQ = sdesc_sw128(sb, 16, 1024);
+      const uint64_t dK = sdesc_sw128(sb + C::OFF_K, 16, 1024);
+      const uint64_t dV = sdesc_sw128(sb + C::OFF_V, BN * 128, 1024);  // MN-major
+      bool ok = mbar_wait(q_full, 0, kStatusTimeoutMma);
+      for (int i = 0; ok && i < n; ++i) {
+        const int s = i % S;
+        ok = mbar_wait(k_full(s), (i / S) & 1, kStatusTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        // (in issue order behind P V of the previous tile, which reads P from these columns)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16(tmem, sdesc_add(dQ, (k >> 2) * BM * 128 + (k & 3) * 32),
+                   sdesc_add(dK, s * C::KV_BYTES + (k >> 2) * BN * 128 + (k & 3) * 32), ID_S, k > 0 ? 1u : 0u);
+        umma_commit(s_full);
+        umma_commit(k_empty(s));
+        ok = mbar_wait(v_full(s), (i / S) & 1, kStatusTimeoutMma) && mbar_wait(p_full, i & 1, kStatusTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          umma_f16_ts(tmem + C::O_COL, tmem + k * 8, sdesc_add(dV, s * C::KV_BYTES + k * 16 * 128), ID_O,
+                      (i > 0 || k > 0) ? 1u : 0u);
+        umma_commit(v_empty(s));
+        umma_commit(o_done);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcSoftmaxRegs));
+    const int r = rg * BM + threadIdx.x;  // row of the kv head
+    const int t = r % a.T;
+    const bool row_ok = r < a.rows && (!TREE || t < sp.drafts);
+    const int pos = sp.len - a.T + t;     // window: position of the row
+    const int32_t* parents = TREE ? a.parents + (long long)seq * a.T : nullptr;
+    int walk = TREE && row_ok ? t : -1;   // tree: next token on the row's path
+    const uint32_t s_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    float m = -FLT_MAX, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int st = i % S;
+      bool draft;
+      const int tok0 = unit_token(sp, tile_at(sp, v0, n, i), BN, draft);
+      const bool whole =
+          !draft && tok0 + BN <= sp.len &&
+          (TREE || (tok0 + BN - 1 <= sp.len - a.T && (tok0 >= sp.len - a.window || tok0 + BN <= a.sinks)));
+      uint32_t keep[4] = {0u, 0u, 0u, 0u};
+      if (!whole) {
+        if (TREE && draft) {
+          while (walk >= tok0) {  // (tokens behind this tile were passed in the tiles behind it)
+            const int x = walk - tok0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if ((x >> 5) == c) keep[c] |= 1u << (x & 31);
+            walk = parent_of(parents, walk);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const long long c0 = tok0 + c * 32;
+            if (TREE) keep[c] = bit_range(0, sp.len - 1 - c0);
+            else keep[c] = (bit_range(pos - a.window + 1 - c0, 31) | bit_range(0, a.sinks - 1 - c0)) & bit_range(0, pos - c0);
+          }
+        }
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, kStatusTimeoutSoftmax));
+      if (!ok) break;
+      tc_fence_after();
+      float x[BN];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+      tmem_wait_ld();
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < BN; ++c)
+          if (!((keep[c >> 5] >> (c & 31)) & 1u)) x[c] = -INFINITY;
+        // V rows that nothing sees -> 0: P is 0 there, but a slot never written (or a box never
+        // loaded) may hold NaN.  Thread = token.
+        ok = __all_sync(0xffffffffu, mbar_wait(v_full(st), (i / S) & 1, kStatusTimeoutSoftmax));
+        if (!ok) break;
+        const int tk = tok0 + threadIdx.x;
+        if (draft ? tk >= sp.drafts : !ctx_visible<TREE>(a, sp, tk)) {
+#pragma unroll
+          for (int c = 0; c < C::KCH; ++c)
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              *reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::KV_BYTES + c * BN * 128 + threadIdx.x * 128 + u * 16) =
+                  make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < BN; ++c) mxp[c & 3] = fmaxf(mxp[c & 3], x[c]);
+      const float mx = fmaxf(fmaxf(mxp[0], mxp[1]), fmaxf(mxp[2], mxp[3])) * a.sl2;
+      // The running maximum follows only jumps of more than 2^8 (P stays <= 256, exact after the final 1/l).
+      float alpha = 1.f;
+      if (mx > m + 8.f) {
+        alpha = ex2(m - mx);
+        m = mx;
+      }
+      const unsigned long long sc2 = f2_pack(a.sl2, a.sl2), nm2 = f2_pack(-m, -m);
+      unsigned long long sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(x[h * 64 + c], x[h * 64 + c + 1]), sc2, nm2), x0, x1);
+          const float p0 = ex2(x0), p1 = ex2(x1);
+          sum2[(c >> 1) & 1] = f2_add(sum2[(c >> 1) & 1], f2_pack(p0, p1));
+          pk[c >> 1] = pack2(p0, p1, BF16);  // P rounded once to the cache's type
+        }
+        tmem_st32(s_addr + h * 32, pk);
+      }
+      float s0, s1, s2, s3;
+      f2_unpack(sum2[0], s0, s1);
+      f2_unpack(sum2[1], s2, s3);
+      l = l * alpha + ((s0 + s1) + (s2 + s3));
+      // P V of the previous tile is complete: S of this one was issued behind it.
+      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(s_addr + C::O_COL + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(s_addr + C::O_COL + c * 32, o);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive_warp(p_full);
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (n - 1) & 1, kStatusTimeoutSoftmax));
+    if (ok) {
+      tc_fence_after();
+      if (!row_ok) l = 0.f;
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const long long row = ((long long)seq * a.Hkv + hkv) * a.rows + r;
+      const long long at = row * a.max_splits + split;
+      using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(s_addr + C::O_COL + c * 32, o);
+          tmem_wait_ld();
+        }
+        // (a row without keys may hold o of nothing: select, do not multiply)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+        if (r >= a.rows) continue;
+        if (n_split <= 1) {
+          T* orow = reinterpret_cast<T*>(a.out) + row * D + c * 32;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint4 w;
+            w.x = pack2(__uint_as_float(o[v * 8 + 0]), __uint_as_float(o[v * 8 + 1]), BF16);
+            w.y = pack2(__uint_as_float(o[v * 8 + 2]), __uint_as_float(o[v * 8 + 3]), BF16);
+            w.z = pack2(__uint_as_float(o[v * 8 + 4]), __uint_as_float(o[v * 8 + 5]), BF16);
+            w.w = pack2(__uint_as_float(o[v * 8 + 6]), __uint_as_float(o[v * 8 + 7]), BF16);
+            *reinterpret_cast<uint4*>(orow + v * 8) = w;
+          }
+        } else {
+          float* po = a.part_o + at * D + c * 32;
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            *reinterpret_cast<uint4*>(po + v * 4) = make_uint4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+        }
+      }
+      if (r < a.rows && n_split > 1) a.part_lse[at] = l > 0.f ? m + lg2(l) : -INFINITY;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// Joins the splits of a row: o = sum 2^(lse_i - M) o_i / sum 2^(lse_i - M).  One warp per row;
+// sequences with one split were written by their only CTA.
+template <typename T, int D, bool TREE>
+__global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ Args a) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), seq = blockIdx.y, lane = threadIdx.x & 31;
+  if (row >= a.Hkv * a.rows) return;
+  const Span sp = make_span<TREE>(a, seq, a.span_unit);
+  const int n = split_count(a, sp);
+  if (n <= 1) return;
+  const long long prow = (long long)seq * a.Hkv * a.rows + row;
+  const float* lse = a.part_lse + prow * a.max_splits;
+  const float* po = a.part_o + prow * a.max_splits * D + lane * (D / 32);
+  float mx = -INFINITY;
+  for (int i = 0; i < n; ++i) mx = fmaxf(mx, lse[i]);
+  float tot = 0.f, acc[D / 32];
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+  if (mx != -INFINITY) {
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float w = ex2(lse[i] - mx);
+      tot += w;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, po[(long long)i * D + e], acc[e]);
+    }
+  }
+  const float inv = tot > 0.f ? 1.f / tot : 0.f;
+  T* orow = reinterpret_cast<T*>(a.out) + prow * D + lane * (D / 32);
+#pragma unroll
+  for (int e = 0; e < D / 32; e += 2)
+    *reinterpret_cast<uint32_t*>(orow + e) =
+        pack2(acc[e] * inv, acc[e + 1] * inv, std::is_same<T, __nv_bfloat16>::value);
+}
+
+// -------------------------------------------------------------------- host --
+struct Plan {
+  bool tc;
+  int unit, span_unit, row_tiles, row_groups, max_splits, split_units;
+  size_t part_lse, total;
+};
+
+// Tokens that a sequence's rows can see, at most.
+static long long max_tokens(const attn_paged_params_t* p, bool tree, int64_t window, int64_t sinks) {
+  const long long ctx = p->max_context;
+  if (tree) return ctx;
+  const long long w = window < ctx ? window + p->seq_q - 1 : ctx, s = sinks < ctx ? sinks : ctx;
+  return ll_min(ctx, w + s);
+}
+
+// Splits: enough CTAs to fill the GPU three times over (the residency of the
+// kernel), none under 128 tokens, where a split's start and its partial cost
+// more than its K/V; at most 2048 tokens, so that ragged batches stay even.
+static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, int64_t sinks) {
+  Plan w;
+  const int rows = p->num_heads_q / p->num_heads_kv * p->seq_q;
+  w.tc = rows > 64;
+  if (w.tc) {
+    w.unit = 128;
+    while (p->block_size % w.unit != 0) w.unit /= 2;
+    w.span_unit = BN;
+    w.row_tiles = BM / 16;
+  } else {
+    w.unit = w.span_unit = p->block_size % 32 == 0 ? 32 : 16;
+    w.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  }
+  w.row_groups = (rows + w.row_tiles * 16 - 1) / (w.row_tiles * 16);
+  const long long tokens = max_tokens(p, tree, window, sinks), u = w.span_unit;
+  // (window: the first and last unit of both pieces may be cut)
+  const long long units = (tokens + u - 1) / u + (tree ? (p->seq_q + u - 1) / u : 3);
+  const long long ctas = (long long)p->num_seqs * p->num_heads_kv * w.row_groups;
+  const long long want = ((w.tc ? 2 : 3) * 148 + ctas - 1) / ctas;
+  const long long least = ll_max(128 / u, 1), most = 2048 / u;
+  w.split_units = (int)ll_min(ll_max((units + want - 1) / want, least), most);
+  w.max_splits = (int)((units + w.split_units - 1) / w.split_units);
+  const size_t parts = (size_t)p->num_seqs * p->num_heads_kv * rows * w.max_splits;
+  w.part_lse = w.max_splits > 1 ? align256(parts * p->head_dim * sizeof(float)) : 0;
+  w.total = w.max_splits > 1 ? w.part_lse + align256(parts * sizeof(float)) : 0;
+  return w;
+}
+
+static int check(const attn_paged_params_t* p) {
+  if (!p || !p->q || !p->key_pool || !p->value_pool || !p->block_table || !p->seq_lengths || !p->out)
+    return ATTN_ERR_INVALID;
+  if (p->num_seqs <= 0 || p->num_heads_q <= 0 || p->num_heads_kv <= 0 || p->seq_q <= 0 || p->num_blocks <= 0 ||
+      p->block_size <= 0 || p->max_blocks_per_seq <= 0 || p->max_context < 0 ||
+      p->num_heads_q % p->num_heads_kv != 0)
+    return ATTN_ERR_INVALID;
+  if (p->num_seqs > 65535) return ATTN_ERR_INVALID;
+  if (p->dtype != ATTN_BF16 && p->dtype != ATTN_F16) return ATTN_ERR_UNSUPPORTED;
+  if ((p->head_dim != 64 && p->head_dim != 128) || p->block_size % 16 != 0) return ATTN_ERR_UNSUPPORTED;
+  if ((long long)p->num_blocks * p->block_size > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;  // (TMA coordinates)
+  for (const void* x : {p->q, p->key_pool, p->value_pool, (const void*)p->out})
+    if (reinterpret_cast<uintptr_t>(x) % 16) return ATTN_ERR_INVALID;
+  return ATTN_OK;
+}
+
+// Sets a kernel's dynamic shared memory once per device.
+template <typename K>
+static bool smem_once(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load() & bit)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (dev < 64) done.fetch_or(bit);
+  return true;
+}
+
+struct Maps {
+  CUtensorMap q, k, v, dk, dv;
+};
+
+template <bool BF16, int D, int U, int RW, bool TREE>
+static int launch_mma(const Maps& t, const Args& a, cudaStream_t st) {
+  using C = MmaCfg<D, U>;
+  static std::atomic<unsigned long long> done{0};
+  auto kern = rows_mma_kernel<BF16, D, U, RW, TREE>;
+  if (!smem_once(kern, C::SMEM, done)) return ATTN_ERR_CUDA;
+  kern<<<dim3(a.Hkv * a.row_groups, a.max_splits, a.N), kMmaThreads, C::SMEM, st>>>(t.k, t.v, t.dk, t.dv, a);
+  return launch_status();
+}
+
+template <bool BF16, int D, bool TREE>
+static int launch_tc(const Maps& t, const Args& a, cudaStream_t st) {
+  using C = TcCfg<D>;
+  static std::atomic<unsigned long long> done{0};
+  auto kern = rows_tc_kernel<BF16, D, TREE>;
+  // The in-kernel register split draws on exactly kTcRegs per thread: with any
+  // other launch count the growing warps could wait forever.
+  static const bool regs_ok = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess && fa.numRegs == kTcRegs;
+  }();
+  if (!regs_ok) return ATTN_ERR_UNSUPPORTED;
+  if (!smem_once(kern, C::SMEM, done)) return ATTN_ERR_CUDA;
+  kern<<<dim3(a.Hkv * a.row_groups, a.max_splits, a.N), kTcThreads, C::SMEM, st>>>(t.q, t.k, t.v, t.dk, t.dv, a);
+  return launch_status();
+}
+
+template <bool BF16, int D, bool TREE>
+static int launch_rows(const Plan& w, const Maps& t, const Args& a, cudaStream_t st) {
+  int rc;
+  if (w.tc)
+    rc = launch_tc<BF16, D, TREE>(t, a, st);
+  else if (w.unit == 32)
+    rc = w.row_tiles == 1   ? launch_mma<BF16, D, 32, 1, TREE>(t, a, st)
+         : w.row_tiles == 2 ? launch_mma<BF16, D, 32, 2, TREE>(t, a, st)
+                            : launch_mma<BF16, D, 32, 4, TREE>(t, a, st);
+  else
+    rc = w.row_tiles == 1   ? launch_mma<BF16, D, 16, 1, TREE>(t, a, st)
+         : w.row_tiles == 2 ? launch_mma<BF16, D, 16, 2, TREE>(t, a, st)
+                            : launch_mma<BF16, D, 16, 4, TREE>(t, a, st);
+  if (rc != ATTN_OK || a.max_splits == 1) return rc;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  rows_join_kernel<T, D, TREE><<<dim3((a.Hkv * a.rows + 7) / 8, a.N), 256, 0, st>>>(a);
+  return launch_status();
+}
+
+static int run(const attn_paged_params_t* p, const attn_paged_tree_t* tree, int64_t window, int64_t sinks,
+               cudaStream_t st) {
+  const Plan w = make_plan(p, tree != nullptr, window, sinks);
+  if (w.total > 0 && (!p->workspace || p->workspace_bytes < w.total)) return ATTN_ERR_WORKSPACE;
+  if (w.max_splits > 65535) return ATTN_ERR_UNSUPPORTED;
+  Maps t;
+  const long long tokens = (long long)p->num_blocks * p->block_size;
+  if (!make_pool_tmap(&t.k, p->dtype, p->key_pool, tokens, p->num_heads_kv, p->head_dim, w.unit) ||
+      !make_pool_tmap(&t.v, p->dtype, p->value_pool, tokens, p->num_heads_kv, p->head_dim, w.unit))
+    return ATTN_ERR_INVALID;
+  if (tree) {
+    if (!make_tmap(&t.dk, p->dtype, tree->draft_keys, p->num_seqs, p->num_heads_kv, p->seq_q, p->head_dim,
+                   tree->k_strides, w.span_unit) ||
+        !make_tmap(&t.dv, p->dtype, tree->draft_values, p->num_seqs, p->num_heads_kv, p->seq_q, p->head_dim,
+                   tree->v_strides, w.span_unit))
+      return ATTN_ERR_INVALID;
+  } else {
+    t.dk = t.k;  // never loaded from
+    t.dv = t.v;
+  }
+  const int rows = p->num_heads_q / p->num_heads_kv * p->seq_q;
+  if (w.tc) {
+    const int64_t qs[3] = {(int64_t)p->num_heads_kv * rows * p->head_dim, (int64_t)rows * p->head_dim, p->head_dim};
+    if (!make_tmap(&t.q, p->dtype, p->q, p->num_seqs, p->num_heads_kv, rows, p->head_dim, qs, BM))
+      return ATTN_ERR_INVALID;
+  }
+  Args a;
+  a.N = p->num_seqs; a.Hq = p->num_heads_q; a.Hkv = p->num_heads_kv; a.T = p->seq_q;
+  a.group = p->num_heads_q / p->num_heads_kv;
+  a.rows = rows;
+  a.row_groups = w.row_groups;
+  a.BS = p->block_size; a.max_blocks = p->max_blocks_per_seq; a.num_blocks = p->num_blocks;
+  a.window = window; a.sinks = sinks;
+  a.unit = w.unit; a.span_unit = w.span_unit; a.max_splits = w.max_splits; a.split_units = w.split_units;
+  a.q = p->q; a.block_table = p->block_table; a.seq_lens = p->seq_lengths;
+  a.parents = tree ? tree->parents : nullptr;
+  a.tree_lens = tree ? tree->tree_lengths : nullptr;
+  a.part_o = reinterpret_cast<float*>(p->workspace);
+  a.part_lse = reinterpret_cast<float*>(reinterpret_cast<char*>(p->workspace) + w.part_lse);
+  a.out = p->out;
+  a.sl2 = p->softmax_scale * kLog2e;
+  const bool bf = p->dtype == ATTN_BF16;
+  if (p->head_dim == 128) {
+    if (tree) return bf ? launch_rows<true, 128, true>(w, t, a, st) : launch_rows<false, 128, true>(w, t, a, st);
+    return bf ? launch_rows<true, 128, false>(w, t, a, st) : launch_rows<false, 128, false>(w, t, a, st);
+  }
+  if (tree) return bf ? launch_rows<true, 64, true>(w, t, a, st) : launch_rows<false, 64, true>(w, t, a, st);
+  return bf ? launch_rows<true, 64, false>(w, t, a, st) : launch_rows<false, 64, false>(w, t, a, st);
+}
+
+static bool window_ok(int64_t window, int64_t sinks) { return window > 0 && sinks >= 0; }
+
+}  // namespace rows
+
+bool rows_take_status(int* status, int* notice) { return take_status_words(status, notice); }
+
+}  // namespace attnb200
+
+using namespace attnb200;
+
+extern "C" {
+
+size_t attn_paged_window_workspace_size(const attn_paged_params_t* p, int64_t window, int64_t num_sinks) {
+  if (rows::check(p) != ATTN_OK || !rows::window_ok(window, num_sinks)) return 0;
+  return rows::make_plan(p, false, window, num_sinks).total;
+}
+
+int attn_paged_window(const attn_paged_params_t* p, int64_t window, int64_t num_sinks, void* stream) {
+  const int rc = rows::check(p);
+  if (rc != ATTN_OK) return rc;
+  if (!rows::window_ok(window, num_sinks)) return ATTN_ERR_INVALID;
+  // (longer than any sequence; keeps the kernels' position arithmetic in range)
+  const int64_t far = 1ll << 40;
+  return rows::run(p, nullptr, window < far ? window : far, num_sinks < far ? num_sinks : far,
+                   reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t attn_paged_tree_workspace_size(const attn_paged_params_t* p) {
+  return rows::check(p) == ATTN_OK ? rows::make_plan(p, true, 0, 0).total : 0;
+}
+
+int attn_paged_tree(const attn_paged_params_t* p, const attn_paged_tree_t* tree, void* stream) {
+  const int rc = rows::check(p);
+  if (rc != ATTN_OK) return rc;
+  if (!tree || !tree->draft_keys || !tree->draft_values || !tree->parents) return ATTN_ERR_INVALID;
+  if (p->seq_q > rows::kMaxTree) return ATTN_ERR_UNSUPPORTED;
+  for (const void* x : {tree->draft_keys, tree->draft_values})
+    if (reinterpret_cast<uintptr_t>(x) % 16) return ATTN_ERR_INVALID;
+  return rows::run(p, tree, 0, 0, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

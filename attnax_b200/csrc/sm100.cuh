@@ -7,6 +7,7 @@
 #pragma once
 #include <cstdint>
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -17,7 +18,8 @@
 namespace attnb200 {
 
 // Set (first writer wins) when a bounded wait gives up; read by attn_device_status().
-__device__ int g_status;
+// One per translation unit.
+static __device__ int g_status;
 
 enum : int { kStatusTimeoutLoad = 0x101, kStatusTimeoutMma = 0x102, kStatusTimeoutSoftmax = 0x103,
              kStatusTimeoutOther = 0x104 };
@@ -25,12 +27,23 @@ enum : int { kStatusTimeoutLoad = 0x101, kStatusTimeoutMma = 0x102, kStatusTimeo
 // Set (first writer wins) when a kernel met input outside its contract that
 // it could still process safely (results follow the documented clamping).
 // Unlike g_status it does not stop other kernels' waits.
-__device__ int g_notice;
+static __device__ int g_notice;
 
 enum : int {
   kNoticeContextOverrun = 0x201,  // a seq_lengths entry above max_context: cut to the planned splits
-  kNoticeTableOverrun = 0x202     // a sequence longer than its block-table row: last entry reused
+  kNoticeTableOverrun = 0x202,    // a sequence longer than its block-table row: last entry reused
+  kNoticeTreeOrder = 0x203,       // a drafted token whose parent is not in front of it: taken as a root
+  kNoticePageList = 0x204         // a page operator met an index it could not use: that entry was skipped
 };
+
+// Host: reads and clears this unit's words.
+[[maybe_unused]] static bool take_status_words(int* status, int* notice) {
+  const int zero = 0;
+  return cudaMemcpyFromSymbol(status, g_status, sizeof(int)) == cudaSuccess &&
+         cudaMemcpyFromSymbol(notice, g_notice, sizeof(int)) == cudaSuccess &&
+         (*status == 0 || cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) == cudaSuccess) &&
+         (*notice == 0 || cudaMemcpyToSymbol(g_notice, &zero, sizeof(int)) == cudaSuccess);
+}
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

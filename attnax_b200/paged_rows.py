@@ -1,0 +1,233 @@
+"""Several query rows per sequence over the paged cache: windows with sinks and trees of drafted tokens.
+
+``paged_window_attention`` is the decode of a model whose layers slide
+(``sink_window_mod`` in training): the query rows are the last positions of
+each sequence, and only the window's pages and the sinks' are read.
+``paged_tree_attention`` scores a tree of drafted tokens in one pass: every
+row sees the cached context and the drafts on its own path.  Both have no
+counterpart in the reference, whose decode lets every row see the whole
+context (attnax/kernels/paged.py:17-84).
+
+bf16/f16 caches with head_dim 64 or 128 and a block size that is a multiple
+of 16 take the fused kernels (one launch, and one that joins the splits);
+other caches gather each sequence and run the flash kernel on it, with one
+host sync.  Both kernels run on the current stream of the cache's device.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._spec import dtype_code
+from .flash import attention, softmax_scale
+from .paged import PagedKVCache, gather_kv
+
+
+def _check_query(query, cache: PagedKVCache):
+    if not isinstance(query, torch.Tensor) or query.dim() != 4:
+        raise ValueError("query must be (num_seqs, num_heads, seq_q, head_dim)")
+    n, hq, t, d = query.shape
+    if n != cache.block_table.shape[0]:
+        raise ValueError(f"query has {n} sequences, the cache {cache.block_table.shape[0]}")
+    if hq % cache.num_kv_heads != 0:
+        raise ValueError(f"num_heads ({hq}) must be divisible by num_kv_heads ({cache.num_kv_heads})")
+    if d != cache.head_dim:
+        raise ValueError(f"query head_dim {d} != cache head_dim {cache.head_dim}")
+    if not query.is_cuda or query.device != cache.key_pool.device:
+        raise RuntimeError("attnax_b200 kernels need the query on the cache's CUDA device; there is no CPU path")
+    return n, hq, t, d
+
+
+def _fused(cache: PagedKVCache) -> bool:
+    return (cache.head_dim in (64, 128) and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
+            and cache.block_size % 16 == 0 and cache.key_pool.is_contiguous() and cache.value_pool.is_contiguous())
+
+
+def _bound(cache: PagedKVCache, max_context):
+    if max_context is not None:
+        return int(max_context)
+    n = int(cache.seq_lengths.max()) if cache.seq_lengths.numel() else 0
+    if n > cache.block_table.shape[1] * cache.block_size:
+        raise ValueError(f"a sequence length ({n}) exceeds max_blocks_per_seq * block_size "
+                         f"({cache.block_table.shape[1]} * {cache.block_size})")
+    return n
+
+
+def _params(query, cache: PagedKVCache, max_context: int):
+    """(PagedParams, out, tensors that the call reads)."""
+    n, hq, t, d = query.shape
+    q = query.to(cache.key_pool.dtype).contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    out = torch.empty_like(q)
+    bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
+    p = _lib.PagedParams()
+    p.dtype = dtype_code(q.dtype)
+    p.num_seqs, p.num_heads_q, p.num_heads_kv, p.head_dim, p.seq_q = n, hq, cache.num_kv_heads, d, t
+    p.num_blocks, p.block_size, p.max_blocks_per_seq = cache.num_blocks, cache.block_size, bt.shape[1]
+    p.max_context = min(max_context, bt.shape[1] * cache.block_size)
+    p.q, p.key_pool, p.value_pool = q.data_ptr(), cache.key_pool.data_ptr(), cache.value_pool.data_ptr()
+    p.block_table, p.seq_lengths, p.out = bt.data_ptr(), sl.data_ptr(), out.data_ptr()
+    p.softmax_scale = softmax_scale(d)
+    return p, out, (q, bt, sl)
+
+
+def _workspace(p, nbytes: int, device):
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+        return ws
+    return None
+
+
+def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_sinks: int = 0, max_context=None):
+    """Sliding-window decode with sinks: ``query (B, Hq, T, D)`` -> same shape and type.
+
+    Row ``t`` of sequence ``b`` stands at position ``seq_lengths[b] - T + t``
+    (append the T tokens' K/V first) and sees the keys ``kv <= position`` with
+    ``position - kv < window_size`` or ``kv < num_sinks``.  Rows in front of
+    the sequence (T > its length) and empty sequences give zeros.  Pages that
+    no row sees are not read: their table entries may be -1 (``free_window``).
+
+    With ``max_context`` (an upper bound of the lengths) there is no host
+    sync; a longer sequence is then cut to the planned splits and noted in
+    ``_lib.device_status()``, as in ``paged_attention_batched``.
+    """
+    if window_size <= 0:
+        raise ValueError(f"window_size must be positive, got {window_size}")
+    if num_sinks < 0:
+        raise ValueError(f"num_sinks must not be negative, got {num_sinks}")
+    n, hq, t, d = _check_query(query, cache)
+    if n == 0 or t == 0:
+        return torch.zeros_like(query)
+    if not _fused(cache):
+        return _window_by_sequence(query, cache, int(window_size), int(num_sinks))
+    lib = _lib.load()
+    p, out, keep = _params(query, cache, _bound(cache, max_context))
+    w, s = min(int(window_size), 1 << 40), min(int(num_sinks), 1 << 40)
+    ws = _workspace(p, lib.attn_paged_window_workspace_size(C.byref(p), w, s), query.device)
+    with torch.cuda.device(query.device):
+        _lib.check(lib.attn_paged_window(C.byref(p), w, s,
+                                         C.c_void_p(torch.cuda.current_stream(query.device).cuda_stream)),
+                   "attn_paged_window")
+    del ws, keep
+    return out.to(query.dtype)
+
+
+def _window_by_sequence(query, cache, window, sinks):
+    out = torch.zeros_like(query)
+    t = query.shape[2]
+    for b in range(query.shape[0]):
+        k, v, n = gather_window(cache, b, t, window, sinks)
+        if n is None:
+            continue
+        kv = n  # positions of the gathered keys
+        length = int(cache.seq_lengths[b])
+        rows = torch.arange(length - t, length, device=query.device)
+        dist = rows[:, None] - kv[None, :]
+        mask = (dist >= 0) & ((dist < window) | (kv < sinks)[None, :])
+        first = max(0, t - length)  # rows in front of the sequence keep their zeros
+        out[b, :, first:] = attention(query[b:b + 1, :, first:].to(k.dtype), k, v, mask=mask[first:])[0].to(query.dtype)
+    return out
+
+
+def gather_window(cache: PagedKVCache, sequence_idx: int, rows: int, window: int, sinks: int):
+    """Contiguous ``(1, Hkv, n, D)`` keys/values of the positions that the last ``rows`` rows see, and the positions."""
+    length = int(cache.seq_lengths[sequence_idx])
+    if length == 0:
+        return None, None, None
+    dev = cache.key_pool.device
+    lo = max(0, length - rows - window + 1)
+    pos = torch.cat([torch.arange(min(sinks, lo), device=dev), torch.arange(lo, length, device=dev)])
+    nb, bs = cache.num_blocks, cache.block_size
+    page = cache.block_table[sequence_idx].long()[(pos // bs).clamp(max=cache.block_table.shape[1] - 1)]
+    page = torch.where(page < 0, page + nb, page).clamp(0, nb - 1)
+    k = cache.key_pool[page, pos % bs].permute(1, 0, 2)[None].contiguous()
+    v = cache.value_pool[page, pos % bs].permute(1, 0, 2)[None].contiguous()
+    return k, v, pos
+
+
+def _tma_ready(x: torch.Tensor) -> torch.Tensor:
+    """Unit stride on head_dim, other strides and the base in 16-byte steps (dimensions of one are not stepped)."""
+    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
+        s % 8 == 0 for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1)
+    return x if ok else x.contiguous().clone() if x.data_ptr() % 16 else x.contiguous()
+
+
+def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, parents, *, tree_lengths=None,
+                         max_context=None):
+    """Attention of drafted tokens: ``query (B, Hq, T, D)`` -> same shape and type.
+
+    ``draft_keys``/``draft_values`` ``(B, Hkv, T, D)`` are the drafts' own K/V
+    (any strides; not in the cache), ``parents (B, T)`` int32 gives each
+    token's parent: an earlier token, or a negative number for a token that
+    continues the context itself.  Row ``t`` sees the whole context
+    (``seq_lengths[b]`` tokens), itself and its ancestors.  With
+    ``tree_lengths (B,)`` the tokens at or past a sequence's length are
+    padding: nothing sees them and their rows are zeros.  A parent that is not
+    in front of its token counts as negative and is noted in
+    ``_lib.device_status()`` (``NOTICE_TREE_ORDER``).  T is at most 1024.
+
+    ``max_context`` as in :func:`paged_window_attention`.  The accepted path
+    goes into the cache with ``append_accepted``.
+    """
+    n, hq, t, d = _check_query(query, cache)
+    for name, x in (("draft_keys", draft_keys), ("draft_values", draft_values)):
+        if not isinstance(x, torch.Tensor) or x.shape != (n, cache.num_kv_heads, t, d):
+            raise ValueError(f"{name} must have shape {(n, cache.num_kv_heads, t, d)}, got "
+                             f"{tuple(getattr(x, 'shape', ()))}")
+        if x.device != query.device:
+            raise RuntimeError(f"{name} must be on the query's device")
+    dev = query.device
+    parents = torch.as_tensor(parents).to(device=dev, dtype=torch.int32).contiguous()
+    if parents.shape != (n, t):
+        raise ValueError(f"parents must have shape {(n, t)}, got {tuple(parents.shape)}")
+    if tree_lengths is not None:
+        tree_lengths = torch.as_tensor(tree_lengths).to(device=dev, dtype=torch.int32).contiguous()
+        if tree_lengths.shape != (n,):
+            raise ValueError(f"tree_lengths must have shape {(n,)}, got {tuple(tree_lengths.shape)}")
+    if t > 1024:
+        raise NotImplementedError(f"{t} drafted tokens; at most 1024")
+    if n == 0 or t == 0:
+        return torch.zeros_like(query)
+    if not _fused(cache):
+        return _tree_by_sequence(query, draft_keys, draft_values, cache, parents, tree_lengths)
+    lib = _lib.load()
+    p, out, keep = _params(query, cache, _bound(cache, max_context))
+    dk, dv = (_tma_ready(x.to(cache.key_pool.dtype)) for x in (draft_keys, draft_values))
+    tr = _lib.PagedTree()
+    tr.draft_keys, tr.draft_values = dk.data_ptr(), dv.data_ptr()
+    tr.k_strides[:], tr.v_strides[:] = dk.stride()[:3], dv.stride()[:3]
+    tr.parents = parents.data_ptr()
+    tr.tree_lengths = None if tree_lengths is None else tree_lengths.data_ptr()
+    ws = _workspace(p, lib.attn_paged_tree_workspace_size(C.byref(p)), dev)
+    with torch.cuda.device(dev):
+        _lib.check(lib.attn_paged_tree(C.byref(p), C.byref(tr),
+                                       C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "attn_paged_tree")
+    del ws, keep
+    return out.to(query.dtype)
+
+
+def _tree_by_sequence(query, dk, dv, cache, parents, tree_lengths):
+    out = torch.zeros_like(query)
+    par = parents.tolist()
+    lens = [query.shape[2]] * query.shape[0] if tree_lengths is None else tree_lengths.tolist()
+    for b in range(query.shape[0]):
+        m = min(max(lens[b], 0), query.shape[2])
+        if m == 0:
+            continue
+        keys, values, n = gather_kv(cache, b)
+        see = torch.zeros(m, n + m, dtype=torch.bool)
+        see[:, :n] = True
+        for t in range(m):
+            if 0 <= par[b][t] < t:
+                see[t, n:] = see[par[b][t], n:]
+            see[t, n + t] = True
+        k = torch.cat([keys.permute(1, 0, 2), dk[b, :, :m].to(keys.dtype)], 1)[None]
+        v = torch.cat([values.permute(1, 0, 2), dv[b, :, :m].to(keys.dtype)], 1)[None]
+        o = attention(query[b:b + 1, :, :m].to(k.dtype), k.contiguous(), v.contiguous(), mask=see.to(query.device))
+        out[b, :, :m] = o[0].to(query.dtype)
+    return out

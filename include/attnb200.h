@@ -148,6 +148,33 @@ int attn_paged_decode(const attn_paged_params_t* p, void* stream);
  * All calls share the array: calls that overlap on the GPU (different
  * streams, no ordering between them) race and corrupt each other. */
 int attn_paged_decode_static(const attn_paged_params_t* p, void* stream);
+/* Decode of several query rows per sequence, the last seq_q positions of the
+ * cache (their K/V already appended): row t stands at seq_lengths - seq_q + t
+ * and sees the keys kv <= it with  it - kv < window  or  kv < num_sinks.  Only
+ * the pages that some row sees are read; table entries of the others may hold
+ * anything.  Rows in front of the sequence (seq_q > seq_lengths) and empty
+ * sequences get zeros.  No counterpart in the reference.
+ * bf16/f16, head_dim 64 or 128, block_size a multiple of 16. */
+size_t attn_paged_window_workspace_size(const attn_paged_params_t* p, int64_t window, int64_t num_sinks);
+int attn_paged_window(const attn_paged_params_t* p, int64_t window, int64_t num_sinks, void* stream);
+/* Attention of a tree of drafted tokens: row t of sequence s sees the whole
+ * cached context [0, seq_lengths[s]) and the drafted tokens on its path: t,
+ * parents[s][t], the parent of that, ... up to a token whose parent is
+ * negative.  The drafts' K/V are tensors of their own, so the cache holds
+ * accepted tokens only (attn_paged_accept appends them).  Tokens at or past
+ * tree_lengths[s] are padding: nothing sees them and their rows are zeros.
+ * A parent at or behind its own token counts as negative and leaves the
+ * notice 0x203.  No counterpart in the reference.  Types and sizes as
+ * attn_paged_window; seq_q is the number of drafted tokens, at most 1024. */
+typedef struct {
+  const void* draft_keys;        /* [num_seqs, heads_kv, seq_q, head_dim], unit stride on head_dim, */
+  const void* draft_values;      /* 16-byte aligned */
+  int64_t k_strides[3], v_strides[3]; /* sequence, head, token: multiples of 16 bytes */
+  const int32_t* parents;        /* [num_seqs, seq_q] */
+  const int32_t* tree_lengths;   /* [num_seqs] or NULL: all seq_q */
+} attn_paged_tree_t;
+size_t attn_paged_tree_workspace_size(const attn_paged_params_t* p);
+int attn_paged_tree(const attn_paged_params_t* p, const attn_paged_tree_t* tree, void* stream);
 /* Contiguous copy of one sequence: keys/values [seq_len, heads_kv, head_dim]
  * from the pages block_table_row[0 .. ceil(seq_len / block_size)).  Entries
  * are read as the reference's pool[block_ids] reads them: negative entries
@@ -299,8 +326,9 @@ int attn_rope(const attn_rope_params_t* p, void* stream);
  * unwound; results are invalid).  0x201: a paged decode met a seq_lengths
  * entry above max_context and attended only its first splits.  0x202: a
  * paged decode met a sequence longer than max_blocks_per_seq * block_size
- * and reused the row's last entry for the pages past it.  A timeout code
- * takes precedence over a notice. */
+ * and reused the row's last entry for the pages past it.  0x203: a drafted
+ * token's parent was not in front of it.  0x204: a page operator skipped an
+ * entry that it could not use.  A timeout code takes precedence over a notice. */
 int attn_device_status(int32_t* status);
 const char* attn_status_string(int status);
 int attn_version(void);
