@@ -9,6 +9,8 @@ hand-written CUDA in ``libattnb200.so`` (C ABI: ``include/attnb200.h``):
 * ``paged_attention`` / ``paged_attention_batched`` over ``PagedKVCache``, and
   ``paged_window_attention`` / ``paged_tree_attention`` for sliding windows with
   sinks and trees of drafted tokens;
+* ``append_accepted``, ``copy_blocks``, ``fork_sequences``, ``free_sequences``,
+  ``free_window`` and ``compact_blocks`` on its pages, a batch at a time;
 * ``kv_cache_attention`` over the contiguous per-layer ``KVLayerCache``;
 * ``apply_rope`` (+ the reference's cos/sin table builders) for Q/K rotation;
 * ``ring_attention`` — sequence parallel over NCCL.
@@ -22,6 +24,8 @@ from .masking import (combine_masks, make_causal_mask, make_document_mask, make_
                       make_sliding_window_mask)
 from .paged import (PagedKVCache, allocate_blocks, append_kv, gather_kv, init_paged_kv_cache,
                     paged_attention, paged_attention_batched)
+from .pages import (append_accepted, compact_blocks, copy_blocks, fork_sequences, free_sequences,
+                    free_window)
 from .paged_rows import paged_tree_attention, paged_window_attention
 from .kv_cache import (KVLayerCache, init_decoder_kv_caches, init_kv_layer_cache, kv_cache_attention,
                        update_kv_layer_cache)
@@ -35,8 +39,8 @@ __all__ = [
     "AttentionFn", "MaskMod", "ScoreMod", "PagedKVCache", "KVLayerCache", "init_kv_layer_cache",
     "update_kv_layer_cache", "init_decoder_kv_caches", "kv_cache_attention", "apply_rope", "apply_rope_table",
     "rope_cos_sin_from_positions", "rope_cos_sin_table", "rope_inv_freq", "additive_bias_mod", "alibi_mod",
-    "alibi_slopes", "allocate_blocks", "append_kv", "causal_mod", "combine_masks",
-    "compose_score_mods", "document_mask_mod", "flash_attention", "gather_kv",
+    "alibi_slopes", "allocate_blocks", "append_accepted", "append_kv", "causal_mod", "combine_masks",
+    "compact_blocks", "compose_score_mods", "copy_blocks", "fork_sequences", "free_sequences", "free_window", "document_mask_mod", "flash_attention", "gather_kv",
     "init_paged_kv_cache", "make_causal_mask", "make_document_mask", "make_padding_mask",
     "make_sliding_window_mask", "mask_mod_to_boolean_mask", "mask_mod_to_score_mod",
     "memory_efficient_attention", "paged_attention", "paged_attention_batched", "paged_tree_attention",

@@ -81,6 +81,14 @@ class PagedTree(C.Structure):
     ]
 
 
+class PagedCacheParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("num_blocks", i32), ("block_size", i32), ("num_heads_kv", i32), ("head_dim", i32),
+        ("key_pool", vp), ("value_pool", vp), ("num_seqs", i32), ("max_blocks_per_seq", i32),
+        ("block_table", vp), ("seq_lengths", vp),
+    ]
+
+
 class RopeParams(C.Structure):
     _fields_ = [
         ("dtype", C.c_int), ("batch", i32), ("heads", i32), ("seq", i32), ("head_dim", i32),
@@ -125,6 +133,15 @@ SIGNATURES = {
     "attn_paged_window": (C.c_int, [C.POINTER(PagedParams), i64, i64, vp]),
     "attn_paged_tree_workspace_size": (szt, [C.POINTER(PagedParams)]),
     "attn_paged_tree": (C.c_int, [C.POINTER(PagedParams), C.POINTER(PagedTree), vp]),
+    "attn_paged_copy": (C.c_int, [C.POINTER(PagedCacheParams), vp, vp, i32, vp]),
+    "attn_paged_fork": (C.c_int, [C.POINTER(PagedCacheParams), vp, vp, i32, vp, i32, vp, vp, vp, vp]),
+    "attn_paged_free_workspace_size": (szt, [C.POINTER(PagedCacheParams)]),
+    "attn_paged_free": (C.c_int, [C.POINTER(PagedCacheParams), vp, i32, vp, vp, vp, vp, vp, szt, vp]),
+    "attn_paged_free_window": (C.c_int, [C.POINTER(PagedCacheParams), i64, i64, vp, vp, vp, vp, szt, vp]),
+    "attn_paged_compact_workspace_size": (szt, [C.POINTER(PagedCacheParams)]),
+    "attn_paged_compact": (C.c_int, [C.POINTER(PagedCacheParams), vp, vp, vp, szt, vp]),
+    "attn_paged_accept": (C.c_int, [C.POINTER(PagedCacheParams), vp, vp, C.POINTER(i64), C.POINTER(i64), i32, vp, i32,
+                                    vp, vp, vp, vp]),
     "attn_paged_gather": (C.c_int, [C.c_int, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, vp]),
     "attn_paged_append": (C.c_int, [C.c_int, vp, vp, i32, i32, i32, i32, vp, i32, i32, i32, vp, vp, vp, vp]),
     "attn_paged_physical_page": (i64, [i32, i32]),

@@ -36,9 +36,23 @@ def _check_query(query, cache: PagedKVCache):
         raise ValueError(f"num_heads ({hq}) must be divisible by num_kv_heads ({cache.num_kv_heads})")
     if d != cache.head_dim:
         raise ValueError(f"query head_dim {d} != cache head_dim {cache.head_dim}")
+    check_tables(cache)
+    return n, hq, t, d
+
+
+def check_tables(cache: PagedKVCache):
+    """The kernels read int32 tables on the pools' device."""
+    for name in ("block_table", "seq_lengths"):
+        x = getattr(cache, name)
+        if x.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32, got {x.dtype}")
+        if x.device != cache.key_pool.device:
+            raise RuntimeError(f"{name} must be on the pools' device")
+
+
+def _need_cuda(query, cache: PagedKVCache):
     if not query.is_cuda or query.device != cache.key_pool.device:
         raise RuntimeError("attnax_b200 kernels need the query on the cache's CUDA device; there is no CPU path")
-    return n, hq, t, d
 
 
 def _fused(cache: PagedKVCache) -> bool:
@@ -101,6 +115,7 @@ def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_
     if num_sinks < 0:
         raise ValueError(f"num_sinks must not be negative, got {num_sinks}")
     n, hq, t, d = _check_query(query, cache)
+    _need_cuda(query, cache)
     if n == 0 or t == 0:
         return torch.zeros_like(query)
     if not _fused(cache):
@@ -191,6 +206,7 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
             raise ValueError(f"tree_lengths must have shape {(n,)}, got {tuple(tree_lengths.shape)}")
     if t > 1024:
         raise NotImplementedError(f"{t} drafted tokens; at most 1024")
+    _need_cuda(query, cache)
     if n == 0 or t == 0:
         return torch.zeros_like(query)
     if not _fused(cache):

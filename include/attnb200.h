@@ -196,6 +196,62 @@ int attn_paged_append(attn_dtype_t dtype, void* key_pool, void* value_pool, int3
                       int32_t block_size, int32_t heads_kv, int32_t head_dim,
                       const int32_t* block_table_row, int32_t max_blocks, int32_t start, int32_t chunk,
                       const void* keys_new, const void* values_new, int32_t* bad_slot, void* stream);
+/* ---- pages of the cache ------------------------------------------------- */
+/* A paged cache as the page operators see it.  They work on whole batches
+ * without a host round trip; index lists live on the device.  An index that
+ * cannot be used (out of range, not allocated, given twice where that is
+ * ambiguous) never writes outside the pool: its entry is skipped and the
+ * notice 0x204 is left.  No counterparts in the reference, which allocates
+ * and appends one sequence at a time (attnax/paged_cache.py:92-198). */
+typedef struct {
+  attn_dtype_t dtype;
+  int32_t num_blocks, block_size, num_heads_kv, head_dim;
+  void* key_pool;                /* [num_blocks, block_size, heads_kv, head_dim] */
+  void* value_pool;
+  int32_t num_seqs, max_blocks_per_seq;
+  const int32_t* block_table;    /* [num_seqs, max_blocks_per_seq], -1 unused */
+  const int32_t* seq_lengths;    /* [num_seqs] */
+} attn_paged_cache_t;
+/* Copies page src[i] over page dst[i], keys and values, i < n.  A dst given
+ * twice takes the first; a page that is a source of another entry is not
+ * written (the entries run in no order); src[i] == dst[i] does nothing. */
+int attn_paged_copy(const attn_paged_cache_t* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+/* Rows dst[i] become copies of rows src[i]: full pages are shared, a last page
+ * that is not full is copied to a page of free_ids (in order of i), and
+ * table_out / lengths_out hold the new table (not aliasing the old one).
+ * *used gets the number of free_ids taken. */
+int attn_paged_fork(const attn_paged_cache_t* c, const int32_t* src, const int32_t* dst, int32_t n,
+                    const int32_t* free_ids, int32_t num_free, int32_t* table_out, int32_t* lengths_out,
+                    int32_t* used, void* stream);
+/* Rows seqs[i] end: -1 entries and length 0 in table_out / lengths_out.
+ * freed [num_blocks] gets the pages that only these rows referred to,
+ * ascending, then -1; *count their number.  The pools are not touched. */
+size_t attn_paged_free_workspace_size(const attn_paged_cache_t* c);
+int attn_paged_free(const attn_paged_cache_t* c, const int32_t* seqs, int32_t n, int32_t* table_out,
+                    int32_t* lengths_out, int32_t* freed, int32_t* count, void* workspace, size_t workspace_bytes,
+                    void* stream);
+/* Every row gives up the pages that no later query of a causal window with
+ * sinks sees: tokens all behind num_sinks and all more than window - 1 in
+ * front of position seq_lengths.  Outputs as attn_paged_free (lengths stay). */
+int attn_paged_free_window(const attn_paged_cache_t* c, int64_t window, int64_t num_sinks, int32_t* table_out,
+                           int32_t* freed, int32_t* count, void* workspace, size_t workspace_bytes, void* stream);
+/* Moves the pages that rows refer to into the first pages of the pool: the
+ * live pages at or past their number *num_live, ascending, go to the pages
+ * below it that are not live, ascending.  table_out refers to the new places;
+ * the pools are rewritten in place. */
+size_t attn_paged_compact_workspace_size(const attn_paged_cache_t* c);
+int attn_paged_compact(const attn_paged_cache_t* c, int32_t* table_out, int32_t* num_live, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Appends the drafted tokens accepted[s][0 .. accepted_lengths[s]) of every
+ * sequence s to its pages, at positions seq_lengths[s].. (pages already in
+ * the table); lengths_out gets the new lengths.  Drafts as in attn_paged_tree
+ * ([num_seqs, heads_kv, num_drafts, head_dim], any strides but the last).
+ * With bad non-NULL (pre-set to INT32_MAX) only checks: the lowest sequence
+ * with an unusable entry is stored there and nothing is written. */
+int attn_paged_accept(const attn_paged_cache_t* c, const void* draft_keys, const void* draft_values,
+                      const int64_t k_strides[3], const int64_t v_strides[3], int32_t num_drafts,
+                      const int32_t* accepted, int32_t max_accepted, const int32_t* accepted_lengths,
+                      int32_t* lengths_out, int32_t* bad, void* stream);
 /* The pool page a block-table entry selects (host copy of the kernels' rule):
  * entry < 0 -> entry + num_blocks, then clamped into [0, num_blocks). */
 int64_t attn_paged_physical_page(int32_t entry, int32_t num_blocks);
