@@ -18,6 +18,24 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
 // Counts `n` kernel launches and reports the launch error state.
 int launch_status(int n = 1);
 
+// Launches `kernel` so that it may start while the previous kernel of the
+// stream drains; it must call pdl_wait_previous() before it reads or writes
+// anything that one touches.
+template <typename... P, typename... A>
+inline void launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);  // (the error state is read by launch_status)
+}
+
 // 4-D tiled map over a (B, H, S, D) tensor (see attnb200.cu).
 bool make_tmap(CUtensorMap* m, attn_dtype_t dt, const void* ptr, int B, int H, int S, int D, const int64_t* s,
                int box_rows);

@@ -11,11 +11,15 @@
 // rows of one kv head (its query heads x T) share every K/V read.  With up to
 // 64 rows the work is bound by HBM (4 * rows flops per byte of K/V); wider
 // trees approach the tensor cores' rate.
-//   rows_mma_kernel  up to 64 rows: warp-level MMA on a TMA ring of 16- or
-//                    32-token units, 1, 2 or 4 row tiles of 16 per CTA
+//   rows_mma_kernel  up to 32 rows: warp-level MMA on a TMA ring of 16- or
+//                    32-token units, one or two row tiles of 16 per CTA
 //   rows_tc_kernel   more rows: tcgen05 on 128-row x 128-token tiles gathered page by page by
 //                    TMA, two CTAs per SM
-//   rows_join_kernel joins the splits
+//   rows_join_kernel joins the splits, its start hidden behind the end of the others
+// Measured on one B200 (64 sequences of 512..32768 tokens, 8 kv heads of 128,
+// bf16, GB/s of K/V): 4 rows 6556 / 5969 (warp MMA / tcgen05), 16 rows 6332 /
+// 5787, 32 rows 5891 / 5692, 48 rows (four row tiles) 3295 / 5511; hence the
+// border at 32.
 #include <cfloat>
 
 #include <atomic>
@@ -28,7 +32,8 @@
 namespace attnb200 {
 namespace rows {
 
-constexpr int kMaxTree = 1024;  // drafted tokens per sequence
+constexpr int kMaxTree = 1024;   // drafted tokens per sequence
+constexpr int kMmaRows = 32;     // rows of a kv head up to which rows_mma_kernel runs
 
 struct Args {
   int N, Hq, Hkv, T, group, rows, row_groups;  // rows = group * T of one kv head
@@ -112,7 +117,7 @@ __device__ __forceinline__ int split_count(const Args& a, const Span& s) {
   return min((s.total + a.split_units - 1) / a.split_units, a.max_splits);
 }
 
-// ---------------------------------------------------- up to 64 query rows --
+// ---------------------------------------------------- up to 32 query rows --
 constexpr int NW = 4;  // consumer warps
 constexpr int kMmaThreads = (NW + 1) * 32;
 
@@ -165,6 +170,10 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
   __syncthreads();
 
   if (warp == NW) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
     // Pages of 32 units at a time are looked up by the 32 lanes.
     for (int i0 = 0; i0 < n; i0 += 32) {
       int row = 0;  // pool row (context) or token (draft) of this lane's unit
@@ -199,12 +208,13 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
     return;
   }
 
+  pdl_launch_next();
   const int rt = warp % RW, tw = warp / RW;  // row tile, share of the units
   const int g = lane >> 2, tig = lane & 3;
   const long long row0 = ((long long)seq * a.Hkv + hkv) * a.rows;  // rows of q / out before this kv head's
   int pos[2];                          // window: position of the fragment rows; tree: drafted token
   bool row_ok[2];
-  unsigned long long anc[2] = {0, 0};  // tree: drafted tokens on the row's path
+  uint32_t anc[2] = {0, 0};            // tree: drafted tokens on the row's path (T <= rows <= 32)
   uint32_t qf[D / 16][4];              // A fragments: [k-step][row g lo, row g + 8 lo, row g hi, row g + 8 hi]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -219,7 +229,7 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
       qf[kk][2 + h] = row_ok[h] ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * tig) : 0u;
     }
     if (TREE && row_ok[h] && v0 + n > sp.n_ctx)
-      for (int p = t; p >= 0; p = parent_of(a.parents + (long long)seq * a.T, p)) anc[h] |= 1ull << p;
+      for (int p = t; p >= 0; p = parent_of(a.parents + (long long)seq * a.T, p)) anc[h] |= 1u << p;
   }
   float o[D / 8][4];
 #pragma unroll
@@ -271,7 +281,7 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
           for (int e = 0; e < 4; ++e) {
             const int tk = tok_a + 8 * x + 2 * tig + (e & 1), h = e >> 1;
             bool keep;
-            if (TREE) keep = draft ? (tk < sp.drafts && ((anc[h] >> (tk & 63)) & 1)) : tk < sp.len;
+            if (TREE) keep = draft ? (tk < sp.drafts && ((anc[h] >> (tk & 31)) & 1)) : tk < sp.len;
             else keep = tk <= pos[h] && (pos[h] - tk < a.window || tk < a.sinks);
             if (!keep) sc[x][e] = -INFINITY;
           }
@@ -378,7 +388,7 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
   }
 }
 
-// ----------------------------------------------- more than 64 query rows --
+// ----------------------------------------------- more than 32 query rows --
 // CTA = 128 rows of one kv head x a split of its 128-token tiles.  Warps 0-3
 // run the softmax (thread = row = TMEM lane), warp 4 gathers the tiles by TMA
 // (one box per page piece, a lane each), warp 5 issues the MMAs; warps 6-7 only
@@ -467,10 +477,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  pdl_launch_next();
   if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcProducerRegs));
     if (warp == 4) {
       if (n > 0 && lane == 0) {
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
         mbar_expect_tx(q_full, C::Q_BYTES);
         for (int c = 0; c < C::KCH; ++c)
           tma_load_4d(sb + c * BM * 128, &tm_q, q_full, c * 64, rg * BM, hkv, seq);
@@ -703,9 +716,10 @@ template <typename T, int D, bool TREE>
 __global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ Args a) {
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), seq = blockIdx.y, lane = threadIdx.x & 31;
   if (row >= a.Hkv * a.rows) return;
-  const Span sp = make_span<TREE>(a, seq, a.span_unit);
+  const Span sp = make_span<TREE>(a, seq, a.span_unit);  // (lengths: not written by the kernel in front)
   const int n = split_count(a, sp);
   if (n <= 1) return;
+  pdl_wait_previous();
   const long long prow = (long long)seq * a.Hkv * a.rows + row;
   const float* lse = a.part_lse + prow * a.max_splits;
   const float* po = a.part_o + prow * a.max_splits * D + lane * (D / 32);
@@ -746,13 +760,16 @@ static long long max_tokens(const attn_paged_params_t* p, bool tree, int64_t win
   return ll_min(ctx, w + s);
 }
 
-// Splits: enough CTAs to fill the GPU three times over (the residency of the
-// kernel), none under 128 tokens, where a split's start and its partial cost
-// more than its K/V; at most 2048 tokens, so that ragged batches stay even.
+// Splits: enough CTAs to fill the GPU as often as the kernel is resident, none
+// under 128 tokens (one sequence of 2500 tokens, one row: 14.7 us at 128 or 256
+// tokens, 18.8 at 512, 31.0 at 1024), and no longer than keeps ragged batches
+// even: 2048 tokens with few rows, where a partial is small next to its K/V;
+// 4096 on tcgen05, whose partials are up to 128 rows x 512 bytes (96 rows:
+// 5094 GB/s at 2048, 5381 at 4096; 256 rows: 1736 us and 1430 us).
 static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, int64_t sinks) {
   Plan w;
   const int rows = p->num_heads_q / p->num_heads_kv * p->seq_q;
-  w.tc = rows > 64;
+  w.tc = rows > kMmaRows;
   if (w.tc) {
     w.unit = 128;
     while (p->block_size % w.unit != 0) w.unit /= 2;
@@ -760,7 +777,7 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
     w.row_tiles = BM / 16;
   } else {
     w.unit = w.span_unit = p->block_size % 32 == 0 ? 32 : 16;
-    w.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    w.row_tiles = rows <= 16 ? 1 : 2;
   }
   w.row_groups = (rows + w.row_tiles * 16 - 1) / (w.row_tiles * 16);
   const long long tokens = max_tokens(p, tree, window, sinks), u = w.span_unit;
@@ -768,7 +785,7 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
   const long long units = (tokens + u - 1) / u + (tree ? (p->seq_q + u - 1) / u : 3);
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * w.row_groups;
   const long long want = ((w.tc ? 2 : 3) * 148 + ctas - 1) / ctas;
-  const long long least = ll_max(128 / u, 1), most = 2048 / u;
+  const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u;
   w.split_units = (int)ll_min(ll_max((units + want - 1) / want, least), most);
   w.max_splits = (int)((units + w.split_units - 1) / w.split_units);
   const size_t parts = (size_t)p->num_seqs * p->num_heads_kv * rows * w.max_splits;
@@ -842,16 +859,12 @@ static int launch_rows(const Plan& w, const Maps& t, const Args& a, cudaStream_t
   if (w.tc)
     rc = launch_tc<BF16, D, TREE>(t, a, st);
   else if (w.unit == 32)
-    rc = w.row_tiles == 1   ? launch_mma<BF16, D, 32, 1, TREE>(t, a, st)
-         : w.row_tiles == 2 ? launch_mma<BF16, D, 32, 2, TREE>(t, a, st)
-                            : launch_mma<BF16, D, 32, 4, TREE>(t, a, st);
+    rc = w.row_tiles == 1 ? launch_mma<BF16, D, 32, 1, TREE>(t, a, st) : launch_mma<BF16, D, 32, 2, TREE>(t, a, st);
   else
-    rc = w.row_tiles == 1   ? launch_mma<BF16, D, 16, 1, TREE>(t, a, st)
-         : w.row_tiles == 2 ? launch_mma<BF16, D, 16, 2, TREE>(t, a, st)
-                            : launch_mma<BF16, D, 16, 4, TREE>(t, a, st);
+    rc = w.row_tiles == 1 ? launch_mma<BF16, D, 16, 1, TREE>(t, a, st) : launch_mma<BF16, D, 16, 2, TREE>(t, a, st);
   if (rc != ATTN_OK || a.max_splits == 1) return rc;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  rows_join_kernel<T, D, TREE><<<dim3((a.Hkv * a.rows + 7) / 8, a.N), 256, 0, st>>>(a);
+  launch_overlapped(rows_join_kernel<T, D, TREE>, dim3((a.Hkv * a.rows + 7) / 8, a.N), dim3(256), 0, st, a);
   return launch_status();
 }
 
