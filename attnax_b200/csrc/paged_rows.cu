@@ -228,8 +228,23 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
       qf[kk][h] = row_ok[h] ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 2 * tig) : 0u;
       qf[kk][2 + h] = row_ok[h] ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8 + 2 * tig) : 0u;
     }
-    if (TREE && row_ok[h] && v0 + n > sp.n_ctx)
-      for (int p = t; p >= 0; p = parent_of(a.parents + (long long)seq * a.T, p)) anc[h] |= 1u << p;
+  }
+  if (TREE && v0 + n > sp.n_ctx) {
+    // Lane x holds drafted token x: its path doubles in length with each step.
+    int p = lane < a.T ? parent_of(a.parents + (long long)seq * a.T, lane) : -1;
+    uint32_t path = 1u << lane;
+#pragma unroll
+    for (int x = 0; x < 5; ++x) {
+      const uint32_t up = __shfl_sync(0xffffffffu, path, p & 31);
+      const int pp = __shfl_sync(0xffffffffu, p, p & 31);
+      if (p >= 0) path |= up;
+      p = p >= 0 ? pp : -1;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t x = __shfl_sync(0xffffffffu, path, pos[h] & 31);
+      anc[h] = row_ok[h] ? x : 0u;
+    }
   }
   float o[D / 8][4];
 #pragma unroll
@@ -414,7 +429,8 @@ struct TcCfg {
   static constexpr int OFF_BAR = OFF_V + STAGES * KV_BYTES;
   static constexpr int NBAR = 4 + 4 * STAGES;
   static constexpr int OFF_TMEMPTR = OFF_BAR + NBAR * 8;
-  static constexpr int SMEM = OFF_TMEMPTR + 16 + 1024;
+  static constexpr int OFF_PARENTS = OFF_TMEMPTR + 16;  // tree: the sequence's parents, 16 bits each
+  static constexpr int SMEM = OFF_PARENTS + kMaxTree * 2 + 1024;
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
   static constexpr uint32_t TMEM_COLS = 256, O_COL = 128;
 };
@@ -455,6 +471,10 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   auto k_empty = [&](int s) { return bar0 + 8u * (4 + 2 * S + s); };
   auto v_empty = [&](int s) { return bar0 + 8u * (4 + 3 * S + s); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEMPTR);
+  int16_t* parents = reinterpret_cast<int16_t*>(smem + C::OFF_PARENTS);
+  if (TREE && v0 + n > sp.n_ctx)  // this split holds drafted tokens
+    for (int x = threadIdx.x; x < a.T; x += kTcThreads)
+      parents[x] = (int16_t)max(parent_of(a.parents + (long long)seq * a.T, x), -1);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(s_full, 1);
@@ -559,7 +579,6 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     const int t = r % a.T;
     const bool row_ok = r < a.rows && (!TREE || t < sp.drafts);
     const int pos = sp.len - a.T + t;     // window: position of the row
-    const int32_t* parents = TREE ? a.parents + (long long)seq * a.T : nullptr;
     int walk = TREE && row_ok ? t : -1;   // tree: next token on the row's path
     const uint32_t s_addr = tmem + ((uint32_t)(warp * 32) << 16);
     float m = -FLT_MAX, l = 0.f;
@@ -579,7 +598,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               if ((x >> 5) == c) keep[c] |= 1u << (x & 31);
-            walk = parent_of(parents, walk);
+            walk = parents[walk];
           }
         } else {
 #pragma unroll
@@ -724,17 +743,31 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ 
   const float* lse = a.part_lse + prow * a.max_splits;
   const float* po = a.part_o + prow * a.max_splits * D + lane * (D / 32);
   float mx = -INFINITY;
-  for (int i = 0; i < n; ++i) mx = fmaxf(mx, lse[i]);
+  for (int i = lane; i < n; i += 32) mx = fmaxf(mx, lse[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float tot = 0.f, acc[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
   if (mx != -INFINITY) {
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float w = ex2(lse[i] - mx);
-      tot += w;
+    constexpr int B = 8;  // partials in flight
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const float wl = i0 + lane < n ? ex2(lse[i0 + lane] - mx) : 0.f;
+      for (int j0 = 0; j0 < min(32, n - i0); j0 += B) {
+        float x[B][D / 32];
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, po[(long long)i * D + e], acc[e]);
+        for (int j = 0; j < B; ++j)
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e)
+            x[j][e] = i0 + j0 + j < n ? po[(long long)(i0 + j0 + j) * D + e] : 0.f;
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+          const float w = __shfl_sync(0xffffffffu, wl, j0 + j);
+          tot += w;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, x[j][e], acc[e]);
+        }
+      }
     }
   }
   const float inv = tot > 0.f ? 1.f / tot : 0.f;
@@ -760,12 +793,14 @@ static long long max_tokens(const attn_paged_params_t* p, bool tree, int64_t win
   return ll_min(ctx, w + s);
 }
 
-// Splits: enough CTAs to fill the GPU as often as the kernel is resident, none
-// under 128 tokens (one sequence of 2500 tokens, one row: 14.7 us at 128 or 256
-// tokens, 18.8 at 512, 31.0 at 1024), and no longer than keeps ragged batches
-// even: 2048 tokens with few rows, where a partial is small next to its K/V;
-// 4096 on tcgen05, whose partials are up to 128 rows x 512 bytes (96 rows:
-// 5094 GB/s at 2048, 5381 at 4096; 256 rows: 1736 us and 1430 us).
+// Splits: the number that ends first if every sequence is as long as it may be,
+// counting waves of resident CTAs and about 256 tokens of time for a CTA's start
+// and its partial.  None under 128 tokens (one sequence of 2500 tokens, one
+// row: 14.7 us at 128 or 256 tokens, 18.8 at 512, 31.0 at 1024), and none longer
+// than keeps ragged batches even: 2048 tokens with few rows, where a partial is
+// small next to its K/V; 4096 on tcgen05, whose partials are up to 128 rows x
+// 512 bytes (96 rows: 5094 GB/s at 2048, 5381 at 4096; 256 rows: 1736 us and
+// 1430 us).
 static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, int64_t sinks) {
   Plan w;
   const int rows = p->num_heads_q / p->num_heads_kv * p->seq_q;
@@ -784,9 +819,17 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
   // (window: the first and last unit of both pieces may be cut)
   const long long units = (tokens + u - 1) / u + (tree ? (p->seq_q + u - 1) / u : 3);
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * w.row_groups;
-  const long long want = ((w.tc ? 2 : 3) * 148 + ctas - 1) / ctas;
-  const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u;
-  w.split_units = (int)ll_min(ll_max((units + want - 1) / want, least), most);
+  const long long slots = (w.tc ? 2 : 3) * 148;
+  const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u, start = 256 / u;
+  const long long s_min = (units + most - 1) / most, s_max = ll_max(ll_min(units / least, s_min + 64), s_min);
+  w.split_units = (int)most;
+  for (long long s = ll_max(s_min, 1), best = -1; s <= s_max; ++s) {
+    const long long len = (units + s - 1) / s, cost = (ctas * s + slots - 1) / slots * (len + start);
+    if (best < 0 || cost < best) {
+      best = cost;
+      w.split_units = (int)ll_max(len, least);
+    }
+  }
   w.max_splits = (int)((units + w.split_units - 1) / w.split_units);
   const size_t parts = (size_t)p->num_seqs * p->num_heads_kv * rows * w.max_splits;
   w.part_lse = w.max_splits > 1 ? align256(parts * p->head_dim * sizeof(float)) : 0;
