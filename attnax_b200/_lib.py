@@ -198,6 +198,24 @@ def check(status: int, what: str):
     raise KernelError(f"{what}: {msg} (status {status})")
 
 
+def run(name: str, device, *args):
+    """Calls entry point ``name`` on the current stream of ``device``, with that device current.
+
+    (The device is switched only where it has to be: a switch costs more host time than a small launch.)
+    """
+    import torch
+
+    fn = getattr(_lib or load(), name)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if status != ATTN_OK:
+        check(status, name)
+
+
 def device_status() -> int:
     """Reads and clears the device status word (non-zero after a timed-out wait)."""
     v = i32(0)

@@ -17,6 +17,7 @@ host sync.  Both kernels run on the current stream of the cache's device.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -42,12 +43,19 @@ def _check_query(query, cache: PagedKVCache):
 
 def check_tables(cache: PagedKVCache):
     """The kernels read int32 tables on the pools' device."""
-    for name in ("block_table", "seq_lengths"):
-        x = getattr(cache, name)
+    dev = cache.key_pool.device
+    for name, x in (("block_table", cache.block_table), ("seq_lengths", cache.seq_lengths)):
         if x.dtype != torch.int32:
             raise ValueError(f"{name} must be int32, got {x.dtype}")
-        if x.device != cache.key_pool.device:
+        if x.device != dev:
             raise RuntimeError(f"{name} must be on the pools' device")
+
+
+def on_device(x, device) -> torch.Tensor:
+    """int32, contiguous, on the device."""
+    if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == device:
+        return x.contiguous()
+    return torch.as_tensor(x).to(device=device, dtype=torch.int32).contiguous()
 
 
 def _need_cuda(query, cache: PagedKVCache):
@@ -78,15 +86,17 @@ def _params(query, cache: PagedKVCache, max_context: int):
         q = q.clone()
     out = torch.empty_like(q)
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    p = _lib.PagedParams()
-    p.dtype = dtype_code(q.dtype)
-    p.num_seqs, p.num_heads_q, p.num_heads_kv, p.head_dim, p.seq_q = n, hq, cache.num_kv_heads, d, t
-    p.num_blocks, p.block_size, p.max_blocks_per_seq = cache.num_blocks, cache.block_size, bt.shape[1]
-    p.max_context = min(max_context, bt.shape[1] * cache.block_size)
-    p.q, p.key_pool, p.value_pool = q.data_ptr(), cache.key_pool.data_ptr(), cache.value_pool.data_ptr()
-    p.block_table, p.seq_lengths, p.out = bt.data_ptr(), sl.data_ptr(), out.data_ptr()
-    p.softmax_scale = softmax_scale(d)
+    nb, bs, hkv, _ = cache.key_pool.shape
+    width = bt.shape[1]
+    p = _lib.PagedParams(dtype_code(q.dtype), n, hq, hkv, d, t, nb, bs, width, min(max_context, width * bs),
+                         q.data_ptr(), cache.key_pool.data_ptr(), cache.value_pool.data_ptr(), bt.data_ptr(),
+                         sl.data_ptr(), out.data_ptr(), _scale(d))
     return p, out, (q, bt, sl)
+
+
+@functools.lru_cache(maxsize=None)
+def _scale(head_dim: int) -> float:
+    return softmax_scale(head_dim)
 
 
 def _workspace(p, nbytes: int, device):
@@ -124,10 +134,7 @@ def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_
     p, out, keep = _params(query, cache, _bound(cache, max_context))
     w, s = min(int(window_size), 1 << 40), min(int(num_sinks), 1 << 40)
     ws = _workspace(p, lib.attn_paged_window_workspace_size(C.byref(p), w, s), query.device)
-    with torch.cuda.device(query.device):
-        _lib.check(lib.attn_paged_window(C.byref(p), w, s,
-                                         C.c_void_p(torch.cuda.current_stream(query.device).cuda_stream)),
-                   "attn_paged_window")
+    _lib.run("attn_paged_window", query.device, C.byref(p), w, s)
     del ws, keep
     return out.to(query.dtype)
 
@@ -169,7 +176,7 @@ def _tma_ready(x: torch.Tensor) -> torch.Tensor:
     """Unit stride on head_dim, other strides and the base in 16-byte steps (dimensions of one are not stepped)."""
     ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
         s % 8 == 0 for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1)
-    return x if ok else x.contiguous().clone() if x.data_ptr() % 16 else x.contiguous()
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
 def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, parents, *, tree_lengths=None,
@@ -197,11 +204,11 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
         if x.device != query.device:
             raise RuntimeError(f"{name} must be on the query's device")
     dev = query.device
-    parents = torch.as_tensor(parents).to(device=dev, dtype=torch.int32).contiguous()
+    parents = on_device(parents, dev)
     if parents.shape != (n, t):
         raise ValueError(f"parents must have shape {(n, t)}, got {tuple(parents.shape)}")
     if tree_lengths is not None:
-        tree_lengths = torch.as_tensor(tree_lengths).to(device=dev, dtype=torch.int32).contiguous()
+        tree_lengths = on_device(tree_lengths, dev)
         if tree_lengths.shape != (n,):
             raise ValueError(f"tree_lengths must have shape {(n,)}, got {tuple(tree_lengths.shape)}")
     if t > 1024:
@@ -214,15 +221,10 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
     lib = _lib.load()
     p, out, keep = _params(query, cache, _bound(cache, max_context))
     dk, dv = (_tma_ready(x.to(cache.key_pool.dtype)) for x in (draft_keys, draft_values))
-    tr = _lib.PagedTree()
-    tr.draft_keys, tr.draft_values = dk.data_ptr(), dv.data_ptr()
-    tr.k_strides[:], tr.v_strides[:] = dk.stride()[:3], dv.stride()[:3]
-    tr.parents = parents.data_ptr()
-    tr.tree_lengths = None if tree_lengths is None else tree_lengths.data_ptr()
+    tr = _lib.PagedTree(dk.data_ptr(), dv.data_ptr(), dk.stride()[:3], dv.stride()[:3], parents.data_ptr(),
+                        None if tree_lengths is None else tree_lengths.data_ptr())
     ws = _workspace(p, lib.attn_paged_tree_workspace_size(C.byref(p)), dev)
-    with torch.cuda.device(dev):
-        _lib.check(lib.attn_paged_tree(C.byref(p), C.byref(tr),
-                                       C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "attn_paged_tree")
+    _lib.run("attn_paged_tree", dev, C.byref(p), C.byref(tr))
     del ws, keep
     return out.to(query.dtype)
 

@@ -23,7 +23,10 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .paged import PagedKVCache
-from .paged_rows import check_tables
+from .paged_rows import check_tables, on_device
+
+
+_Strides = C.c_int64 * 3
 
 
 def _params(cache: PagedKVCache):
@@ -31,30 +34,22 @@ def _params(cache: PagedKVCache):
     if not cache.key_pool.is_cuda:
         raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
     check_tables(cache)
-    if not (cache.key_pool.is_contiguous() and cache.value_pool.is_contiguous()):
+    kp, vpool = cache.key_pool, cache.value_pool
+    if not (kp.is_contiguous() and vpool.is_contiguous()):
         raise ValueError("page operators write the pools in place and need them contiguous")
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    p = _lib.PagedCacheParams()
-    p.dtype = dtype_code(cache.key_pool.dtype)
-    p.num_blocks, p.block_size = cache.num_blocks, cache.block_size
-    p.num_heads_kv, p.head_dim = cache.num_kv_heads, cache.head_dim
-    p.key_pool, p.value_pool = cache.key_pool.data_ptr(), cache.value_pool.data_ptr()
-    p.num_seqs, p.max_blocks_per_seq = bt.shape
-    p.block_table, p.seq_lengths = bt.data_ptr(), sl.data_ptr()
+    p = _lib.PagedCacheParams(dtype_code(kp.dtype), *kp.shape, kp.data_ptr(), vpool.data_ptr(), *bt.shape,
+                              bt.data_ptr(), sl.data_ptr())
     return p, (bt, sl)
-
-
-def _call(device, name: str, *args):
-    with torch.cuda.device(device):
-        stream = C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-        _lib.check(getattr(_lib.load(), name)(*args, stream), name)
 
 
 def _indices(x, device, limit: int, what: str, distinct: bool = False) -> torch.Tensor:
     """int32 indices on the device; what comes from the host is checked there."""
-    t = torch.as_tensor(x)
+    t = x if isinstance(x, torch.Tensor) else torch.as_tensor(x)
     if t.dim() != 1:
         raise ValueError(f"{what} must be one-dimensional, got shape {tuple(t.shape)}")
+    if t.is_cuda and t.dtype == torch.int32 and t.device == device:
+        return t.contiguous()
     if t.numel() and (t.is_floating_point() or t.dtype == torch.bool):
         raise ValueError(f"{what} must be integers, got {t.dtype}")
     if not t.is_cuda:
@@ -85,7 +80,7 @@ def copy_blocks(cache: PagedKVCache, src_blocks, dst_blocks) -> PagedKVCache:
             raise ValueError(f"page {int(both[0])} is both a source and a destination")
     p, keep = _params(cache)
     if src.numel():
-        _call(dev, "attn_paged_copy", C.byref(p), src.data_ptr(), dst.data_ptr(), src.numel())
+        _lib.run("attn_paged_copy", dev, C.byref(p), src.data_ptr(), dst.data_ptr(), src.numel())
     del keep
     return cache
 
@@ -116,22 +111,26 @@ def fork_sequences(cache: PagedKVCache, src_sequences, dst_sequences, free_block
         if need > free.numel():
             raise ValueError(f"free_block_ids has {free.numel()} entries but {need} are needed")
     p, keep = _params(cache)
-    table = torch.empty_like(cache.block_table, memory_format=torch.contiguous_format)
-    lens = torch.empty_like(cache.seq_lengths, memory_format=torch.contiguous_format)
+    table = torch.empty(cache.block_table.shape, dtype=torch.int32, device=dev)
+    lens = torch.empty(cache.seq_lengths.shape, dtype=torch.int32, device=dev)
     used = torch.empty((), dtype=torch.int32, device=dev)
-    _call(dev, "attn_paged_fork", C.byref(p), src.data_ptr(), dst.data_ptr(), src.numel(),
+    _lib.run("attn_paged_fork", dev, C.byref(p), src.data_ptr(), dst.data_ptr(), src.numel(),
           free.data_ptr() if free.numel() else None, free.numel(), table.data_ptr(), lens.data_ptr(), used.data_ptr())
     del keep
     return PagedKVCache(cache.key_pool, cache.value_pool, table, lens), used
 
 
+def _scratch(ws):
+    return (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
+
+
 def _freed(cache: PagedKVCache, p):
     dev = cache.key_pool.device
-    nbytes = _lib.load().attn_paged_free_workspace_size(C.byref(p))
-    return (torch.empty_like(cache.block_table, memory_format=torch.contiguous_format),
+    nbytes = _lib.load().attn_paged_free_workspace_size(C.byref(p))  # 0 but for huge pools
+    return (torch.empty(cache.block_table.shape, dtype=torch.int32, device=dev),
             torch.empty(cache.num_blocks, dtype=torch.int32, device=dev),
             torch.empty((), dtype=torch.int32, device=dev),
-            torch.empty(nbytes, dtype=torch.uint8, device=dev))
+            torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None)
 
 
 def free_sequences(cache: PagedKVCache, sequences):
@@ -145,9 +144,9 @@ def free_sequences(cache: PagedKVCache, sequences):
     seqs = _indices(sequences, dev, cache.block_table.shape[0], "sequences")
     p, keep = _params(cache)
     table, freed, count, ws = _freed(cache, p)
-    lens = torch.empty_like(cache.seq_lengths, memory_format=torch.contiguous_format)
-    _call(dev, "attn_paged_free", C.byref(p), seqs.data_ptr() if seqs.numel() else None, seqs.numel(),
-          table.data_ptr(), lens.data_ptr(), freed.data_ptr(), count.data_ptr(), ws.data_ptr(), ws.numel())
+    lens = torch.empty(cache.seq_lengths.shape, dtype=torch.int32, device=dev)
+    _lib.run("attn_paged_free", dev, C.byref(p), seqs.data_ptr() if seqs.numel() else None, seqs.numel(),
+          table.data_ptr(), lens.data_ptr(), freed.data_ptr(), count.data_ptr(), *_scratch(ws))
     del keep
     return PagedKVCache(cache.key_pool, cache.value_pool, table, lens), freed, count
 
@@ -167,8 +166,8 @@ def free_window(cache: PagedKVCache, *, window_size: int, num_sinks: int = 0):
     dev = cache.key_pool.device
     p, keep = _params(cache)
     table, freed, count, ws = _freed(cache, p)
-    _call(dev, "attn_paged_free_window", C.byref(p), min(int(window_size), 1 << 40), min(int(num_sinks), 1 << 40),
-          table.data_ptr(), freed.data_ptr(), count.data_ptr(), ws.data_ptr(), ws.numel())
+    _lib.run("attn_paged_free_window", dev, C.byref(p), min(int(window_size), 1 << 40), min(int(num_sinks), 1 << 40),
+          table.data_ptr(), freed.data_ptr(), count.data_ptr(), *_scratch(ws))
     del keep
     return PagedKVCache(cache.key_pool, cache.value_pool, table, cache.seq_lengths), freed, count
 
@@ -183,10 +182,10 @@ def compact_blocks(cache: PagedKVCache):
     """
     dev = cache.key_pool.device
     p, keep = _params(cache)
-    table = torch.empty_like(cache.block_table, memory_format=torch.contiguous_format)
+    table = torch.empty(cache.block_table.shape, dtype=torch.int32, device=dev)
     live = torch.empty((), dtype=torch.int32, device=dev)
     ws = torch.empty(_lib.load().attn_paged_compact_workspace_size(C.byref(p)), dtype=torch.uint8, device=dev)
-    _call(dev, "attn_paged_compact", C.byref(p), table.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel())
+    _lib.run("attn_paged_compact", dev, C.byref(p), table.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel())
     del keep
     return PagedKVCache(cache.key_pool, cache.value_pool, table, cache.seq_lengths), live
 
@@ -218,8 +217,7 @@ def append_accepted(cache: PagedKVCache, draft_keys, draft_values, accepted, acc
     if draft_keys.shape != draft_values.shape:
         raise ValueError(f"draft_keys shape {tuple(draft_keys.shape)} != draft_values shape "
                          f"{tuple(draft_values.shape)}")
-    acc = torch.as_tensor(accepted).to(device=dev, dtype=torch.int32).contiguous()
-    lens = torch.as_tensor(accepted_lengths).to(device=dev, dtype=torch.int32).contiguous()
+    acc, lens = on_device(accepted, dev), on_device(accepted_lengths, dev)
     if acc.dim() != 2 or acc.shape[0] != n:
         raise ValueError(f"accepted must have shape ({n}, A), got {tuple(acc.shape)}")
     if lens.shape != (n,):
@@ -230,17 +228,17 @@ def append_accepted(cache: PagedKVCache, draft_keys, draft_values, accepted, acc
         if check and n and bool((lens != 0).any()):
             raise ValueError("accepted_lengths counts tokens that are not there")
         return cache
-    kd, vd = (x.to(cache.key_pool.dtype) for x in (draft_keys, draft_values))
-    kd, vd = (x if x.stride(-1) == 1 else x.contiguous() for x in (kd, vd))
-    ks, vs = (C.c_int64 * 3)(*kd.stride()[:3]), (C.c_int64 * 3)(*vd.stride()[:3])
+    kd, vd = draft_keys.to(cache.key_pool.dtype), draft_values.to(cache.key_pool.dtype)
+    kd, vd = (x if x.stride(3) == 1 else x.contiguous() for x in (kd, vd))
+    ks, vs = _Strides(*kd.stride()[:3]), _Strides(*vd.stride()[:3])
     args = (C.byref(p), kd.data_ptr(), vd.data_ptr(), ks, vs, t, acc.data_ptr(), acc.shape[1], lens.data_ptr())
     if check:
         bad = torch.full((), 2**31 - 1, dtype=torch.int32, device=dev)
-        _call(dev, "attn_paged_accept", *args, None, bad.data_ptr())
+        _lib.run("attn_paged_accept", dev, *args, None, bad.data_ptr())
         if int(bad) != 2**31 - 1:
             raise ValueError(f"sequence {int(bad)}: an accepted index, its count or the page for it is out of "
                              "range; call allocate_blocks before append_accepted")
-    out = torch.empty_like(cache.seq_lengths, memory_format=torch.contiguous_format)
-    _call(dev, "attn_paged_accept", *args, out.data_ptr(), None)
+    out = torch.empty(cache.seq_lengths.shape, dtype=torch.int32, device=dev)
+    _lib.run("attn_paged_accept", dev, *args, out.data_ptr(), None)
     del keep
     return PagedKVCache(cache.key_pool, cache.value_pool, cache.block_table, out)

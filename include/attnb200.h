@@ -223,7 +223,8 @@ int attn_paged_copy(const attn_paged_cache_t* c, const int32_t* src, const int32
 int attn_paged_fork(const attn_paged_cache_t* c, const int32_t* src, const int32_t* dst, int32_t n,
                     const int32_t* free_ids, int32_t num_free, int32_t* table_out, int32_t* lengths_out,
                     int32_t* used, void* stream);
-/* Rows seqs[i] end: -1 entries and length 0 in table_out / lengths_out.
+/* (attn_paged_free*: the workspace is needed, and its size not 0, only for pools of more than 819200 pages.)
+ * Rows seqs[i] end: -1 entries and length 0 in table_out / lengths_out.
  * freed [num_blocks] gets the pages that only these rows referred to,
  * ascending, then -1; *count their number.  The pools are not touched. */
 size_t attn_paged_free_workspace_size(const attn_paged_cache_t* c);

@@ -160,7 +160,9 @@ def test_c_entries_refuse_windows_trees_and_lists():
     c.num_seqs, c.max_blocks_per_seq, c.block_table, c.seq_lengths = 1, 1, 16, 32
     # the new table may not be the old one; scratch is the caller's
     assert lib.attn_paged_fork(C.byref(c), 16, 16, 1, 16, 1, 16, 48, 16, None) == _lib.ATTN_ERR_INVALID
+    c.num_blocks = 1 << 20
     assert lib.attn_paged_free(C.byref(c), 16, 1, 48, 48, 48, 48, None, 0, None) == _lib.ATTN_ERR_WORKSPACE
+    c.num_blocks = 8
     assert lib.attn_paged_free_window(C.byref(c), 0, 0, 48, 48, 48, 16, 1024, None) == _lib.ATTN_ERR_INVALID
     assert lib.attn_paged_compact(C.byref(c), 48, 48, None, 0, None) == _lib.ATTN_ERR_WORKSPACE
     s = (C.c_int64 * 3)(64, 64, 64)

@@ -71,6 +71,23 @@ def test_copy_skips_what_it_cannot_do():
     assert _lib.device_status() == _lib.NOTICE_PAGE_LIST
 
 
+def test_copy_long_lists():
+    """Many entries share their look through the lists; the rules stay."""
+    cache, _ = rand_cache(1, [1], 1, 8, 1, BF, spare=4000)
+    k, v, table, lens = host(cache)
+    nb = cache.num_blocks
+    perm = torch.randperm(nb, generator=torch.Generator().manual_seed(5)).to(torch.int32)
+    src, dst = perm[:1999].clone(), perm[1999:3998].clone()
+    src[500], dst[1300], src[77] = nb, -5, dst[77]    # skipped, skipped, onto itself
+    dst[1501] = dst[1500]                             # the first wins
+    src[1998] = dst[40]                               # entry 40 may not write a source
+    ok = [i for i in range(1999) if i not in (500, 1300, 77, 1501, 40)]
+    k[dst[ok].long()], v[dst[ok].long()] = k[src[ok].long()], v[src[ok].long()]
+    out = ax.copy_blocks(cache, src.to(DEV), dst.to(DEV))
+    check(out, k, v, table, lens)
+    assert _lib.device_status() == _lib.NOTICE_PAGE_LIST
+
+
 def fork_model(bs, table, lens, src, dst, free):
     """(table, lens, page copies, used) of the forks, one after the other on the old table."""
     new, newlen, moves, used = [list(r) for r in table], list(lens), [], 0
@@ -249,6 +266,28 @@ def test_append_accepted_refuses_or_skips():
         k[table[s][pos // 16], pos % 16] = dk[s, :, tok].cpu()
         v[table[s][pos // 16], pos % 16] = dv[s, :, tok].cpu()
     check(out, k, v, table, [15, 22, 7])
+
+
+@pytest.mark.parametrize("nb,rows", [(819200, 3), (819201, 3), (1200000, 400)])
+def test_sets_of_many_pages(nb, rows):
+    """Pools on both sides of what the bit maps in shared memory hold."""
+    g = torch.Generator().manual_seed(nb)
+    pool = torch.arange(nb, dtype=torch.float32, device=DEV).view(nb, 1, 1, 1)
+    ids = torch.randperm(nb, generator=g)[:rows * 700].view(rows, 700).to(torch.int32)
+    ids[0, 0], ids[1, 3] = nb - 1, 0
+    cache = ax.PagedKVCache(pool, pool.clone(), ids.to(DEV), torch.full((rows,), 700, dtype=torch.int32, device=DEV))
+    out, freed, n = ax.free_sequences(cache, [0, rows - 1])
+    left = set(ids[1:rows - 1].flatten().tolist())
+    want = sorted(set(ids[[0, rows - 1]].flatten().tolist()) - left)
+    assert int(n) == len(want) and freed[:len(want)].tolist() == want and bool((freed[len(want):] == -1).all())
+    new, live = ax.compact_blocks(out)
+    assert int(live) == len(left)
+    t, old = new.block_table[1:rows - 1].cpu(), ids[1:rows - 1]
+    assert sorted(set(t.flatten().tolist())) == list(range(len(left)))
+    assert torch.equal(new.key_pool.flatten()[t.to(DEV).long()].cpu().to(torch.int32), old)
+    assert torch.equal(new.value_pool.flatten()[t.to(DEV).long()].cpu().to(torch.int32), old)
+    stay = old < len(left)
+    assert torch.equal(t[stay], old[stay])
 
 
 def test_pools_past_32_bits():
