@@ -36,6 +36,25 @@ inline void launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_
   cudaLaunchKernelEx(&cfg, kernel, P(args)...);  // (the error state is read by launch_status)
 }
 
+// Launches `kernel` in clusters of `cluster` CTAs along y.
+template <typename... P, typename... A>
+inline void launch_cluster_y(void (*kernel)(P...), int cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                             const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1;
+  at[0].val.clusterDim.y = cluster;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // 4-D tiled map over a (B, H, S, D) tensor (see attnb200.cu).
 bool make_tmap(CUtensorMap* m, attn_dtype_t dt, const void* ptr, int B, int H, int S, int D, const int64_t* s,
                int box_rows);

@@ -15,7 +15,11 @@
 //                    32-token units, one or two row tiles of 16 per CTA
 //   rows_tc_kernel   more rows: tcgen05 on 128-row x 128-token tiles gathered page by page by
 //                    TMA, two CTAs per SM
-//   rows_join_kernel joins the splits, its start hidden behind the end of the others
+//   rows_join_kernel joins the splits, its start hidden behind the end of the others; up to 8
+//                    splits of rows_mma_kernel that all run at once form a cluster and join through
+//                    each other's shared memory instead (one launch, no partials in memory; on
+//                    tcgen05 a 64 KB tile per CTA makes that the slower way: 4 sequences of 8000, 64
+//                    rows: 39.8 us joined by a launch, 46.3 us in clusters)
 // Measured on one B200 (64 sequences of 512..32768 tokens, 8 kv heads of 128,
 // bf16, GB/s of K/V): 4 rows 6556 / 5969 (warp MMA / tcgen05), 16 rows 6332 /
 // 5787, 32 rows 5891 / 5692, 48 rows (four row tiles) 3295 / 5511; hence the
@@ -42,6 +46,7 @@ struct Args {
   int unit;                      // tokens of a TMA box
   int span_unit;                 // tokens of the units that splits count: `unit`, or the 128 of a tile
   int max_splits, split_units;   // units per split
+  bool cluster;                  // the splits of a row are a cluster and join in it
   const void* q;
   const int32_t* block_table;
   const int32_t* seq_lens;
@@ -117,6 +122,44 @@ __device__ __forceinline__ int split_count(const Args& a, const Span& s) {
   return min((s.total + a.split_units - 1) / a.split_units, a.max_splits);
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Address of `p` (this CTA's shared memory) in CTA `rank` of the cluster.
+template <typename T>
+__device__ __forceinline__ T* in_cluster(T* p, int rank) {
+  uint64_t out;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<T*>(out);
+}
+
+// One row joined from the splits' normalised rows `o` (this lane's D / 32
+// values) and log-sum-exps `lse` in the CTAs [0, n) of the cluster, n <= 32.
+template <int D, typename T, bool BF16>
+__device__ __forceinline__ void join_in_cluster(float* o, float* lse, int n, int lane, T* out) {
+  const float mine = lane < n ? *in_cluster(lse, lane) : -INFINITY;
+  float mx = mine;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  const float w = mx == -INFINITY ? 0.f : ex2(mine - mx);
+  float tot = 0.f, acc[D / 32];
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float* oi = in_cluster(o, i);
+    const float wi = __shfl_sync(0xffffffffu, w, i);
+    tot += wi;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wi, oi[e], acc[e]);
+  }
+  const float inv = tot > 0.f ? 1.f / tot : 0.f;
+#pragma unroll
+  for (int e = 0; e < D / 32; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e) = pack2(acc[e] * inv, acc[e + 1] * inv, BF16);
+}
+
 // ---------------------------------------------------- up to 32 query rows --
 constexpr int NW = 4;  // consumer warps
 constexpr int kMmaThreads = (NW + 1) * 32;
@@ -128,7 +171,9 @@ struct MmaCfg {
   static constexpr int STAGES = 65536 / (2 * SLICE);
   static constexpr int MS = D + 4;               // padded row of the merge buffer
   static constexpr int SMEM = 1024 + STAGES * 2 * SLICE + 2 * STAGES * 8;
-  static_assert(NW * 16 * (MS + 2) * 4 <= STAGES * 2 * SLICE, "the merge buffer fits the drained ring");
+  // After the ring has drained: the warps' states, then (cluster) up to 32 joined rows and their LSE.
+  static constexpr int OFF_ROWS = NW * 16 * (MS + 2) * 4;
+  static_assert(OFF_ROWS + kMmaRows * (D + 1) * 4 <= STAGES * 2 * SLICE, "the merge buffers fit the drained ring");
 };
 
 // RW row tiles of 16 per CTA, one per warp; the other NW / RW warps of a row
@@ -146,7 +191,7 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
   const int split = blockIdx.y, seq = blockIdx.z;
   const Span sp = make_span<TREE>(a, seq, U);
   const int n_split = split_count(a, sp);
-  if (split >= n_split && split > 0) return;
+  if (split >= n_split && split > 0 && !(a.cluster && n_split > 1)) return;
   if (split == 0 && threadIdx.x == 0 && sp.total > a.max_splits * a.split_units)
     atomicCAS(&g_notice, 0, kNoticeContextOverrun);
   const int v0 = split * a.split_units;
@@ -156,10 +201,13 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
   const uint32_t raw_base = smem_u32(smem_raw);
   const uint32_t sb = (raw_base + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sb - raw_base);
+  float* rows_o = reinterpret_cast<float*>(smem + C::OFF_ROWS);  // [RW * 16][D], then their LSE
+  float* rows_lse = rows_o + RW * 16 * D;
   const uint32_t k_base = sb, v_base = sb + S * C::SLICE, bar0 = sb + 2 * S * C::SLICE;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (S + s); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row0 = ((long long)seq * a.Hkv + hkv) * a.rows;  // rows of q / out before this kv head's
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full(s), 1);
@@ -205,13 +253,10 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
       }
       if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
     }
-    return;
-  }
-
+  } else {
   pdl_launch_next();
   const int rt = warp % RW, tw = warp / RW;  // row tile, share of the units
   const int g = lane >> 2, tig = lane & 3;
-  const long long row0 = ((long long)seq * a.Hkv + hkv) * a.rows;  // rows of q / out before this kv head's
   int pos[2];                          // window: position of the fragment rows; tree: drafted token
   bool row_ok[2];
   uint32_t anc[2] = {0, 0};            // tree: drafted tokens on the row's path (T <= rows <= 32)
@@ -368,10 +413,10 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
     }
   }
   named_bar_sync(1, NW * 32);
-  if (!__all_sync(0xffffffffu, ok)) return;
+  ok = __all_sync(0xffffffffu, ok);
   for (int j = warp; j < RW * 16; j += NW) {
     const int r = rg * RW * 16 + j;
-    if (r >= a.rows) continue;
+    if (r >= a.rows || !ok) continue;
     const int t = j >> 4, jr = j & 15;  // row tile and row in it: warps t, t + RW, ...
     float mx = -FLT_MAX;
 #pragma unroll
@@ -394,12 +439,30 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
 #pragma unroll
       for (int e = 0; e < D / 32; e += 2)
         *reinterpret_cast<uint32_t*>(orow + e) = pack2(acc[e] * inv, acc[e + 1] * inv, BF16);
+    } else if (a.cluster) {
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) rows_o[j * D + lane * (D / 32) + e] = acc[e] * inv;
+      if (lane == 0) rows_lse[j] = lt > 0.f ? mx + lg2(lt) : -INFINITY;
     } else {
       const long long at = (row0 + r) * a.max_splits + split;
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) a.part_o[at * D + lane * (D / 32) + e] = acc[e] * inv;
       if (lane == 0) a.part_lse[at] = lt > 0.f ? mx + lg2(lt) : -INFINITY;
     }
+  }
+  }
+  if (a.cluster && n_split > 1) {
+    // Each CTA of the cluster joins a share of the rows; none leaves before its rows are read.
+    __syncwarp();
+    cluster_sync();
+    if (warp < NW)
+      for (int j = split + a.max_splits * warp; j < RW * 16; j += a.max_splits * NW) {
+        const int r = rg * RW * 16 + j;
+        if (r < a.rows)
+          join_in_cluster<D, T, BF16>(rows_o + j * D + lane * (D / 32), rows_lse + j, n_split, lane,
+                                      reinterpret_cast<T*>(a.out) + (row0 + r) * D + lane * (D / 32));
+      }
+    cluster_sync();
   }
 }
 
@@ -496,6 +559,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
 
   pdl_launch_next();
   if (warp >= 4) {
@@ -687,7 +751,6 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       const float inv = l > 0.f ? 1.f / l : 0.f;
       const long long row = ((long long)seq * a.Hkv + hkv) * a.rows + r;
       const long long at = row * a.max_splits + split;
-      using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -780,7 +843,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ 
 
 // -------------------------------------------------------------------- host --
 struct Plan {
-  bool tc;
+  bool tc, cluster;
   int unit, span_unit, row_tiles, row_groups, max_splits, split_units;
   size_t part_lse, total;
 };
@@ -794,13 +857,21 @@ static long long max_tokens(const attn_paged_params_t* p, bool tree, int64_t win
 }
 
 // Splits: the number that ends first if every sequence is as long as it may be,
-// counting waves of resident CTAs and about 256 tokens of time for a CTA's start
-// and its partial.  None under 128 tokens (one sequence of 2500 tokens, one
+// counting waves of resident CTAs.  None under 128 tokens (one sequence of 2500 tokens, one
 // row: 14.7 us at 128 or 256 tokens, 18.8 at 512, 31.0 at 1024), and none longer
 // than keeps ragged batches even: 2048 tokens with few rows, where a partial is
 // small next to its K/V; 4096 on tcgen05, whose partials are up to 128 rows x
 // 512 bytes (96 rows: 5094 GB/s at 2048, 5381 at 4096; 256 rows: 1736 us and
 // 1430 us).
+// Splits that join in a cluster: as many as a cluster holds everywhere, and
+// only where every CTA runs at once (a CTA of a short sequence waits for its
+// cluster, which would keep the next wave's CTAs out).
+static bool cluster_fits(bool tc, long long splits, long long waves) { return !tc && splits <= 8 && waves <= 1; }
+// A CTA's start and its partial, and a launch of rows_join_kernel, in the time
+// of so many tokens of a CTA (one sequence of 2500 tokens, one row: 10.2 us in
+// 20 splits and a join, 12.5 us in a cluster of 8; of 1028 tokens: 9.0 and 8.4).
+constexpr int kStartTokens = 256, kJoinTokens = 96;
+
 static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, int64_t sinks) {
   Plan w;
   const int rows = p->num_heads_q / p->num_heads_kv * p->seq_q;
@@ -820,18 +891,21 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
   const long long units = (tokens + u - 1) / u + (tree ? (p->seq_q + u - 1) / u : 3);
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * w.row_groups;
   const long long slots = (w.tc ? 2 : 3) * 148;
-  const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u, start = 256 / u;
+  const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u;
   const long long s_min = (units + most - 1) / most, s_max = ll_max(ll_min(units / least, s_min + 64), s_min);
   w.split_units = (int)most;
   for (long long s = ll_max(s_min, 1), best = -1; s <= s_max; ++s) {
-    const long long len = (units + s - 1) / s, cost = (ctas * s + slots - 1) / slots * (len + start);
+    const long long len = (units + s - 1) / s, waves = (ctas * s + slots - 1) / slots;
+    const bool joins = s > 1 && !cluster_fits(w.tc, s, waves);
+    const long long cost = waves * (ll_max(len, least) * u + kStartTokens) + (joins ? kJoinTokens : 0);
     if (best < 0 || cost < best) {
       best = cost;
       w.split_units = (int)ll_max(len, least);
     }
   }
   w.max_splits = (int)((units + w.split_units - 1) / w.split_units);
-  const size_t parts = (size_t)p->num_seqs * p->num_heads_kv * rows * w.max_splits;
+  w.cluster = w.max_splits > 1 && cluster_fits(w.tc, w.max_splits, (ctas * w.max_splits + slots - 1) / slots);
+  const size_t parts = w.cluster ? 0 : (size_t)p->num_seqs * p->num_heads_kv * rows * w.max_splits;
   w.part_lse = w.max_splits > 1 ? align256(parts * p->head_dim * sizeof(float)) : 0;
   w.total = w.max_splits > 1 ? w.part_lse + align256(parts * sizeof(float)) : 0;
   return w;
@@ -875,7 +949,9 @@ static int launch_mma(const Maps& t, const Args& a, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   auto kern = rows_mma_kernel<BF16, D, U, RW, TREE>;
   if (!smem_once(kern, C::SMEM, done)) return ATTN_ERR_CUDA;
-  kern<<<dim3(a.Hkv * a.row_groups, a.max_splits, a.N), kMmaThreads, C::SMEM, st>>>(t.k, t.v, t.dk, t.dv, a);
+  const dim3 grid(a.Hkv * a.row_groups, a.max_splits, a.N);
+  if (a.cluster) launch_cluster_y(kern, a.max_splits, grid, dim3(kMmaThreads), C::SMEM, st, t.k, t.v, t.dk, t.dv, a);
+  else kern<<<grid, kMmaThreads, C::SMEM, st>>>(t.k, t.v, t.dk, t.dv, a);
   return launch_status();
 }
 
@@ -905,7 +981,7 @@ static int launch_rows(const Plan& w, const Maps& t, const Args& a, cudaStream_t
     rc = w.row_tiles == 1 ? launch_mma<BF16, D, 32, 1, TREE>(t, a, st) : launch_mma<BF16, D, 32, 2, TREE>(t, a, st);
   else
     rc = w.row_tiles == 1 ? launch_mma<BF16, D, 16, 1, TREE>(t, a, st) : launch_mma<BF16, D, 16, 2, TREE>(t, a, st);
-  if (rc != ATTN_OK || a.max_splits == 1) return rc;
+  if (rc != ATTN_OK || a.max_splits == 1 || a.cluster) return rc;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   launch_overlapped(rows_join_kernel<T, D, TREE>, dim3((a.Hkv * a.rows + 7) / 8, a.N), dim3(256), 0, st, a);
   return launch_status();
@@ -945,6 +1021,7 @@ static int run(const attn_paged_params_t* p, const attn_paged_tree_t* tree, int6
   a.BS = p->block_size; a.max_blocks = p->max_blocks_per_seq; a.num_blocks = p->num_blocks;
   a.window = window; a.sinks = sinks;
   a.unit = w.unit; a.span_unit = w.span_unit; a.max_splits = w.max_splits; a.split_units = w.split_units;
+  a.cluster = w.cluster;
   a.q = p->q; a.block_table = p->block_table; a.seq_lens = p->seq_lengths;
   a.parents = tree ? tree->parents : nullptr;
   a.tree_lens = tree ? tree->tree_lengths : nullptr;
