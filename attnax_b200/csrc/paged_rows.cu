@@ -467,35 +467,39 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
 }
 
 // ----------------------------------------------- more than 32 query rows --
-// CTA = 128 rows of one kv head x a split of its 128-token tiles.  Warps 0-3
-// run the softmax (thread = row = TMEM lane), warp 4 gathers the tiles by TMA
-// (one box per page piece, a lane each), warp 5 issues the MMAs; warps 6-7 only
-// complete the warpgroup that hands its registers to the softmax warps.  TMEM:
-// S in [0, 128), P over its first 64 columns, O in [128, 128 + D).  One CTA's
-// chain S -> softmax -> P V is serial; the second CTA on the SM fills its gaps,
-// which is enough to stay on HBM at 128 rows (one tile per CTA and stage, 96 KB
-// of shared memory).
+// CTA = NT tiles of 128 rows of one kv head x a split of its 128-token tiles.
+// Warps 0-3 (and 4-7) run the softmax of a row tile (thread = row = TMEM lane),
+// the next warp gathers the K/V tiles by TMA (one box per page piece, a lane
+// each), the one behind it issues the MMAs; two more only complete the warpgroup
+// that hands its registers to the softmax warps.  TMEM: S of tile x in [128 x,
+// 128 x + 128), P over its first 64 columns, the O's behind the S's.
+//   NT = 1 (up to 128 rows): a CTA's chain S -> softmax -> P V is serial; a second
+//     CTA on the SM fills its gaps, which is enough to stay on HBM.
+//   NT = 2 (more rows): the two tiles share every K/V tile and fill each other's
+//     gaps (order P V_0, S_0, P V_1, S_1), one CTA per SM.  With one tile per CTA
+//     the tiles' K/V came from L2 at 64 KB per 128 x 128 tile, about 14 TB/s.
 constexpr int BM = 128, BN = 128;
-constexpr int kTcThreads = 256;
-// Register split (setmaxnreg) of a CTA launched at kTcRegs per thread.
-constexpr int kTcRegs = 128, kTcProducerRegs = 56, kTcSoftmaxRegs = 200;
-static_assert(128 * (kTcProducerRegs + kTcSoftmaxRegs) == kTcThreads * kTcRegs, "register split");
-
-template <int D>
+template <int D, int NT>
 struct TcCfg {
   static constexpr int KCH = D / 64;
-  static constexpr int STAGES = D == 64 ? 2 : 1;
-  static constexpr int Q_BYTES = KCH * BM * 128;
+  static constexpr int STAGES = (NT == 1 ? 128 : 256) / D;  // 1 or 2 at D = 128, 2 or 4 at D = 64
+  static constexpr int THREADS = 128 * (NT + 1);
+  // Register split (setmaxnreg) of a CTA launched at REGS per thread.
+  static constexpr int REGS = NT == 1 ? 128 : 168, PRODUCER_REGS = NT == 1 ? 56 : 104, SOFTMAX_REGS = 200;
+  static_assert(128 * (PRODUCER_REGS + NT * SOFTMAX_REGS) == THREADS * REGS, "register split");
+  static constexpr int Q_BYTES = KCH * BM * 128;  // one row tile
   static constexpr int KV_BYTES = KCH * BN * 128;
-  static constexpr int OFF_K = Q_BYTES;
+  static constexpr int OFF_K = NT * Q_BYTES;
   static constexpr int OFF_V = OFF_K + STAGES * KV_BYTES;
   static constexpr int OFF_BAR = OFF_V + STAGES * KV_BYTES;
-  static constexpr int NBAR = 4 + 4 * STAGES;
+  static constexpr int NBAR = 2 + 2 * NT + 4 * STAGES;
   static constexpr int OFF_TMEMPTR = OFF_BAR + NBAR * 8;
   static constexpr int OFF_PARENTS = OFF_TMEMPTR + 16;  // tree: the sequence's parents, 16 bits each
   static constexpr int SMEM = OFF_PARENTS + kMaxTree * 2 + 1024;
-  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
-  static constexpr uint32_t TMEM_COLS = 256, O_COL = 128;
+  static constexpr int CTAS = NT == 1 ? 2 : 1;  // per SM
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "resident CTAs");
+  static constexpr uint32_t TMEM_COLS = 256 * NT;
+  __host__ __device__ static constexpr uint32_t o_col(int x) { return 128 * NT + x * D; }
 };
 
 // The tile that position i of the split visits: context tiles in order, drafted
@@ -505,13 +509,13 @@ __device__ __forceinline__ int tile_at(const Span& s, int v0, int n, int i) {
   return v < ctx ? v : max(v0, ctx) + (v0 + n - 1 - v);
 }
 
-template <bool BF16, int D, bool TREE>
-__global__ void __launch_bounds__(kTcThreads, 2)
+template <bool BF16, int D, int NT, bool TREE>
+__global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
     rows_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_dk,
                    const __grid_constant__ CUtensorMap tm_dv, const __grid_constant__ Args a) {
-  using C = TcCfg<D>;
-  constexpr int S = C::STAGES;
+  using C = TcCfg<D, NT>;
+  constexpr int S = C::STAGES, kTma = 4 * NT, kMma = 4 * NT + 1;  // warps
   const int hkv = blockIdx.x / a.row_groups, rg = blockIdx.x % a.row_groups;
   const int split = blockIdx.y, seq = blockIdx.z;
   const Span sp = make_span<TREE>(a, seq, BN);
@@ -528,21 +532,25 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   uint8_t* smem = smem_raw + (sb - raw_base);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bar0 = sb + C::OFF_BAR;
-  const uint32_t q_full = bar0, s_full = bar0 + 8, p_full = bar0 + 16, o_done = bar0 + 24;
-  auto k_full = [&](int s) { return bar0 + 8u * (4 + s); };
-  auto v_full = [&](int s) { return bar0 + 8u * (4 + S + s); };
-  auto k_empty = [&](int s) { return bar0 + 8u * (4 + 2 * S + s); };
-  auto v_empty = [&](int s) { return bar0 + 8u * (4 + 3 * S + s); };
+  const uint32_t q_full = bar0, o_done = bar0 + 8;
+  auto s_full = [&](int x) { return bar0 + 8u * (2 + x); };
+  auto p_full = [&](int x) { return bar0 + 8u * (2 + NT + x); };
+  auto k_full = [&](int s) { return bar0 + 8u * (2 + 2 * NT + s); };
+  auto v_full = [&](int s) { return bar0 + 8u * (2 + 2 * NT + S + s); };
+  auto k_empty = [&](int s) { return bar0 + 8u * (2 + 2 * NT + 2 * S + s); };
+  auto v_empty = [&](int s) { return bar0 + 8u * (2 + 2 * NT + 3 * S + s); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEMPTR);
   int16_t* parents = reinterpret_cast<int16_t*>(smem + C::OFF_PARENTS);
   if (TREE && v0 + n > sp.n_ctx)  // this split holds drafted tokens
-    for (int x = threadIdx.x; x < a.T; x += kTcThreads)
+    for (int x = threadIdx.x; x < a.T; x += C::THREADS)
       parents[x] = (int16_t)max(parent_of(a.parents + (long long)seq * a.T, x), -1);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);  // one arrival per softmax warp
     mbar_init(o_done, 1);
+    for (int x = 0; x < NT; ++x) {
+      mbar_init(s_full(x), 1);
+      mbar_init(p_full(x), 4);  // one arrival per softmax warp
+    }
     for (int s = 0; s < S; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(v_full(s), 1);
@@ -551,7 +559,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     }
     fence_mbar_init();
   }
-  if (warp == 5) {
+  if (warp == kMma) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -562,15 +570,16 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
 
   pdl_launch_next();
-  if (warp >= 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcProducerRegs));
-    if (warp == 4) {
+  if (warp >= kTma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::PRODUCER_REGS));
+    if (warp == kTma) {
       if (n > 0 && lane == 0) {
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
-        mbar_expect_tx(q_full, C::Q_BYTES);
-        for (int c = 0; c < C::KCH; ++c)
-          tma_load_4d(sb + c * BM * 128, &tm_q, q_full, c * 64, rg * BM, hkv, seq);
+        mbar_expect_tx(q_full, NT * C::Q_BYTES);
+        for (int x = 0; x < NT; ++x)
+          for (int c = 0; c < C::KCH; ++c)
+            tma_load_4d(sb + x * C::Q_BYTES + c * BM * 128, &tm_q, q_full, c * 64, (rg * NT + x) * BM, hkv, seq);
       }
       const int ub = a.unit;  // tokens per box: a page, or the power of two that divides it
       for (int i = 0; i < n; ++i) {
@@ -606,45 +615,65 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         }
         if (!ok) break;
       }
-    } else if (warp == 5 && lane == 0 && n > 0) {
+    } else if (warp == kMma && lane == 0 && n > 0) {
       constexpr int FMT = BF16 ? 1 : 0;
       constexpr uint32_t ID_S = idesc_f16(128, BN, FMT, 0, 0);
       constexpr uint32_t ID_O = idesc_f16(128, D, FMT, 0, 1);
       const uint64_t dQ = sdesc_sw128(sb, 16, 1024);
       const uint64_t dK = sdesc_sw128(sb + C::OFF_K, 16, 1024);
       const uint64_t dV = sdesc_sw128(sb + C::OFF_V, BN * 128, 1024);  // MN-major
-      bool ok = mbar_wait(q_full, 0, kStatusTimeoutMma);
-      for (int i = 0; ok && i < n; ++i) {
-        const int s = i % S;
-        ok = mbar_wait(k_full(s), (i / S) & 1, kStatusTimeoutMma);
-        if (!ok) break;
-        tc_fence_after();
-        // (in issue order behind P V of the previous tile, which reads P from these columns)
+      auto issue_s = [&](int x, int s) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_f16(tmem, sdesc_add(dQ, (k >> 2) * BM * 128 + (k & 3) * 32),
+          umma_f16(tmem + x * 128, sdesc_add(dQ, x * C::Q_BYTES + (k >> 2) * BM * 128 + (k & 3) * 32),
                    sdesc_add(dK, s * C::KV_BYTES + (k >> 2) * BN * 128 + (k & 3) * 32), ID_S, k > 0 ? 1u : 0u);
-        umma_commit(s_full);
-        umma_commit(k_empty(s));
-        ok = mbar_wait(v_full(s), (i / S) & 1, kStatusTimeoutMma) && mbar_wait(p_full, i & 1, kStatusTimeoutMma);
-        if (!ok) break;
+        umma_commit(s_full(x));
+      };
+      auto issue_pv = [&](int x, int i) -> bool {
+        if (!mbar_wait(p_full(x), i & 1, kStatusTimeoutMma)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < BN / 16; ++k)
-          umma_f16_ts(tmem + C::O_COL, tmem + k * 8, sdesc_add(dV, s * C::KV_BYTES + k * 16 * 128), ID_O,
-                      (i > 0 || k > 0) ? 1u : 0u);
-        umma_commit(v_empty(s));
-        umma_commit(o_done);
+          umma_f16_ts(tmem + C::o_col(x), tmem + x * 128 + k * 8, sdesc_add(dV, (i % S) * C::KV_BYTES + k * 16 * 128),
+                      ID_O, (i > 0 || k > 0) ? 1u : 0u);
+        return true;
+      };
+      // S of a row tile is issued behind its P V of the previous tile, which reads P from the same columns.
+      bool ok = mbar_wait(q_full, 0, kStatusTimeoutMma);
+      for (int i = 0; ok && i <= n; ++i) {
+        if (i > 0) {
+          ok = mbar_wait(v_full((i - 1) % S), ((i - 1) / S) & 1, kStatusTimeoutMma) && issue_pv(0, i - 1);
+          if (!ok) break;
+          if (NT == 1) umma_commit(v_empty((i - 1) % S));
+        }
+        if (i < n) {
+          ok = mbar_wait(k_full(i % S), (i / S) & 1, kStatusTimeoutMma);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(0, i % S);
+        }
+        if (NT == 2 && i > 0) {
+          ok = issue_pv(1, i - 1);
+          if (!ok) break;
+          umma_commit(v_empty((i - 1) % S));
+        }
+        if (i < n) {
+          if (NT == 2) issue_s(1, i % S);
+          umma_commit(k_empty(i % S));
+        }
       }
+      if (ok) umma_commit(o_done);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcSoftmaxRegs));
-    const int r = rg * BM + threadIdx.x;  // row of the kv head
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+    const int x_tile = warp >> 2, rl = threadIdx.x & 127;  // row tile, row in it == TMEM lane
+    const int r = (rg * NT + x_tile) * BM + rl;            // row of the kv head
     const int t = r % a.T;
     const bool row_ok = r < a.rows && (!TREE || t < sp.drafts);
     const int pos = sp.len - a.T + t;     // window: position of the row
     int walk = TREE && row_ok ? t : -1;   // tree: next token on the row's path
-    const uint32_t s_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lanes + x_tile * 128, o_addr = lanes + 128 * NT + x_tile * D;
     float m = -FLT_MAX, l = 0.f;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
@@ -673,7 +702,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           }
         }
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(s_full, i & 1, kStatusTimeoutSoftmax));
+      ok = __all_sync(0xffffffffu, mbar_wait(s_full(x_tile), i & 1, kStatusTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
       float x[BN];
@@ -685,16 +714,16 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         for (int c = 0; c < BN; ++c)
           if (!((keep[c >> 5] >> (c & 31)) & 1u)) x[c] = -INFINITY;
         // V rows that nothing sees -> 0: P is 0 there, but a slot never written (or a box never
-        // loaded) may hold NaN.  Thread = token.
+        // loaded) may hold NaN.  Thread = token; with two row tiles both write the same zeros.
         ok = __all_sync(0xffffffffu, mbar_wait(v_full(st), (i / S) & 1, kStatusTimeoutSoftmax));
         if (!ok) break;
-        const int tk = tok0 + threadIdx.x;
+        const int tk = tok0 + rl;
         if (draft ? tk >= sp.drafts : !ctx_visible<TREE>(a, sp, tk)) {
 #pragma unroll
           for (int c = 0; c < C::KCH; ++c)
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::KV_BYTES + c * BN * 128 + threadIdx.x * 128 + u * 16) =
+              *reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::KV_BYTES + c * BN * 128 + rl * 128 + u * 16) =
                   make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
@@ -733,18 +762,18 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          tmem_ld32(s_addr + C::O_COL + c * 32, o);
+          tmem_ld32(o_addr + c * 32, o);
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(s_addr + C::O_COL + c * 32, o);
+          tmem_st32(o_addr + c * 32, o);
         }
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive_warp(p_full);
+      mbar_arrive_warp(p_full(x_tile));
     }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (n - 1) & 1, kStatusTimeoutSoftmax));
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done, 0, kStatusTimeoutSoftmax));
     if (ok) {
       tc_fence_after();
       if (!row_ok) l = 0.f;
@@ -755,7 +784,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         if (n > 0) {
-          tmem_ld32(s_addr + C::O_COL + c * 32, o);
+          tmem_ld32(o_addr + c * 32, o);
           tmem_wait_ld();
         }
         // (a row without keys may hold o of nothing: select, do not multiply)
@@ -785,7 +814,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == kMma) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
@@ -880,7 +909,7 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
     w.unit = 128;
     while (p->block_size % w.unit != 0) w.unit /= 2;
     w.span_unit = BN;
-    w.row_tiles = BM / 16;
+    w.row_tiles = (rows > BM ? 2 : 1) * (BM / 16);
   } else {
     w.unit = w.span_unit = p->block_size % 32 == 0 ? 32 : 16;
     w.row_tiles = rows <= 16 ? 1 : 2;
@@ -890,7 +919,7 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
   // (window: the first and last unit of both pieces may be cut)
   const long long units = (tokens + u - 1) / u + (tree ? (p->seq_q + u - 1) / u : 3);
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * w.row_groups;
-  const long long slots = (w.tc ? 2 : 3) * 148;
+  const long long slots = (w.tc ? (rows > BM ? 1 : 2) : 3) * 148;
   const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u;
   const long long s_min = (units + most - 1) / most, s_max = ll_max(ll_min(units / least, s_min + 64), s_min);
   w.split_units = (int)most;
@@ -955,20 +984,20 @@ static int launch_mma(const Maps& t, const Args& a, cudaStream_t st) {
   return launch_status();
 }
 
-template <bool BF16, int D, bool TREE>
+template <bool BF16, int D, int NT, bool TREE>
 static int launch_tc(const Maps& t, const Args& a, cudaStream_t st) {
-  using C = TcCfg<D>;
+  using C = TcCfg<D, NT>;
   static std::atomic<unsigned long long> done{0};
-  auto kern = rows_tc_kernel<BF16, D, TREE>;
-  // The in-kernel register split draws on exactly kTcRegs per thread: with any
+  auto kern = rows_tc_kernel<BF16, D, NT, TREE>;
+  // The in-kernel register split draws on exactly C::REGS per thread: with any
   // other launch count the growing warps could wait forever.
   static const bool regs_ok = [&] {
     cudaFuncAttributes fa;
-    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess && fa.numRegs == kTcRegs;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess && fa.numRegs == C::REGS;
   }();
   if (!regs_ok) return ATTN_ERR_UNSUPPORTED;
   if (!smem_once(kern, C::SMEM, done)) return ATTN_ERR_CUDA;
-  kern<<<dim3(a.Hkv * a.row_groups, a.max_splits, a.N), kTcThreads, C::SMEM, st>>>(t.q, t.k, t.v, t.dk, t.dv, a);
+  kern<<<dim3(a.Hkv * a.row_groups, a.max_splits, a.N), C::THREADS, C::SMEM, st>>>(t.q, t.k, t.v, t.dk, t.dv, a);
   return launch_status();
 }
 
@@ -976,7 +1005,7 @@ template <bool BF16, int D, bool TREE>
 static int launch_rows(const Plan& w, const Maps& t, const Args& a, cudaStream_t st) {
   int rc;
   if (w.tc)
-    rc = launch_tc<BF16, D, TREE>(t, a, st);
+    rc = a.rows > BM ? launch_tc<BF16, D, 2, TREE>(t, a, st) : launch_tc<BF16, D, 1, TREE>(t, a, st);
   else if (w.unit == 32)
     rc = w.row_tiles == 1 ? launch_mma<BF16, D, 32, 1, TREE>(t, a, st) : launch_mma<BF16, D, 32, 2, TREE>(t, a, st);
   else
