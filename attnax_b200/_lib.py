@@ -45,7 +45,7 @@ class FwdParams(C.Structure):
         ("q_strides", i64 * 3), ("k_strides", i64 * 3), ("v_strides", i64 * 3),
         ("o_strides", i64 * 3), ("lse", vp), ("softmax_scale", f32),
         ("fix_masked_rows", i32), ("mask", AttnMask), ("workspace", vp),
-        ("workspace_bytes", szt),
+        ("workspace_bytes", szt), ("out_rest", vp),
     ]
 
 
@@ -59,7 +59,7 @@ class BwdParams(C.Structure):
         ("o_strides", i64 * 3), ("do_strides", i64 * 3), ("dq_strides", i64 * 3),
         ("dk_strides", i64 * 3), ("dv_strides", i64 * 3), ("softmax_scale", f32),
         ("fix_masked_rows", i32), ("mask", AttnMask), ("workspace", vp),
-        ("workspace_bytes", szt),
+        ("workspace_bytes", szt), ("out_rest", vp),
     ]
 
 

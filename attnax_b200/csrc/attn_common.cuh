@@ -179,6 +179,20 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
+// What rounding a and b to the 16-bit pair `packed` left of them, rounded to the same type.
+template <bool BF16>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t packed) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&packed);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a - __low2float(h), b - __high2float(h));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 h = *reinterpret_cast<const __half2*>(&packed);
+    const __half2 r = __floats2half2_rn(a - __low2float(h), b - __high2float(h));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
 // Per-thread constants for transforming one row of a score tile held in
 // registers.  Columns are kv positions (forward, dQ) or q positions
 // (dK/dV, "transposed").  d(c) = q - kv at column c = d0 + dstep * c.

@@ -251,7 +251,7 @@ static int launch_sm100_fwd2(const attn_fwd_params_t* p, float* lse, const int2*
   a.group = p->num_heads_q / p->num_heads_kv;
   a.n_ctas = fwd2_ctas(p->seq_q);
   a.sl2 = p->softmax_scale * kLog2e;
-  a.out = p->out;
+  a.out = p->out; a.out_rest = p->out_rest;
   a.o_s0 = p->o_strides[0]; a.o_s1 = p->o_strides[1]; a.o_s2 = p->o_strides[2];
   a.lse = lse; a.mask = p->mask;
   a.doc_q_tiles = dq_t; a.doc_kv_tiles = dkv_t; a.doc_jrange = djr;
@@ -304,7 +304,7 @@ static int launch_sm100_fwd(const attn_fwd_params_t* p, float* lse, const int2* 
   a.group = p->num_heads_q / p->num_heads_kv;
   a.nq_tiles = (p->seq_q + fwd::BM - 1) / fwd::BM;
   a.sl2 = p->softmax_scale * kLog2e;
-  a.out = p->out;
+  a.out = p->out; a.out_rest = p->out_rest;
   a.o_s0 = p->o_strides[0]; a.o_s1 = p->o_strides[1]; a.o_s2 = p->o_strides[2];
   a.lse = lse; a.mask = p->mask;
   a.doc_q_tiles = dq_t; a.doc_kv_tiles = dkv_t; a.doc_jrange = djr;
@@ -404,6 +404,8 @@ int attn_fwd(const attn_fwd_params_t* p, void* stream) {
 
   const bool tc = tc_layout_ok(p);
   if (!tc && !simt_dim_ok(p->head_dim)) return ATTN_ERR_UNSUPPORTED;
+  if (p->out_rest && (!tc || p->mask.num_sinks <= 0 || reinterpret_cast<uintptr_t>(p->out_rest) % 16))
+    return ATTN_ERR_INVALID;
   int2 *dq_t = nullptr, *dkv_t = nullptr, *djr = nullptr;
   int* order = nullptr;
   if (p->mask.doc_q && tc) {
@@ -563,9 +565,10 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   {
     constexpr int rows_per_block = kPrepRowsPerBlock / (D / 8);
-    prep_rows_kernel<T, D><<<dim3((Sq_pad + rows_per_block - 1) / rows_per_block, p->num_heads_q, p->batch), 256, 0,
-                             st>>>(
-        reinterpret_cast<const T*>(p->out), reinterpret_cast<const T*>(p->d_out), p->o_strides[0], p->o_strides[1],
+    auto prep = p->out_rest ? prep_rows_kernel<T, D, true> : prep_rows_kernel<T, D, false>;
+    prep<<<dim3((Sq_pad + rows_per_block - 1) / rows_per_block, p->num_heads_q, p->batch), 256, 0, st>>>(
+        reinterpret_cast<const T*>(p->out), reinterpret_cast<const T*>(p->out_rest),
+        reinterpret_cast<const T*>(p->d_out), p->o_strides[0], p->o_strides[1],
         p->o_strides[2], p->do_strides[0], p->do_strides[1], p->do_strides[2], p->lse, delta, lse2,
         p->num_heads_q, p->seq_q, Sq_pad, (D == 128 && bwd_fused_dq(p) && !CfgKV<128, true>::RED) ? dq_acc : nullptr);
   }
@@ -665,6 +668,7 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
   if (!check_mask(p->mask, p->batch)) return ATTN_ERR_INVALID;
   const bool tc = bwd_tc_ok(p);
   if (!tc && !simt_dim_ok(p->head_dim)) return ATTN_ERR_UNSUPPORTED;
+  if (p->out_rest && (!tc || reinterpret_cast<uintptr_t>(p->out_rest) % 16)) return ATTN_ERR_INVALID;
   const size_t need = attn_bwd_workspace_size(p);
   if (!p->workspace || p->workspace_bytes < need) return ATTN_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

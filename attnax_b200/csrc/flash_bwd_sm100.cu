@@ -1178,8 +1178,9 @@ __global__ void dq_convert_kernel(const float* acc, T* dq, long long s0, long lo
 // padded rows (+inf, 0), and zeroes the row of the fused-dQ accumulator when
 // there is one.  D/8 lanes share a row (16 bytes each) and every warp keeps
 // kPasses rows-per-pass of loads in flight before reducing.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) prep_rows_kernel(const T* out, const T* dout, long long os0, long long os1,
+// REST: O is `out` plus the rounding rest `rest` (same strides).
+template <typename T, int D, bool REST = false>
+__global__ void __launch_bounds__(256) prep_rows_kernel(const T* out, const T* rest, const T* dout, long long os0, long long os1,
                                                         long long os2, long long ds0, long long ds1, long long ds2,
                                                         const float* lse, float* delta, float* lse2, int H, int S,
                                                         int S_pad, float* dq_acc) {
@@ -1191,15 +1192,17 @@ __global__ void __launch_bounds__(256) prep_rows_kernel(const T* out, const T* d
   const int h = blockIdx.y, b = blockIdx.z;
   const int row0 = (blockIdx.x * (blockDim.x >> 5) + warp) * RPW + lane / L;
   const int cl = (lane % L) * 8;
-  uint4 ov[kPasses], dv[kPasses];
+  uint4 ov[kPasses], dv[kPasses], rv[REST ? kPasses : 1];
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     const int row = row0 + p * RPP;
     if (row < S) {
       ov[p] = *reinterpret_cast<const uint4*>(out + b * os0 + h * os1 + (long long)row * os2 + cl);
       dv[p] = *reinterpret_cast<const uint4*>(dout + b * ds0 + h * ds1 + (long long)row * ds2 + cl);
+      if constexpr (REST) rv[p] = *reinterpret_cast<const uint4*>(rest + b * os0 + h * os1 + (long long)row * os2 + cl);
     } else {
       ov[p] = dv[p] = make_uint4(0, 0, 0, 0);
+      if constexpr (REST) rv[p] = make_uint4(0, 0, 0, 0);
     }
   }
 #pragma unroll
@@ -1209,6 +1212,11 @@ __global__ void __launch_bounds__(256) prep_rows_kernel(const T* out, const T* d
     float acc = 0.f;
 #pragma unroll
     for (int x = 0; x < 8; ++x) acc = fmaf(to_f32(oh[x]), to_f32(dh[x]), acc);
+    if constexpr (REST) {
+      const T* rh = reinterpret_cast<const T*>(&rv[p]);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc = fmaf(to_f32(rh[x]), to_f32(dh[x]), acc);
+    }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     const int row = row0 + p * RPP;

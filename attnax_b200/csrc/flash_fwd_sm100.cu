@@ -49,6 +49,7 @@ struct Args {
   int B, Hq, Hkv, Sq, Skv, group, nq_tiles;
   float sl2;  // softmax scale * log2(e)
   void* out;
+  void* out_rest;  // SINK: the rounding rest of out, or null
   long long o_s0, o_s1, o_s2;
   float* lse;
   attn_mask_t mask;
@@ -302,6 +303,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             w.z = pack2(__uint_as_float(o[v * 8 + 4]) * inv, __uint_as_float(o[v * 8 + 5]) * inv, BF16);
             w.w = pack2(__uint_as_float(o[v * 8 + 6]) * inv, __uint_as_float(o[v * 8 + 7]) * inv, BF16);
             *reinterpret_cast<uint4*>(orow + c * 32 + v * 8) = w;
+            if constexpr (SINK) {
+              if (a.out_rest) {
+                auto val = [&](int e) { return __uint_as_float(o[v * 8 + e]) * inv; };
+                const uint4 d = make_uint4(rest2<BF16>(val(0), val(1), w.x), rest2<BF16>(val(2), val(3), w.y),
+                                           rest2<BF16>(val(4), val(5), w.z), rest2<BF16>(val(6), val(7), w.w));
+                *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out_rest) + (orow - reinterpret_cast<T*>(a.out)) +
+                                          c * 32 + v * 8) = d;
+              }
+            }
           }
         }
       }

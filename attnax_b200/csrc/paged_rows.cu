@@ -69,6 +69,10 @@ template <bool TREE>
 __device__ __forceinline__ Span make_span(const Args& a, int seq, int U) {
   Span s;
   s.len = max(a.seq_lens[seq], 0);
+  if (s.len > a.max_blocks * a.BS) {  // (no more tokens than the table row has pages for)
+    atomicCAS(&g_notice, 0, kNoticeTableOverrun);
+    s.len = a.max_blocks * a.BS;
+  }
   s.drafts = 0;
   s.lo = 0;
   s.n_sink = 0;
@@ -99,12 +103,7 @@ __device__ __forceinline__ bool ctx_visible(const Args& a, const Span& s, int c)
 }
 
 __device__ __forceinline__ int page_of(const Args& a, int seq, int tok) {
-  int col = tok / a.BS;
-  if (col >= a.max_blocks) {
-    atomicCAS(&g_notice, 0, kNoticeTableOverrun);
-    col = a.max_blocks - 1;
-  }
-  return (int)paged_phys_page(a.block_table[(long long)seq * a.max_blocks + col], a.num_blocks);
+  return (int)paged_phys_page(a.block_table[(long long)seq * a.max_blocks + tok / a.BS], a.num_blocks);
 }
 
 // Parent of drafted token t: negative, or in front of t.
@@ -951,6 +950,7 @@ static int check(const attn_paged_params_t* p) {
   if (p->dtype != ATTN_BF16 && p->dtype != ATTN_F16) return ATTN_ERR_UNSUPPORTED;
   if ((p->head_dim != 64 && p->head_dim != 128) || p->block_size % 16 != 0) return ATTN_ERR_UNSUPPORTED;
   if ((long long)p->num_blocks * p->block_size > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;  // (TMA coordinates)
+  if ((long long)p->max_blocks_per_seq * p->block_size > 0x7fffffffll - 4096) return ATTN_ERR_UNSUPPORTED;
   for (const void* x : {p->q, p->key_pool, p->value_pool, (const void*)p->out})
     if (reinterpret_cast<uintptr_t>(x) % 16) return ATTN_ERR_INVALID;
   return ATTN_OK;

@@ -63,8 +63,8 @@ def softmax_scale(head_dim: int) -> float:
     return float(torch.tensor(1.0 / math.sqrt(head_dim), dtype=torch.float32))
 
 
-def fwd_raw(q, k, v, spec, *, want_lse=True, out=None, lse=None):
-    """One ``attn_fwd`` call; returns ``(out, lse)``."""
+def fwd_raw(q, k, v, spec, *, want_lse=True, out=None, lse=None, rest=None):
+    """One ``attn_fwd`` call; returns ``(out, lse)``.  ``rest`` (like out, contiguous) gets out's rounding rest."""
     lib = _lib.load()
     B, Hq, Hkv, Sq, Skv, D = check_qkv(q, k, v)
     out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
@@ -80,6 +80,7 @@ def fwd_raw(q, k, v, spec, *, want_lse=True, out=None, lse=None):
     p.softmax_scale = softmax_scale(D)
     p.fix_masked_rows = int(spec.fix_masked_rows)
     p.mask = spec.struct
+    p.out_rest = None if rest is None else rest.data_ptr()
     nbytes = lib.attn_fwd_workspace_size(C.byref(p))
     ws = None
     if nbytes:
@@ -90,7 +91,7 @@ def fwd_raw(q, k, v, spec, *, want_lse=True, out=None, lse=None):
     return out, lse
 
 
-def bwd_raw(q, k, v, out, lse, dout, spec):
+def bwd_raw(q, k, v, out, lse, dout, spec, *, rest=None):
     lib = _lib.load()
     B, Hq, Hkv, Sq, Skv, D = check_qkv(q, k, v)
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -108,6 +109,7 @@ def bwd_raw(q, k, v, out, lse, dout, spec):
     p.softmax_scale = softmax_scale(D)
     p.fix_masked_rows = int(spec.fix_masked_rows)
     p.mask = spec.struct
+    p.out_rest = None if rest is None else rest.data_ptr()
     nbytes = lib.attn_bwd_workspace_size(C.byref(p))
     ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
@@ -119,15 +121,20 @@ def bwd_raw(q, k, v, out, lse, dout, spec):
 class _FlashAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, spec):
-        out, lse = fwd_raw(q, k, v, spec)
-        ctx.save_for_backward(q, k, v, out, lse)
+        # A window of few keys shows the rounding of out in rowsum(dO * O): with sinks
+        # (16-bit types on the tensor cores) the rounding rest is kept for the backward.
+        rest = None
+        if spec.struct.num_sinks > 0 and q.dtype != torch.float32 and q.shape[-1] in (64, 128):
+            rest = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out, lse = fwd_raw(q, k, v, spec, rest=rest)
+        ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.spec = spec
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = bwd_raw(q, k, v, out, lse, _prep(dout), ctx.spec)
+        q, k, v, out, lse, rest = ctx.saved_tensors
+        dq, dk, dv = bwd_raw(q, k, v, out, lse, _prep(dout), ctx.spec, rest=rest)
         return dq, dk, dv, None
 
 

@@ -92,6 +92,10 @@ typedef struct {
   int32_t fix_masked_rows;       /* 1: rows with no kept key average all of V */
   attn_mask_t mask;
   void* workspace; size_t workspace_bytes;
+  /* NULL, or like out: what rounding left of it, out_rest = round(O - round(O)).  Handed to attn_bwd it
+   * takes the rounding of O out of rowsum(dO * O), which windows of few keys show in dQ and dK.
+   * Only with num_sinks > 0, a 16-bit dtype and head_dim 64 or 128. */
+  void* out_rest;
 } attn_fwd_params_t;
 
 typedef struct {
@@ -106,6 +110,7 @@ typedef struct {
   int32_t fix_masked_rows;       /* 1: rows with no kept key add dO/seq_kv to all of dV */
   attn_mask_t mask;
   void* workspace; size_t workspace_bytes;
+  const void* out_rest;          /* from attn_fwd (strides of out), or NULL */
 } attn_bwd_params_t;
 
 typedef struct {
@@ -383,7 +388,8 @@ int attn_rope(const attn_rope_params_t* p, void* stream);
  * unwound; results are invalid).  0x201: a paged decode met a seq_lengths
  * entry above max_context and attended only its first splits.  0x202: a
  * paged decode met a sequence longer than max_blocks_per_seq * block_size
- * and reused the row's last entry for the pages past it.  0x203: a drafted
+ * and reused the row's last entry for the pages past it (attn_paged_window and
+ * attn_paged_tree read such a sequence as if it ended with its row).  0x203: a drafted
  * token's parent was not in front of it.  0x204: a page operator skipped an
  * entry that it could not use.  A timeout code takes precedence over a notice. */
 int attn_device_status(int32_t* status);

@@ -217,6 +217,21 @@ def test_lengths_above_the_bound_are_cut_and_noted():
     assert_within(got[1:2], want, bound, "sequence within the bound")
 
 
+@pytest.mark.parametrize("t", [1, 20])
+def test_lengths_past_the_table_row_are_cut_and_noted(t):
+    """No more tokens than the row's pages hold: the sequence is read as if it ended there."""
+    cache = make_cache(2, [64, 40], 1, 128, 16, BF)
+    q = randn(1, 2, 4, t, 128)
+    wrong = ax.PagedKVCache(cache.key_pool, cache.value_pool, cache.block_table,
+                            torch.tensor([100, 40], dtype=torch.int32, device=DEV))
+    assert _lib.device_status() == 0
+    got = ax.paged_window_attention(q, wrong, window_size=30, num_sinks=2, max_context=100)
+    assert _lib.device_status() == _lib.NOTICE_TABLE_OVERRUN
+    check_window(cache, [64, 40], q, got, 30, 2)
+    with pytest.raises(ValueError):
+        ax.paged_window_attention(q, wrong, window_size=30)
+
+
 def test_another_stream_and_a_captured_graph():
     """On a side stream, and captured twice into graphs whose replays follow new lengths and queries."""
     lens, window, sinks, t = [300, 129], 64, 4, 3
