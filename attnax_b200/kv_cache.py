@@ -92,9 +92,39 @@ def _decode_block_size(cache: KVLayerCache, query: torch.Tensor):
     return next((bs for bs in _BLOCK_SIZES if cache.max_len % bs == 0), None)
 
 
-def kv_cache_attention(query: torch.Tensor, cache: KVLayerCache, *, mask=None, score_mod=None) -> torch.Tensor:
+def _window_attention(query, cache: KVLayerCache, n: int, mask, score_mod, window: int, sinks: int):
+    from .flash import attention
+    from .paged_rows import paged_window_attention
+
+    b, hq, sq, d = query.shape
+    k, v = cache.keys, cache.values
+    hkv = k.shape[1]
+    bs = next((x for x in _BLOCK_SIZES if cache.max_len % x == 0), None)
+    if (mask is None and score_mod is None and bs is not None and d in (64, 128) and k.is_contiguous()
+            and v.is_contiguous() and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float16)):
+        nseq, nblk = b * hkv, cache.max_len // bs
+        pool = PagedKVCache(k.view(nseq * nblk, bs, 1, d), v.view(nseq * nblk, bs, 1, d),
+                            _identity_table(nseq, nblk, query.device),
+                            torch.full((nseq,), n, dtype=torch.int32, device=query.device))
+        q = query.contiguous().view(nseq, hq // hkv, sq, d)
+        return paged_window_attention(q, pool, window_size=window, num_sinks=sinks, max_context=n).view(b, hq, sq, d)
+    qi = torch.arange(n - sq, n, device=query.device)[:, None]
+    ki = torch.arange(n, device=query.device)[None, :]
+    win = ((ki <= qi) & ((qi - ki < window) | (ki < sinks)))[None, None]
+    m = win if mask is None else torch.as_tensor(mask, device=query.device) & win
+    return attention(query.to(k.dtype), k[:, :, :n], v[:, :, :n], mask=m, score_mod=score_mod).to(query.dtype)
+
+
+def kv_cache_attention(query: torch.Tensor, cache: KVLayerCache, *, mask=None, score_mod=None,
+                       window_size=None, num_sinks: int = 0) -> torch.Tensor:
     """``query (batch, num_heads, seq_q, head_dim)`` against the first
     ``cache.length`` cached positions; returns the query's shape and dtype.
+
+    With ``window_size`` the query rows are the last ``seq_q`` cached positions
+    and see a causal window of that many keys plus the first ``num_sinks``
+    ones (no counterpart in the reference): the kernels of
+    ``paged_window_attention`` read only those, on the cache itself (bf16/f16,
+    head_dim 64 or 128, ``max_len`` a multiple of 16, no mask/score_mod).
 
     bf16/f16 buffers with head_dim 128, ``max_len`` a multiple of 16 and no
     mask/score_mod take the split-K decode kernel; otherwise the flash kernel
@@ -112,9 +142,15 @@ def kv_cache_attention(query: torch.Tensor, cache: KVLayerCache, *, mask=None, s
         raise ValueError(f"num_heads ({hq}) must be divisible by num_kv_heads ({hkv})")
     if not query.is_cuda:
         raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
+    if window_size is None and num_sinks:
+        raise ValueError("num_sinks needs a window_size")
+    if window_size is not None and (window_size <= 0 or num_sinks < 0):
+        raise ValueError(f"window_size must be positive and num_sinks not negative, got {window_size}, {num_sinks}")
     n = int(cache.length)
     if n == 0:
         return torch.zeros_like(query)
+    if window_size is not None:
+        return _window_attention(query, cache, n, mask, score_mod, int(window_size), int(num_sinks))
     bs = _decode_block_size(cache, query) if mask is None and score_mod is None else None
     if bs is not None:
         nseq, nblk = b * hkv, cache.max_len // bs

@@ -18,7 +18,7 @@ import torch
 
 from ._api import compose_score_mods
 from .flash import flash_attention
-from .kv_cache import KVLayerCache, update_kv_layer_cache
+from .kv_cache import KVLayerCache, kv_cache_attention, update_kv_layer_cache
 from .rope import apply_rope_table, rope_cos_sin_table
 from .score_mods import sink_window_mod, sliding_window_mod
 
@@ -73,6 +73,10 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
         v = new_cache.values[:, :, :new_cache.length]
 
     mods = compose_score_mods(base_score_mod, score_mod)
+    if past and attention_sinks and mask is None and mods is None and attention_fn is flash_attention:
+        # a cached step of a window with sinks: the decode reads only the keys that it sees
+        out = kv_cache_attention(q, new_cache, window_size=attention_window, num_sinks=attention_sinks)
+        return out.transpose(1, 2).reshape(b, seq_q, num_heads * head_dim), new_cache
     if attention_window is not None and self_attention:
         if past == 0:
             # the reference's boolean window mask (attention.py:417-431) is this band

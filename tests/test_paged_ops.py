@@ -37,6 +37,14 @@ def test_window_arguments():
             ax.free_window(cpu_cache(), **kw)
 
 
+def test_contiguous_cache_arguments():
+    cache = ax.init_kv_layer_cache(1, 2, 64, 32, torch.bfloat16, device="cpu")
+    q = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    for kw in ({"num_sinks": 2}, {"window_size": 0}, {"window_size": 4, "num_sinks": -1}):
+        with pytest.raises((ValueError, RuntimeError)):
+            ax.kv_cache_attention(q, cache, **kw)
+
+
 def test_tree_arguments():
     c = cpu_cache()
     for dk, dv in ((DRAFT[:, :1], DRAFT), (DRAFT, DRAFT[:, :, :1]), (DRAFT, None)):

@@ -286,3 +286,22 @@ def test_kv_offsets_past_32_bits():
     dk, dv = randn(4, 1, hkv, 1, d), randn(5, 1, hkv, 1, d)
     par = torch.full((1, 1), -1, dtype=torch.int32)
     check_tree(cache, [300], q, dk, dv, par, [1], ax.paged_tree_attention(q, dk, dv, cache, par))
+
+
+@pytest.mark.parametrize("d,max_len,dt", [(128, 512, BF), (64, 400, HF), (128, 333, BF), (32, 64, F32)])
+@pytest.mark.parametrize("t", [1, 5])
+def test_contiguous_cache(d, max_len, dt, t):
+    """kv_cache_attention with a window: fused on the buffer, or the flash kernel where that cannot be."""
+    b, hq, hkv, n = 2, 4, 2, max_len - 7
+    cache = ax.init_kv_layer_cache(b, hkv, d, max_len, dt)
+    cache = ax.update_kv_layer_cache(cache, randn(1, b, hkv, n, d, dt=dt), randn(2, b, hkv, n, d, dt=dt), 0)
+    q = randn(3, b, hq, t, d, dt=dt)
+    got = ax.kv_cache_attention(q, cache, window_size=21, num_sinks=3)
+    row, col = torch.arange(n - t, n, device=DEV)[:, None], torch.arange(n, device=DEV)[None]
+    keep = (col <= row) & ((row - col < 21) | (col < 3))
+    want, bound = attention64(q, cache.keys[:, :, :n], cache.values[:, :, :n], keep)
+    assert_within(got, want, bound, "window over a contiguous cache")
+    mask = (torch.arange(n, device=DEV) % 3 != 0)[None, None, None]
+    got = ax.kv_cache_attention(q, cache, window_size=21, num_sinks=3, mask=mask)
+    want, bound = attention64(q, cache.keys[:, :, :n], cache.values[:, :, :n], keep & mask[0, 0])
+    assert_within(got, want, bound, "and a mask")
