@@ -828,8 +828,8 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ 
   if (row >= a.Hkv * a.rows) return;
   const Span sp = make_span<TREE>(a, seq, a.span_unit);  // (lengths: not written by the kernel in front)
   const int n = split_count(a, sp);
+  pdl_wait_previous();  // (also where there is nothing to join: this kernel must not end before that one)
   if (n <= 1) return;
-  pdl_wait_previous();
   const long long prow = (long long)seq * a.Hkv * a.rows + row;
   const float* lse = a.part_lse + prow * a.max_splits;
   const float* po = a.part_o + prow * a.max_splits * D + lane * (D / 32);
@@ -946,7 +946,7 @@ static int check(const attn_paged_params_t* p) {
       p->block_size <= 0 || p->max_blocks_per_seq <= 0 || p->max_context < 0 ||
       p->num_heads_q % p->num_heads_kv != 0)
     return ATTN_ERR_INVALID;
-  if (p->num_seqs > 65535) return ATTN_ERR_INVALID;
+  if (p->num_seqs > 65535) return ATTN_ERR_UNSUPPORTED;  // (a grid dimension)
   if (p->dtype != ATTN_BF16 && p->dtype != ATTN_F16) return ATTN_ERR_UNSUPPORTED;
   if ((p->head_dim != 64 && p->head_dim != 128) || p->block_size % 16 != 0) return ATTN_ERR_UNSUPPORTED;
   if ((long long)p->num_blocks * p->block_size > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;  // (TMA coordinates)

@@ -683,9 +683,9 @@ int attn_paged_accept(const attn_paged_cache_t* c, const void* draft_keys, const
                       const int32_t* accepted, int32_t max_accepted, const int32_t* accepted_lengths,
                       int32_t* lengths_out, int32_t* bad, void* stream) {
   if (!pages::cache_ok(c, true, true) || !draft_keys || !draft_values || !k_strides || !v_strides || num_drafts <= 0 ||
-      max_accepted < 0 || (max_accepted > 0 && !accepted) || !accepted_lengths || (!lengths_out && !bad) ||
-      c->num_seqs > 65535)
+      max_accepted < 0 || (max_accepted > 0 && !accepted) || !accepted_lengths || (!lengths_out && !bad))
     return ATTN_ERR_INVALID;
+  if (c->num_seqs > 65535) return ATTN_ERR_UNSUPPORTED;  // (a grid dimension)
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const long long es = dtype_size(c->dtype), row = c->head_dim * es;
   int vec = pages::vec_bytes(row, pages::addr(c->key_pool) | pages::addr(c->value_pool) | pages::addr(draft_keys) |

@@ -108,11 +108,17 @@ def _window_attention(query, cache: KVLayerCache, n: int, mask, score_mod, windo
                             torch.full((nseq,), n, dtype=torch.int32, device=query.device))
         q = query.contiguous().view(nseq, hq // hkv, sq, d)
         return paged_window_attention(q, pool, window_size=window, num_sinks=sinks, max_context=n).view(b, hq, sq, d)
-    qi = torch.arange(n - sq, n, device=query.device)[:, None]
+    first = max(0, sq - n)  # rows in front of the cache see nothing
+    qi = torch.arange(n - sq + first, n, device=query.device)[:, None]
     ki = torch.arange(n, device=query.device)[None, :]
     win = ((ki <= qi) & ((qi - ki < window) | (ki < sinks)))[None, None]
-    m = win if mask is None else torch.as_tensor(mask, device=query.device) & win
-    return attention(query.to(k.dtype), k[:, :, :n], v[:, :, :n], mask=m, score_mod=score_mod).to(query.dtype)
+    if mask is not None:
+        mask = torch.as_tensor(mask, device=query.device)
+        win = win & (mask[..., first:, :] if mask.dim() > 1 and mask.shape[-2] == sq else mask)
+    out = torch.zeros_like(query)
+    out[:, :, first:] = attention(query[:, :, first:].to(k.dtype), k[:, :, :n], v[:, :, :n], mask=win,
+                                  score_mod=score_mod).to(query.dtype)
+    return out
 
 
 def kv_cache_attention(query: torch.Tensor, cache: KVLayerCache, *, mask=None, score_mod=None,

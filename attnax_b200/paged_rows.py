@@ -175,7 +175,7 @@ def gather_window(cache: PagedKVCache, sequence_idx: int, rows: int, window: int
 def _tma_ready(x: torch.Tensor) -> torch.Tensor:
     """Unit stride on head_dim, other strides and the base in 16-byte steps (dimensions of one are not stepped)."""
     ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
-        s % 8 == 0 for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1)
+        s > 0 and s % 8 == 0 for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1)
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 

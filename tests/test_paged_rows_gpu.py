@@ -191,6 +191,22 @@ def test_tree_other_caches(d, bs, dt):
     check_tree(cache, lens, q, dk, dv, par, [9, 4, 0], got)
 
 
+@pytest.mark.parametrize("layout", ["expanded", "odd", "sliced"])
+def test_draft_layouts(layout):
+    """Drafts broadcast over heads, at an odd address, and as a slice of a wider tensor."""
+    lens, t, hkv, d = [70, 5], 5, 2, 128
+    cache = make_cache(4, lens, hkv, d, 16, BF)
+    q = randn(1, 2, 4, t, d)
+    if layout == "expanded":
+        dk, dv = (randn(s, 2, 1, t, d).expand(2, hkv, t, d) for s in (2, 3))
+    elif layout == "odd":
+        dk, dv = (randn(s, 2 * hkv * t * d + 1)[1:].view(2, hkv, t, d) for s in (2, 3))
+    else:
+        dk, dv = (randn(s, 2, hkv, t, 3 * d)[..., d:2 * d] for s in (2, 3))
+    par = random_tree(3, 2, t)
+    check_tree(cache, lens, q, dk, dv, par, [t, t], ax.paged_tree_attention(q, dk, dv, cache, par))
+
+
 def test_parents_out_of_order_are_roots():
     """A parent at or behind its token cannot be on a path: taken as a root, with a notice."""
     lens, t = [50], 6
@@ -301,6 +317,9 @@ def test_contiguous_cache(d, max_len, dt, t):
     keep = (col <= row) & ((row - col < 21) | (col < 3))
     want, bound = attention64(q, cache.keys[:, :, :n], cache.values[:, :, :n], keep)
     assert_within(got, want, bound, "window over a contiguous cache")
+    few = ax.KVLayerCache(cache.keys, cache.values, 3)     # more rows than positions
+    got = ax.kv_cache_attention(randn(4, b, hq, 5, d, dt=dt), few, window_size=2, num_sinks=0)
+    assert float(got[:, :, :2].abs().max()) == 0.0 and bool((got[:, :, 2:] != 0).any())
     mask = (torch.arange(n, device=DEV) % 3 != 0)[None, None, None]
     got = ax.kv_cache_attention(q, cache, window_size=21, num_sinks=3, mask=mask)
     want, bound = attention64(q, cache.keys[:, :, :n], cache.values[:, :, :n], keep & mask[0, 0])
