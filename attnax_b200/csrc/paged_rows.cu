@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
 //   NT = 1 (up to 128 rows): a CTA's chain S -> softmax -> P V is serial; a second
 //     CTA on the SM fills its gaps, which is enough to stay on HBM.
 //   NT = 2 (more rows): the two tiles share every K/V tile and fill each other's
-//     gaps (order P V_0, S_0, P V_1, S_1), one CTA per SM.  With one tile per CTA
-//     the tiles' K/V came from L2 at 64 KB per 128 x 128 tile, about 14 TB/s.
+//     gaps (order P V_0, S_0, P V_1, S_1), one CTA per SM (2 sequences of 100000,
+//     512 rows per kv head: 512 us with one tile per CTA, 488 us with two).
 constexpr int BM = 128, BN = 128;
 template <int D, int NT>
 struct TcCfg {
