@@ -673,6 +673,25 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
     int walk = TREE && row_ok ? t : -1;   // tree: next token on the row's path
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_addr = lanes + x_tile * 128, o_addr = lanes + 128 * NT + x_tile * D;
+    // A warp without rows (33 to 96 rows of a tile) leaves the exponentials to the others (64 rows:
+    // the two idle warps' share of the SM was half of all).
+    const bool idle = r - lane >= a.rows;
+    // V rows that nothing sees -> 0: P is 0 there, but a slot never written (or a box never
+    // loaded) may hold NaN.  Thread = token; with two row tiles both write the same zeros.
+    auto clear_v = [&](int st, int i, int tok0, bool draft) -> bool {
+      if (!__all_sync(0xffffffffu, mbar_wait(v_full(st), (i / S) & 1, kStatusTimeoutSoftmax))) return false;
+      const int tk = tok0 + rl;
+      if (draft ? tk >= sp.drafts : !ctx_visible<TREE>(a, sp, tk)) {
+#pragma unroll
+        for (int c = 0; c < C::KCH; ++c)
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::KV_BYTES + c * BN * 128 + rl * 128 + u * 16) =
+                make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      return true;
+    };
     float m = -FLT_MAX, l = 0.f;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
@@ -704,6 +723,13 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
       ok = __all_sync(0xffffffffu, mbar_wait(s_full(x_tile), i & 1, kStatusTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
+      if (idle) {
+        // No rows here: P and O of these lanes may hold anything, the tile's V rows are still cleared below.
+        if (!whole && !clear_v(st, i, tok0, draft)) { ok = false; break; }
+        tc_fence_before();
+        mbar_arrive_warp(p_full(x_tile));
+        continue;
+      }
       float x[BN];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
@@ -712,20 +738,8 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
 #pragma unroll
         for (int c = 0; c < BN; ++c)
           if (!((keep[c >> 5] >> (c & 31)) & 1u)) x[c] = -INFINITY;
-        // V rows that nothing sees -> 0: P is 0 there, but a slot never written (or a box never
-        // loaded) may hold NaN.  Thread = token; with two row tiles both write the same zeros.
-        ok = __all_sync(0xffffffffu, mbar_wait(v_full(st), (i / S) & 1, kStatusTimeoutSoftmax));
+        ok = clear_v(st, i, tok0, draft);
         if (!ok) break;
-        const int tk = tok0 + rl;
-        if (draft ? tk >= sp.drafts : !ctx_visible<TREE>(a, sp, tk)) {
-#pragma unroll
-          for (int c = 0; c < C::KCH; ++c)
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              *reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::KV_BYTES + c * BN * 128 + rl * 128 + u * 16) =
-                  make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
       }
       float mxp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
