@@ -346,7 +346,7 @@ using namespace attnb200;
 
 extern "C" {
 
-int attn_version(void) { return 1; }
+int attn_version(void) { return 2; }  // 2: attn_mask_t, attn_fwd_params_t, attn_bwd_params_t grew (sinks)
 
 uint64_t attn_launch_count(void) { return g_launches.load(); }
 

@@ -212,3 +212,42 @@ def test_attention_core_with_sinks_and_cache():
     want, bound = attention64(*heads, _keep(n + m, n + m, window, sinks))
     got = torch.cat([first, second], 1).view(b, n + m, hq, d).transpose(1, 2)
     assert_within(got, want, bound, "attention_core")
+
+
+def test_two_graphs_of_a_training_step():
+    """Forward and gradients captured twice, with ALiBi; replays follow the leaves.
+
+    (No eager graph of the same leaves is alive meanwhile: PyTorch ties a leaf's node to the stream of
+    the first graph that uses it, and waiting for that stream ends the capture.)"""
+    b, hq, hkv, s, d, window, sinks = 1, 4, 2, 700, 128, 90, 4
+    q, k, v, do = _inputs(31, b, hq, hkv, s, s, d, BF)
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    mod = ax.compose_score_mods(ax.sink_window_mod(window, sinks), ax.alibi_mod(hq))
+    def step():
+        out = ax.flash_attention(q, k, v, score_mod=mod)
+        return (out, *torch.autograd.grad(out, (q, k, v), do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, res))
+    with torch.no_grad():
+        new = _inputs(32, b, hq, hkv, s, s, d, BF)
+        for t, x in zip((q, k, v, do), new):
+            t.copy_(x)
+    for g, _ in graphs:
+        g.replay()
+    dist = (torch.arange(s, device=DEV)[:, None] - torch.arange(s, device=DEV)[None]).abs().double()
+    bias = -ax.alibi_slopes(hq).double().to(DEV)[None, :, None, None] * dist
+    want, bound, grads, bounds = attention64(q.detach(), k.detach(), v.detach(), _keep(s, s, window, sinks), do, bias)
+    for _, (out, *gs) in graphs:
+        assert_within(out, want, bound, "out")
+        for name, g, w, bd in zip(("dq", "dk", "dv"), gs, grads, bounds):
+            assert_within(g, w, bd, name)
