@@ -10,6 +10,8 @@ import ctypes as C
 import os
 import threading
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libattnb200.so")
 
@@ -203,15 +205,13 @@ def run(name: str, device, *args):
 
     (The device is switched only where it has to be: a switch costs more host time than a small launch.)
     """
-    import torch
-
     fn = getattr(_lib or load(), name)
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    if index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    current = torch.cuda.current_device()
+    if device.index is None or device.index == current:
+        status = fn(*args, torch.cuda.current_stream().cuda_stream)
     else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream().cuda_stream)
     if status != ATTN_OK:
         check(status, name)
 

@@ -78,10 +78,14 @@ def _bound(cache: PagedKVCache, max_context):
     return n
 
 
+def cast(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return x if x.dtype == dtype else x.to(dtype)
+
+
 def _params(query, cache: PagedKVCache, max_context: int):
     """(PagedParams, out, tensors that the call reads)."""
     n, hq, t, d = query.shape
-    q = query.to(cache.key_pool.dtype).contiguous()
+    q = cast(query, cache.key_pool.dtype).contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     out = torch.empty_like(q)
@@ -136,7 +140,7 @@ def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_
     ws = _workspace(p, lib.attn_paged_window_workspace_size(C.byref(p), w, s), query.device)
     _lib.run("attn_paged_window", query.device, C.byref(p), w, s)
     del ws, keep
-    return out.to(query.dtype)
+    return cast(out, query.dtype)
 
 
 def _window_by_sequence(query, cache, window, sinks):
@@ -174,8 +178,10 @@ def gather_window(cache: PagedKVCache, sequence_idx: int, rows: int, window: int
 
 def _tma_ready(x: torch.Tensor) -> torch.Tensor:
     """Unit stride on head_dim, other strides and the base in 16-byte steps (dimensions of one are not stepped)."""
-    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
-        s > 0 and s % 8 == 0 for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1)
+    a, b, c, unit = x.stride()
+    na, nb, nc, _ = x.shape
+    ok = (unit == 1 and x.data_ptr() % 16 == 0 and (na == 1 or (a > 0 and a % 8 == 0))
+          and (nb == 1 or (b > 0 and b % 8 == 0)) and (nc == 1 or (c > 0 and c % 8 == 0)))
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
@@ -220,13 +226,13 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
         return _tree_by_sequence(query, draft_keys, draft_values, cache, parents, tree_lengths)
     lib = _lib.load()
     p, out, keep = _params(query, cache, _bound(cache, max_context))
-    dk, dv = (_tma_ready(x.to(cache.key_pool.dtype)) for x in (draft_keys, draft_values))
+    dk, dv = (_tma_ready(cast(x, cache.key_pool.dtype)) for x in (draft_keys, draft_values))
     tr = _lib.PagedTree(dk.data_ptr(), dv.data_ptr(), dk.stride()[:3], dv.stride()[:3], parents.data_ptr(),
                         None if tree_lengths is None else tree_lengths.data_ptr())
     ws = _workspace(p, lib.attn_paged_tree_workspace_size(C.byref(p)), dev)
     _lib.run("attn_paged_tree", dev, C.byref(p), C.byref(tr))
     del ws, keep
-    return out.to(query.dtype)
+    return cast(out, query.dtype)
 
 
 def _tree_by_sequence(query, dk, dv, cache, parents, tree_lengths):

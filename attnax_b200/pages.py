@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .paged import PagedKVCache
-from .paged_rows import check_tables, on_device
+from .paged_rows import cast, check_tables, on_device
 
 
 _Strides = C.c_int64 * 3
@@ -228,7 +228,7 @@ def append_accepted(cache: PagedKVCache, draft_keys, draft_values, accepted, acc
         if check and n and bool((lens != 0).any()):
             raise ValueError("accepted_lengths counts tokens that are not there")
         return cache
-    kd, vd = draft_keys.to(cache.key_pool.dtype), draft_values.to(cache.key_pool.dtype)
+    kd, vd = cast(draft_keys, cache.key_pool.dtype), cast(draft_values, cache.key_pool.dtype)
     kd, vd = (x if x.stride(3) == 1 else x.contiguous() for x in (kd, vd))
     ks, vs = _Strides(*kd.stride()[:3]), _Strides(*vd.stride()[:3])
     args = (C.byref(p), kd.data_ptr(), vd.data_ptr(), ks, vs, t, acc.data_ptr(), acc.shape[1], lens.data_ptr())
