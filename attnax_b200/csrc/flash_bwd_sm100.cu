@@ -1012,6 +1012,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const long long qg_row = a.mask.q_offset + q0 + r;
     const unsigned long long sl2x2 = f2_pack(a.sl2, a.sl2), delta2 = f2_pack(delta, delta);
     const unsigned long long step2 = f2_pack(8.f * slope_l2, 8.f * slope_l2);
+    // SINK: boundary tiles of a band with sinks take the full-tile arithmetic too, a keep mask per 32
+    // columns then zeroes the dropped dS (three of the seven tiles that a 511-key window visits are
+    // boundary tiles: B3 Hq12 Hkv4 S1999 D64, kernel 111 us without this).
+    const bool bits_mask =
+        SINK && fast_mask && !a.mask.prefix_len && !a.mask.doc_q && !a.mask.bias && !a.mask.bool_mask;
     int i = 0;
     bool ok = true;
     for (int t = j_lo - n_sk; t < j_hi; ++t) {
@@ -1041,7 +1046,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_warp(s_free(i % NSB));
         }
         const int c0 = j * KT + half * HC + cc * 32;
-        if (st == kFull && fast_mask) {
+        if ((st == kFull && fast_mask) || (SINK && bits_mask)) {
           const float rowc = -slope_l2 * (float)clamp_i32(qg_row - (a.mask.kv_offset + c0)) - lse2;
           unsigned long long addv[4];  // rowc + slope*c for the column pairs, 4 independent chains
 #pragma unroll
@@ -1055,6 +1060,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             addv[q] = f2_add(addv[q], step2);
             const unsigned long long p2 = f2_pack(ex2(x0), ex2(x1));
             f2_unpack(f2_mul(p2, f2_sub(f2_pack(dp[c], dp[c + 1]), delta2)), dp[c], dp[c + 1]);
+          }
+          if (SINK && st == kPartial) {
+            const long long d0 = qg_row - (a.mask.kv_offset + c0);  // q - kv at column e is d0 - e
+            const uint32_t keep =
+                bit_range(0, (long long)a.Skv - c0 - 1) &
+                (bit_range(d0 - a.mask.band_hi, d0 - a.mask.band_lo) |
+                 bit_range(0, ll_min(a.mask.num_sinks - (a.mask.kv_offset + c0) - 1, d0 - a.mask.band_lo)));
+#pragma unroll
+            for (int c = 0; c < 32; ++c) dp[c] = ((keep >> c) & 1u) ? dp[c] : 0.f;
           }
         } else {
           const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, q0 + r, c0, max(0, min(32, a.Skv - c0)), false);
