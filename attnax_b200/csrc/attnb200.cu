@@ -265,6 +265,10 @@ static int launch_sm100_fwd2(const attn_fwd_params_t* p, float* lse, const int2*
   a.acc_final_from = acc ? acc->final_from : 0;
   constexpr int smem = fwd2::Cfg<D>::SMEM;
   const bool sink = p->mask.num_sinks > 0;
+  if (sink && (!make_tmap(&a.tm_out, p->dtype, p->out, p->batch, p->num_heads_q, p->seq_q, D, p->o_strides, fwd2::BM) ||
+               (p->out_rest && !make_tmap(&a.tm_rest, p->dtype, p->out_rest, p->batch, p->num_heads_q, p->seq_q, D,
+                                          p->o_strides, fwd2::BM))))
+    return ATTN_ERR_INVALID;
   if (acc && sink) return ATTN_ERR_UNSUPPORTED;  // (the ring's entry points take no sinks)
   const int variant = acc ? 1 : sink ? 2 : 0;
   auto kern = acc ? fwd2::flash_fwd2_kernel<D, BF16, true>

@@ -94,6 +94,8 @@ struct Args {
   float* acc_o;
   float* acc_lse;
   int acc_rows, acc_row0, acc_final_from;
+  // SINK: maps of out and out_rest (64 features x BM rows), for the staged stores.
+  alignas(64) CUtensorMap tm_out, tm_rest;
 };
 
 // Cubic fit of 2^f on [-1/2, 1/2] (max relative error 7.6e-5), our own fit.
@@ -634,7 +636,55 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (row_ok) a.acc_lse[arow] = lnew;
-    } else if (ok && my_act) {
+    } else if (SINK && my_act) {
+      // Rows staged over the tile's own Q (its last S product is done) in the swizzled layout of the maps,
+      // then stored by TMA: a thread's own 16-byte stores at a row's stride cost 80 us per output at B2 Hq16
+      // S16384 D128 (of 467).  Every warp takes part in the barriers, whatever `ok` says.
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      uint8_t* stage = sp + C::OFF_Q + x * C::Q_BYTES;
+      for (int pass = 0; pass < (a.out_rest ? 2 : 1); ++pass) {  // the rounded rows, what rounding left
+        if (ok) {
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            if (i > 0) {
+              tmem_ld32(tmem + lane_base + C::o_col(x) + c * 32, o);
+              tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float lo = __uint_as_float(o[v * 8 + 2 * e]) * inv, hi = __uint_as_float(o[v * 8 + 2 * e + 1]) * inv;
+                w[e] = pack2(lo, hi, BF16);
+                if (pass == 1) w[e] = rest2<BF16>(lo, hi, w[e]);
+              }
+              const int unit = c * 4 + v;  // 16 bytes of the row
+              *reinterpret_cast<uint4*>(stage + (unit >> 3) * BM * 128 + r * 128 + (((unit & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        named_bar_sync(1 + x, 128);
+        if (r == 0 && ok) {
+          for (int c = 0; c < C::KCH; ++c)
+            tma_store_4d(pass ? &a.tm_rest : &a.tm_out, smem_u32(stage) + c * BM * 128, c * 64, my_q0, hq, b);
+          bulk_commit();
+          bulk_wait_read_all();
+        }
+        named_bar_sync(1 + x, 128);  // (the stage may be written again)
+      }
+      if (r == 0) bulk_wait_all();
+      if (ok && (my_q0 + r) < a.Sq && a.lse)
+        a.lse[((long long)b * a.Hq + hq) * a.Sq + my_q0 + r] =
+            (m_run == -FLT_MAX || l_run <= 0.f) ? -INFINITY : (m_run + lg2(l_run)) * kLn2;
+    } else if (!SINK && ok && my_act) {
       tc_fence_after();
       const bool row_ok = (my_q0 + r) < a.Sq;
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
@@ -660,15 +710,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             w.z = pack2(__uint_as_float(o[v * 8 + 4]) * inv, __uint_as_float(o[v * 8 + 5]) * inv, BF16);
             w.w = pack2(__uint_as_float(o[v * 8 + 6]) * inv, __uint_as_float(o[v * 8 + 7]) * inv, BF16);
             *reinterpret_cast<uint4*>(orow + c * 32 + v * 8) = w;
-            if constexpr (SINK) {
-              if (a.out_rest) {
-                auto val = [&](int e) { return __uint_as_float(o[v * 8 + e]) * inv; };
-                const uint4 d = make_uint4(rest2<BF16>(val(0), val(1), w.x), rest2<BF16>(val(2), val(3), w.y),
-                                           rest2<BF16>(val(4), val(5), w.z), rest2<BF16>(val(6), val(7), w.w));
-                *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out_rest) + (orow - reinterpret_cast<T*>(a.out)) +
-                                          c * 32 + v * 8) = d;
-              }
-            }
           }
         }
       }
