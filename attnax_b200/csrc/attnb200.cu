@@ -18,6 +18,7 @@
 #include "flash_fwd_sm100.cu"
 #include "flash_fwd2_sm100.cu"
 #include "flash_simt.cu"
+#include "flash_simt_tiled.cu"
 #include "flash_bwd_sm100.cu"
 #include "paged.cu"
 #include "ring.cu"
@@ -230,6 +231,43 @@ static int launch_simt_fwd(const attn_fwd_params_t* p, float* lse, cudaStream_t 
   return launch_status();
 }
 
+// fp32 with sinks: the register-tiled kernels where every row starts on 16 bytes.
+static bool rows_aligned(const void* p, const int64_t* s) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
+}
+template <typename P>
+static bool tiled_ok(const P* p) {
+  return p->dtype == ATTN_F32 && p->mask.num_sinks > 0 && (p->head_dim == 64 || p->head_dim == 128) &&
+         rows_aligned(p->q, p->q_strides) && rows_aligned(p->k, p->k_strides) && rows_aligned(p->v, p->v_strides) &&
+         rows_aligned(p->out, p->o_strides);
+}
+
+template <typename P>
+static tiled::Args tiled_args(const P* p) {
+  tiled::Args a{};
+  a.B = p->batch; a.Hq = p->num_heads_q; a.Hkv = p->num_heads_kv; a.Sq = p->seq_q; a.Skv = p->seq_kv;
+  a.group = p->num_heads_q / p->num_heads_kv;
+  a.q = static_cast<const float*>(p->q); a.k = static_cast<const float*>(p->k); a.v = static_cast<const float*>(p->v);
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = p->q_strides[i]; a.ks[i] = p->k_strides[i]; a.vs[i] = p->v_strides[i];
+  }
+  a.scale = p->softmax_scale; a.sl2 = p->softmax_scale * kLog2e; a.mask = p->mask;
+  return a;
+}
+
+template <int D>
+static int launch_tiled_fwd(const attn_fwd_params_t* p, float* lse, cudaStream_t st) {
+  tiled::Args a = tiled_args(p);
+  a.out = static_cast<float*>(p->out);
+  for (int i = 0; i < 3; ++i) a.os[i] = p->o_strides[i];
+  a.lse = lse;
+  const size_t smem = tiled::Lay<D>::fwd_smem;
+  if (cudaFuncSetAttribute(tiled::fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return ATTN_ERR_CUDA;
+  tiled::fwd_kernel<D><<<dim3((p->seq_q + tiled::TB - 1) / tiled::TB, a.Hq, a.B), tiled::kThreads, smem, st>>>(a);
+  return launch_status();
+}
+
 // Accumulation target of a ring step (see fwd2::Args::acc_o); null for a plain forward.
 struct RingAcc {
   float* o;
@@ -436,6 +474,8 @@ int attn_fwd(const attn_fwd_params_t* p, void* stream) {
     else
       rc = bf ? launch_sm100_fwd<64, true>(p, lse, dq_t, dkv_t, djr, st, order)
               : launch_sm100_fwd<64, false>(p, lse, dq_t, dkv_t, djr, st, order);
+  } else if (tiled_ok(p)) {
+    rc = p->head_dim == 128 ? launch_tiled_fwd<128>(p, lse, st) : launch_tiled_fwd<64>(p, lse, st);
   } else if (p->dtype == ATTN_F32) {
     rc = launch_simt_fwd<float>(p, lse, st);
   } else if (p->dtype == ATTN_BF16) {
@@ -480,6 +520,11 @@ static bool bwd_tc_ok(const attn_bwd_params_t* p) {
 static int bwd_seq_pad(const attn_bwd_params_t* p) { return (p->seq_q + 127) / 128 * 128; }
 
 static bool bwd_fused_dq(const attn_bwd_params_t* p) { return ATTN_BWD_FUSED_DQ && p->head_dim == 128; }
+
+static bool tiled_bwd_ok(const attn_bwd_params_t* p) {
+  return tiled_ok(p) && rows_aligned(p->d_out, p->do_strides) && rows_aligned(p->dq, p->dq_strides) &&
+         rows_aligned(p->dk, p->dk_strides) && rows_aligned(p->dv, p->dv_strides);
+}
 
 struct BwdWorkspace {
   size_t lse2 = 0, dq_acc = 0, doc_q = 0, doc_kv = 0, doc_q_jr = 0, doc_kv_qr = 0, doc_kv_order = 0,
@@ -536,6 +581,10 @@ static BwdWorkspace bwd_workspace_layout(const attn_bwd_params_t* p) {
       off += align256((size_t)p->batch * bwd_kv_tiles(p->seq_kv) * sizeof(int));
     }
   }
+  if (tiled_bwd_ok(p)) {
+    w.sink_part = off;
+    off += align256((size_t)2 * p->batch * p->num_heads_q * p->seq_kv * p->head_dim * sizeof(float));
+  }
   if (tc && p->mask.num_sinks > 0) {
     const SinkSplit s = sink_split(p->mask, p->seq_q, p->seq_kv, p->num_heads_q / p->num_heads_kv);
     w.sink_part = off;
@@ -543,6 +592,30 @@ static BwdWorkspace bwd_workspace_layout(const attn_bwd_params_t* p) {
   }
   w.total = off;
   return w;
+}
+
+template <int D>
+static int launch_tiled_bwd(const attn_bwd_params_t* p, const float* delta, const float* lse2, float* part,
+                            cudaStream_t st) {
+  tiled::Args a = tiled_args(p);
+  a.dout = static_cast<const float*>(p->d_out);
+  a.dq = static_cast<float*>(p->dq); a.dk = static_cast<float*>(p->dk); a.dv = static_cast<float*>(p->dv);
+  for (int i = 0; i < 3; ++i) {
+    a.dos[i] = p->do_strides[i]; a.dqs[i] = p->dq_strides[i];
+    a.dks[i] = p->dk_strides[i]; a.dvs[i] = p->dv_strides[i];
+  }
+  a.lse2 = lse2; a.delta = delta; a.part = part;
+  using L = tiled::Lay<D>;
+  if (cudaFuncSetAttribute(tiled::dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::dq_smem) !=
+          cudaSuccess ||
+      cudaFuncSetAttribute(tiled::dkv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::dkv_smem) !=
+          cudaSuccess)
+    return ATTN_ERR_CUDA;
+  tiled::dq_kernel<D><<<dim3((a.Sq + tiled::TB - 1) / tiled::TB, a.Hq, a.B), tiled::kThreads, L::dq_smem, st>>>(a);
+  tiled::dkv_kernel<D><<<dim3((a.Skv + tiled::TB - 1) / tiled::TB, a.Hq, a.B), tiled::kThreads, L::dkv_smem, st>>>(a);
+  constexpr int rows = 256 / (D / 4);
+  tiled::group_sum_kernel<D><<<dim3((a.Skv + rows - 1) / rows, a.Hkv, 2 * a.B), 256, 0, st>>>(a);
+  return launch_status(3);
 }
 
 struct BwdDocTables {
@@ -742,6 +815,12 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
         reinterpret_cast<const T*>(p->out), reinterpret_cast<const T*>(p->d_out), p->o_strides[0],
         p->o_strides[1], p->o_strides[2], p->do_strides[0], p->do_strides[1], p->do_strides[2], p->lse,
         delta, lse2, p->num_heads_q, p->seq_q, p->head_dim);
+    int rc = ATTN_OK;
+    const bool tl = tiled_bwd_ok(p);
+    if (tl)
+      rc = p->head_dim == 128 ? launch_tiled_bwd<128>(p, delta, lse2, sink_part, st)
+                              : launch_tiled_bwd<64>(p, delta, lse2, sink_part, st);
+    if (rc != ATTN_OK) return rc;
 #define ATTN_SIMT_BWD(DD)                                                                         \
   case DD: {                                                                                      \
     using L = simt::Lay<DD>;                                                                      \
@@ -751,7 +830,7 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
         <<<dim3((p->seq_kv + L::RPB - 1) / L::RPB, p->num_heads_kv, p->batch), simt::kThreads, 0, st>>>(a); \
     break;                                                                                        \
   }
-    switch (p->head_dim) {
+    if (!tl) switch (p->head_dim) {
       ATTN_SIMT_BWD(8) ATTN_SIMT_BWD(16) ATTN_SIMT_BWD(32) ATTN_SIMT_BWD(64) ATTN_SIMT_BWD(128)
       default: return ATTN_ERR_UNSUPPORTED;
     }
@@ -762,7 +841,7 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
           reinterpret_cast<T*>(p->dv), p->dv_strides[0], p->dv_strides[1], p->dv_strides[2], p->lse,
           p->num_heads_q, p->seq_q, p->seq_kv, p->head_dim, grp);
     }
-    return launch_status(p->fix_masked_rows ? 4 : 3);
+    return launch_status((tl ? 1 : 3) + (p->fix_masked_rows ? 1 : 0));
   };
   if (p->dtype == ATTN_F32) return run(float{});
   if (p->dtype == ATTN_BF16) return run(__nv_bfloat16{});

@@ -1,0 +1,335 @@
+// fp32 flash attention with sinks on register tiles (CUDA cores): forward,
+// dQ, and dK/dV per query head.
+//
+// The one-row-per-thread-group kernels of flash_simt.cu read every K/V value
+// from shared memory for a single multiply-add per row; they stay the path of
+// everything that ran on them.  Here a block of 256 threads owns 64 x 64 score
+// tiles, 4 x 4 per thread: 64 multiply-adds per 8 shared-memory vectors, so the
+// FMA pipe bounds the products.  dK/dV of a kv head are computed per query head
+// (a small batch then fills the GPU) and summed over the group in a fixed order.
+#include <cfloat>
+
+#include "attn_common.cuh"
+
+namespace attnb200 {
+namespace tiled {
+
+constexpr int TB = 64;        // rows of a tile, q or kv
+constexpr int kThreads = 256; // 16 x 16: thread (ty, tx) owns rows 4 ty.., columns tx + 16 j
+constexpr int LP = TB + 4;    // row stride of a staged score tile
+
+template <int D>
+struct Lay {
+  static constexpr int LD = D + 4;  // row stride of a staged tile (16 rows apart in different banks)
+  static constexpr int TILE = TB * LD;
+  static constexpr int NC = D / TB;  // float4 columns of an output row per thread
+  static constexpr size_t fwd_smem = sizeof(float) * (3 * TILE + TB * LP);
+  static constexpr size_t dq_smem = sizeof(float) * (4 * TILE + TB * LP);
+  static constexpr size_t dkv_smem = sizeof(float) * (4 * TILE + 2 * TB * LP + 2 * TB);
+  static_assert(dkv_smem <= 232448, "shared memory of a block");
+};
+
+struct Args {
+  int B, Hq, Hkv, Sq, Skv, group;
+  const float *q, *k, *v, *dout;
+  float *out, *dq, *dk, *dv;
+  long long qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];
+  float* lse;                 // forward
+  const float *lse2, *delta;  // backward, [B][Hq][Sq]
+  float* part;                // [2][B][Hq][Skv][D]: dV and dK per query head
+  float scale, sl2;
+  attn_mask_t mask;
+};
+
+// Rows [r0, r0 + TB) of a tensor into shared memory, zeros past its end.
+template <int D>
+__device__ __forceinline__ void load_tile(float* dst, const float* src, long long stride, int r0, int rows) {
+  for (int x = threadIdx.x; x < TB * (D / 4); x += kThreads) {
+    const int r = x / (D / 4), c = x % (D / 4) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r0 + r < rows) v = *reinterpret_cast<const float4*>(src + (r0 + r) * stride + c);
+    *reinterpret_cast<float4*>(dst + r * Lay<D>::LD + c) = v;
+  }
+}
+
+// acc[i][j] = A[4 ty + i] . B[tx + 16 j]
+template <int D>
+__device__ __forceinline__ void rows_dot(const float* A, const float* B, int ty, int tx, float (&acc)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < D; d += 4) {
+    float4 a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(A + (4 * ty + i) * Lay<D>::LD + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(B + (tx + 16 * j) * Lay<D>::LD + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = fmaf(a[i].x, b[j].x, acc[i][j]);
+        acc[i][j] = fmaf(a[i].y, b[j].y, acc[i][j]);
+        acc[i][j] = fmaf(a[i].z, b[j].z, acc[i][j]);
+        acc[i][j] = fmaf(a[i].w, b[j].w, acc[i][j]);
+      }
+  }
+}
+
+// acc[i][c] += sum_k P[4 ty + i][k] * X[k][64 c + 4 tx ..]
+template <int D>
+__device__ __forceinline__ void add_product(const float* P, const float* X, int ty, int tx,
+                                            float4 (&acc)[4][Lay<D>::NC]) {
+#pragma unroll 2
+  for (int k = 0; k < TB; k += 4) {
+    float4 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(P + (4 * ty + i) * LP + k);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < Lay<D>::NC; ++c) {
+        const float4 x = *reinterpret_cast<const float4*>(X + (k + e) * Lay<D>::LD + c * TB + 4 * tx);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+          acc[i][c].x = fmaf(w, x.x, acc[i][c].x);
+          acc[i][c].y = fmaf(w, x.y, acc[i][c].y);
+          acc[i][c].z = fmaf(w, x.z, acc[i][c].z);
+          acc[i][c].w = fmaf(w, x.w, acc[i][c].w);
+        }
+      }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void clear(float4 (&acc)[4][Lay<D>::NC]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < Lay<D>::NC; ++c) acc[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+template <int D>
+__device__ __forceinline__ void store_rows(float* dst, long long stride, int r0, int rows, int ty, int tx,
+                                           const float4 (&acc)[4][Lay<D>::NC], const float (&mul)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + 4 * ty + i;
+    if (r >= rows) continue;
+#pragma unroll
+    for (int c = 0; c < Lay<D>::NC; ++c)
+      *reinterpret_cast<float4*>(dst + r * stride + c * TB + 4 * tx) =
+          make_float4(acc[i][c].x * mul[i], acc[i][c].y * mul[i], acc[i][c].z * mul[i], acc[i][c].w * mul[i]);
+  }
+}
+
+// Log2-domain score of (row, col), -FLT_MAX where dropped or outside.
+__device__ __forceinline__ float score(const Args& a, float raw, float slope_l2, int b, int hq, int row, int col,
+                                       bool partial) {
+  if (row >= a.Sq || col >= a.Skv) return -FLT_MAX;
+  return mask_score(a.mask, raw, a.sl2, slope_l2, b, hq, row, col, a.Skv, partial);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ Args a) {
+  using L = Lay<D>;
+  extern __shared__ float sm[];
+  float *sq = sm, *sk = sq + L::TILE, *sv = sk + L::TILE, *sp = sv + L::TILE;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int q0 = (gridDim.x - 1 - blockIdx.x) * TB, hq = blockIdx.y, b = blockIdx.z, hkv = hq / a.group;
+  const int q1 = min(q0 + TB, a.Sq);
+  const float* K = a.k + b * a.ks[0] + hkv * a.ks[1];
+  const float* V = a.v + b * a.vs[0] + hkv * a.vs[1];
+  load_tile<D>(sq, a.q + b * a.qs[0] + hq * a.qs[1], a.qs[2], q0, a.Sq);
+  const float slope_l2 = a.mask.alibi_slopes ? a.mask.alibi_slopes[hq] * kLog2e : 0.f;
+  float4 o[4][L::NC];
+  clear<D>(o);
+  float m[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -FLT_MAX;
+    l[i] = 0.f;
+  }
+  int j_lo, j_hi;
+  band_tile_range(a.mask, q0, q1, a.Skv, TB, &j_lo, &j_hi);
+  const int n_sk = sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, TB), j_lo, j_hi);
+  for (int t = j_lo - n_sk; t < j_hi; ++t) {
+    const int j = t < j_lo ? t - (j_lo - n_sk) : t, k0 = j * TB;
+    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, min(k0 + TB, a.Skv), TB);
+    if (st == kSkip) continue;
+    __syncthreads();
+    load_tile<D>(sk, K, a.ks[2], k0, a.Skv);
+    load_tile<D>(sv, V, a.vs[2], k0, a.Skv);
+    __syncthreads();
+    float s[4][4];
+    rows_dot<D>(sq, sk, ty, tx, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = m[i];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[i][c] = score(a, s[i][c], slope_l2, b, hq, q0 + 4 * ty + i, k0 + tx + 16 * c, st == kPartial);
+        mx = fmaxf(mx, s[i][c]);
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float alpha = exp2f(m[i] - mx);
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float p = s[i][c] == -FLT_MAX ? 0.f : exp2f(s[i][c] - mx);
+        sum += p;
+        sp[(4 * ty + i) * LP + tx + 16 * c] = p;
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l[i] = l[i] * alpha + sum;
+      m[i] = mx;
+#pragma unroll
+      for (int c = 0; c < L::NC; ++c) {
+        o[i][c].x *= alpha; o[i][c].y *= alpha; o[i][c].z *= alpha; o[i][c].w *= alpha;
+      }
+    }
+    __syncwarp();  // (a row's 16 threads share a warp)
+    add_product<D>(sp, sv, ty, tx, o);
+  }
+  float inv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    inv[i] = l[i] > 0.f ? 1.f / l[i] : 0.f;
+    const int r = q0 + 4 * ty + i;
+    if (a.lse && tx == 0 && r < a.Sq)
+      a.lse[((long long)b * a.Hq + hq) * a.Sq + r] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+  }
+  store_rows<D>(a.out + b * a.os[0] + hq * a.os[1], a.os[2], q0, a.Sq, ty, tx, o, inv);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Args a) {
+  using L = Lay<D>;
+  extern __shared__ float sm[];
+  float *sq = sm, *sd = sq + L::TILE, *sk = sd + L::TILE, *sv = sk + L::TILE, *sp = sv + L::TILE;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int q0 = (gridDim.x - 1 - blockIdx.x) * TB, hq = blockIdx.y, b = blockIdx.z, hkv = hq / a.group;
+  const int q1 = min(q0 + TB, a.Sq);
+  const float* K = a.k + b * a.ks[0] + hkv * a.ks[1];
+  const float* V = a.v + b * a.vs[0] + hkv * a.vs[1];
+  load_tile<D>(sq, a.q + b * a.qs[0] + hq * a.qs[1], a.qs[2], q0, a.Sq);
+  load_tile<D>(sd, a.dout + b * a.dos[0] + hq * a.dos[1], a.dos[2], q0, a.Sq);
+  const float slope_l2 = a.mask.alibi_slopes ? a.mask.alibi_slopes[hq] * kLog2e : 0.f;
+  float lse2[4], delta[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = q0 + 4 * ty + i;
+    const long long at = ((long long)b * a.Hq + hq) * a.Sq + r;
+    lse2[i] = r < a.Sq ? a.lse2[at] : INFINITY;
+    delta[i] = r < a.Sq ? a.delta[at] : 0.f;
+  }
+  float4 dq[4][L::NC];
+  clear<D>(dq);
+  int j_lo, j_hi;
+  band_tile_range(a.mask, q0, q1, a.Skv, TB, &j_lo, &j_hi);
+  const int n_sk = sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, TB), j_lo, j_hi);
+  for (int t = j_lo - n_sk; t < j_hi; ++t) {
+    const int j = t < j_lo ? t - (j_lo - n_sk) : t, k0 = j * TB;
+    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, min(k0 + TB, a.Skv), TB);
+    if (st == kSkip) continue;
+    __syncthreads();
+    load_tile<D>(sk, K, a.ks[2], k0, a.Skv);
+    load_tile<D>(sv, V, a.vs[2], k0, a.Skv);
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    rows_dot<D>(sq, sk, ty, tx, s);
+    rows_dot<D>(sd, sv, ty, tx, dp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float x = score(a, s[i][c], slope_l2, b, hq, q0 + 4 * ty + i, k0 + tx + 16 * c, st == kPartial);
+        const float p = x == -FLT_MAX ? 0.f : exp2f(x - lse2[i]);
+        sp[(4 * ty + i) * LP + tx + 16 * c] = x == -FLT_MAX ? 0.f : p * (dp[i][c] - delta[i]);  // (dropped dP may be anything)
+      }
+    __syncwarp();
+    add_product<D>(sp, sk, ty, tx, dq);
+  }
+  const float mul[4] = {a.scale, a.scale, a.scale, a.scale};
+  store_rows<D>(a.dq + b * a.dqs[0] + hq * a.dqs[1], a.dqs[2], q0, a.Sq, ty, tx, dq, mul);
+}
+
+// dV and dK of 64 kv rows from one query head, into a.part.
+template <int D>
+__global__ void __launch_bounds__(kThreads) dkv_kernel(const __grid_constant__ Args a) {
+  using L = Lay<D>;
+  extern __shared__ float sm[];
+  float *sk = sm, *sv = sk + L::TILE, *sq = sv + L::TILE, *sd = sq + L::TILE, *sp = sd + L::TILE, *ss = sp + TB * LP;
+  float *sl = ss + TB * LP, *se = sl + TB;  // lse2 and delta of the q tile
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int k0 = blockIdx.x * TB, hq = blockIdx.y, b = blockIdx.z, hkv = hq / a.group;
+  const int k1 = min(k0 + TB, a.Skv);
+  const float* Q = a.q + b * a.qs[0] + hq * a.qs[1];
+  const float* G = a.dout + b * a.dos[0] + hq * a.dos[1];
+  load_tile<D>(sk, a.k + b * a.ks[0] + hkv * a.ks[1], a.ks[2], k0, a.Skv);
+  load_tile<D>(sv, a.v + b * a.vs[0] + hkv * a.vs[1], a.vs[2], k0, a.Skv);
+  const float slope_l2 = a.mask.alibi_slopes ? a.mask.alibi_slopes[hq] * kLog2e : 0.f;
+  float4 dk[4][L::NC], dv[4][L::NC];
+  clear<D>(dk);
+  clear<D>(dv);
+  for (int q0 = 0; q0 < a.Sq; q0 += TB) {
+    const int q1 = min(q0 + TB, a.Sq);
+    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, TB);
+    if (st == kSkip) continue;
+    __syncthreads();
+    load_tile<D>(sq, Q, a.qs[2], q0, a.Sq);
+    load_tile<D>(sd, G, a.dos[2], q0, a.Sq);
+    if (threadIdx.x < TB) {
+      const int r = q0 + threadIdx.x;
+      const long long at = ((long long)b * a.Hq + hq) * a.Sq + r;
+      sl[threadIdx.x] = r < a.Sq ? a.lse2[at] : INFINITY;
+      se[threadIdx.x] = r < a.Sq ? a.delta[at] : 0.f;
+    }
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    rows_dot<D>(sk, sq, ty, tx, s);   // S^T: rows are kv, columns q
+    rows_dot<D>(sv, sd, ty, tx, dp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int e = tx + 16 * c;
+        const float x = score(a, s[i][c], slope_l2, b, hq, q0 + e, k0 + 4 * ty + i, st == kPartial);
+        const float p = x == -FLT_MAX ? 0.f : exp2f(x - sl[e]);
+        sp[(4 * ty + i) * LP + e] = p;
+        ss[(4 * ty + i) * LP + e] = x == -FLT_MAX ? 0.f : p * (dp[i][c] - se[e]);
+      }
+    __syncwarp();
+    add_product<D>(sp, sd, ty, tx, dv);
+    add_product<D>(ss, sq, ty, tx, dk);
+  }
+  const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {a.scale, a.scale, a.scale, a.scale};
+  float* part = a.part + ((long long)b * a.Hq + hq) * a.Skv * D;
+  store_rows<D>(part, D, k0, a.Skv, ty, tx, dv, one);
+  store_rows<D>(part + (long long)a.B * a.Hq * a.Skv * D, D, k0, a.Skv, ty, tx, dk, mul);
+}
+
+// Sum over a kv head's query heads, in their order.
+template <int D>
+__global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ Args a) {
+  const int r = blockIdx.x * (256 / (D / 4)) + threadIdx.x / (D / 4), c = threadIdx.x % (D / 4) * 4;
+  const int hkv = blockIdx.y, b = blockIdx.z % a.B, which = blockIdx.z / a.B;  // dV, dK
+  if (r >= a.Skv) return;
+  const float* p = a.part + (long long)which * a.B * a.Hq * a.Skv * D +
+                   ((long long)b * a.Hq + hkv * a.group) * a.Skv * D + (long long)r * D + c;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g = 0; g < a.group; ++g) {
+    const float4 x = *reinterpret_cast<const float4*>(p + (long long)g * a.Skv * D);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  float* dst = which ? a.dk + b * a.dks[0] + hkv * a.dks[1] + r * a.dks[2] : a.dv + b * a.dvs[0] + hkv * a.dvs[1] + r * a.dvs[2];
+  *reinterpret_cast<float4*>(dst + c) = s;
+}
+
+}  // namespace tiled
+}  // namespace attnb200

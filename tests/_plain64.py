@@ -84,4 +84,9 @@ def assert_within(got, want, bound, what=""):
     rel = float(err.sum()) / total if total else 0.0
     print(f"[plain64] {what}: worst error / bound {worst:.3f}, mean-rel {rel:.2e}")
     assert worst <= 1.0, f"{what}: an element is {worst:.3f} times its bound off"
+    # A relative error says nothing of values that are smaller than what they may be off by: with a
+    # single visible key P = 1 and dS = dP - delta is 0, but dP and delta are sums of D products in 32
+    # bits in two orders, each off by up to D 2^-24 of the sum of magnitudes (the bound above).
+    if total < float(bound.expand_as(want).sum()):
+        return
     assert rel <= MEAN_REL, f"{what}: mean relative error {rel:.3e}"

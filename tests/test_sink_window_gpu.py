@@ -47,7 +47,11 @@ CASES = [
     (1, 2, 1, 1, 128, BF, 5, 2),           # one token
     (1, 4, 1, 6001, 128, BF, 64, 4),       # the sinks' gradient split over several CTAs
     (1, 2, 2, 6001, 64, HF, 30, 300),
-    (2, 4, 2, 200, 64, F32, 33, 4),        # 32-bit path
+    (2, 4, 2, 200, 64, F32, 33, 4),        # 32-bit path, register tiles
+    (1, 6, 1, 321, 128, F32, 100, 70),
+    (2, 3, 3, 65, 128, F32, 64, 1),
+    (1, 4, 2, 1030, 64, F32, 200, 131),
+    (1, 2, 2, 1, 128, F32, 1, 1),
     (1, 2, 1, 150, 32, BF, 17, 5),         # head dims of the CUDA-core path
     (1, 2, 1, 90, 8, F32, 7, 40),
 ]
@@ -80,6 +84,21 @@ def test_with_alibi_and_documents(d, dt):
             assert_within(g, w, bd, name)
 
 
+def test_bias_in_32_bits():
+    """An additive bias and a boolean mask on the 32-bit path."""
+    b, hq, hkv, s, d, window, sinks = 1, 4, 2, 150, 64, 40, 3
+    q, k, v, do = _inputs(6, b, hq, hkv, s, s, d, F32)
+    bias = _inputs(7, 1, hq, 1, s, s, 8, F32)[0][..., :1] * torch.ones(1, 1, 1, s, device=DEV)
+    mask = torch.rand(1, 1, s, s, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) > 0.2
+    mask |= torch.eye(s, dtype=torch.bool, device=DEV)
+    mod = ax.compose_score_mods(ax.sink_window_mod(window, sinks), ax.additive_bias_mod(bias))
+    out, *gs = _run(q, k, v, do, mod, mask)
+    want, bound, grads, bounds = attention64(q, k, v, _keep(s, s, window, sinks) & mask, do, bias.double())
+    assert_within(out, want, bound, "out")
+    for name, g, w, bd in zip(("dq", "dk", "dv"), gs, grads, bounds):
+        assert_within(g, w, bd, name)
+
+
 def test_boolean_mask_and_rows_without_keys():
     """A mask on top: rows that keep nothing average all of V (the framework's rule)."""
     b, hq, hkv, s, d, window, sinks = 1, 2, 1, 400, 128, 50, 4
@@ -104,7 +123,7 @@ def test_boolean_mask_and_rows_without_keys():
 
 
 @pytest.mark.parametrize("sq,skv", [(300, 700), (700, 300), (5, 900), (900, 1)])
-@pytest.mark.parametrize("d,dt", [(128, BF), (64, HF), (16, F32)])
+@pytest.mark.parametrize("d,dt", [(128, BF), (64, HF), (16, F32), (64, F32), (128, F32)])
 def test_unequal_lengths(sq, skv, d, dt):
     """More queries than keys: late rows keep only sinks; more keys than queries: late keys get no gradient."""
     window, sinks = 40, 3
@@ -117,13 +136,14 @@ def test_unequal_lengths(sq, skv, d, dt):
 
 
 @pytest.mark.parametrize("q_off,kv_off", [(0, 0), (512, 0), (512, 256), (300, 300), (2, 0)])
-def test_global_offsets(q_off, kv_off):
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_global_offsets(q_off, kv_off, dt):
     """One chunk pair of a longer sequence (the ring's step): sinks go by global key positions."""
     from attnax_b200._spec import build_spec
     from attnax_b200.flash import bwd_raw, fwd_raw
 
     window, sinks, s = 200, 260, 512
-    q, k, v, do = _inputs(q_off + 3, 1, 2, 1, s, s, 128, BF)
+    q, k, v, do = _inputs(q_off + 3, 1, 2, 1, s, s, 128, dt)
     spec = build_spec(ax.sink_window_mod(window, sinks), None, batch=1, heads_q=2, seq_q=s, seq_kv=s,
                       device=q.device, q_offset=q_off, kv_offset=kv_off)
     spec.fix_masked_rows = False
@@ -148,11 +168,12 @@ def test_strided_inputs():
         assert_within(g, w, bd, name)
 
 
-def test_dropped_keys_may_hold_anything_large():
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_dropped_keys_may_hold_anything_large(dt):
     """Keys that no row keeps: their scores overflow nowhere and their gradient is zero."""
     s, window, sinks = 600, 50, 4
-    q, k, v, do = _inputs(21, 1, 2, 1, 40, s, 128, BF)
-    k[:, :, 60:] = 3e38
+    q, k, v, do = _inputs(21, 1, 2, 1, 40, s, 128, dt)
+    k[:, :, 60:], v[:, :, 60:] = 3e38, -3e38
     out, dq, dk, dv = _run(q, k, v, do, ax.sink_window_mod(window, sinks))
     k0, v0 = k[:, :, :60], v[:, :, :60]
     want, bound, grads, bounds = attention64(q, k0, v0, _keep(40, 60, window, sinks), do)
