@@ -46,8 +46,8 @@ __host__ __device__ inline long long ll_max(long long a, long long b) { return a
 
 // Classifies the tile [q0,q1) x [k0,k1) of batch b (local positions).
 // doc_q_tiles/doc_kv_tiles hold (min,max) ids per kDocTile-row tile; when
-// they are null a document mask makes every tile partial.  SINK: the mask may
-// hold sinks (num_sinks); the instantiations without it never look.
+// they are null a document mask makes every tile partial.  SINK: the mask
+// holds sinks (num_sinks > 0); the instantiations without it never look.
 template <bool SINK = false>
 __host__ __device__ inline int tile_state(const attn_mask_t& m, const int2* doc_q_tiles,
                                           const int2* doc_kv_tiles, int nq_doc, int nk_doc, int b,
@@ -133,7 +133,10 @@ __device__ __forceinline__ float load_bias(const void* p, attn_dtype_t dt, long 
 }
 
 // Element transform for one score: raw q.k -> log2-domain score t, with
-// every mask and additive term.  `row`/`col` are local positions.
+// every mask and additive term.  `row`/`col` are local positions.  SINK as in
+// tile_state: only with num_sinks > 0 (without sinks `kvg < num_sinks` would
+// hold for keys at negative positions).
+template <bool SINK = false>
 __device__ __forceinline__ float mask_score(const attn_mask_t& m, float raw, float sl2,
                                             float slope_l2, int b, int h, int row, int col,
                                             int seq_kv, bool partial) {
@@ -145,7 +148,7 @@ __device__ __forceinline__ float mask_score(const attn_mask_t& m, float raw, flo
   bool keep = true;
   if (m.has_band) {
     const long long d = qg - kvg;
-    keep = keep && d >= m.band_lo && (d <= m.band_hi || kvg < m.num_sinks);
+    keep = keep && d >= m.band_lo && (d <= m.band_hi || (SINK && kvg < m.num_sinks));
   }
   if (m.prefix_len) keep = keep && (kvg < (long long)m.prefix_len[b] || kvg <= qg);
   if (m.doc_q)

@@ -220,7 +220,8 @@ static int launch_simt_fwd(const attn_fwd_params_t* p, float* lse, cudaStream_t 
 #define ATTN_SIMT_FWD(DD)                                                                   \
   case DD: {                                                                                \
     dim3 g((p->seq_q + simt::Lay<DD>::RPB - 1) / simt::Lay<DD>::RPB, p->num_heads_q, p->batch); \
-    simt::simt_fwd_kernel<T, DD><<<g, simt::kThreads, 0, st>>>(a);                          \
+    if (a.mask.num_sinks > 0) simt::simt_fwd_kernel<T, DD, true><<<g, simt::kThreads, 0, st>>>(a); \
+    else simt::simt_fwd_kernel<T, DD><<<g, simt::kThreads, 0, st>>>(a);                     \
     break;                                                                                  \
   }
   switch (p->head_dim) {
@@ -840,10 +841,15 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
 #define ATTN_SIMT_BWD(DD)                                                                         \
   case DD: {                                                                                      \
     using L = simt::Lay<DD>;                                                                      \
-    simt::simt_bwd_dq_kernel<T, DD>                                                               \
-        <<<dim3((p->seq_q + L::RPB - 1) / L::RPB, p->num_heads_q, p->batch), simt::kThreads, 0, st>>>(a); \
-    simt::simt_bwd_dkv_kernel<T, DD>                                                              \
-        <<<dim3((p->seq_kv + L::RPB - 1) / L::RPB, p->num_heads_kv, p->batch), simt::kThreads, 0, st>>>(a); \
+    const dim3 gq((p->seq_q + L::RPB - 1) / L::RPB, p->num_heads_q, p->batch);                    \
+    const dim3 gkv((p->seq_kv + L::RPB - 1) / L::RPB, p->num_heads_kv, p->batch);                 \
+    if (a.mask.num_sinks > 0) {                                                                   \
+      simt::simt_bwd_dq_kernel<T, DD, true><<<gq, simt::kThreads, 0, st>>>(a);                    \
+      simt::simt_bwd_dkv_kernel<T, DD, true><<<gkv, simt::kThreads, 0, st>>>(a);                  \
+    } else {                                                                                      \
+      simt::simt_bwd_dq_kernel<T, DD><<<gq, simt::kThreads, 0, st>>>(a);                          \
+      simt::simt_bwd_dkv_kernel<T, DD><<<gkv, simt::kThreads, 0, st>>>(a);                        \
+    }                                                                                             \
     break;                                                                                        \
   }
     if (!tl) switch (p->head_dim) {

@@ -8,7 +8,7 @@
 // Layout: a query (or key) row is owned by TPR = max(1, D/32) consecutive
 // lanes, each holding EPT = D/TPR contiguous features; dot products reduce
 // over those lanes with shuffles.  K/V (or Q/dO) tiles of KT rows are staged
-// in shared memory as fp32.
+// in shared memory as fp32.  SINK: the mask holds sinks (num_sinks > 0).
 #include <cfloat>
 
 #include "attn_common.cuh"
@@ -42,7 +42,7 @@ struct FwdArgs {
   attn_mask_t mask;
 };
 
-template <typename T, int D>
+template <typename T, int D, bool SINK = false>
 __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const FwdArgs a) {
   using L = Lay<D>;
   __shared__ float sk[KT][D];
@@ -68,11 +68,11 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const FwdArgs a) {
   int j_lo, j_hi;
   band_tile_range(a.mask, q0, q1, a.Skv, KT, &j_lo, &j_hi);
   // the sinks' tiles in front of the band's run first
-  const int n_sk = a.mask.num_sinks > 0 ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
+  const int n_sk = SINK ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
   for (int t0 = j_lo - n_sk; t0 < j_hi; ++t0) {
-    const int j = t0 < j_lo ? t0 - (j_lo - n_sk) : t0;
+    const int j = SINK && t0 < j_lo ? t0 - (j_lo - n_sk) : t0;
     const int k0 = j * KT, k1 = min(k0 + KT, a.Skv);
-    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
+    const int st = tile_state<SINK>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
     if (st == kSkip) continue;
     __syncthreads();
     for (int x = tid; x < KT * D; x += kThreads) {
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < L::EPT; ++e) acc = fmaf(q[e], sk[c][part * L::EPT + e], acc);
       acc = group_sum<L::TPR>(acc);
-      t[c] = mask_score(a.mask, acc, a.sl2, slope_l2, b, hq, row, k0 + c, a.Skv, st == kPartial);
+      t[c] = mask_score<SINK>(a.mask, acc, a.sl2, slope_l2, b, hq, row, k0 + c, a.Skv, st == kPartial);
       mx = fmaxf(mx, t[c]);
     }
     const float alpha = exp2f(m - mx);
@@ -154,7 +154,7 @@ struct BwdArgs {
 };
 
 // dQ: one query row per TPR lanes, K/V tiles staged.
-template <typename T, int D>
+template <typename T, int D, bool SINK = false>
 __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) {
   using L = Lay<D>;
   __shared__ float sk[KT][D];
@@ -183,11 +183,11 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) 
   int j_lo, j_hi;
   band_tile_range(a.mask, q0, q1, a.Skv, KT, &j_lo, &j_hi);
   // the sinks' tiles in front of the band's run first
-  const int n_sk = a.mask.num_sinks > 0 ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
+  const int n_sk = SINK ? sink_tiles_before(sink_tile_count(a.mask, q1, a.Skv, KT), j_lo, j_hi) : 0;
   for (int t0 = j_lo - n_sk; t0 < j_hi; ++t0) {
-    const int j = t0 < j_lo ? t0 - (j_lo - n_sk) : t0;
+    const int j = SINK && t0 < j_lo ? t0 - (j_lo - n_sk) : t0;
     const int k0 = j * KT, k1 = min(k0 + KT, a.Skv);
-    const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
+    const int st = tile_state<SINK>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, KT);
     if (st == kSkip) continue;
     __syncthreads();
     for (int x = tid; x < KT * D; x += kThreads) {
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) 
       }
       s = group_sum<L::TPR>(s);
       dp = group_sum<L::TPR>(dp);
-      const float t = mask_score(a.mask, s, a.sl2, slope_l2, b, hq, row, k0 + c, a.Skv, st == kPartial);
+      const float t = mask_score<SINK>(a.mask, s, a.sl2, slope_l2, b, hq, row, k0 + c, a.Skv, st == kPartial);
       const float p = (t == -FLT_MAX) ? 0.f : exp2f(t - lse2);
       const float ds = p * (dp - delta);
 #pragma unroll
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) 
 
 // dK, dV: one key row per TPR lanes, summed over the query heads of its
 // group (the transpose of the reference's jnp.repeat, attention.py:32-39).
-template <typename T, int D>
+template <typename T, int D, bool SINK = false>
 __global__ void __launch_bounds__(kThreads) simt_bwd_dkv_kernel(const BwdArgs a) {
   using L = Lay<D>;
   __shared__ float sq[KT][D];
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dkv_kernel(const BwdArgs a)
     const int nqt = (a.Sq + KT - 1) / KT;
     for (int i = 0; i < nqt; ++i) {
       const int q0 = i * KT, q1 = min(q0 + KT, a.Sq);
-      const int st = tile_state<true>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, L::RPB);
+      const int st = tile_state<SINK>(a.mask, nullptr, nullptr, 0, 0, b, q0, q1, k0, k1, L::RPB);
       if (st == kSkip) continue;
       __syncthreads();
       for (int x = tid; x < KT * D; x += kThreads) {
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dkv_kernel(const BwdArgs a)
         }
         s = group_sum<L::TPR>(s);
         dp = group_sum<L::TPR>(dp);
-        const float t = mask_score(a.mask, s, a.sl2, slope_l2, b, hq, q0 + rr, col, a.Skv,
+        const float t = mask_score<SINK>(a.mask, s, a.sl2, slope_l2, b, hq, q0 + rr, col, a.Skv,
                                    st == kPartial || q0 + rr >= a.Sq);
         const float p = (t == -FLT_MAX || !col_ok) ? 0.f : exp2f(t - slse[rr]);
         const float ds = p * (dp - sdelta[rr]);

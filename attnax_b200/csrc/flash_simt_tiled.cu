@@ -135,7 +135,7 @@ __device__ __forceinline__ void store_rows(float* dst, long long stride, int r0,
 __device__ __forceinline__ float score(const Args& a, float raw, float slope_l2, int b, int hq, int row, int col,
                                        bool partial) {
   if (row >= a.Sq || col >= a.Skv) return -FLT_MAX;
-  return mask_score(a.mask, raw, a.sl2, slope_l2, b, hq, row, col, a.Skv, partial);
+  return mask_score<true>(a.mask, raw, a.sl2, slope_l2, b, hq, row, col, a.Skv, partial);
 }
 
 template <int D, int R>

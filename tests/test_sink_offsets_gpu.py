@@ -1,0 +1,50 @@
+"""Windows at global offsets (chunks of a longer sequence), with and without sinks, against the formula in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+import attnax_b200 as ax
+from attnax_b200._spec import build_spec
+from attnax_b200.flash import bwd_raw, fwd_raw
+from tests._plain64 import assert_within, attention64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _inputs(seed, hq, hkv, sq, skv, d, dt):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    mk = lambda *s: torch.randn(s, generator=g, device=DEV).to(dt)  # noqa: E731
+    return mk(1, hq, sq, d), mk(1, hkv, skv, d), mk(1, hkv, skv, d), mk(1, hq, sq, d)
+
+
+def _spec(mod, hq, sq, skv, q_off, kv_off):
+    spec = build_spec(mod, None, batch=1, heads_q=hq, seq_q=sq, seq_kv=skv, device=torch.device(DEV, 0),
+                      q_offset=q_off, kv_offset=kv_off)
+    spec.fix_masked_rows = False
+    return spec
+
+
+def _positions(sq, skv, q_off, kv_off):
+    return torch.arange(sq, device=DEV)[:, None] + q_off, torch.arange(skv, device=DEV)[None, :] + kv_off
+
+
+@pytest.mark.parametrize("d,dt", [(64, F32), (128, F32), (8, F32), (32, BF), (16, HF), (128, BF), (64, HF)])
+@pytest.mark.parametrize("q_off,kv_off", [(0, -512), (-40, -512), (0, -7)])
+@pytest.mark.parametrize("window", [10, 130])
+def test_plain_window_over_keys_in_front_of_position_zero(d, dt, q_off, kv_off, window):
+    """Without sinks no key is one, whatever its position: the band alone decides, at negative positions too."""
+    hq, hkv, sq, skv = 4, 2, 150, 700
+    q, k, v, do = _inputs(window, hq, hkv, sq, skv, d, dt)
+    spec = _spec(ax.sliding_window_mod(window), hq, sq, skv, q_off, kv_off)
+    out, lse = fwd_raw(q, k, v, spec)
+    qi, ki = _positions(sq, skv, q_off, kv_off)
+    keep = (ki <= qi) & (qi - ki < window)
+    assert bool(keep.any(1).all())
+    want, bound, grads, bounds = attention64(q, k, v, keep, do)
+    assert_within(out, want, bound, "out")
+    for name, g, w, bd in zip(("dq", "dk", "dv"), bwd_raw(q, k, v, out, lse, do, spec), grads, bounds):
+        assert_within(g, w, bd, name)
