@@ -637,9 +637,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (row_ok) a.acc_lse[arow] = lnew;
     } else if (SINK && my_act) {
-      // Rows staged over the tile's own Q (its last S product is done) in the swizzled layout of the maps,
+      // Rows staged over the tile's own Q (its last S product is done; a tile that kept no kv tile had none, and
+      // waits for Q's load, which may still be landing there) in the swizzled layout of the maps,
       // then stored by TMA: a thread's own 16-byte stores at a row's stride cost 80 us per output at B2 Hq16
       // S16384 D128 (of 467).  Every warp takes part in the barriers, whatever `ok` says.
+      if (i == 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(q_full, 0, kStatusTimeoutSoftmax));
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
       uint8_t* stage = sp + C::OFF_Q + x * C::Q_BYTES;
       for (int pass = 0; pass < (a.out_rest ? 2 : 1); ++pass) {  // the rounded rows, what rounding left

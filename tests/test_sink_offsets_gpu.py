@@ -48,3 +48,34 @@ def test_plain_window_over_keys_in_front_of_position_zero(d, dt, q_off, kv_off, 
     assert_within(out, want, bound, "out")
     for name, g, w, bd in zip(("dq", "dk", "dv"), bwd_raw(q, k, v, out, lse, do, spec), grads, bounds):
         assert_within(g, w, bd, name)
+
+
+@pytest.mark.parametrize("d,dt", [(128, BF), (64, HF), (128, F32)])
+@pytest.mark.parametrize("q_off,kv_off,rows", [(1024, 512, 512), (1150, 512, 512), (1150, 512, 200), (5000, 512, 700)])
+@pytest.mark.parametrize("rested", [False, True])
+def test_row_tiles_that_keep_no_key(d, dt, q_off, kv_off, rows, rested):
+    """Chunks behind the window and without a sink: zeros and -inf, no gradients, also of the rounding rest."""
+    window, sinks, skv, hq, hkv = 200, 260, 512, 4, 2
+    if rested and dt == F32:
+        pytest.skip("the rest is the 16-bit types'")
+    q, k, v, do = _inputs(q_off, hq, hkv, rows, skv, d, dt)
+    spec = _spec(ax.sink_window_mod(window, sinks), hq, rows, skv, q_off, kv_off)
+    rest = torch.full_like(q, 7.0) if rested else None
+    qi, ki = _positions(rows, skv, q_off, kv_off)
+    keep = (ki <= qi) & ((qi - ki < window) | (ki < sinks))
+    empty = ~keep.any(1)
+    # 128-row tiles without any key, alone in their pair or beside a tile with keys
+    tiles = torch.cat([empty, empty.new_ones(-rows % 128)]).view(-1, 128).all(1)
+    assert bool(tiles.any())
+    zero = tiles.repeat_interleave(128)[:rows]
+    want, bound, grads, bounds = attention64(q, k, v, keep, do)
+    for _ in range(20):
+        out, lse = fwd_raw(q, k, v, spec, rest=rest)
+        assert float(out[:, :, zero].abs().max()) == 0.0
+        if rested:
+            assert float(rest[:, :, zero].abs().max()) == 0.0
+        assert bool((lse[:, :, empty] == -math.inf).all()) and bool(torch.isfinite(lse[:, :, ~empty]).all())
+    if bool((~empty).any()):
+        assert_within(out[:, :, ~empty], want[:, :, ~empty], bound[:, :, ~empty], "out")
+    for name, g, w, bd in zip(("dq", "dk", "dv"), bwd_raw(q, k, v, out, lse, do, spec, rest=rest), grads, bounds):
+        assert_within(g, w, bd, name)
