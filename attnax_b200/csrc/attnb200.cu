@@ -545,20 +545,32 @@ struct BwdWorkspace {
 // How dkdv_kernel splits the rows behind the window of the kv tiles that hold
 // sinks: chunks of about the q tiles that a window's kv tile visits, not under
 // 32 (query head, q tile) pairs (a CTA's start and its partial then cost a few
-// per cent), and at most 64 chunks (the partials stay small next to dK and dV).
+// per cent).  Of the chunks there are at most 64, and fewer the more tiles hold
+// sinks: either their partials are no more rows than dK and dV have (or 8192),
+// or the chunks' CTAs are no more than four waves.  Tiles that would be left in
+// one piece are not split at all.  (B1 Hq32 Hkv8 S32768 W512, 64 chunks for any
+// number of sinks -> this rule: 1000 sinks 3.09 -> 2.96 ms, 4096 8.17 -> 6.85 ms
+// and 1.6 GiB -> 0.3 GiB of partials, 32768 34.3 -> 25.5 ms and 13 GiB -> none.)
 struct SinkSplit {
-  int rows = 0, tiles = 0, chunks = 0, chunk_tiles = 1;
+  int rows = 0, tiles = 0, chunks = 0, chunk_tiles = 1, whole = 0;
 };
-static SinkSplit sink_split(const attn_mask_t& m, int seq_q, int seq_kv, int group) {
+static SinkSplit sink_split(const attn_mask_t& m, int seq_q, int seq_kv, int group, long long kv_heads) {
   SinkSplit s;
   const long long rows = ll_min(m.num_sinks - m.kv_offset, seq_kv);
   if (m.num_sinks <= 0 || rows <= 0) return s;
+  const int tiles = (int)((rows + bwd::KROWS - 1) / bwd::KROWS), n_kt = (seq_kv + bwd::KROWS - 1) / bwd::KROWS;
+  const long long by_rows = ll_max(64, n_kt) / tiles, ctas = tiles * kv_heads, by_ctas = (4 * 148 + ctas - 1) / ctas;
+  const long long most = ll_min(64, ll_max(by_rows, by_ctas));
+  if (most < 2) {
+    s.whole = 1;
+    return s;
+  }
   s.rows = (int)rows;
-  s.tiles = (s.rows + bwd::KROWS - 1) / bwd::KROWS;
+  s.tiles = tiles;
   const int nq = (seq_q + bwd::QT - 1) / bwd::QT;
   const int left = nq - bwd::sink_q_first(m, 0, seq_kv < bwd::KROWS ? seq_kv : bwd::KROWS, seq_q);
   const long long band = ll_min((m.band_hi - m.band_lo) / bwd::QT, nq) + bwd::KROWS / bwd::QT + 1;
-  s.chunk_tiles = (int)ll_max(ll_max(band, (31 + group) / group), (left + 63) / 64);
+  s.chunk_tiles = (int)ll_max(ll_max(band, (31 + group) / group), (left + most - 1) / most);
   s.chunks = left > 0 ? (left + s.chunk_tiles - 1) / s.chunk_tiles : 0;
   return s;
 }
@@ -597,7 +609,8 @@ static BwdWorkspace bwd_workspace_layout(const attn_bwd_params_t* p) {
     off += align256((size_t)2 * p->batch * p->num_heads_q * p->seq_kv * p->head_dim * sizeof(float));
   }
   if (tc && p->mask.num_sinks > 0) {
-    const SinkSplit s = sink_split(p->mask, p->seq_q, p->seq_kv, p->num_heads_q / p->num_heads_kv);
+    const SinkSplit s = sink_split(p->mask, p->seq_q, p->seq_kv, p->num_heads_q / p->num_heads_kv,
+                                   (long long)p->batch * p->num_heads_kv);
     w.sink_part = off;
     off += align256((size_t)(1 + s.chunks) * p->batch * p->num_heads_kv * s.rows * 2 * p->head_dim * sizeof(float));
   }
@@ -688,10 +701,10 @@ static int launch_sm100_bwd(const attn_bwd_params_t* p, float* delta, float* lse
     return ATTN_ERR_INVALID;
   // With an order table, blockIdx.x walks (rank, kv head) with heads fastest.
   const int sink = p->mask.num_sinks > 0;
-  const SinkSplit split = sink_split(p->mask, Sq, Skv, a.group);
+  const SinkSplit split = sink_split(p->mask, Sq, Skv, a.group, (long long)B * Hkv);
   a.sink_part = sink_part;
   a.sink_rows = split.rows; a.sink_tiles = split.tiles;
-  a.sink_chunks = split.chunks; a.sink_chunk_tiles = split.chunk_tiles;
+  a.sink_chunks = split.chunks; a.sink_chunk_tiles = split.chunk_tiles; a.sink_whole = split.whole;
   const int items = a.n_kt + split.tiles * split.chunks;
   const dim3 grid_kv = a.kv_order ? dim3(items * Hkv, 1, B) : dim3(items, Hkv, B);
   auto reduce_sinks = [&] {

@@ -123,9 +123,10 @@ struct Args {
   // each a CTA of its own (grid indices in front of the n_kt kv tiles, since they may be
   // the longest: kv tile slowest, chunk fastest).  The first sink_rows kv rows leave fp32 partials
   // [1 + sink_chunks][B][Hkv][sink_rows][dV, dK][D]: slot 0 from the kv tile's
-  // window, slot 1 + c from chunk c; sink_reduce_kernel sums them.
+  // window, slot 1 + c from chunk c; sink_reduce_kernel sums them.  sink_whole: nothing is split (the
+  // other four are 0), a sink's kv tile visits the rows behind its window itself.
   float* sink_part;
-  int sink_rows, sink_tiles, sink_chunks, sink_chunk_tiles;
+  int sink_rows, sink_tiles, sink_chunks, sink_chunk_tiles, sink_whole;
 };
 
 // q-tile index range [lo, hi) (tiles of QT) that the band allows for kv rows [k0, k1).
@@ -259,7 +260,8 @@ struct CfgKV {
 // one CTA it walked all q tiles alone (B2 Hq16 Hkv4 S16384 W512, 16 sinks: the
 // whole call 2.76 ms), so the rows behind its window are split over CTAs of
 // about the other kv tiles' length (Args::sink_chunks) that leave fp32 partials
-// of the sinks' dK/dV rows, summed in a fixed order.
+// of the sinks' dK/dV rows, summed in a fixed order.  Where the sinks' own tiles
+// fill the GPU they do without (Args::sink_whole; see sink_split).
 template <int D, bool BF16, bool FQ, bool SINK = false>
 __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
     dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -347,6 +349,9 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
     const int nq = (a.Sq + QT - 1) / QT;
     t_lo = min(nq, sink_q_first(a.mask, k0, k1, a.Sq) + chunk * a.sink_chunk_tiles);
     t_hi = min(nq, t_lo + a.sink_chunk_tiles);
+  } else if (SINK && a.sink_whole && a.mask.kv_offset + k0 < a.mask.num_sinks) {
+    if (t_hi <= t_lo) t_lo = sink_q_first(a.mask, k0, k1, a.Sq);
+    t_hi = (a.Sq + QT - 1) / QT;
   }
   if (a.doc_kv_qr) {
     static_assert(KROWS == kDocTile && kDocTile % QT == 0, "document tiles vs kv / q tiles");

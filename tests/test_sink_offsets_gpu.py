@@ -79,3 +79,29 @@ def test_row_tiles_that_keep_no_key(d, dt, q_off, kv_off, rows, rested):
         assert_within(out[:, :, ~empty], want[:, :, ~empty], bound[:, :, ~empty], "out")
     for name, g, w, bd in zip(("dq", "dk", "dv"), bwd_raw(q, k, v, out, lse, do, spec, rest=rest), grads, bounds):
         assert_within(g, w, bd, name)
+
+
+@pytest.mark.parametrize("b,hq,hkv,s,d,dt,window,sinks", [
+    (1, 18, 18, 4300, 128, BF, 64, 4200),   # sinks in more than half of the kv tiles, 594 tiles: nothing split
+    (1, 17, 17, 4500, 64, HF, 700, 9000),   # every key a sink
+    (1, 4, 1, 4300, 128, BF, 64, 4200),     # as many sinks on one kv head: chunks to fill the GPU
+    (2, 6, 2, 2000, 64, BF, 100, 1500),     # several sink tiles, a few chunks each
+])
+def test_many_sinks(b, hq, hkv, s, d, dt, window, sinks):
+    """However the rows behind the windows of the sinks' tiles are shared out."""
+    g = torch.Generator(device=DEV).manual_seed(s)
+    mk = lambda h: torch.randn(b, h, s, d, generator=g, device=DEV).to(dt)  # noqa: E731
+    q, k, v, do = mk(hq).requires_grad_(True), mk(hkv).requires_grad_(True), mk(hkv).requires_grad_(True), mk(hq)
+    out = ax.flash_attention(q, k, v, score_mod=ax.sink_window_mod(window, sinks))
+    gs = torch.autograd.grad(out, (q, k, v), do)
+    qi, ki = _positions(s, s, 0, 0)
+    keep = (ki <= qi) & ((qi - ki < window) | (ki < sinks))
+    grp = hq // hkv
+    for x in range(b):
+        for h in range(hkv):  # one kv head at a time: the 64-bit scores of all take too much memory
+            qs, ks = slice(h * grp, (h + 1) * grp), slice(h, h + 1)
+            want, bound, grads, bounds = attention64(q.detach()[x:x + 1, qs], k.detach()[x:x + 1, ks],
+                                                     v.detach()[x:x + 1, ks], keep, do[x:x + 1, qs])
+            assert_within(out[x:x + 1, qs], want, bound, "out")
+            for name, y, w, bd, hs in zip(("dq", "dk", "dv"), gs, grads, bounds, (qs, ks, ks)):
+                assert_within(y[x:x + 1, hs], w, bd, name)
