@@ -48,6 +48,17 @@ class PagedKVCache:
         return int(self.key_pool.shape[3])
 
 
+def check_pools(cache: PagedKVCache):
+    """Both pools alike: the kernels take their shape, type and device from ``key_pool``."""
+    k, v = cache.key_pool, cache.value_pool
+    if k.dim() != 4:
+        raise ValueError(f"key_pool must be (num_blocks, block_size, num_kv_heads, head_dim), got {tuple(k.shape)}")
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"value_pool {tuple(v.shape)} {v.dtype} != key_pool {tuple(k.shape)} {k.dtype}")
+    if v.device != k.device:
+        raise RuntimeError(f"value_pool is on {v.device}, key_pool on {k.device}")
+
+
 def init_paged_kv_cache(*, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
                         batch_size: int, max_blocks_per_seq: int, dtype=torch.bfloat16,
                         device="cuda") -> PagedKVCache:
@@ -81,6 +92,7 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
     if keys_new.shape != values_new.shape:
         raise ValueError(f"keys_new shape {tuple(keys_new.shape)} != values_new shape "
                          f"{tuple(values_new.shape)}")
+    check_pools(cache)
     lib = _lib.load()
     chunk = int(keys_new.shape[0])
     start = int(cache.seq_lengths[sequence_idx])
@@ -108,6 +120,7 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
 
 def gather_kv(cache: PagedKVCache, sequence_idx: int):
     """Contiguous ``(seq_len, Hkv, D)`` keys/values of one sequence (paged_cache.py:201-231)."""
+    check_pools(cache)
     lib = _lib.load()
     seq_len = int(cache.seq_lengths[sequence_idx])
     shape = (seq_len, cache.num_kv_heads, cache.head_dim)
@@ -134,6 +147,7 @@ def paged_decode_raw(query, cache: PagedKVCache, *, block_table=None, seq_length
     and reported by ``_lib.device_status()`` (``NOTICE_CONTEXT_OVERRUN`` /
     ``NOTICE_TABLE_OVERRUN``) instead of raising.
     """
+    check_pools(cache)
     lib = _lib.load()
     bt = cache.block_table if block_table is None else block_table
     sl = cache.seq_lengths if seq_lengths is None else seq_lengths

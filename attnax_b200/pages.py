@@ -31,9 +31,9 @@ _Strides = C.c_int64 * 3
 
 def _params(cache: PagedKVCache):
     """(PagedCacheParams, tensors it points into)."""
+    check_tables(cache)
     if not cache.key_pool.is_cuda:
         raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
-    check_tables(cache)
     kp, vpool = cache.key_pool, cache.value_pool
     if not (kp.is_contiguous() and vpool.is_contiguous()):
         raise ValueError("page operators write the pools in place and need them contiguous")

@@ -1,0 +1,54 @@
+"""What the paged entry points refuse about the cache itself, without a GPU: its fields have to describe each other."""
+
+import pytest
+import torch
+
+import attnax_b200 as ax
+
+BF = torch.bfloat16
+
+
+def cpu_cache():
+    return ax.init_paged_kv_cache(num_blocks=8, block_size=16, num_kv_heads=2, head_dim=64, batch_size=3,
+                                  max_blocks_per_seq=4, device="cpu")
+
+
+Q = torch.zeros(3, 4, 2, 64, dtype=BF)
+DRAFT = torch.zeros(3, 2, 2, 64, dtype=BF)
+PAR = torch.full((3, 2), -1, dtype=torch.int32)
+
+ROWS = [
+    lambda c: ax.paged_window_attention(Q, c, window_size=4),
+    lambda c: ax.paged_tree_attention(Q, DRAFT, DRAFT, c, PAR),
+]
+PAGES = [
+    lambda c: ax.copy_blocks(c, [0], [1]), lambda c: ax.fork_sequences(c, [0], [1], [2]),
+    lambda c: ax.free_sequences(c, [0]), lambda c: ax.free_window(c, window_size=3),
+    lambda c: ax.compact_blocks(c), lambda c: ax.append_accepted(c, DRAFT, DRAFT, [[0]] * 3, [1] * 3),
+]
+OLDER = [
+    lambda c: ax.append_kv(c, 0, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64)),
+    lambda c: ax.gather_kv(c, 0),
+    lambda c: ax.paged_attention_batched(torch.zeros(3, 4, 2, 64, dtype=BF), c),
+]
+
+POOLS = {
+    "fewer pages": lambda v: v[:4], "smaller pages": lambda v: v[:, :8], "fewer heads": lambda v: v[:, :, :1],
+    "smaller head": lambda v: v[..., :32], "wider": lambda v: v.float(), "other type": lambda v: v.to(torch.float16),
+    "flat": lambda v: v.flatten(),
+}
+
+
+@pytest.mark.parametrize("call", ROWS + PAGES + OLDER)
+@pytest.mark.parametrize("pool", POOLS)
+def test_value_pool_unlike_the_key_pool(call, pool):
+    c = cpu_cache()
+    with pytest.raises(ValueError, match="value_pool"):
+        call(ax.PagedKVCache(c.key_pool, POOLS[pool](c.value_pool), c.block_table, c.seq_lengths))
+
+
+@pytest.mark.parametrize("call", ROWS + PAGES + OLDER)
+def test_value_pool_on_another_device(call):
+    c = cpu_cache()
+    with pytest.raises(RuntimeError, match="value_pool"):
+        call(ax.PagedKVCache(c.key_pool, c.value_pool.to("meta"), c.block_table, c.seq_lengths))
