@@ -59,6 +59,15 @@ def check_pools(cache: PagedKVCache):
         raise RuntimeError(f"value_pool is on {v.device}, key_pool on {k.device}")
 
 
+def check_rows(block_table: torch.Tensor, seq_lengths: torch.Tensor):
+    """One table row and one length per sequence."""
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be (num_seqs, max_blocks_per_seq), got {tuple(block_table.shape)}")
+    if seq_lengths.dim() != 1 or seq_lengths.shape[0] != block_table.shape[0]:
+        raise ValueError(f"seq_lengths {tuple(seq_lengths.shape)} do not match the {block_table.shape[0]} rows of "
+                         "block_table")
+
+
 def init_paged_kv_cache(*, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
                         batch_size: int, max_blocks_per_seq: int, dtype=torch.bfloat16,
                         device="cuda") -> PagedKVCache:
@@ -151,9 +160,12 @@ def paged_decode_raw(query, cache: PagedKVCache, *, block_table=None, seq_length
     lib = _lib.load()
     bt = cache.block_table if block_table is None else block_table
     sl = cache.seq_lengths if seq_lengths is None else seq_lengths
+    check_rows(bt, sl)
     if query.dim() != 4:
         raise ValueError("query must be (num_seqs, num_heads, seq_q, head_dim)")
     n, hq, sq, d = query.shape
+    if n != bt.shape[0]:
+        raise ValueError(f"query has {n} sequences, the cache {bt.shape[0]}")
     if hq % cache.num_kv_heads != 0:
         raise ValueError(f"num_heads ({hq}) must be divisible by num_kv_heads "
                          f"({cache.num_kv_heads}) for paged attention")

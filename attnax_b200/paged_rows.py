@@ -24,7 +24,7 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .flash import attention, softmax_scale
-from .paged import PagedKVCache, check_pools, gather_kv
+from .paged import PagedKVCache, check_pools, check_rows, gather_kv
 
 
 def _check_query(query, cache: PagedKVCache):
@@ -42,8 +42,9 @@ def _check_query(query, cache: PagedKVCache):
 
 
 def check_tables(cache: PagedKVCache):
-    """The kernels read int32 tables on the pools' device, and two pools alike."""
+    """The kernels read int32 tables on the pools' device, a row and a length per sequence, and two pools alike."""
     check_pools(cache)
+    check_rows(cache.block_table, cache.seq_lengths)
     dev = cache.key_pool.device
     for name, x in (("block_table", cache.block_table), ("seq_lengths", cache.seq_lengths)):
         if x.dtype != torch.int32:

@@ -52,3 +52,23 @@ def test_value_pool_on_another_device(call):
     c = cpu_cache()
     with pytest.raises(RuntimeError, match="value_pool"):
         call(ax.PagedKVCache(c.key_pool, c.value_pool.to("meta"), c.block_table, c.seq_lengths))
+
+
+@pytest.mark.parametrize("call", ROWS + PAGES)
+def test_lengths_and_table_rows_that_do_not_match(call):
+    c = cpu_cache()
+    for table, lens in ((c.block_table, c.seq_lengths[:2]), (c.block_table, c.seq_lengths[None]),
+                        (c.block_table, c.seq_lengths[0]), (c.block_table.flatten(), c.seq_lengths),
+                        (c.block_table[None], c.seq_lengths), (c.block_table, torch.zeros(4, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            call(ax.PagedKVCache(c.key_pool, c.value_pool, table, lens))
+
+
+def test_decode_rows():
+    from attnax_b200.paged import paged_decode_raw
+
+    c = cpu_cache()
+    for q, kw in ((Q[:2], {}), (torch.cat([Q, Q]), {}), (Q, {"seq_lengths": c.seq_lengths[:2]}),
+                  (Q, {"block_table": c.block_table[:2]}), (Q, {"block_table": c.block_table[0]})):
+        with pytest.raises(ValueError):
+            paged_decode_raw(q, c, **kw)
