@@ -100,7 +100,9 @@ def _window_attention(query, cache: KVLayerCache, n: int, mask, score_mod, windo
     k, v = cache.keys, cache.values
     hkv = k.shape[1]
     bs = next((x for x in _BLOCK_SIZES if cache.max_len % x == 0), None)
-    if (mask is None and score_mod is None and bs is not None and d in (64, 128) and k.is_contiguous()
+    # (the page kernels have no backward; the flash kernel below has)
+    grads = torch.is_grad_enabled() and (query.requires_grad or k.requires_grad or v.requires_grad)
+    if (not grads and mask is None and score_mod is None and bs is not None and d in (64, 128) and k.is_contiguous()
             and v.is_contiguous() and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float16)):
         nseq, nblk = b * hkv, cache.max_len // bs
         pool = PagedKVCache(k.view(nseq * nblk, bs, 1, d), v.view(nseq * nblk, bs, 1, d),
@@ -130,7 +132,9 @@ def kv_cache_attention(query: torch.Tensor, cache: KVLayerCache, *, mask=None, s
     and see a causal window of that many keys plus the first ``num_sinks``
     ones (no counterpart in the reference): the kernels of
     ``paged_window_attention`` read only those, on the cache itself (bf16/f16,
-    head_dim 64 or 128, ``max_len`` a multiple of 16, no mask/score_mod).
+    head_dim 64 or 128, ``max_len`` a multiple of 16, no mask/score_mod, and
+    no gradient asked for: where the query or the cache requires one, the
+    flash kernel and its backward run on a boolean mask).
 
     bf16/f16 buffers with head_dim 128, ``max_len`` a multiple of 16 and no
     mask/score_mod take the split-K decode kernel; otherwise the flash kernel

@@ -74,7 +74,7 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
 
     mods = compose_score_mods(base_score_mod, score_mod)
     if past and attention_sinks and mask is None and mods is None and attention_fn is flash_attention:
-        # a cached step of a window with sinks: the decode reads only the keys that it sees
+        # a cached step of a window with sinks: without gradients the decode reads only the keys that it sees
         out = kv_cache_attention(q, new_cache, window_size=attention_window, num_sinks=attention_sinks)
         return out.transpose(1, 2).reshape(b, seq_q, num_heads * head_dim), new_cache
     if attention_window is not None and self_attention:

@@ -12,6 +12,8 @@ bf16/f16 caches with head_dim 64 or 128 and a block size that is a multiple
 of 16 take the fused kernels (one launch, and one that joins the splits);
 other caches gather each sequence and run the flash kernel on it, with one
 host sync.  Both kernels run on the current stream of the cache's device.
+Like the paged decode they are for inference: the fused kernels have no backward,
+and what they return carries no gradient.
 """
 
 from __future__ import annotations

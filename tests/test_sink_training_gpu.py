@@ -1,0 +1,59 @@
+"""Training through windows with sinks on a contiguous cache."""
+
+import pytest
+import torch
+
+import attnax_b200 as ax
+from attnax_b200.mha import attention_core
+from tests._plain64 import assert_within, attention64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def randn(seed, *shape, dt=BF):
+    return torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(dt)
+
+
+def _keep(rows, n, window, sinks):
+    """The last ``rows`` of ``n`` positions."""
+    q = torch.arange(n - rows, n, device=DEV)[:, None]
+    k = torch.arange(n, device=DEV)[None, :]
+    return (k <= q) & ((q - k < window) | (k < sinks))
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32])
+@pytest.mark.parametrize("masked", [False, True])
+def test_cached_continuation_is_differentiable(dt, masked):
+    """attention_core on a cache: gradients of the continuation's query, key and value, in every type."""
+    b, hq, hkv, d, n, m, window, sinks = 2, 4, 2, 128, 200, 37, 64, 5
+    qkv = [randn(i, b, n + m, h * d, dt=dt) for i, h in enumerate((hq, hkv, hkv))]
+    do = randn(9, b, m, hq * d, dt=dt)
+    kw = dict(num_heads=hq, num_kv_heads=hkv, attention_window=window, attention_sinks=sinks)
+    mask = torch.ones(1, 1, m, n + m, dtype=torch.bool, device=DEV) if masked else None
+    with torch.no_grad():
+        _, cache = attention_core(*(t[:, :n] for t in qkv), kv_cache=ax.init_kv_layer_cache(b, hkv, d, 256, dt), **kw)
+    step = [t[:, n:].clone().requires_grad_(True) for t in qkv]
+    out, _ = attention_core(*step, kv_cache=cache, mask=mask, **kw)
+    got = torch.autograd.grad(out, step, do)
+    heads = [t.view(b, n + m, -1, d).transpose(1, 2) for t in qkv]
+    dh = do.view(b, m, hq, d).transpose(1, 2)
+    want, bound, grads, bounds = attention64(heads[0][:, :, n:], heads[1], heads[2], _keep(m, n + m, window, sinks), dh)
+    assert_within(out.view(b, m, hq, d).transpose(1, 2), want, bound, "out")
+    for name, g, w, bd in zip(("dq", "dk", "dv"), got, grads, bounds):
+        assert_within(g.view(b, m, -1, d).transpose(1, 2), w[:, :, -m:], bd[:, :, -m:], name)
+
+
+@pytest.mark.parametrize("d,dt", [(128, BF), (64, HF), (32, F32)])
+def test_window_over_a_contiguous_cache_is_differentiable(d, dt):
+    b, hq, hkv, n, t = 1, 4, 2, 150, 9
+    cache = ax.init_kv_layer_cache(b, hkv, d, 160, dt)
+    cache = ax.update_kv_layer_cache(cache, randn(1, b, hkv, n, d, dt=dt), randn(2, b, hkv, n, d, dt=dt), 0)
+    q, do = randn(3, b, hq, t, d, dt=dt).requires_grad_(True), randn(4, b, hq, t, d, dt=dt)
+    out = ax.kv_cache_attention(q, cache, window_size=21, num_sinks=3)
+    dq, = torch.autograd.grad(out, q, do)
+    want, bound, grads, bounds = attention64(q.detach(), cache.keys[:, :, :n], cache.values[:, :, :n],
+                                             _keep(t, n, 21, 3), do)
+    assert_within(out, want, bound, "out")
+    assert_within(dq, grads[0], bounds[0], "dq")
