@@ -110,16 +110,14 @@ def _window_attention(query, cache: KVLayerCache, n: int, mask, score_mod, windo
                             torch.full((nseq,), n, dtype=torch.int32, device=query.device))
         q = query.contiguous().view(nseq, hq // hkv, sq, d)
         return paged_window_attention(q, pool, window_size=window, num_sinks=sinks, max_context=n).view(b, hq, sq, d)
-    first = max(0, sq - n)  # rows in front of the cache see nothing
-    qi = torch.arange(n - sq + first, n, device=query.device)[:, None]
+    qi = torch.arange(n - sq, n, device=query.device)[:, None]
     ki = torch.arange(n, device=query.device)[None, :]
     win = ((ki <= qi) & ((qi - ki < window) | (ki < sinks)))[None, None]
     if mask is not None:
-        mask = torch.as_tensor(mask, device=query.device)
-        win = win & (mask[..., first:, :] if mask.dim() > 1 and mask.shape[-2] == sq else mask)
-    out = torch.zeros_like(query)
-    out[:, :, first:] = attention(query[:, :, first:].to(k.dtype), k[:, :, :n], v[:, :, :n], mask=win,
-                                  score_mod=score_mod).to(query.dtype)
+        win = win & torch.as_tensor(mask, device=query.device).to(torch.bool)
+    out = attention(query.to(k.dtype), k[:, :, :n], v[:, :, :n], mask=win, score_mod=score_mod).to(query.dtype)
+    if sq > n:  # rows in front of the cache see nothing
+        out = torch.cat([torch.zeros_like(out[:, :, :sq - n]), out[:, :, sq - n:]], 2)
     return out
 
 

@@ -57,3 +57,21 @@ def test_window_over_a_contiguous_cache_is_differentiable(d, dt):
                                              _keep(t, n, 21, 3), do)
     assert_within(out, want, bound, "out")
     assert_within(dq, grads[0], bounds[0], "dq")
+
+
+@pytest.mark.parametrize("d,dt", [(64, F32), (128, BF)])
+def test_score_mod_of_rows_in_front_of_the_cache(d, dt):
+    """More rows than positions: a score_mod is given all rows, those that see nothing are zeros without a gradient."""
+    b, hq, hkv, n, t = 1, 4, 2, 11, 16
+    cache = ax.init_kv_layer_cache(b, hkv, d, 32, dt)
+    cache = ax.update_kv_layer_cache(cache, randn(1, b, hkv, n, d, dt=dt), randn(2, b, hkv, n, d, dt=dt), 0)
+    q, do = randn(3, b, hq, t, d, dt=dt).requires_grad_(True), randn(4, b, hq, t, d, dt=dt)
+    bias = randn(5, b, hq, t, n, dt=dt)
+    got = ax.kv_cache_attention(q, cache, window_size=6, num_sinks=2, score_mod=ax.additive_bias_mod(bias))
+    dq, = torch.autograd.grad(got, q, do)
+    want, bound, grads, bounds = attention64(q.detach(), cache.keys[:, :, :n], cache.values[:, :, :n],
+                                             _keep(t, n, 6, 2), do, bias.double())
+    first = t - n
+    assert float(got[:, :, :first].abs().max()) == 0.0 and float(dq[:, :, :first].abs().max()) == 0.0
+    assert_within(got[:, :, first:], want[:, :, first:], bound[:, :, first:], "out")
+    assert_within(dq[:, :, first:], grads[0][:, :, first:], bounds[0][:, :, first:], "dq")
