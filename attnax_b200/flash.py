@@ -38,6 +38,11 @@ def _prep(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or its copy at an address that is a multiple of 16 bytes (a slice may start anywhere)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def check_qkv(query, key, value):
     """Validates shapes like the reference and returns (B, Hq, Hkv, Sq, Skv, D)."""
     for name, t in (("query", query), ("key", key), ("value", value)):
@@ -125,6 +130,7 @@ class _FlashAttnFn(torch.autograd.Function):
         # (16-bit types on the tensor cores) the rounding rest is kept for the backward.
         rest = None
         if spec.struct.num_sinks > 0 and q.dtype != torch.float32 and q.shape[-1] in (64, 128):
+            q, k, v = _aligned(q), _aligned(k), _aligned(v)
             rest = torch.empty_like(q, memory_format=torch.contiguous_format)
         out, lse = fwd_raw(q, k, v, spec, rest=rest)
         ctx.save_for_backward(q, k, v, out, lse, rest)
@@ -134,7 +140,10 @@ class _FlashAttnFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse, rest = ctx.saved_tensors
-        dq, dk, dv = bwd_raw(q, k, v, out, lse, _prep(dout), ctx.spec, rest=rest)
+        dout = _prep(dout)
+        if rest is not None:
+            dout = _aligned(dout)
+        dq, dk, dv = bwd_raw(q, k, v, out, lse, dout, ctx.spec, rest=rest)
         return dq, dk, dv, None
 
 

@@ -75,3 +75,20 @@ def test_score_mod_of_rows_in_front_of_the_cache(d, dt):
     assert float(got[:, :, :first].abs().max()) == 0.0 and float(dq[:, :, :first].abs().max()) == 0.0
     assert_within(got[:, :, first:], want[:, :, first:], bound[:, :, first:], "out")
     assert_within(dq[:, :, first:], grads[0][:, :, first:], bounds[0][:, :, first:], "dq")
+
+
+@pytest.mark.parametrize("d,dt", [(128, BF), (64, HF), (128, F32)])
+@pytest.mark.parametrize("odd", ["q", "k", "v", "do"])
+def test_training_at_odd_addresses(d, dt, odd):
+    """One of the tensors starts at an address that is no multiple of 16 bytes."""
+    b, hq, hkv, s, window, sinks = 1, 4, 2, 300, 40, 3
+    def at(seed, h, shift):  # (contiguous, `shift` elements behind an aligned address)
+        return randn(seed, b * h * s * d + 8, dt=dt)[shift:shift + b * h * s * d].view(b, h, s, d)
+    t = {n: at(i, h, 1 if n == odd else 0) for i, (n, h) in enumerate((("q", hq), ("k", hkv), ("v", hkv), ("do", hq)))}
+    q, k, v = (t[n].requires_grad_(True) for n in ("q", "k", "v"))
+    out = ax.flash_attention(q, k, v, score_mod=ax.sink_window_mod(window, sinks))
+    gs = torch.autograd.grad(out, (q, k, v), t["do"])
+    want, bound, grads, bounds = attention64(q.detach(), k.detach(), v.detach(), _keep(s, s, window, sinks), t["do"])
+    assert_within(out, want, bound, "out")
+    for name, g, w, bd in zip(("dq", "dk", "dv"), gs, grads, bounds):
+        assert_within(g, w, bd, name)
