@@ -83,7 +83,7 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
         elif isinstance(p, AlibiMod):
             if p.num_heads != heads_q:
                 raise ValueError(f"alibi_mod({p.num_heads}) used with {heads_q} query heads")
-            # (on the device once per mod: a copy from the host per call would wait for it, and could not be captured)
+            # (kept on the device by the mod: a copy from the host per call would wait for it, and could not be captured)
             s = p._device_tensor("slopes", p.slopes, device)
             slopes = s if slopes is None else slopes + s
         elif isinstance(p, PrefixLMMod):

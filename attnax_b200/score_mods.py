@@ -41,11 +41,14 @@ class TaggedScoreMod:
     kind = "tagged"
 
     def _device_tensor(self, name, t, device):
+        """``t`` on the device.  From the host it is copied once, and again when its values have changed."""
+        if t.device.type != "cpu" or torch.device(device).type == "cpu":
+            return t.to(device).contiguous()
         cache = self.__dict__.setdefault("_dev_cache", {})
         key = (name, str(device))
-        if key not in cache:
-            cache[key] = t.to(device).contiguous()
-        return cache[key]
+        if key not in cache or cache[key][0].dtype != t.dtype or not torch.equal(cache[key][0], t):
+            cache[key] = (t.clone(), t.to(device).contiguous())
+        return cache[key][1]
 
 
 class CausalMod(TaggedScoreMod):

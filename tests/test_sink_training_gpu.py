@@ -92,3 +92,27 @@ def test_training_at_odd_addresses(d, dt, odd):
     assert_within(out, want, bound, "out")
     for name, g, w, bd in zip(("dq", "dk", "dv"), gs, grads, bounds):
         assert_within(g, w, bd, name)
+
+
+def test_slopes_that_change_between_calls():
+    """The kernels follow a mod's slopes: replaced, or written in place on either device."""
+    hq, s, d = 4, 90, 64
+    q, k, v = (randn(i, 1, hq, s, d) for i in range(3))
+    mod = ax.alibi_mod(hq)
+    dist = (torch.arange(s, device=DEV)[:, None] - torch.arange(s, device=DEV)[None]).abs().double()
+
+    def check(what):
+        got = ax.flash_attention(q, k, v, score_mod=ax.compose_score_mods(ax.sink_window_mod(30, 2), mod))
+        bias = -mod.slopes.double().to(DEV)[None, :, None, None] * dist
+        want, bound = attention64(q, k, v, _keep(s, s, 30, 2), None, bias)
+        assert_within(got, want, bound, what)
+
+    check("as made")
+    mod.slopes = mod.slopes * 3
+    check("replaced")
+    mod.slopes *= 0.1
+    check("written in place")
+    mod.slopes = mod.slopes.to(DEV)
+    check("on the device")
+    mod.slopes.mul_(5)
+    check("written in place on the device")

@@ -1,0 +1,39 @@
+"""What build_spec hands to the kernels follows the mods' values, on the CPU."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import attnax_b200 as ax
+from attnax_b200._spec import build_spec
+
+
+def _spec(mod, s=8, heads=4):
+    return build_spec(mod, None, batch=1, heads_q=heads, seq_q=s, seq_kv=s, device="cpu")
+
+
+def _slopes(spec, n):
+    return list((C.c_float * n).from_address(spec.struct.alibi_slopes))
+
+
+def test_slopes_follow_the_mod():
+    mod = ax.alibi_mod(4)
+    assert _slopes(_spec(mod), 4) == mod.slopes.tolist()
+    mod.slopes = mod.slopes * 3
+    assert _slopes(_spec(mod), 4) == mod.slopes.tolist()
+    mod.slopes *= 0.5
+    assert _slopes(_spec(mod), 4) == mod.slopes.tolist()
+
+
+def test_device_copies_follow_their_values():
+    """The copy kept for a device (a stand-in here) is made again when the host's values, length or type change."""
+    mod = ax.alibi_mod(4)
+    one = mod._device_tensor("slopes", mod.slopes, "meta")
+    assert mod._device_tensor("slopes", mod.slopes, "meta") is one
+    assert mod._device_tensor("slopes", mod.slopes.clone(), "meta") is one
+    mod.slopes[2] += 1
+    two = mod._device_tensor("slopes", mod.slopes, "meta")
+    assert two is not one and mod._device_tensor("slopes", mod.slopes, "meta") is two
+    assert mod._device_tensor("slopes", mod.slopes.double(), "meta").dtype == torch.float64
+    assert mod._device_tensor("slopes", mod.slopes[:3], "meta").shape == (3,)
