@@ -75,6 +75,8 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
             lo = max(lo, 0 if p.causal else -(w - 1))
             hi = min(hi, w - 1)
             has_band = True
+        elif isinstance(p, SinkWindowMod) and p.num_sinks == 0:  # a plain causal window
+            lo, hi, has_band = max(lo, 0), min(hi, p.window_size - 1), True
         elif isinstance(p, SinkWindowMod):
             if sink is not None and (sink.window_size, sink.num_sinks) != (p.window_size, p.num_sinks):
                 raise NotImplementedError("two different sink_window_mod windows in one chain")

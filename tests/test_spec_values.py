@@ -37,3 +37,19 @@ def test_device_copies_follow_their_values():
     assert two is not one and mod._device_tensor("slopes", mod.slopes, "meta") is two
     assert mod._device_tensor("slopes", mod.slopes.double(), "meta").dtype == torch.float64
     assert mod._device_tensor("slopes", mod.slopes[:3], "meta").shape == (3,)
+
+
+def test_a_sink_window_without_sinks_is_a_plain_window():
+    """It composes like one: with wider and narrower windows, with other windows without sinks, and with sinks."""
+    def band(*mods):
+        m = _spec(ax.compose_score_mods(*mods)).struct
+        return m.has_band, m.band_lo, m.band_hi, m.num_sinks
+
+    assert band(ax.sink_window_mod(4, 0), ax.sliding_window_mod(9)) == (1, 0, 3, 0)
+    assert band(ax.sliding_window_mod(3, causal=False), ax.sink_window_mod(4, 0)) == (1, 0, 2, 0)
+    assert band(ax.sink_window_mod(4, 0), ax.sink_window_mod(7, 0)) == (1, 0, 3, 0)
+    assert band(ax.sink_window_mod(4, 0), ax.sink_window_mod(7, 2)) == (1, 0, 3, 0)
+    assert band(ax.sink_window_mod(7, 2), ax.sink_window_mod(7, 0)) == (1, 0, 6, 0)
+    assert band(ax.sink_window_mod(4, 0)) == (1, 0, 3, 0)
+    with pytest.raises(NotImplementedError):
+        band(ax.sink_window_mod(7, 2), ax.sink_window_mod(9, 0))
