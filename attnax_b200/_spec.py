@@ -117,7 +117,7 @@ def build_spec(score_mod, mask, *, batch, heads_q, seq_q, seq_kv, device, q_offs
             raise NotImplementedError(f"{sink!r} composed with a wider sliding window")
         # a plain window no wider than the sinks' own drops everything that the sinks add
         if hi == BAND_INF:
-            hi, m.num_sinks = sink.window_size - 1, sink.num_sinks
+            hi, m.num_sinks = min(sink.window_size - 1, BAND_INF), min(sink.num_sinks, BAND_INF)
     if has_band:
         m.has_band, m.band_lo, m.band_hi = 1, lo, hi
     if prefix is not None:

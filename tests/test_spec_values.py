@@ -53,3 +53,14 @@ def test_a_sink_window_without_sinks_is_a_plain_window():
     assert band(ax.sink_window_mod(4, 0)) == (1, 0, 3, 0)
     with pytest.raises(NotImplementedError):
         band(ax.sink_window_mod(7, 2), ax.sink_window_mod(9, 0))
+
+
+@pytest.mark.parametrize("window,sinks", [(1 << 70, 4), (5, (1 << 64) + 3), ((1 << 64) + 5, (1 << 64) + 3)])
+def test_windows_and_sinks_beyond_64_bits(window, sinks):
+    """Longer than any sequence, not their low 64 bits."""
+    m = _spec(ax.sink_window_mod(window, sinks)).struct
+    assert m.has_band and m.band_lo == 0
+    assert m.band_hi == (window - 1 if window < 1 << 60 else m.band_hi) and m.band_hi >= min(window - 1, 1 << 60)
+    assert m.num_sinks == (sinks if sinks < 1 << 60 else m.num_sinks) and m.num_sinks >= min(sinks, 1 << 60)
+    # positions up to 2^40 added on either side stay within 64 bits
+    assert m.band_hi + (1 << 40) < 1 << 63 and m.num_sinks + (1 << 40) < 1 << 63
