@@ -204,10 +204,10 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ A
   float inv[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    inv[i] = l[i] > 0.f ? 1.f / l[i] : 0.f;
+    inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];  // (0: no kept key; NaN scores make it NaN)
     const int r = q0 + R * ty + i;
     if (a.lse && tx == 0 && r < a.Sq)
-      a.lse[((long long)b * a.Hq + hq) * a.Sq + r] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+      a.lse[((long long)b * a.Hq + hq) * a.Sq + r] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
   }
   store_rows<D, R>(a.out + b * a.os[0] + hq * a.os[1], a.os[2], q0, a.Sq, ty, tx, o, inv);
 }

@@ -7,7 +7,9 @@
 // whole context (attnax/kernels/paged.py:17-84).
 //
 // Both are softmax(q k^T * scale | keep) v in one pass with a running maximum
-// and sum, split over the visible tokens and joined by their log-sum-exp.  The
+// and sum, split over the visible tokens and joined by their log-sum-exp.  A
+// row sum of exactly 0 means that the row saw nothing (zeros, lse -inf); a NaN
+// score makes it NaN, and the row with it.  The
 // rows of one kv head (its query heads x T) share every K/V read.  With up to
 // 64 rows the work is bound by HBM (4 * rows flops per byte of K/V); wider
 // trees approach the tensor cores' rate.
@@ -141,7 +143,7 @@ __device__ __forceinline__ void join_in_cluster(float* o, float* lse, int n, int
   float mx = mine;
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-  const float w = mx == -INFINITY ? 0.f : ex2(mine - mx);
+  const float w = mine == -INFINITY ? 0.f : ex2(mine - mx);  // (fmaxf skips NaN, this does not)
   float tot = 0.f, acc[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
@@ -153,7 +155,7 @@ __device__ __forceinline__ void join_in_cluster(float* o, float* lse, int n, int
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wi, oi[e], acc[e]);
   }
-  const float inv = tot > 0.f ? 1.f / tot : 0.f;
+  const float inv = tot == 0.f ? 0.f : 1.f / tot;
 #pragma unroll
   for (int e = 0; e < D / 32; e += 2)
     *reinterpret_cast<uint32_t*>(out + e) = pack2(acc[e] * inv, acc[e + 1] * inv, BF16);
@@ -427,12 +429,12 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
     for (int w = 0; w < TW; ++w) {
       const int at = (w * RW + t) * 16 + jr;
       const float lw = ml[at * 2 + 1];
-      const float f = lw > 0.f ? ex2(ml[at * 2] - mx) : 0.f;  // (a row without keys holds o of nothing)
+      const float f = lw == 0.f ? 0.f : ex2(ml[at * 2] - mx);  // (a row without keys holds o of nothing)
       lt += f * lw;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] += f > 0.f ? f * mo[at * MS + lane * (D / 32) + e] : 0.f;
+      for (int e = 0; e < D / 32; ++e) acc[e] += f == 0.f ? 0.f : f * mo[at * MS + lane * (D / 32) + e];
     }
-    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
     if (n_split <= 1) {
       T* orow = reinterpret_cast<T*>(a.out) + (row0 + r) * D + lane * (D / 32);
 #pragma unroll
@@ -441,12 +443,12 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
     } else if (a.cluster) {
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) rows_o[j * D + lane * (D / 32) + e] = acc[e] * inv;
-      if (lane == 0) rows_lse[j] = lt > 0.f ? mx + lg2(lt) : -INFINITY;
+      if (lane == 0) rows_lse[j] = lt == 0.f ? -INFINITY : mx + lg2(lt);
     } else {
       const long long at = (row0 + r) * a.max_splits + split;
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) a.part_o[at * D + lane * (D / 32) + e] = acc[e] * inv;
-      if (lane == 0) a.part_lse[at] = lt > 0.f ? mx + lg2(lt) : -INFINITY;
+      if (lane == 0) a.part_lse[at] = lt == 0.f ? -INFINITY : mx + lg2(lt);
     }
   }
   }
@@ -800,7 +802,7 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
     if (ok) {
       tc_fence_after();
       if (!row_ok) l = 0.f;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long row = ((long long)seq * a.Hkv + hkv) * a.rows + r;
       const long long at = row * a.max_splits + split;
 #pragma unroll
@@ -812,7 +814,7 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
         }
         // (a row without keys may hold o of nothing: select, do not multiply)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+        for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
         if (r >= a.rows) continue;
         if (n_split <= 1) {
           T* orow = reinterpret_cast<T*>(a.out) + row * D + c * 32;
@@ -832,7 +834,7 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
             *reinterpret_cast<uint4*>(po + v * 4) = make_uint4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
         }
       }
-      if (r < a.rows && n_split > 1) a.part_lse[at] = l > 0.f ? m + lg2(l) : -INFINITY;
+      if (r < a.rows && n_split > 1) a.part_lse[at] = l == 0.f ? -INFINITY : m + lg2(l);
     }
   }
   tc_fence_before();
@@ -864,28 +866,27 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ 
   float tot = 0.f, acc[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-  if (mx != -INFINITY) {
-    constexpr int B = 8;  // partials in flight
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const float wl = i0 + lane < n ? ex2(lse[i0 + lane] - mx) : 0.f;
-      for (int j0 = 0; j0 < min(32, n - i0); j0 += B) {
-        float x[B][D / 32];
+  constexpr int B = 8;  // partials in flight
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const float x0 = i0 + lane < n ? lse[i0 + lane] : -INFINITY;
+    const float wl = x0 == -INFINITY ? 0.f : ex2(x0 - mx);  // (all may be -inf, or NaN)
+    for (int j0 = 0; j0 < min(32, n - i0); j0 += B) {
+      float x[B][D / 32];
 #pragma unroll
-        for (int j = 0; j < B; ++j)
+      for (int j = 0; j < B; ++j)
 #pragma unroll
-          for (int e = 0; e < D / 32; ++e)
-            x[j][e] = i0 + j0 + j < n ? po[(long long)(i0 + j0 + j) * D + e] : 0.f;
+        for (int e = 0; e < D / 32; ++e)
+          x[j][e] = i0 + j0 + j < n ? po[(long long)(i0 + j0 + j) * D + e] : 0.f;
 #pragma unroll
-        for (int j = 0; j < B; ++j) {
-          const float w = __shfl_sync(0xffffffffu, wl, j0 + j);
-          tot += w;
+      for (int j = 0; j < B; ++j) {
+        const float w = __shfl_sync(0xffffffffu, wl, j0 + j);
+        tot += w;
 #pragma unroll
-          for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, x[j][e], acc[e]);
-        }
+        for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, x[j][e], acc[e]);
       }
     }
   }
-  const float inv = tot > 0.f ? 1.f / tot : 0.f;
+  const float inv = tot == 0.f ? 0.f : 1.f / tot;
   T* orow = reinterpret_cast<T*>(a.out) + prow * D + lane * (D / 32);
 #pragma unroll
   for (int e = 0; e < D / 32; e += 2)

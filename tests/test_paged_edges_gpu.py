@@ -1,0 +1,61 @@
+"""Window, tree and page operators at the edge of their contract."""
+
+import pytest
+import torch
+
+import attnax_b200 as ax
+from tests.test_paged_rows_gpu import make_cache, randn, random_tree
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+NAN = float("nan")
+
+
+# rows per kv head: 2, 20 (warp MMA); 48, 160, 320 (tcgen05).  Contexts in one split, in a cluster, in joined splits.
+@pytest.mark.parametrize("t,hq,hkv", [(1, 4, 2), (5, 4, 1), (12, 8, 2), (40, 4, 1), (40, 8, 1)])
+@pytest.mark.parametrize("n", [60, 900, 9000])
+@pytest.mark.parametrize("where", ["query", "key"])
+def test_nan_stays_nan(t, hq, hkv, n, where):
+    """A row whose scores hold NaN is NaN, as in the formula; the other sequence's rows are untouched."""
+    lens = [n, n]
+    cache = make_cache(t + n, lens, hkv, 128, 16, BF)
+    q, dk, dv = randn(1, 2, hq, t, 128), randn(2, 2, hkv, t, 128), randn(3, 2, hkv, t, 128)
+    par = random_tree(4, 2, t)
+    if where == "query":
+        q[0, 1, -1, 3] = NAN
+    else:  # the newest key of sequence 0, seen by its last row (window) and by every row (tree)
+        cache.key_pool[cache.block_table[0, (n - 1) // 16].long(), (n - 1) % 16, :, 5] = NAN
+    window = ax.paged_window_attention(q, cache, window_size=n, num_sinks=2)
+    tree = ax.paged_tree_attention(q, dk, dv, cache, par)
+    for got in (window, tree):
+        bad = got.isnan().any(-1)
+        assert bool((bad == got.isnan().all(-1)).all())
+        assert not bool(bad[1].any())
+    if where == "query":
+        assert bool(window[0, 1, -1].isnan().all()) and int(window.isnan().any(-1).sum()) == 1
+        assert bool(tree[0, 1, -1].isnan().all()) and int(tree.isnan().any(-1).sum()) == 1
+    else:
+        assert bool(window[0, :, -1].isnan().all()) and int(window.isnan().any(-1).sum()) == hq
+        assert bool(tree[0].isnan().all())
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_stays_nan_in_32_bits(d, masked):
+    """fp32 with sinks: a row with a NaN score is no row without keys (zeros, or the mean of V under a mask)."""
+    s, hq, hkv = 200, 4, 2
+    q, k, v, do = (randn(i, 1, h, s, d, dt=F32) for i, h in enumerate((hq, hkv, hkv, hq)))
+    q[0, 1, 70, 3] = NAN
+    k[0, 1, 150, 5] = NAN          # seen by rows 150..179 of heads 2 and 3
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    mask = torch.ones(1, 1, s, s, dtype=torch.bool, device=DEV) if masked else None
+    out = ax.flash_attention(q, k, v, score_mod=ax.sink_window_mod(30, 4), mask=mask)
+    dq, = torch.autograd.grad(out, q, do)
+    want = torch.zeros(1, hq, s, dtype=torch.bool, device=DEV)
+    want[0, 1, 70] = True
+    want[0, 2:, 150:180] = True
+    assert torch.equal(out.isnan().any(-1), want) and torch.equal(out.isnan().all(-1), want)
+    # dQ = dS K: where dS is 0 a NaN in K still makes the product NaN, so heads 2 and 3 may hold more
+    assert bool(dq.isnan().all(-1)[want].all())
+    assert torch.equal(dq.isnan().any(-1)[:, :2], want[:, :2])
