@@ -51,21 +51,23 @@ class PagedKVCache:
 def check_pools(cache: PagedKVCache):
     """Both pools alike: the kernels take their shape, type and device from ``key_pool``."""
     k, v = cache.key_pool, cache.value_pool
-    if k.dim() != 4:
-        raise ValueError(f"key_pool must be (num_blocks, block_size, num_kv_heads, head_dim), got {tuple(k.shape)}")
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError(f"value_pool {tuple(v.shape)} {v.dtype} != key_pool {tuple(k.shape)} {k.dtype}")
+    shape = k.shape
+    if len(shape) == 4 and v.shape == shape and v.dtype == k.dtype and v.device == k.device:
+        return
+    if len(shape) != 4:
+        raise ValueError(f"key_pool must be (num_blocks, block_size, num_kv_heads, head_dim), got {tuple(shape)}")
     if v.device != k.device:
         raise RuntimeError(f"value_pool is on {v.device}, key_pool on {k.device}")
+    raise ValueError(f"value_pool {tuple(v.shape)} {v.dtype} != key_pool {tuple(shape)} {k.dtype}")
 
 
 def check_rows(block_table: torch.Tensor, seq_lengths: torch.Tensor):
     """One table row and one length per sequence."""
-    if block_table.dim() != 2:
-        raise ValueError(f"block_table must be (num_seqs, max_blocks_per_seq), got {tuple(block_table.shape)}")
-    if seq_lengths.dim() != 1 or seq_lengths.shape[0] != block_table.shape[0]:
-        raise ValueError(f"seq_lengths {tuple(seq_lengths.shape)} do not match the {block_table.shape[0]} rows of "
-                         "block_table")
+    shape = block_table.shape
+    if len(shape) != 2:
+        raise ValueError(f"block_table must be (num_seqs, max_blocks_per_seq), got {tuple(shape)}")
+    if seq_lengths.shape != shape[:1]:
+        raise ValueError(f"seq_lengths {tuple(seq_lengths.shape)} do not match the {shape[0]} rows of block_table")
 
 
 def init_paged_kv_cache(*, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,

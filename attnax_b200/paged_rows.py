@@ -46,9 +46,11 @@ def _check_query(query, cache: PagedKVCache):
 def check_tables(cache: PagedKVCache):
     """The kernels read int32 tables on the pools' device, a row and a length per sequence, and two pools alike."""
     check_pools(cache)
-    check_rows(cache.block_table, cache.seq_lengths)
-    dev = cache.key_pool.device
-    for name, x in (("block_table", cache.block_table), ("seq_lengths", cache.seq_lengths)):
+    table, lengths, dev = cache.block_table, cache.seq_lengths, cache.key_pool.device
+    check_rows(table, lengths)
+    if table.dtype is torch.int32 and lengths.dtype is torch.int32 and table.device == dev and lengths.device == dev:
+        return
+    for name, x in (("block_table", table), ("seq_lengths", lengths)):
         if x.dtype != torch.int32:
             raise ValueError(f"{name} must be int32, got {x.dtype}")
         if x.device != dev:
