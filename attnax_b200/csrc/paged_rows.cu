@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kMmaThreads, 3)
   }
   if (TREE && v0 + n > sp.n_ctx) {
     // Lane x holds drafted token x: its path doubles in length with each step.
-    int p = lane < a.T ? parent_of(a.parents + (long long)seq * a.T, lane) : -1;
+    int p = lane < sp.drafts ? parent_of(a.parents + (long long)seq * a.T, lane) : -1;  // (padding may hold anything)
     uint32_t path = 1u << lane;
 #pragma unroll
     for (int x = 0; x < 5; ++x) {
@@ -542,8 +542,8 @@ __global__ void __launch_bounds__(128 * (NT + 1), NT == 1 ? 2 : 1)
   auto v_empty = [&](int s) { return bar0 + 8u * (2 + 2 * NT + 3 * S + s); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEMPTR);
   int16_t* parents = reinterpret_cast<int16_t*>(smem + C::OFF_PARENTS);
-  if (TREE && v0 + n > sp.n_ctx)  // this split holds drafted tokens
-    for (int x = threadIdx.x; x < a.T; x += C::THREADS)
+  if (TREE && v0 + n > sp.n_ctx)  // this split holds drafted tokens (what the padding behind them holds is not read)
+    for (int x = threadIdx.x; x < sp.drafts; x += C::THREADS)
       parents[x] = (int16_t)max(parent_of(a.parents + (long long)seq * a.T, x), -1);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);

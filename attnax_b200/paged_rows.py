@@ -201,7 +201,8 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
     continues the context itself.  Row ``t`` sees the whole context
     (``seq_lengths[b]`` tokens), itself and its ancestors.  With
     ``tree_lengths (B,)`` the tokens at or past a sequence's length are
-    padding: nothing sees them and their rows are zeros.  A parent that is not
+    padding: nothing sees them, their rows are zeros and their parents are not
+    looked at.  A parent that is not
     in front of its token counts as negative and is noted in
     ``_lib.device_status()`` (``NOTICE_TREE_ORDER``).  T is at most 1024.
 

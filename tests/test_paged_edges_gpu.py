@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import attnax_b200 as ax
-from tests.test_paged_rows_gpu import make_cache, randn, random_tree
+from attnax_b200 import _lib
+from tests.test_paged_rows_gpu import check_tree, make_cache, randn, random_tree
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -59,3 +60,18 @@ def test_nan_stays_nan_in_32_bits(d, masked):
     # dQ = dS K: where dS is 0 a NaN in K still makes the product NaN, so heads 2 and 3 may hold more
     assert bool(dq.isnan().all(-1)[want].all())
     assert torch.equal(dq.isnan().any(-1)[:, :2], want[:, :2])
+
+
+@pytest.mark.parametrize("t", [6, 20, 70])
+def test_padding_parents_are_not_looked_at(t):
+    """What stands behind a tree's length is padding: any parents, no notice."""
+    lens, tl = [100, 40], [t // 2, t]
+    cache = make_cache(2, lens, 1, 128, 16, BF)
+    q, dk, dv = randn(1, 2, 4, t, 128), randn(2, 2, 1, t, 128), randn(3, 2, 1, t, 128)
+    par = random_tree(5, 2, t)
+    wild = par.clone()
+    wild[0, tl[0]:] = torch.arange(t - tl[0]).to(torch.int32) + 1000
+    assert _lib.device_status() == 0
+    got = ax.paged_tree_attention(q, dk, dv, cache, wild, tree_lengths=tl)
+    assert _lib.device_status() == 0
+    check_tree(cache, lens, q, dk, dv, par, tl, got)
