@@ -57,11 +57,23 @@ def check_tables(cache: PagedKVCache):
             raise RuntimeError(f"{name} must be on the pools' device")
 
 
+def narrow(x: torch.Tensor, device) -> torch.Tensor:
+    """Integers as contiguous int32 on the device; what 32 bits do not hold becomes their end of the range,
+    which no index reaches."""
+    if x.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
+            if x.numel():
+                raise ValueError(f"indices and lengths must be integers, got {x.dtype}")
+        else:
+            x = x.clamp(-2**31, 2**31 - 1)
+    return x.to(device=device, dtype=torch.int32).contiguous()
+
+
 def on_device(x, device) -> torch.Tensor:
     """int32, contiguous, on the device."""
     if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == device:
         return x.contiguous()
-    return torch.as_tensor(x).to(device=device, dtype=torch.int32).contiguous()
+    return narrow(torch.as_tensor(x), device)
 
 
 def _need_cuda(query, cache: PagedKVCache):

@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .paged import PagedKVCache
-from .paged_rows import cast, check_tables, on_device
+from .paged_rows import cast, check_tables, narrow, on_device
 
 
 _Strides = C.c_int64 * 3
@@ -58,7 +58,7 @@ def _indices(x, device, limit: int, what: str, distinct: bool = False) -> torch.
             raise ValueError(f"{what} has entry {int(t[bad][0])}, outside [0, {limit})")
         if distinct and t.unique().numel() != t.numel():
             raise ValueError(f"{what} names an index twice")
-    return t.to(device=device, dtype=torch.int32).contiguous()
+    return narrow(t, device)
 
 
 def copy_blocks(cache: PagedKVCache, src_blocks, dst_blocks) -> PagedKVCache:

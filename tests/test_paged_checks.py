@@ -72,3 +72,29 @@ def test_decode_rows():
                   (Q, {"block_table": c.block_table[:2]}), (Q, {"block_table": c.block_table[0]})):
         with pytest.raises(ValueError):
             paged_decode_raw(q, c, **kw)
+
+
+def test_wide_integers_are_not_cut_to_their_low_half():
+    from attnax_b200.paged_rows import on_device
+
+    dev = torch.device("cpu")
+    far = [1 << 32, -(1 << 32), (1 << 40) + 5, 7, -1, 2**31 - 1, -2**31]
+    want = [2**31 - 1, -2**31, 2**31 - 1, 7, -1, 2**31 - 1, -2**31]
+    for x in (far, torch.tensor(far)):
+        got = on_device(x, dev)
+        assert got.dtype == torch.int32 and got.tolist() == want
+    assert on_device(torch.tensor([3, 250], dtype=torch.uint8), dev).tolist() == [3, 250]
+    assert on_device([], dev).tolist() == []
+
+
+@pytest.mark.parametrize("wrong", [torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.bool)])
+def test_indices_must_be_integers(wrong):
+    c = cpu_cache()
+    with pytest.raises(ValueError):
+        ax.paged_tree_attention(Q, DRAFT, DRAFT, c, wrong)
+    with pytest.raises(ValueError):
+        ax.paged_tree_attention(Q, DRAFT, DRAFT, c, PAR, tree_lengths=wrong[:, 0])
+    with pytest.raises(ValueError):
+        ax.append_accepted(c, DRAFT, DRAFT, wrong, [1] * 3)
+    with pytest.raises(ValueError):
+        ax.append_accepted(c, DRAFT, DRAFT, [[0]] * 3, wrong[:, 0])

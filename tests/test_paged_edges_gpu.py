@@ -75,3 +75,29 @@ def test_padding_parents_are_not_looked_at(t):
     got = ax.paged_tree_attention(q, dk, dv, cache, wild, tree_lengths=tl)
     assert _lib.device_status() == 0
     check_tree(cache, lens, q, dk, dv, par, tl, got)
+
+
+def test_indices_wider_than_32_bits_on_the_device():
+    """64-bit indices on the device that 32 bits do not hold are out of range, not their low half."""
+    cache = make_cache(1, [40, 20], 1, 64, 16, BF)
+    kp, vp, table = cache.key_pool.clone(), cache.value_pool.clone(), cache.block_table.clone()
+    far = (1 << 32) + 1
+    mk = lambda *x: torch.tensor(x, dtype=torch.int64, device=DEV)  # noqa: E731
+    assert _lib.device_status() == 0
+    ax.copy_blocks(cache, mk(0, far), mk(far, 2))
+    assert _lib.device_status() == _lib.NOTICE_PAGE_LIST
+    assert torch.equal(cache.key_pool.nan_to_num(7), kp.nan_to_num(7))
+    assert torch.equal(cache.value_pool.nan_to_num(7), vp.nan_to_num(7))
+    out, freed, count = ax.free_sequences(cache, mk(far))
+    assert _lib.device_status() == _lib.NOTICE_PAGE_LIST
+    assert torch.equal(out.block_table, table) and int(count) == 0
+    # parents and accepted drafts from the host
+    t = 4
+    q, dk, dv = randn(1, 2, 2, t, 64), randn(2, 2, 1, t, 64), randn(3, 2, 1, t, 64)
+    par = torch.tensor([[-1, 1 << 32, -(1 << 32), 2], [-1, 0, 0, 0]])
+    good = torch.tensor([[-1, -1, -1, 2], [-1, 0, 0, 0]], dtype=torch.int32)
+    got = ax.paged_tree_attention(q, dk, dv, cache, par)
+    assert _lib.device_status() == _lib.NOTICE_TREE_ORDER
+    check_tree(cache, [40, 20], q, dk, dv, good, [t, t], got)
+    with pytest.raises(ValueError):
+        ax.append_accepted(cache, dk, dv, [[1 << 32], [0]], [1, 1])
