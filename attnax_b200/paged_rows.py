@@ -10,8 +10,9 @@ context (attnax/kernels/paged.py:17-84).
 
 bf16/f16 caches with head_dim 64 or 128 and a block size that is a multiple
 of 16 take the fused kernels (one launch, and one that joins the splits);
-other caches gather each sequence and run the flash kernel on it, with one
-host sync.  Both kernels run on the current stream of the cache's device.
+other caches gather each sequence and run the flash kernel on it, waiting for
+the lengths (``max_context`` is not used there).  Both kernels run on the
+current stream of the cache's device.
 Like the paged decode they are for inference: the fused kernels have no backward,
 and what they return carries no gradient.
 """
@@ -151,6 +152,7 @@ def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_
     if n == 0 or t == 0:
         return torch.zeros_like(query)
     if not _fused(cache):
+        _bound(cache, None)
         return _window_by_sequence(query, cache, int(window_size), int(num_sinks))
     lib = _lib.load()
     p, out, keep = _params(query, cache, _bound(cache, max_context))
@@ -242,6 +244,7 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
     if n == 0 or t == 0:
         return torch.zeros_like(query)
     if not _fused(cache):
+        _bound(cache, None)
         return _tree_by_sequence(query, draft_keys, draft_values, cache, parents, tree_lengths)
     lib = _lib.load()
     p, out, keep = _params(query, cache, _bound(cache, max_context))

@@ -101,3 +101,15 @@ def test_indices_wider_than_32_bits_on_the_device():
     check_tree(cache, [40, 20], q, dk, dv, good, [t, t], got)
     with pytest.raises(ValueError):
         ax.append_accepted(cache, dk, dv, [[1 << 32], [0]], [1, 1])
+
+
+def test_overlong_sequences_are_refused_on_other_caches():
+    """A length past its table row raises for the caches that are gathered, as for the others."""
+    cache = make_cache(5, [45, 30], 2, 32, 4, F32)
+    wrong = ax.PagedKVCache(cache.key_pool, cache.value_pool, cache.block_table,
+                            torch.tensor([45 + 4, 30], dtype=torch.int32, device=DEV))
+    q = randn(6, 2, 4, 2, 32, dt=F32)
+    with pytest.raises(ValueError):
+        ax.paged_window_attention(q, wrong, window_size=21, num_sinks=2)
+    with pytest.raises(ValueError):
+        ax.paged_tree_attention(q, q[:, :2], q[:, :2], wrong, [[-1, 0]] * 2)
