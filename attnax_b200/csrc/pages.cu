@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(256) fork_kernel(Pool p, ForkArgs a) {
   twice = __syncthreads_or(twice);
   const int k = sum;
   const bool takes = takes_page(a, i);
+  // (a fork that is skipped below has taken its id all the same: the ids go by the list alone)
   if (i == a.n - 1 && threadIdx.x == 0) *a.used = min(k + (takes ? 1 : 0), a.num_free);
   const int s = a.src[i], d = a.dst[i];
   if (!in_range(s, a.num_seqs) || !in_range(d, a.num_seqs) || twice) {
@@ -142,7 +143,9 @@ __global__ void __launch_bounds__(256) fork_kernel(Pool p, ForkArgs a) {
   if (takes) {
     tail = row[cols - 1];
     fresh = k < a.num_free ? a.free_ids[k] : -1;
-    if (!in_range(fresh, p.num_blocks) || !in_range(tail, p.num_blocks)) {
+    bool taken = false;  // an id listed twice is the first one's
+    for (int j = threadIdx.x; j < min(k, a.num_free); j += blockDim.x) taken = taken || a.free_ids[j] == fresh;
+    if (__syncthreads_or(taken) || !in_range(fresh, p.num_blocks) || !in_range(tail, p.num_blocks)) {
       // no page for the copy: the row keeps its full pages and their tokens
       if (threadIdx.x == 0) skip_notice();
       fresh = -1;

@@ -93,8 +93,12 @@ def fork_sequences(cache: PagedKVCache, src_sequences, dst_sequences, free_block
     int32 on the device) is the number of ids taken from the front of the
     list.  Pages that only a replaced row held are not freed (call
     ``free_sequences`` first).  With fewer ids than forks this waits for the
-    lengths and raises ``ValueError`` if they are too few; ids on the device
-    that are no pages leave the copy with its full pages and a note.
+    lengths and raises ``ValueError`` if they are too few.
+
+    On the device: ids that are no pages, or are listed again, leave the copy
+    with its full pages and a note; of forks onto one row the first wins, the
+    others are skipped and noted.  ``used`` counts the ids of such forks too
+    (compare the new table with the list to have those pages back).
     """
     dev = cache.key_pool.device
     n_seq = cache.block_table.shape[0]

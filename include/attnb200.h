@@ -224,7 +224,9 @@ int attn_paged_copy(const attn_paged_cache_t* c, const int32_t* src, const int32
 /* Rows dst[i] become copies of rows src[i]: full pages are shared, a last page
  * that is not full is copied to a page of free_ids (in order of i), and
  * table_out / lengths_out hold the new table (not aliasing the old one).
- * *used gets the number of free_ids taken. */
+ * *used gets the number of free_ids taken, those of skipped forks (a row
+ * replaced twice: the first wins; an id out of range or listed again: the row
+ * keeps its full pages) included. */
 int attn_paged_fork(const attn_paged_cache_t* c, const int32_t* src, const int32_t* dst, int32_t n,
                     const int32_t* free_ids, int32_t num_free, int32_t* table_out, int32_t* lengths_out,
                     int32_t* used, void* stream);

@@ -113,3 +113,23 @@ def test_overlong_sequences_are_refused_on_other_caches():
         ax.paged_window_attention(q, wrong, window_size=21, num_sinks=2)
     with pytest.raises(ValueError):
         ax.paged_tree_attention(q, q[:, :2], q[:, :2], wrong, [[-1, 0]] * 2)
+
+
+def test_fork_with_an_id_listed_twice_on_the_device():
+    """The first fork has the page; the second keeps its full pages, as with an id that is no page."""
+    lens, bs = [37, 20, 5, 0, 0, 0], 16
+    g = torch.Generator().manual_seed(1)
+    pools = [torch.randn(20, bs, 1, 64, generator=g).to(BF).to(DEV) for _ in range(2)]
+    table = torch.tensor([[0, 1, 2], [3, 4, -1], [5, -1, -1], [-1] * 3, [-1] * 3, [-1] * 3], dtype=torch.int32)
+    cache = ax.PagedKVCache(*pools, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    k, v = cache.key_pool.clone(), cache.value_pool.clone()
+    mk = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    assert _lib.device_status() == 0
+    out, used = ax.fork_sequences(cache, mk([0, 1, 2]), mk([3, 4, 5]), mk([9, 9, 10]))
+    assert _lib.device_status() == _lib.NOTICE_PAGE_LIST
+    assert int(used) == 3
+    assert out.block_table[3:].tolist() == [[0, 1, 9], [3, -1, -1], [10, -1, -1]]
+    assert out.seq_lengths.tolist() == [37, 20, 5, 37, 16, 5]
+    for a, b in ((2, 9), (5, 10)):
+        k[b], v[b] = k[a], v[a]
+    assert torch.equal(cache.key_pool, k) and torch.equal(cache.value_pool, v)
