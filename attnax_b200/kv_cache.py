@@ -75,12 +75,19 @@ _tables: dict = {}
 
 
 def _identity_table(nseq: int, nblocks: int, device) -> torch.Tensor:
-    """Block table ``[s, i] = s * nblocks + i`` (cached per shape and device)."""
+    """Block table ``[s, i] = s * nblocks + i``, kept per shape and device.
+
+    Inside a capture it belongs to the graph (nothing writes it before a
+    replay), so it is not kept; outside, it is complete before any other
+    stream can be given it.
+    """
     key = (nseq, nblocks, str(device))
     t = _tables.get(key)
     if t is None:
         t = torch.arange(nseq * nblocks, dtype=torch.int32, device=device).view(nseq, nblocks)
-        _tables[key] = t
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()
+            _tables[key] = t
     return t
 
 
