@@ -61,6 +61,19 @@ def check_pools(cache: PagedKVCache):
     raise ValueError(f"value_pool {tuple(v.shape)} {v.dtype} != key_pool {tuple(shape)} {k.dtype}")
 
 
+def pools_contiguous(cache: PagedKVCache) -> bool:
+    """Whether the kernels can address the pools; others are read through torch's indexing."""
+    return cache.key_pool.is_contiguous() and cache.value_pool.is_contiguous()
+
+
+def gather_positions(cache: PagedKVCache, sequence_idx: int, pos: torch.Tensor):
+    """``(n, Hkv, D)`` keys/values at positions ``pos`` of one sequence, from pools of any strides."""
+    nb, bs = cache.num_blocks, cache.block_size
+    page = cache.block_table[sequence_idx].long()[(pos // bs).clamp(max=cache.block_table.shape[1] - 1)]
+    page = torch.where(page < 0, page + nb, page).clamp(0, nb - 1)
+    return cache.key_pool[page, pos % bs], cache.value_pool[page, pos % bs]
+
+
 def check_rows(block_table: torch.Tensor, seq_lengths: torch.Tensor):
     """One table row and one length per sequence."""
     shape = block_table.shape
@@ -104,6 +117,8 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
         raise ValueError(f"keys_new shape {tuple(keys_new.shape)} != values_new shape "
                          f"{tuple(values_new.shape)}")
     check_pools(cache)
+    if not pools_contiguous(cache):
+        raise ValueError("append_kv writes the pools in place and needs them contiguous")
     lib = _lib.load()
     chunk = int(keys_new.shape[0])
     start = int(cache.seq_lengths[sequence_idx])
@@ -132,8 +147,13 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
 def gather_kv(cache: PagedKVCache, sequence_idx: int):
     """Contiguous ``(seq_len, Hkv, D)`` keys/values of one sequence (paged_cache.py:201-231)."""
     check_pools(cache)
-    lib = _lib.load()
     seq_len = int(cache.seq_lengths[sequence_idx])
+    if not pools_contiguous(cache):
+        if seq_len > cache.block_table.shape[1] * cache.block_size:
+            raise ValueError(f"sequence length {seq_len} exceeds its {cache.block_table.shape[1]} table entries")
+        k, v = gather_positions(cache, sequence_idx, torch.arange(seq_len, device=cache.key_pool.device))
+        return k.contiguous(), v.contiguous(), seq_len
+    lib = _lib.load()
     shape = (seq_len, cache.num_kv_heads, cache.head_dim)
     k = torch.empty(shape, dtype=cache.key_pool.dtype, device=cache.key_pool.device)
     v = torch.empty_like(k)
@@ -159,6 +179,8 @@ def paged_decode_raw(query, cache: PagedKVCache, *, block_table=None, seq_length
     ``NOTICE_TABLE_OVERRUN``) instead of raising.
     """
     check_pools(cache)
+    if not pools_contiguous(cache):
+        raise ValueError("paged_decode_raw reads the pools where they are and needs them contiguous")
     lib = _lib.load()
     bt = cache.block_table if block_table is None else block_table
     sl = cache.seq_lengths if seq_lengths is None else seq_lengths
@@ -209,7 +231,7 @@ def _fast_decode_ok(query, cache: PagedKVCache) -> bool:
     bs = cache.block_size
     return (cache.head_dim == 128 and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
             and ((bs % 16 == 0 and bs <= 256) or bs <= 48)
-            and query.dtype in (torch.bfloat16, torch.float16, torch.float32))
+            and query.dtype in (torch.bfloat16, torch.float16, torch.float32) and pools_contiguous(cache))
 
 
 def paged_attention(query, cache: PagedKVCache, sequence_idx: int, *, mask=None, score_mod=None,

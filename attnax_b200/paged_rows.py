@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .flash import attention, softmax_scale
-from .paged import PagedKVCache, check_pools, check_rows, gather_kv
+from .paged import PagedKVCache, check_pools, check_rows, gather_kv, gather_positions, pools_contiguous
 
 
 def _check_query(query, cache: PagedKVCache):
@@ -84,7 +84,7 @@ def _need_cuda(query, cache: PagedKVCache):
 
 def _fused(cache: PagedKVCache) -> bool:
     return (cache.head_dim in (64, 128) and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
-            and cache.block_size % 16 == 0 and cache.key_pool.is_contiguous() and cache.value_pool.is_contiguous())
+            and cache.block_size % 16 == 0 and pools_contiguous(cache))
 
 
 def _bound(cache: PagedKVCache, max_context):
@@ -188,11 +188,7 @@ def gather_window(cache: PagedKVCache, sequence_idx: int, rows: int, window: int
     dev = cache.key_pool.device
     lo = max(0, length - rows - window + 1)
     pos = torch.cat([torch.arange(min(sinks, lo), device=dev), torch.arange(lo, length, device=dev)])
-    nb, bs = cache.num_blocks, cache.block_size
-    page = cache.block_table[sequence_idx].long()[(pos // bs).clamp(max=cache.block_table.shape[1] - 1)]
-    page = torch.where(page < 0, page + nb, page).clamp(0, nb - 1)
-    k = cache.key_pool[page, pos % bs].permute(1, 0, 2)[None].contiguous()
-    v = cache.value_pool[page, pos % bs].permute(1, 0, 2)[None].contiguous()
+    k, v = (x.permute(1, 0, 2)[None].contiguous() for x in gather_positions(cache, sequence_idx, pos))
     return k, v, pos
 
 

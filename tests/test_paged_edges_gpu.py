@@ -5,7 +5,8 @@ import torch
 
 import attnax_b200 as ax
 from attnax_b200 import _lib
-from tests.test_paged_rows_gpu import check_tree, make_cache, randn, random_tree
+from tests._plain64 import assert_within, attention64
+from tests.test_paged_rows_gpu import check_tree, check_window, history, make_cache, randn, random_tree
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -133,3 +134,52 @@ def test_fork_with_an_id_listed_twice_on_the_device():
     for a, b in ((2, 9), (5, 10)):
         k[b], v[b] = k[a], v[a]
     assert torch.equal(cache.key_pool, k) and torch.equal(cache.value_pool, v)
+
+
+def _odd_pools(kind, nb, bs, hkv, d, dt):
+    """Pools that are not contiguous, or contiguous at an odd address."""
+    g = torch.Generator(device=DEV).manual_seed(nb)
+    mk = lambda *s: torch.randn(*s, generator=g, device=DEV).to(dt)  # noqa: E731
+    if kind == "interleaved":          # K and V of a page side by side
+        both = mk(nb, 2, bs, hkv, d)
+        return both[:, 0], both[:, 1]
+    if kind == "head major":
+        return tuple(mk(nb, hkv, bs, d).transpose(1, 2) for _ in range(2))
+    return tuple(mk(nb * bs * hkv * d + 1)[1:].view(nb, bs, hkv, d) for _ in range(2))
+
+
+@pytest.mark.parametrize("kind", ["interleaved", "head major"])
+@pytest.mark.parametrize("d,bs,dt", [(128, 16, BF), (64, 32, HF), (32, 4, F32)])
+def test_pools_of_other_layouts(kind, d, bs, dt):
+    """Windows, trees, gathers and decodes read such pools where their tokens are."""
+    lens, hq, hkv, t = [45, 0, 70], 4, 2, 3
+    kp, vp = _odd_pools(kind, 30, bs, hkv, d, dt)
+    table = torch.randperm(30, generator=torch.Generator().manual_seed(1)).to(torch.int32)[:3 * (30 // 3)].view(3, -1)
+    table = torch.cat([table, table[:, :10].flip(0)], 1)[:, :18]   # (rows may share pages)
+    cache = ax.PagedKVCache(kp, vp, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    q = randn(1, 3, hq, t, d, dt=dt)
+    check_window(cache, lens, q, ax.paged_window_attention(q, cache, window_size=21, num_sinks=2), 21, 2)
+    dk, dv, par = randn(2, 3, hkv, t, d, dt=dt), randn(3, 3, hkv, t, d, dt=dt), random_tree(4, 3, t)
+    check_tree(cache, lens, q, dk, dv, par, [t] * 3, ax.paged_tree_attention(q, dk, dv, cache, par))
+    full = ax.paged_attention_batched(q, cache)
+    for i, n in enumerate(lens):
+        k, v = history(cache, i, n)
+        keys, values, m = ax.gather_kv(cache, i)
+        assert m == n and torch.equal(keys, k[0].transpose(0, 1)) and torch.equal(values, v[0].transpose(0, 1))
+        if n == 0:
+            assert float(full[i].abs().max()) == 0.0
+            continue
+        want, bound = attention64(q[i:i + 1], k, v, torch.ones(t, n, dtype=torch.bool, device=DEV))
+        assert_within(full[i:i + 1], want, bound, "decode")
+
+
+@pytest.mark.parametrize("kind", ["interleaved", "head major"])
+def test_appending_needs_contiguous_pools(kind):
+    """What is written in place is not written to where it does not belong."""
+    kp, vp = _odd_pools(kind, 6, 16, 2, 64, BF)
+    cache = ax.PagedKVCache(kp, vp, torch.tensor([[0, 1]], dtype=torch.int32, device=DEV),
+                            torch.tensor([3], dtype=torch.int32, device=DEV))
+    before = kp.clone()
+    with pytest.raises(ValueError, match="contiguous"):
+        ax.append_kv(cache, 0, randn(1, 2, 2, 64), randn(2, 2, 2, 64))
+    assert torch.equal(kp, before)
