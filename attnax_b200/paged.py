@@ -66,6 +66,11 @@ def pools_contiguous(cache: PagedKVCache) -> bool:
     return cache.key_pool.is_contiguous() and cache.value_pool.is_contiguous()
 
 
+def pools_by_tma(cache: PagedKVCache) -> bool:
+    """Whether TMA can fetch pages: contiguous pools that start on 16 bytes."""
+    return pools_contiguous(cache) and (cache.key_pool.data_ptr() | cache.value_pool.data_ptr()) % 16 == 0
+
+
 def gather_positions(cache: PagedKVCache, sequence_idx: int, pos: torch.Tensor):
     """``(n, Hkv, D)`` keys/values at positions ``pos`` of one sequence, from pools of any strides."""
     nb, bs = cache.num_blocks, cache.block_size
@@ -231,7 +236,7 @@ def _fast_decode_ok(query, cache: PagedKVCache) -> bool:
     bs = cache.block_size
     return (cache.head_dim == 128 and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
             and ((bs % 16 == 0 and bs <= 256) or bs <= 48)
-            and query.dtype in (torch.bfloat16, torch.float16, torch.float32) and pools_contiguous(cache))
+            and query.dtype in (torch.bfloat16, torch.float16, torch.float32) and pools_by_tma(cache))
 
 
 def paged_attention(query, cache: PagedKVCache, sequence_idx: int, *, mask=None, score_mod=None,

@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .flash import attention, softmax_scale
-from .paged import PagedKVCache, check_pools, check_rows, gather_kv, gather_positions, pools_contiguous
+from .paged import PagedKVCache, check_pools, check_rows, gather_kv, gather_positions, pools_by_tma
 
 
 def _check_query(query, cache: PagedKVCache):
@@ -84,7 +84,7 @@ def _need_cuda(query, cache: PagedKVCache):
 
 def _fused(cache: PagedKVCache) -> bool:
     return (cache.head_dim in (64, 128) and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
-            and cache.block_size % 16 == 0 and pools_contiguous(cache))
+            and cache.block_size % 16 == 0 and pools_by_tma(cache))
 
 
 def _bound(cache: PagedKVCache, max_context):

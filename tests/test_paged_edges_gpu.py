@@ -148,7 +148,7 @@ def _odd_pools(kind, nb, bs, hkv, d, dt):
     return tuple(mk(nb * bs * hkv * d + 1)[1:].view(nb, bs, hkv, d) for _ in range(2))
 
 
-@pytest.mark.parametrize("kind", ["interleaved", "head major"])
+@pytest.mark.parametrize("kind", ["interleaved", "head major", "odd address"])
 @pytest.mark.parametrize("d,bs,dt", [(128, 16, BF), (64, 32, HF), (32, 4, F32)])
 def test_pools_of_other_layouts(kind, d, bs, dt):
     """Windows, trees, gathers and decodes read such pools where their tokens are."""
@@ -183,3 +183,14 @@ def test_appending_needs_contiguous_pools(kind):
     with pytest.raises(ValueError, match="contiguous"):
         ax.append_kv(cache, 0, randn(1, 2, 2, 64), randn(2, 2, 2, 64))
     assert torch.equal(kp, before)
+
+
+def test_appending_at_an_odd_address():
+    kp, vp = _odd_pools("odd address", 6, 16, 2, 64, BF)
+    cache = ax.PagedKVCache(kp, vp, torch.tensor([[4, 1]], dtype=torch.int32, device=DEV),
+                            torch.tensor([3], dtype=torch.int32, device=DEV))
+    k, v = randn(1, 20, 2, 64), randn(2, 20, 2, 64)
+    want = kp.clone()
+    want[4, 3:], want[1, :7] = k[:13], k[13:]
+    out = ax.append_kv(cache, 0, k, v)
+    assert torch.equal(out.key_pool, want) and out.seq_lengths.tolist() == [23]
