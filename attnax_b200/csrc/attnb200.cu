@@ -771,6 +771,8 @@ int attn_bwd(const attn_bwd_params_t* p, void* stream) {
   if (!tc && !simt_dim_ok(p->head_dim)) return ATTN_ERR_UNSUPPORTED;
   if (p->out_rest && (!tc || reinterpret_cast<uintptr_t>(p->out_rest) % 16)) return ATTN_ERR_INVALID;
   const size_t need = attn_bwd_workspace_size(p);
+  // (these kernels move 16 bytes at a time there)
+  if ((tc || tiled_bwd_ok(p)) && reinterpret_cast<uintptr_t>(p->workspace) % 16) return ATTN_ERR_INVALID;
   if (!p->workspace || p->workspace_bytes < need) return ATTN_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const BwdWorkspace wl = bwd_workspace_layout(p);

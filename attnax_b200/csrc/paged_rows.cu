@@ -1044,6 +1044,7 @@ static int launch_rows(const Plan& w, const Maps& t, const Args& a, cudaStream_t
 static int run(const attn_paged_params_t* p, const attn_paged_tree_t* tree, int64_t window, int64_t sinks,
                cudaStream_t st) {
   const Plan w = make_plan(p, tree != nullptr, window, sinks);
+  if (w.total > 0 && reinterpret_cast<uintptr_t>(p->workspace) % 16) return ATTN_ERR_INVALID;  // (float4 partials)
   if (w.total > 0 && (!p->workspace || p->workspace_bytes < w.total)) return ATTN_ERR_WORKSPACE;
   if (w.max_splits > 65535) return ATTN_ERR_UNSUPPORTED;
   Maps t;

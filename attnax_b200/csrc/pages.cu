@@ -561,6 +561,7 @@ static int free_pages(const attn_paged_cache_t* c, FreeArgs a, void* workspace, 
     return launch_status();
   }
   const size_t need = 2 * map_bytes(c);
+  if (addr(workspace) % 4) return ATTN_ERR_INVALID;
   if (!workspace || bytes < need) return ATTN_ERR_WORKSPACE;
   if (cudaMemsetAsync(workspace, 0, need, st) != cudaSuccess) return ATTN_ERR_CUDA;
   a.live = reinterpret_cast<uint32_t*>(workspace);
@@ -646,6 +647,7 @@ size_t attn_paged_compact_workspace_size(const attn_paged_cache_t* c) {
 int attn_paged_compact(const attn_paged_cache_t* c, int32_t* table_out, int32_t* num_live, void* workspace,
                        size_t workspace_bytes, void* stream) {
   if (!pages::cache_ok(c, true, true) || !table_out || !num_live) return ATTN_ERR_INVALID;
+  if (pages::addr(workspace) % 4) return ATTN_ERR_INVALID;
   if (!workspace || workspace_bytes < attn_paged_compact_workspace_size(c)) return ATTN_ERR_WORKSPACE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   char* ws = reinterpret_cast<char*>(workspace);

@@ -4,7 +4,8 @@
  * Plain C: device pointers, element strides, sizes, and CUDA streams passed
  * as `void*` (a `cudaStream_t`).  Every entry point returns an attn_status_t
  * (0 = success) and never allocates device memory: work buffers come from
- * the caller through `workspace`, sized by the matching *_workspace_size().
+ * the caller through `workspace`, sized by the matching *_workspace_size()
+ * and starting on 16 bytes.
  * Tensors use the reference's (batch, heads, seq, head_dim) layout with a
  * unit stride on head_dim; the other strides are free but must be multiples
  * of 16 bytes for the tensor-core paths.

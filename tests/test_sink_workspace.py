@@ -35,3 +35,37 @@ def test_sinks_take_a_bounded_workspace(b, hq, hkv, s, d, window):
         last = extra
     if b * hkv * -(-s // 128) >= 4 * 148 and s > 8192:
         assert last == 0    # every key a sink: causal attention, and no partials
+
+
+def test_c_entries_refuse_workspaces_off_their_alignment():
+    """Before anything is launched (and before their size is looked at)."""
+    lib = _lib.load()
+    p = _lib.PagedParams()
+    p.dtype, p.num_seqs, p.num_heads_q, p.num_heads_kv, p.head_dim, p.seq_q = _lib.ATTN_BF16, 2, 4, 2, 128, 1
+    p.num_blocks, p.block_size, p.max_blocks_per_seq, p.max_context = 8, 16, 4096, 65536
+    p.q = p.key_pool = p.value_pool = p.block_table = p.seq_lengths = p.out = 16    # never followed
+    t = _lib.PagedTree()
+    t.draft_keys = t.draft_values = t.parents = 16
+    for at, status in ((24, _lib.ATTN_ERR_INVALID), (32, _lib.ATTN_ERR_WORKSPACE)):
+        p.workspace, p.workspace_bytes = at, 64
+        assert lib.attn_paged_window_workspace_size(C.byref(p), 1 << 20, 0) > 64
+        assert lib.attn_paged_window(C.byref(p), 1 << 20, 0, None) == status
+        assert lib.attn_paged_tree(C.byref(p), C.byref(t), None) == status
+    for dtype, d in ((_lib.ATTN_BF16, 128), (_lib.ATTN_F16, 64), (_lib.ATTN_F32, 128)):
+        b = _lib.BwdParams()
+        b.dtype, b.batch, b.num_heads_q, b.num_heads_kv, b.seq_q, b.seq_kv, b.head_dim = dtype, 1, 2, 1, 200, 200, d
+        for name in ("q", "k", "v", "out", "d_out", "dq", "dk", "dv", "lse"):
+            setattr(b, name, 16)
+        for name in ("q", "k", "v", "o", "do", "dq", "dk", "dv"):
+            setattr(b, name + "_strides", (C.c_int64 * 3)(400 * d, 200 * d, d))
+        b.mask.has_band, b.mask.band_hi, b.mask.num_sinks = 1, 30, 4
+        for at, status in ((24, _lib.ATTN_ERR_INVALID), (32, _lib.ATTN_ERR_WORKSPACE)):
+            b.workspace, b.workspace_bytes = at, 64
+            assert lib.attn_bwd(C.byref(b), None) == status
+    c = _lib.PagedCacheParams()
+    c.dtype, c.num_blocks, c.block_size, c.num_heads_kv, c.head_dim = _lib.ATTN_BF16, 1 << 20, 16, 1, 64
+    c.key_pool = c.value_pool = c.block_table = c.seq_lengths = 16
+    c.num_seqs = c.max_blocks_per_seq = 1
+    for at, status in ((18, _lib.ATTN_ERR_INVALID), (20, _lib.ATTN_ERR_WORKSPACE)):
+        assert lib.attn_paged_compact(C.byref(c), 48, 48, at, 64, None) == status
+        assert lib.attn_paged_free(C.byref(c), 16, 1, 48, 48, 48, 48, at, 64, None) == status
