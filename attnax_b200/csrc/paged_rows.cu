@@ -924,6 +924,10 @@ static bool cluster_fits(bool tc, long long splits, long long waves) { return !t
 // of so many tokens of a CTA (one sequence of 2500 tokens, one row: 10.2 us in
 // 20 splits and a join, 12.5 us in a cluster of 8; of 1028 tokens: 9.0 and 8.4).
 constexpr int kStartTokens = 256, kJoinTokens = 96;
+// Many long sequences with many rows each have CTAs enough: there the longest
+// split grows instead of the partials (8 sequences of 131072, 1024 drafts, 64
+// heads: 39.5 ms and 9.3 GiB in splits of 4096, 33.1 ms and 0.8 GiB so).
+constexpr long long kMaxPartials = 1ll << 30;
 
 static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, int64_t sinks) {
   Plan w;
@@ -945,7 +949,11 @@ static Plan make_plan(const attn_paged_params_t* p, bool tree, int64_t window, i
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * w.row_groups;
   const long long slots = (w.tc ? (rows > BM ? 1 : 2) : 3) * 148;
   const long long least = ll_max(128 / u, 1), most = (w.tc ? 4096 : 2048) / u;
-  const long long s_min = (units + most - 1) / most, s_max = ll_max(ll_min(units / least, s_min + 64), s_min);
+  // (partials: not over 1 GiB, unless it takes more for four waves of CTAs, see kMaxPartials)
+  const long long per_split = (long long)p->num_seqs * p->num_heads_kv * rows * (p->head_dim + 1) * sizeof(float);
+  const long long s_cap = ll_max(ll_max(kMaxPartials / per_split, (4 * slots + ctas - 1) / ctas), 1);
+  const long long s_min = ll_min((units + most - 1) / most, s_cap);
+  const long long s_max = ll_max(ll_min(ll_min(units / least, s_min + 64), s_cap), s_min);
   w.split_units = (int)most;
   for (long long s = ll_max(s_min, 1), best = -1; s <= s_max; ++s) {
     const long long len = (units + s - 1) / s, waves = (ctas * s + slots - 1) / slots;

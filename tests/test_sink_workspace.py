@@ -69,3 +69,20 @@ def test_c_entries_refuse_workspaces_off_their_alignment():
     for at, status in ((18, _lib.ATTN_ERR_INVALID), (20, _lib.ATTN_ERR_WORKSPACE)):
         assert lib.attn_paged_compact(C.byref(c), 48, 48, at, 64, None) == status
         assert lib.attn_paged_free(C.byref(c), 16, 1, 48, 48, 48, 48, at, 64, None) == status
+
+
+@pytest.mark.parametrize("n,hq,hkv,t,ctx", [
+    (1, 8, 2, 1, 2500), (64, 64, 8, 16, 32768), (8, 64, 8, 64, 8000),        # as few rows as ever
+    (64, 64, 8, 1024, 131072), (8, 64, 8, 1024, 131072), (1, 64, 8, 1024, 1 << 20), (256, 64, 8, 128, 32768),
+    (1000, 32, 8, 32, 65536), (65535, 8, 1, 1, 1 << 20), (1, 128, 1, 1024, 1 << 24),
+])
+def test_partials_of_window_and_tree_stay_small(n, hq, hkv, t, ctx):
+    """However many rows and tokens: 1 GiB (four waves of CTAs with partials take less than that)."""
+    lib = _lib.load()
+    p = _lib.PagedParams()
+    p.dtype, p.num_seqs, p.num_heads_q, p.num_heads_kv, p.head_dim, p.seq_q = _lib.ATTN_BF16, n, hq, hkv, 128, t
+    p.num_blocks, p.block_size, p.max_blocks_per_seq, p.max_context = 8, 16, ctx // 16 + 1, ctx
+    p.q = p.key_pool = p.value_pool = p.block_table = p.seq_lengths = p.out = 16
+    assert lib.attn_paged_tree_workspace_size(C.byref(p)) <= (1 << 30) + 512
+    for window in (1, 1000, ctx // 2, 2 * ctx):
+        assert lib.attn_paged_window_workspace_size(C.byref(p), window, 4) <= (1 << 30) + 512
