@@ -34,28 +34,36 @@ def _check_query(query, cache: PagedKVCache):
     if not isinstance(query, torch.Tensor) or query.dim() != 4:
         raise ValueError("query must be (num_seqs, num_heads, seq_q, head_dim)")
     n, hq, t, d = query.shape
-    if n != cache.block_table.shape[0]:
-        raise ValueError(f"query has {n} sequences, the cache {cache.block_table.shape[0]}")
-    if hq % cache.num_kv_heads != 0:
-        raise ValueError(f"num_heads ({hq}) must be divisible by num_kv_heads ({cache.num_kv_heads})")
-    if d != cache.head_dim:
-        raise ValueError(f"query head_dim {d} != cache head_dim {cache.head_dim}")
-    check_tables(cache)
-    return n, hq, t, d
+    pool, rows = check_tables(cache)
+    if n != rows[0]:
+        raise ValueError(f"query has {n} sequences, the cache {rows[0]}")
+    if hq % pool[2] != 0:
+        raise ValueError(f"num_heads ({hq}) must be divisible by num_kv_heads ({pool[2]})")
+    if d != pool[3]:
+        raise ValueError(f"query head_dim {d} != cache head_dim {pool[3]}")
+    return n, hq, t, d, pool, rows
 
 
 def check_tables(cache: PagedKVCache):
-    """The kernels read int32 tables on the pools' device, a row and a length per sequence, and two pools alike."""
+    """The kernels read int32 tables on the pools' device, a row and a length per sequence, and two pools alike.
+
+    Returns the pools' shape and the table's.
+    """
+    k, v, table, lengths = cache.key_pool, cache.value_pool, cache.block_table, cache.seq_lengths
+    pool, rows, dev = k.shape, table.shape, k.device
+    # (one pass where all is well: these checks are a good part of a small call's host time)
+    if (len(pool) == 4 and v.shape == pool and v.dtype is k.dtype and v.device == dev
+            and len(rows) == 2 and lengths.shape == rows[:1] and table.dtype is torch.int32
+            and lengths.dtype is torch.int32 and table.device == dev and lengths.device == dev):
+        return pool, rows
     check_pools(cache)
-    table, lengths, dev = cache.block_table, cache.seq_lengths, cache.key_pool.device
     check_rows(table, lengths)
-    if table.dtype is torch.int32 and lengths.dtype is torch.int32 and table.device == dev and lengths.device == dev:
-        return
     for name, x in (("block_table", table), ("seq_lengths", lengths)):
         if x.dtype != torch.int32:
             raise ValueError(f"{name} must be int32, got {x.dtype}")
         if x.device != dev:
             raise RuntimeError(f"{name} must be on the pools' device")
+    return pool, rows
 
 
 def narrow(x: torch.Tensor, device) -> torch.Tensor:
@@ -82,9 +90,9 @@ def _need_cuda(query, cache: PagedKVCache):
         raise RuntimeError("attnax_b200 kernels need the query on the cache's CUDA device; there is no CPU path")
 
 
-def _fused(cache: PagedKVCache) -> bool:
-    return (cache.head_dim in (64, 128) and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
-            and cache.block_size % 16 == 0 and pools_by_tma(cache))
+def _fused(cache: PagedKVCache, pool) -> bool:
+    return (pool[3] in (64, 128) and cache.key_pool.dtype in (torch.bfloat16, torch.float16)
+            and pool[1] % 16 == 0 and pools_by_tma(cache))
 
 
 def _bound(cache: PagedKVCache, max_context):
@@ -101,18 +109,17 @@ def cast(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return x if x.dtype == dtype else x.to(dtype)
 
 
-def _params(query, cache: PagedKVCache, max_context: int):
-    """(PagedParams, out, tensors that the call reads)."""
-    n, hq, t, d = query.shape
-    q = cast(query, cache.key_pool.dtype).contiguous()
+def _params(query, dims, cache: PagedKVCache, max_context: int):
+    """(PagedParams, out, tensors that the call reads); ``dims`` as _check_query returns them."""
+    n, hq, t, d, (nb, bs, hkv, _), (_, width) = dims
+    kp = cache.key_pool
+    q = cast(query, kp.dtype).contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     out = torch.empty_like(q)
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    nb, bs, hkv, _ = cache.key_pool.shape
-    width = bt.shape[1]
-    p = _lib.PagedParams(dtype_code(q.dtype), n, hq, hkv, d, t, nb, bs, width, min(max_context, width * bs),
-                         q.data_ptr(), cache.key_pool.data_ptr(), cache.value_pool.data_ptr(), bt.data_ptr(),
+    p = _lib.PagedParams(dtype_code(kp.dtype), n, hq, hkv, d, t, nb, bs, width, min(max_context, width * bs),
+                         q.data_ptr(), kp.data_ptr(), cache.value_pool.data_ptr(), bt.data_ptr(),
                          sl.data_ptr(), out.data_ptr(), _scale(d))
     return p, out, (q, bt, sl)
 
@@ -147,15 +154,15 @@ def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_
         raise ValueError(f"window_size must be positive, got {window_size}")
     if num_sinks < 0:
         raise ValueError(f"num_sinks must not be negative, got {num_sinks}")
-    n, hq, t, d = _check_query(query, cache)
+    n, hq, t, d, pool, _ = dims = _check_query(query, cache)
     _need_cuda(query, cache)
     if n == 0 or t == 0:
         return torch.zeros_like(query)
-    if not _fused(cache):
+    if not _fused(cache, pool):
         _bound(cache, None)
         return _window_by_sequence(query, cache, int(window_size), int(num_sinks))
     lib = _lib.load()
-    p, out, keep = _params(query, cache, _bound(cache, max_context))
+    p, out, keep = _params(query, dims, cache, _bound(cache, max_context))
     w, s = min(int(window_size), 1 << 40), min(int(num_sinks), 1 << 40)
     ws = _workspace(p, lib.attn_paged_window_workspace_size(C.byref(p), w, s), query.device)
     _lib.run("attn_paged_window", query.device, C.byref(p), w, s)
@@ -219,10 +226,10 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
     ``max_context`` as in :func:`paged_window_attention`.  The accepted path
     goes into the cache with ``append_accepted``.
     """
-    n, hq, t, d = _check_query(query, cache)
+    n, hq, t, d, pool, _ = dims = _check_query(query, cache)
     for name, x in (("draft_keys", draft_keys), ("draft_values", draft_values)):
-        if not isinstance(x, torch.Tensor) or x.shape != (n, cache.num_kv_heads, t, d):
-            raise ValueError(f"{name} must have shape {(n, cache.num_kv_heads, t, d)}, got "
+        if not isinstance(x, torch.Tensor) or x.shape != (n, pool[2], t, d):
+            raise ValueError(f"{name} must have shape {(n, pool[2], t, d)}, got "
                              f"{tuple(getattr(x, 'shape', ()))}")
         if x.device != query.device:
             raise RuntimeError(f"{name} must be on the query's device")
@@ -239,11 +246,11 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
     _need_cuda(query, cache)
     if n == 0 or t == 0:
         return torch.zeros_like(query)
-    if not _fused(cache):
+    if not _fused(cache, pool):
         _bound(cache, None)
         return _tree_by_sequence(query, draft_keys, draft_values, cache, parents, tree_lengths)
     lib = _lib.load()
-    p, out, keep = _params(query, cache, _bound(cache, max_context))
+    p, out, keep = _params(query, dims, cache, _bound(cache, max_context))
     dk, dv = (_tma_ready(cast(x, cache.key_pool.dtype)) for x in (draft_keys, draft_values))
     tr = _lib.PagedTree(dk.data_ptr(), dv.data_ptr(), dk.stride()[:3], dv.stride()[:3], parents.data_ptr(),
                         None if tree_lengths is None else tree_lengths.data_ptr())

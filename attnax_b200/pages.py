@@ -31,14 +31,14 @@ _Strides = C.c_int64 * 3
 
 def _params(cache: PagedKVCache):
     """(PagedCacheParams, tensors it points into)."""
-    check_tables(cache)
-    if not cache.key_pool.is_cuda:
-        raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
+    pool, rows = check_tables(cache)
     kp, vpool = cache.key_pool, cache.value_pool
+    if not kp.is_cuda:
+        raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
     if not (kp.is_contiguous() and vpool.is_contiguous()):
         raise ValueError("page operators write the pools in place and need them contiguous")
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    p = _lib.PagedCacheParams(dtype_code(kp.dtype), *kp.shape, kp.data_ptr(), vpool.data_ptr(), *bt.shape,
+    p = _lib.PagedCacheParams(dtype_code(kp.dtype), *pool, kp.data_ptr(), vpool.data_ptr(), *rows,
                               bt.data_ptr(), sl.data_ptr())
     return p, (bt, sl)
 
