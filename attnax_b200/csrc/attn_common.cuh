@@ -133,7 +133,8 @@ __device__ __forceinline__ float load_bias(const void* p, attn_dtype_t dt, long 
 }
 
 // Element transform for one score: raw q.k -> log2-domain score t, with
-// every mask and additive term.  `row`/`col` are local positions.  SINK as in
+// every mask and additive term.  `row`/`col` are local positions; the row must
+// be inside the sequence, a column past its end needs `partial`.  SINK as in
 // tile_state: only with num_sinks > 0 (without sinks `kvg < num_sinks` would
 // hold for keys at negative positions).
 template <bool SINK = false>
@@ -229,7 +230,9 @@ __device__ __forceinline__ int clamp_i32(long long x) {
   return (int)(x < -(1ll << 30) ? -(1ll << 30) : (x > (1ll << 30) ? (1ll << 30) : x));
 }
 
-// row/col0 are local positions of this thread's row and of column 0.
+// row/col0 are local positions of this thread's row and of column 0.  The row
+// must be inside the sequence (its document id, mask and bias rows are read);
+// rows of a last tile past the end take the last row's, their results are dropped.
 // transposed: the row is a kv position and columns are q positions.
 __device__ __forceinline__ RowCtx make_row_ctx(const attn_mask_t& m, float sl2, int b, int hq,
                                                int row, int col0, int ncols, bool transposed) {

@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(CfgKV<D, FQ>::THREADS, 1)
           }
         }
       } else {
-        const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, k0 + r, c0, max(0, min(HC, a.Sq - c0)), true);
+        const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, min(k0 + r, a.Skv - 1), c0, max(0, min(HC, a.Sq - c0)), true);
         transform_row<HC, SINK>(sc, rc, st == kPartial || k0 + r >= a.Skv);
         const bool row_ok = k0 + r < a.Skv;
 #pragma unroll
@@ -1076,7 +1076,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 32; ++c) dp[c] = ((keep >> c) & 1u) ? dp[c] : 0.f;
           }
         } else {
-          const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, q0 + r, c0, max(0, min(32, a.Skv - c0)), false);
+          const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, min(q0 + r, a.Sq - 1), c0, max(0, min(32, a.Skv - c0)), false);
           transform_row<32, SINK>(sc, rc, st == kPartial);
 #pragma unroll
           for (int c = 0; c < 32; ++c) {

@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) t[e] = __uint_as_float(raw[e]);
-          const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, my_q0 + r, k0 + c * 32,
+          const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, min(my_q0 + r, a.Sq - 1), k0 + c * 32,
                                          max(0, min(32, a.Skv - (k0 + c * 32))), false);
           transform_row<32, SINK>(t, rc, true);
 #pragma unroll

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_warp(s_free(i & 1));
 
       const int k0 = j * BN;
-      const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, q0 + r, k0, min(BN, a.Skv - k0), false);
+      const RowCtx rc = make_row_ctx(a.mask, a.sl2, b, hq, min(q0 + r, a.Sq - 1), k0, min(BN, a.Skv - k0), false);
       transform_row<BN, SINK>(s, rc, st == kPartial);
       float mx = m_run;
 #pragma unroll
