@@ -860,33 +860,39 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ 
   const float* lse = a.part_lse + prow * a.max_splits;
   const float* po = a.part_o + prow * a.max_splits * D + lane * (D / 32);
   float mx = -INFINITY;
-  for (int i = lane; i < n; i += 32) mx = fmaxf(mx, lse[i]);
+  bool nan = false;  // (fmaxf skips NaN)
+  for (int i = lane; i < n; i += 32) {
+    mx = fmaxf(mx, lse[i]);
+    nan = nan || lse[i] != lse[i];
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  nan = __any_sync(0xffffffffu, nan);
   float tot = 0.f, acc[D / 32];
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-  constexpr int B = 8;  // partials in flight
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const float x0 = i0 + lane < n ? lse[i0 + lane] : -INFINITY;
-    const float wl = x0 == -INFINITY ? 0.f : ex2(x0 - mx);  // (all may be -inf, or NaN)
-    for (int j0 = 0; j0 < min(32, n - i0); j0 += B) {
-      float x[B][D / 32];
+  if (mx != -INFINITY) {
+    constexpr int B = 8;  // partials in flight
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const float wl = i0 + lane < n ? ex2(lse[i0 + lane] - mx) : 0.f;
+      for (int j0 = 0; j0 < min(32, n - i0); j0 += B) {
+        float x[B][D / 32];
 #pragma unroll
-      for (int j = 0; j < B; ++j)
+        for (int j = 0; j < B; ++j)
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e)
-          x[j][e] = i0 + j0 + j < n ? po[(long long)(i0 + j0 + j) * D + e] : 0.f;
+          for (int e = 0; e < D / 32; ++e)
+            x[j][e] = i0 + j0 + j < n ? po[(long long)(i0 + j0 + j) * D + e] : 0.f;
 #pragma unroll
-      for (int j = 0; j < B; ++j) {
-        const float w = __shfl_sync(0xffffffffu, wl, j0 + j);
-        tot += w;
+        for (int j = 0; j < B; ++j) {
+          const float w = __shfl_sync(0xffffffffu, wl, j0 + j);
+          tot += w;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, x[j][e], acc[e]);
+          for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(w, x[j][e], acc[e]);
+        }
       }
     }
   }
-  const float inv = tot == 0.f ? 0.f : 1.f / tot;
+  const float inv = nan ? NAN : tot > 0.f ? 1.f / tot : 0.f;
   T* orow = reinterpret_cast<T*>(a.out) + prow * D + lane * (D / 32);
 #pragma unroll
   for (int e = 0; e < D / 32; e += 2)
