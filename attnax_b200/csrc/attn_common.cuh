@@ -133,8 +133,8 @@ __device__ __forceinline__ float load_bias(const void* p, attn_dtype_t dt, long 
 }
 
 // Element transform for one score: raw q.k -> log2-domain score t, with
-// every mask and additive term.  `row`/`col` are local positions; the row must
-// be inside the sequence, a column past its end needs `partial`.  SINK as in
+// every mask and additive term.  `row`/`col` are local positions; with `partial`
+// the row must be inside the sequence, a column past its end needs it.  SINK as in
 // tile_state: only with num_sinks > 0 (without sinks `kvg < num_sinks` would
 // hold for keys at negative positions).
 template <bool SINK = false>

@@ -51,8 +51,8 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const FwdArgs a) {
   const int rloc = tid / L::TPR, part = tid % L::TPR;
   const int hq = blockIdx.y, b = blockIdx.z, hkv = hq / a.group;
   const int q0 = blockIdx.x * L::RPB;
-  const int row = q0 + rloc, mrow = min(row, a.Sq - 1);  // (past the end: the last row's masks, see mask_score)
-  const bool row_ok = row < a.Sq;
+  const int row = min(q0 + rloc, a.Sq - 1);  // (past the end: the last row's masks, see mask_score)
+  const bool row_ok = q0 + rloc < a.Sq;
   const int q1 = min(q0 + L::RPB, a.Sq);
   const T* Q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hq * a.qs[1];
   const T* K = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + hkv * a.ks[1];
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < L::EPT; ++e) acc = fmaf(q[e], sk[c][part * L::EPT + e], acc);
       acc = group_sum<L::TPR>(acc);
-      t[c] = mask_score<SINK>(a.mask, acc, a.sl2, slope_l2, b, hq, mrow, k0 + c, a.Skv, st == kPartial);
+      t[c] = mask_score<SINK>(a.mask, acc, a.sl2, slope_l2, b, hq, row, k0 + c, a.Skv, st == kPartial);
       mx = fmaxf(mx, t[c]);
     }
     const float alpha = exp2f(m - mx);
@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) 
   const int tid = threadIdx.x;
   const int rloc = tid / L::TPR, part = tid % L::TPR;
   const int hq = blockIdx.y, b = blockIdx.z, hkv = hq / a.group;
-  const int q0 = blockIdx.x * L::RPB, row = q0 + rloc, mrow = min(row, a.Sq - 1);
-  const bool row_ok = row < a.Sq;
+  const int q0 = blockIdx.x * L::RPB, row = min(q0 + rloc, a.Sq - 1);
+  const bool row_ok = q0 + rloc < a.Sq;
   const int q1 = min(q0 + L::RPB, a.Sq);
   const T* Q = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + hq * a.qs[1];
   const T* DO = reinterpret_cast<const T*>(a.dout) + b * a.dos[0] + hq * a.dos[1];
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dq_kernel(const BwdArgs a) 
       }
       s = group_sum<L::TPR>(s);
       dp = group_sum<L::TPR>(dp);
-      const float t = mask_score<SINK>(a.mask, s, a.sl2, slope_l2, b, hq, mrow, k0 + c, a.Skv, st == kPartial);
+      const float t = mask_score<SINK>(a.mask, s, a.sl2, slope_l2, b, hq, row, k0 + c, a.Skv, st == kPartial);
       const float p = (t == -FLT_MAX) ? 0.f : exp2f(t - lse2);
       const float ds = p * (dp - delta);
 #pragma unroll
@@ -277,8 +277,9 @@ __global__ void __launch_bounds__(kThreads) simt_bwd_dkv_kernel(const BwdArgs a)
         }
         s = group_sum<L::TPR>(s);
         dp = group_sum<L::TPR>(dp);
-        const float t = mask_score<SINK>(a.mask, s, a.sl2, slope_l2, b, hq, min(q0 + rr, a.Sq - 1), col, a.Skv,
-                                         st == kPartial || q0 + rr >= a.Sq);
+        // (a row past the end has no masks to look up: its lse2 of +inf makes p 0)
+        const float t = mask_score<SINK>(a.mask, s, a.sl2, slope_l2, b, hq, q0 + rr, col, a.Skv,
+                                         st == kPartial && q0 + rr < a.Sq);
         const float p = (t == -FLT_MAX || !col_ok) ? 0.f : exp2f(t - slse[rr]);
         const float ds = p * (dp - sdelta[rr]);
 #pragma unroll
