@@ -161,7 +161,8 @@ def free_window(cache: PagedKVCache, *, window_size: int, num_sinks: int = 0):
     A page goes when all its tokens lie behind the first ``num_sinks`` and in
     front of the window of the next token (position ``seq_lengths``); its entry
     becomes -1 and the lengths stay.  Whatever reads the whole context
-    (``paged_attention``, ``gather_kv``) must not be used on such rows.
+    (``paged_attention``, ``paged_tree_attention``, ``gather_kv``) must not be
+    used on such rows.
     """
     if window_size <= 0:
         raise ValueError(f"window_size must be positive, got {window_size}")
