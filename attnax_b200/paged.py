@@ -80,7 +80,10 @@ def gather_positions(cache: PagedKVCache, sequence_idx: int, pos: torch.Tensor):
 
 
 def check_rows(block_table: torch.Tensor, seq_lengths: torch.Tensor):
-    """One table row and one length per sequence."""
+    """One table row and one length per sequence, int32 as the kernels read them."""
+    for name, x in (("block_table", block_table), ("seq_lengths", seq_lengths)):
+        if x.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32, got {x.dtype}")
     shape = block_table.shape
     if len(shape) != 2:
         raise ValueError(f"block_table must be (num_seqs, max_blocks_per_seq), got {tuple(shape)}")
@@ -122,6 +125,7 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
         raise ValueError(f"keys_new shape {tuple(keys_new.shape)} != values_new shape "
                          f"{tuple(values_new.shape)}")
     check_pools(cache)
+    check_rows(cache.block_table, cache.seq_lengths)
     if not pools_contiguous(cache):
         raise ValueError("append_kv writes the pools in place and needs them contiguous")
     lib = _lib.load()
@@ -152,6 +156,7 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
 def gather_kv(cache: PagedKVCache, sequence_idx: int):
     """Contiguous ``(seq_len, Hkv, D)`` keys/values of one sequence (paged_cache.py:201-231)."""
     check_pools(cache)
+    check_rows(cache.block_table, cache.seq_lengths)
     seq_len = int(cache.seq_lengths[sequence_idx])
     if not pools_contiguous(cache):
         if seq_len > cache.block_table.shape[1] * cache.block_size:

@@ -59,8 +59,6 @@ def check_tables(cache: PagedKVCache):
     check_pools(cache)
     check_rows(table, lengths)
     for name, x in (("block_table", table), ("seq_lengths", lengths)):
-        if x.dtype != torch.int32:
-            raise ValueError(f"{name} must be int32, got {x.dtype}")
         if x.device != dev:
             raise RuntimeError(f"{name} must be on the pools' device")
     return pool, rows

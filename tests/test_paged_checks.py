@@ -98,3 +98,12 @@ def test_indices_must_be_integers(wrong):
         ax.append_accepted(c, DRAFT, DRAFT, wrong, [1] * 3)
     with pytest.raises(ValueError):
         ax.append_accepted(c, DRAFT, DRAFT, [[0]] * 3, wrong[:, 0])
+
+
+@pytest.mark.parametrize("call", ROWS + PAGES + OLDER)
+def test_tables_and_lengths_of_other_types(call):
+    c = cpu_cache()
+    for table, lens in ((c.block_table.long(), c.seq_lengths), (c.block_table, c.seq_lengths.long()),
+                        (c.block_table.to(torch.int16), c.seq_lengths), (c.block_table, c.seq_lengths.float())):
+        with pytest.raises(ValueError, match="int32"):
+            call(ax.PagedKVCache(c.key_pool, c.value_pool, table, lens))
