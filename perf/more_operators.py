@@ -418,7 +418,7 @@ def _exact_page(page, old, old_scale, pool):
     """Values ``(tokens, kv heads, dim)`` of an 8-bit page, the first ``old`` of them codes of ``old_scale (kv heads)``."""
     most = {"e4m3": 448.0, "int8": 127.0}[pool]
     amax = page[old:].abs().amax((0, 2))
-    s = torch.ldexp(torch.ones_like(amax), torch.round(torch.log2(amax / most)) + 1)  # one or two steps too large
+    s = torch.ldexp(torch.ones_like(amax), (torch.round(torch.log2(amax / most)) + 1).int())  # one or two steps too large
     s = torch.where(amax <= most * s / 4, s / 4, torch.where(amax <= most * s / 2, s / 2, s)).clamp(min=2.0 ** -100)
     s = torch.maximum(s, old_scale)[:, None]
     return torch.cat([_exact_round(page[:old] * (old_scale[:, None] / s), pool), _exact_round(page[old:] / s, pool)]) * s
