@@ -11,8 +11,13 @@ hand-written CUDA in ``libattnb200.so`` (C ABI: ``include/attnb200.h``):
   sinks and trees of drafted tokens;
 * ``append_accepted``, ``copy_blocks``, ``fork_sequences``, ``free_sequences``,
   ``free_window`` and ``compact_blocks`` on its pages, a batch at a time;
+* ``append_tokens`` / ``gather_tokens``, batches of tokens into and out of pages, keys and
+  queries rotated on the way, and ``QuantizedPagedKVCache`` with ``paged_quantized_attention``
+  for pages in 8 bits;
 * ``kv_cache_attention`` over the contiguous per-layer ``KVLayerCache``;
 * ``apply_rope`` (+ the reference's cos/sin table builders) for Q/K rotation;
+* ``rotary_plan`` / ``apply_rotary``: both pair layouts, part of the head, scaled frequencies,
+  with gradients;
 * ``ring_attention`` — sequence parallel over NCCL.
 """
 
@@ -29,6 +34,9 @@ from .pages import (append_accepted, compact_blocks, copy_blocks, fork_sequences
 from .paged_rows import paged_tree_attention, paged_window_attention
 from .kv_cache import (KVLayerCache, init_decoder_kv_caches, init_kv_layer_cache, kv_cache_attention,
                        update_kv_layer_cache)
+from .quantized import (QuantizedPagedKVCache, append_tokens, gather_tokens, init_quantized_paged_kv_cache,
+                        paged_quantized_attention)
+from .rotary import (RotaryPlan, apply_rotary, rotary_frequencies, rotary_plan, rotary_plan_from_frequencies)
 from .ring import ring_attention, ring_attention_reference
 from .rope import (apply_rope, apply_rope_table, rope_cos_sin_from_positions, rope_cos_sin_table,
                    rope_inv_freq)
@@ -46,5 +54,8 @@ __all__ = [
     "memory_efficient_attention", "paged_attention", "paged_attention_batched", "paged_tree_attention",
     "paged_window_attention",
     "pallas_flash_attention", "prefix_lm_mod", "ring_attention", "ring_attention_reference",
+    "QuantizedPagedKVCache", "RotaryPlan", "append_tokens", "apply_rotary", "gather_tokens",
+    "init_quantized_paged_kv_cache", "paged_quantized_attention", "rotary_frequencies", "rotary_plan",
+    "rotary_plan_from_frequencies",
     "score_mods", "sink_window_mod", "sliding_window_mod", "standard_attention",
 ]

@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libattnb200.so")
 ATTN_OK, ATTN_ERR_INVALID, ATTN_ERR_UNSUPPORTED, ATTN_ERR_CUDA, ATTN_ERR_NCCL, \
     ATTN_ERR_WORKSPACE, ATTN_ERR_TIMEOUT = range(7)
 ATTN_F32, ATTN_BF16, ATTN_F16 = 0, 1, 2
+POOL_E4M3, POOL_INT8 = 16, 17  # pools of 8-bit codes
 # Device status codes (attn_device_status): bounded-wait timeouts and notices.
 STATUS_TIMEOUTS = (0x101, 0x102, 0x103, 0x104)
 NOTICE_CONTEXT_OVERRUN = 0x201   # a paged decode met a length above max_context
@@ -99,6 +100,50 @@ class RopeParams(C.Structure):
     ]
 
 
+class RotarySpec(C.Structure):
+    _fields_ = [("turns", vp), ("rotary_dim", i32), ("interleaved", i32), ("magnitude", f32)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("batch", i32), ("seq", i32), ("head_dim", i32), ("heads_q", i32), ("heads_k", i32),
+        ("q", vp), ("q_out", vp), ("k", vp), ("k_out", vp),
+        ("q_strides", i64 * 3), ("q_out_strides", i64 * 3), ("k_strides", i64 * 3), ("k_out_strides", i64 * 3),
+        ("rotary", RotarySpec), ("inverse", i32), ("positions", vp), ("positions_64", i32),
+        ("position_strides", i64 * 2),
+    ]
+
+
+class PagedAppendParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("pool_format", i32), ("num_blocks", i32), ("block_size", i32), ("num_heads_kv", i32),
+        ("head_dim", i32), ("key_pool", vp), ("value_pool", vp), ("key_scales", vp), ("value_scales", vp),
+        ("num_seqs", i32), ("max_blocks_per_seq", i32), ("block_table", vp), ("seq_lengths", vp),
+        ("keys", vp), ("values", vp), ("k_strides", i64 * 3), ("v_strides", i64 * 3), ("num_new", i32),
+        ("new_lengths", vp), ("rotary", RotarySpec), ("num_heads_q", i32), ("q", vp), ("q_out", vp),
+        ("q_strides", i64 * 3), ("q_out_strides", i64 * 3), ("lengths_out", vp), ("bad", vp),
+    ]
+
+
+class PagedGatherParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("pool_format", i32), ("num_blocks", i32), ("block_size", i32), ("num_heads_kv", i32),
+        ("head_dim", i32), ("key_pool", vp), ("value_pool", vp), ("key_scales", vp), ("value_scales", vp),
+        ("num_seqs", i32), ("max_blocks_per_seq", i32), ("block_table", vp), ("seq_lengths", vp),
+        ("starts", vp), ("count", i32), ("keys_out", vp), ("values_out", vp),
+    ]
+
+
+class PagedAttend8Params(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("pool_format", i32), ("num_seqs", i32), ("num_heads_q", i32), ("num_heads_kv", i32),
+        ("head_dim", i32), ("seq_q", i32), ("num_blocks", i32), ("block_size", i32), ("max_blocks_per_seq", i32),
+        ("max_context", i32), ("q", vp), ("key_pool", vp), ("value_pool", vp), ("key_scales", vp),
+        ("value_scales", vp), ("block_table", vp), ("seq_lengths", vp), ("out", vp), ("softmax_scale", f32),
+        ("workspace", vp), ("workspace_bytes", szt),
+    ]
+
+
 class RingParams(C.Structure):
     _fields_ = [
         ("dtype", C.c_int), ("batch", i32), ("num_heads_q", i32), ("num_heads_kv", i32),
@@ -149,6 +194,11 @@ SIGNATURES = {
     "attn_paged_physical_page": (i64, [i32, i32]),
     "attn_lse_merge": (C.c_int, [C.c_int, i64, i32, vp, vp, vp, vp, vp, vp]),
     "attn_rope": (C.c_int, [C.POINTER(RopeParams), vp]),
+    "attn_rotary": (C.c_int, [C.POINTER(RotaryParams), vp]),
+    "attn_paged_append_tokens": (C.c_int, [C.POINTER(PagedAppendParams), vp]),
+    "attn_paged_gather_tokens": (C.c_int, [C.POINTER(PagedGatherParams), vp]),
+    "attn_paged_attend8_workspace_size": (szt, [C.POINTER(PagedAttend8Params)]),
+    "attn_paged_attend8": (C.c_int, [C.POINTER(PagedAttend8Params), vp]),
     "attn_comm_unique_id": (C.c_int, [vp, szt]),
     "attn_comm_init": (C.c_int, [C.POINTER(vp), i32, i32, vp, szt]),
     "attn_comm_destroy": (C.c_int, [vp]),

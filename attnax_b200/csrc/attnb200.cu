@@ -422,7 +422,7 @@ int attn_device_status(int32_t* status) {
   const int zero = 0;
   if (cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) != cudaSuccess) return ATTN_ERR_CUDA;
   if (cudaMemcpyToSymbol(g_notice, &zero, sizeof(int)) != cudaSuccess) return ATTN_ERR_CUDA;
-  for (auto take : {&rows_take_status, &pages_take_status}) {
+  for (auto take : {&rows_take_status, &pages_take_status, &rotary_take_status, &attend8_take_status}) {
     int v1 = 0, n1 = 0;
     if (!take(&v1, &n1)) return ATTN_ERR_CUDA;
     if (!v) v = v1;

@@ -66,5 +66,7 @@ bool make_pool_tmap(CUtensorMap* m, attn_dtype_t dt, const void* pool, long long
 // read and clear those of the others for attn_device_status.
 bool rows_take_status(int* status, int* notice);
 bool pages_take_status(int* status, int* notice);
+bool rotary_take_status(int* status, int* notice);
+bool attend8_take_status(int* status, int* notice);
 
 }  // namespace attnb200

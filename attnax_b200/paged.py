@@ -13,7 +13,7 @@ new tokens too.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
@@ -53,6 +53,7 @@ def check_pools(cache: PagedKVCache):
     k, v = cache.key_pool, cache.value_pool
     shape = k.shape
     if len(shape) == 4 and v.shape == shape and v.dtype == k.dtype and v.device == k.device:
+        dtype_code(k.dtype)  # (8-bit pools have scales, which the operators of this class would not read)
         return
     if len(shape) != 4:
         raise ValueError(f"key_pool must be (num_blocks, block_size, num_kv_heads, head_dim), got {tuple(shape)}")
@@ -115,7 +116,7 @@ def allocate_blocks(cache: PagedKVCache, *, sequence_idx: int, num_new_tokens: i
     table = cache.block_table.clone()
     if new > 0:
         table[sequence_idx, have:have + new] = free[:new].to(device=table.device, dtype=torch.int32)
-    return PagedKVCache(cache.key_pool, cache.value_pool, table, cache.seq_lengths), new
+    return replace(cache, block_table=table), new
 
 
 def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,

@@ -29,6 +29,9 @@
  *                       (attnax/embeddings.py:126-184), the rotation
  *                       MultiHeadAttention applies to Q and K before attention
  *                       (attnax/attention.py:340-381)
+ * Beside the reference: attn_paged_window, attn_paged_tree, the page operators,
+ * attn_rotary, attn_paged_append_tokens, attn_paged_gather_tokens and
+ * attn_paged_attend8.
  */
 #ifndef ATTNB200_H_
 #define ATTNB200_H_
@@ -384,6 +387,112 @@ typedef struct {
 } attn_rope_params_t;
 
 int attn_rope(const attn_rope_params_t* p, void* stream);
+
+/* ---- rotary positions ---------------------------------------------------- */
+/* Each pair (a, b) of the first rotary_dim channels turns by position * w:
+ *   a' = m (a cos - b sin), b' = m (a sin + b cos);
+ * the channels behind them are copied.  turns[i] is pair i's frequency as a
+ * fraction of a turn per position, w / (2 pi) * 2^64 modulo 2^64, so angles
+ * are exact at any position.  interleaved 0: pair (i, i + rotary_dim / 2);
+ * 1: pair (2 i, 2 i + 1). */
+typedef struct {
+  const uint64_t* turns;     /* device, [rotary_dim / 2] */
+  int32_t rotary_dim;        /* even, at most head_dim */
+  int32_t interleaved;
+  float magnitude;
+} attn_rotary_spec_t;
+/* Queries and keys in one launch (heads_k 0: one tensor).  inverse 1 turns
+ * backwards, which is the gradient.  Strides in elements, unit on head_dim,
+ * any others; *_out may alias its input.  Math in fp32, one rounding. */
+typedef struct {
+  attn_dtype_t dtype;
+  int32_t batch, seq, head_dim, heads_q, heads_k;
+  const void* q; void* q_out;        /* (batch, heads_q, seq, head_dim) */
+  const void* k; void* k_out;
+  int64_t q_strides[3], q_out_strides[3], k_strides[3], k_out_strides[3];
+  attn_rotary_spec_t rotary;
+  int32_t inverse;
+  const void* positions;             /* int32 or int64, or NULL: 0 .. seq - 1 */
+  int32_t positions_64;
+  int64_t position_strides[2];       /* elements: batch (0: shared), seq */
+} attn_rotary_params_t;
+int attn_rotary(const attn_rotary_params_t* p, void* stream);
+
+/* ---- tokens into and out of a paged cache ---------------------------------- */
+/* What a pool holds: an attn_dtype_t, or 8-bit codes.  The codes of one page
+ * and kv head stand for code * scale, scales float32 [num_blocks, heads_kv],
+ * powers of two where attn_paged_append_tokens wrote them. */
+enum { ATTN_POOL_E4M3 = 16, ATTN_POOL_INT8 = 17 };
+/* Appends the tokens [0, new_lengths[s]) of every sequence s to its pages at
+ * positions seq_lengths[s].., keys turned by their position on the way (turns
+ * NULL: not turned), and turns the query rows: row i by seq_lengths[s] + i,
+ * padding rows too.  lengths_out gets the new lengths.  A page of 8-bit codes
+ * keeps the larger of its old scale and the one that the new tokens need; its
+ * old codes are restated if it grows.  Infinities and NaN become NaN codes;
+ * int8 has none, so the page's scale becomes NaN until it is begun anew.  A
+ * page that gets tokens must belong to one sequence.  Tokens without a page,
+ * and new_lengths outside [0, num_new], are skipped or cut and leave the
+ * notice 0x204.  With bad non-NULL (pre-set to INT32_MAX) only checks: the
+ * lowest such sequence is stored there and nothing is written. */
+typedef struct {
+  attn_dtype_t dtype;                /* keys, values, q, q_out */
+  int32_t pool_format;
+  int32_t num_blocks, block_size, num_heads_kv, head_dim;
+  void* key_pool; void* value_pool;
+  float* key_scales; float* value_scales;          /* 8-bit pools */
+  int32_t num_seqs, max_blocks_per_seq;
+  const int32_t* block_table; const int32_t* seq_lengths;
+  const void* keys; const void* values;            /* (num_seqs, heads_kv, num_new, head_dim), any strides but the last */
+  int64_t k_strides[3], v_strides[3];
+  int32_t num_new;
+  const int32_t* new_lengths;        /* [num_seqs] or NULL: all num_new */
+  attn_rotary_spec_t rotary;
+  int32_t num_heads_q;               /* 0: no query */
+  const void* q; void* q_out;
+  int64_t q_strides[3], q_out_strides[3];
+  int32_t* lengths_out; int32_t* bad;
+} attn_paged_append_params_t;
+int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream);
+/* keys_out/values_out [num_seqs, count, heads_kv, head_dim] in `dtype`: the
+ * tokens at positions starts[s] .. starts[s] + count (starts NULL: from 0) of
+ * every sequence, 8-bit codes as the values that they stand for; zeros in
+ * front of a sequence and from its length on.  Table entries are read as
+ * attn_paged_gather reads them; positions past the table row give zeros and
+ * the notice 0x202. */
+typedef struct {
+  attn_dtype_t dtype;
+  int32_t pool_format;
+  int32_t num_blocks, block_size, num_heads_kv, head_dim;
+  const void* key_pool; const void* value_pool;
+  const float* key_scales; const float* value_scales;
+  int32_t num_seqs, max_blocks_per_seq;
+  const int32_t* block_table; const int32_t* seq_lengths;
+  const int32_t* starts;
+  int32_t count;
+  void* keys_out; void* values_out;
+} attn_paged_gather_params_t;
+int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream);
+/* Attention over 8-bit pages: query row i of sequence s stands at position
+ * seq_lengths[s] - seq_q + i and sees the keys up to it; rows in front of the
+ * sequence give zeros.  head_dim 64 or 128, block_size a multiple of 16, pools
+ * on 16 bytes; others are ATTN_ERR_UNSUPPORTED.  max_context bounds the
+ * lengths: a longer sequence is cut to the planned splits (notice 0x201), one
+ * longer than its table row ends with the row (0x202). */
+typedef struct {
+  attn_dtype_t dtype;                /* q and out */
+  int32_t pool_format;
+  int32_t num_seqs, num_heads_q, num_heads_kv, head_dim, seq_q;
+  int32_t num_blocks, block_size, max_blocks_per_seq, max_context;
+  const void* q;                     /* [num_seqs, heads_q, seq_q, head_dim] */
+  const void* key_pool; const void* value_pool;
+  const float* key_scales; const float* value_scales;
+  const int32_t* block_table; const int32_t* seq_lengths;
+  void* out;
+  float softmax_scale;
+  void* workspace; size_t workspace_bytes;
+} attn_paged_attend8_params_t;
+size_t attn_paged_attend8_workspace_size(const attn_paged_attend8_params_t* p);
+int attn_paged_attend8(const attn_paged_attend8_params_t* p, void* stream);
 
 /* ---- diagnostics -------------------------------------------------------- */
 /* Reads and clears the device status words (0 = none).  Synchronises the
