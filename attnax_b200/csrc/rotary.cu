@@ -62,6 +62,35 @@ struct alignas(sizeof(T) * N) Vec {
   T e[N];
 };
 
+// Vectors are moved as machine words: as structs, the compiler split those that it keeps for several heads into
+// elements (training shape, one direction: 280 us instead of 115).
+template <int BYTES> struct Word;
+template <> struct Word<1> { using T = uint8_t; };
+template <> struct Word<2> { using T = uint16_t; };
+template <> struct Word<4> { using T = uint32_t; };
+template <> struct Word<8> { using T = uint2; };
+template <> struct Word<16> { using T = uint4; };
+template <typename T, int N>
+using Bits = typename Word<sizeof(T) * N>::T;
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> unpack(const Bits<T, N>& w) {
+  Vec<T, N> v;
+  static_assert(sizeof(v) == sizeof(w), "");
+  memcpy(&v, &w, sizeof(v));
+  return v;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* at, const Vec<T, N>& v) {
+  constexpr int M = sizeof(T) * N > 16 ? 16 / sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N / M; ++i) {
+    Bits<T, M> w;
+    memcpy(&w, v.e + i * M, sizeof(w));
+    reinterpret_cast<Bits<T, M>*>(at)[i] = w;
+  }
+}
+
 // One item: NP pairs, in two vectors of NP elements at o1 and o2, or elements behind the turned part.
 struct Item {
   int o1, o2;
@@ -108,12 +137,21 @@ __device__ __forceinline__ void turn(float (&v)[2 * NP], const float (&cs)[NP], 
   }
 }
 
+// An item as it lies in memory.
 template <typename T, int NP>
-__device__ __forceinline__ void load_item(const T* row, const Item& it, float (&v)[2 * NP]) {
-  using V = Vec<T, NP>;
-  const V a = *reinterpret_cast<const V*>(row + it.o1);
-  V b{};
-  if (it.second) b = *reinterpret_cast<const V*>(row + it.o2);
+struct Raw {
+  Bits<T, NP> a, b;
+};
+template <typename T, int NP>
+__device__ __forceinline__ Raw<T, NP> load_raw(const T* row, const Item& it) {
+  Raw<T, NP> r{};
+  r.a = *reinterpret_cast<const Bits<T, NP>*>(row + it.o1);
+  if (it.second) r.b = *reinterpret_cast<const Bits<T, NP>*>(row + it.o2);
+  return r;
+}
+template <typename T, int NP>
+__device__ __forceinline__ void widen(const Raw<T, NP>& r, float (&v)[2 * NP]) {
+  const Vec<T, NP> a = unpack<T, NP>(r.a), b = unpack<T, NP>(r.b);
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
     v[j] = to_f32(a.e[j]);
@@ -123,15 +161,14 @@ __device__ __forceinline__ void load_item(const T* row, const Item& it, float (&
 
 template <typename T, int NP>
 __device__ __forceinline__ void store_item(T* row, const Item& it, const float (&v)[2 * NP]) {
-  using V = Vec<T, NP>;
-  V a, b;
+  Vec<T, NP> a, b;
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
     a.e[j] = from_f32<T>(v[j]);
     b.e[j] = from_f32<T>(v[NP + j]);
   }
-  *reinterpret_cast<V*>(row + it.o1) = a;
-  if (it.second) *reinterpret_cast<V*>(row + it.o2) = b;
+  store_vec<T, NP>(row + it.o1, a);
+  if (it.second) store_vec<T, NP>(row + it.o2, b);
 }
 
 // A (batch, heads, seq, dim) tensor with unit stride on dim; strides in elements.
@@ -148,39 +185,58 @@ struct Args {
   Spec sp;
   const void* positions;
   long long ps[2];
-  int positions_64, batch, seq, dim, items, head_group;
+  const int32_t* first;  // [batch] added to the positions, or null
+  int positions_64, seq, dim, items, head_group, head_lanes, cta_tokens;
+  int tokens;
 };
 
-// Thread = (token, item); it walks over the head_group heads of blockIdx.y
-// (of both tensors in a row), kUnroll of them in flight.
+// Heads whose loads a thread has in flight together.  (The output may alias the input, so the compiler keeps loads
+// behind the stores in front of them: they are issued by hand.)
+constexpr int kHeads = 2;
+
+// CTA = cta_tokens tokens and the head_group heads of blockIdx.y, of both tensors in a row; thread = (token, one of
+// head_lanes heads in turn, item).  Four head lanes make a warp's accesses neighbours in memory where a token's heads
+// lie side by side, one where a head's tokens do.
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Args a) {
-  const long long w = blockIdx.x * 256ll + threadIdx.x;
-  const long long tok = w / a.items;
-  if (tok >= (long long)a.batch * a.seq) return;
-  const int c = (int)(w % a.items);
-  const int b = (int)(tok / a.seq), s = (int)(tok % a.seq);
-  const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
-  float cs[NP], sn[NP];
-  if (it.turned) {
-    long long pos = s;
-    if (a.positions) {
-      const long long at = b * a.ps[0] + s * a.ps[1];
-      pos = a.positions_64 ? reinterpret_cast<const long long*>(a.positions)[at]
-                           : reinterpret_cast<const int*>(a.positions)[at];
-    }
-    item_angles<NP>(a.sp, pos, c, cs, sn);
+__global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ Args a) {
+  const int in_cta = threadIdx.x / a.items / a.head_lanes, sub = threadIdx.x / a.items % a.head_lanes;
+  const int tok = blockIdx.x * a.cta_tokens + in_cta;
+  if (in_cta >= a.cta_tokens || tok >= a.tokens) return;
+  const int b = tok / a.seq, s = tok % a.seq;
+  long long pos = s;
+  if (a.positions) {
+    const long long at = b * a.ps[0] + s * a.ps[1];
+    pos = a.positions_64 ? reinterpret_cast<const long long*>(a.positions)[at]
+                         : reinterpret_cast<const int*>(a.positions)[at];
   }
-  const int h1 = min((int)(blockIdx.y + 1) * a.head_group, a.t[0].heads + a.t[1].heads);
-#pragma unroll 2
-  for (int h = blockIdx.y * a.head_group; h < h1; ++h) {
-    const bool second = h >= a.t[0].heads;
-    const Rows& r = a.t[second];
-    const int hh = second ? h - a.t[0].heads : h;
-    float v[2 * NP];
-    load_item<T, NP>(reinterpret_cast<const T*>(r.x) + b * r.xs[0] + hh * r.xs[1] + s * r.xs[2], it, v);
-    if (it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
-    store_item<T, NP>(reinterpret_cast<T*>(r.out) + b * r.os[0] + hh * r.os[1] + s * r.os[2], it, v);
+  if (a.first) pos += a.first[b];
+  const int hq = a.t[0].heads, hl = a.head_lanes;
+  const int h0 = blockIdx.y * a.head_group, h1 = min(h0 + a.head_group, hq + a.t[1].heads);
+  const T* x0 = reinterpret_cast<const T*>(a.t[0].x) + b * a.t[0].xs[0] + s * a.t[0].xs[2];
+  const T* x1 = reinterpret_cast<const T*>(a.t[1].x) + b * a.t[1].xs[0] + s * a.t[1].xs[2];
+  T* y0 = reinterpret_cast<T*>(a.t[0].out) + b * a.t[0].os[0] + s * a.t[0].os[2];
+  T* y1 = reinterpret_cast<T*>(a.t[1].out) + b * a.t[1].os[0] + s * a.t[1].os[2];
+  for (int c = threadIdx.x % a.items; c < a.items; c += 256) {  // (more than 256 items: one token per CTA)
+    const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
+    float cs[NP], sn[NP];
+    if (it.turned) item_angles<NP>(a.sp, pos, c, cs, sn);
+    for (int h = h0 + sub; h < h1; h += kHeads * hl) {
+      Raw<T, NP> raw[kHeads];
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int x = h + u * hl;
+        if (x < h1) raw[u] = load_raw<T, NP>(x < hq ? x0 + x * a.t[0].xs[1] : x1 + (x - hq) * a.t[1].xs[1], it);
+      }
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int x = h + u * hl;
+        if (x >= h1) break;
+        float v[2 * NP];
+        widen<T, NP>(raw[u], v);
+        if (it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
+        store_item<T, NP>(x < hq ? y0 + x * a.t[0].os[1] : y1 + (x - hq) * a.t[1].os[1], it, v);
+      }
+    }
   }
 }
 
@@ -191,7 +247,7 @@ struct AppendArgs {
   float *ks, *vs;
   const int32_t *table, *lens, *new_lens;
   int32_t *lens_out, *bad;
-  int num_seqs, max_blocks, num_blocks, bs, dim, num_new, items, head_group, page_slots, q_ctas;
+  int num_seqs, max_blocks, num_blocks, bs, dim, num_new, items, head_group, head_lanes, cta_tokens, page_slots, page_heads, page_ctas, q_ctas, angles;
 };
 
 __device__ __forceinline__ int new_tokens(const AppendArgs& a, int s) {
@@ -220,41 +276,53 @@ __global__ void append_check_kernel(const __grid_constant__ AppendArgs a) {
   if (bad) atomicMin(a.bad, s);
 }
 
-// Pools of TO from rows of TI: one rounding, after the turn.  Thread = (token,
-// item) as in rotary_kernel, over query heads, key heads and value heads.
+// Pools of TO from rows of TI: one rounding, after the turn.  CTAs and threads as in rotary_kernel, over the query
+// heads, the key heads and the value heads of every token.
 template <typename TI, typename TO, int NP>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
-  const long long w = blockIdx.x * 256ll + threadIdx.x;
-  const long long tok = w / a.items;
-  if (tok >= (long long)a.num_seqs * a.num_new) return;
-  const int c = (int)(w % a.items);
-  const int s = (int)(tok / a.num_new), i = (int)(tok % a.num_new);
-  const bool first = c == 0 && blockIdx.y == 0;
+__global__ void __launch_bounds__(256, 3) append_kernel(const __grid_constant__ AppendArgs a) {
+  const int in_cta = threadIdx.x / a.items / a.head_lanes, sub = threadIdx.x / a.items % a.head_lanes;
+  const int tok = blockIdx.x * a.cta_tokens + in_cta;
+  if (in_cta >= a.cta_tokens || tok >= a.num_seqs * a.num_new) return;
+  const int s = tok / a.num_new, i = tok % a.num_new;
+  const bool first = threadIdx.x % a.items == 0 && sub == 0 && blockIdx.y == 0;
   if (first && i == 0) write_length(a, s);
   const long long pos = (long long)a.lens[s] + i;
   const bool there = i < new_tokens(a, s);
   const int page = there ? write_page(a, s, pos) : -1;
   if (there && page < 0 && first) skip_notice();
-  const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
-  float cs[NP], sn[NP];
-  if (it.turned) item_angles<NP>(a.sp, pos, c, cs, sn);
-  const int hq = a.q.heads, hk = a.k.heads;
-  const int h1 = min((int)(blockIdx.y + 1) * a.head_group, hq + 2 * hk);
-  const long long slot = ((long long)page * a.bs + pos % a.bs) * hk;
-#pragma unroll 2
-  for (int h = blockIdx.y * a.head_group; h < h1; ++h) {
-    float v[2 * NP];
-    if (h < hq) {
-      load_item<TI, NP>(reinterpret_cast<const TI*>(a.q.x) + s * a.q.xs[0] + h * a.q.xs[1] + i * a.q.xs[2], it, v);
-      if (it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
-      store_item<TI, NP>(reinterpret_cast<TI*>(a.q.out) + s * a.q.os[0] + h * a.q.os[1] + i * a.q.os[2], it, v);
-    } else if (page >= 0) {
-      const bool key = h < hq + hk;
-      const Rows& r = key ? a.k : a.v;
-      const int hh = key ? h - hq : h - hq - hk;
-      load_item<TI, NP>(reinterpret_cast<const TI*>(r.x) + s * r.xs[0] + hh * r.xs[1] + i * r.xs[2], it, v);
-      if (key && it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
-      store_item<TO, NP>(reinterpret_cast<TO*>(r.out) + (slot + hh) * a.dim, it, v);
+  const int hq = a.q.heads, hk = a.k.heads, hl = a.head_lanes, h0 = blockIdx.y * a.head_group;
+  const int h1 = min(h0 + a.head_group, page < 0 ? hq : hq + 2 * hk);
+  const TI* xq = reinterpret_cast<const TI*>(a.q.x) + s * a.q.xs[0] + i * a.q.xs[2];
+  const TI* xk = reinterpret_cast<const TI*>(a.k.x) + s * a.k.xs[0] + i * a.k.xs[2];
+  const TI* xv = reinterpret_cast<const TI*>(a.v.x) + s * a.v.xs[0] + i * a.v.xs[2];
+  TI* yq = reinterpret_cast<TI*>(a.q.out) + s * a.q.os[0] + i * a.q.os[2];
+  const long long slot = ((long long)page * a.bs + pos % a.bs) * hk * a.dim;
+  for (int c = threadIdx.x % a.items; c < a.items; c += 256) {
+    const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
+    float cs[NP], sn[NP];
+    if (it.turned && h0 < hq + hk) item_angles<NP>(a.sp, pos, c, cs, sn);
+    for (int h = h0 + sub; h < h1; h += kHeads * hl) {
+      Raw<TI, NP> raw[kHeads];
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int x = h + u * hl;
+        if (x < h1)
+          raw[u] = load_raw<TI, NP>(x < hq        ? xq + x * a.q.xs[1]
+                                    : x < hq + hk ? xk + (x - hq) * a.k.xs[1]
+                                                  : xv + (x - hq - hk) * a.v.xs[1],
+                                    it);
+      }
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int x = h + u * hl;
+        if (x >= h1) break;
+        float v[2 * NP];
+        widen<TI, NP>(raw[u], v);
+        if (it.turned && x < hq + hk) turn<NP>(v, cs, sn, a.sp.interleaved);
+        if (x < hq) store_item<TI, NP>(yq + x * a.q.os[1], it, v);
+        else if (x < hq + hk) store_item<TO, NP>(reinterpret_cast<TO*>(a.k.out) + slot + (x - hq) * a.dim, it, v);
+        else store_item<TO, NP>(reinterpret_cast<TO*>(a.v.out) + slot + (x - hq - hk) * a.dim, it, v);
+      }
     }
   }
 }
@@ -267,6 +335,11 @@ struct E4m3 {
   static constexpr bool kHasNan = true;
   __device__ static uint8_t code(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
   __device__ static float value(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
+  // four codes of values in range
+  __device__ static uint32_t code4(float a, float b, float c, float d) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+  }
 };
 struct Int8 {
   // 127 = 1.984375 * 2^6
@@ -276,7 +349,38 @@ struct Int8 {
   // (NaN becomes 0: the page's scale is NaN then)
   __device__ static uint8_t code(float x) { return (uint8_t)(int8_t)min(max(__float2int_rn(x), -127), 127); }
   __device__ static float value(uint8_t c) { return (float)(int8_t)c; }
+  // 1.5 * 2^23 + x holds x rounded to even in its low bits (the conversion instruction runs at a quarter of the rate)
+  __device__ static uint32_t code4(float a, float b, float c, float d) {
+    constexpr float kRound = 12582912.f;
+    const uint32_t ab = __byte_perm(__float_as_uint(a + kRound), __float_as_uint(b + kRound), 0x0040);
+    const uint32_t cd = __byte_perm(__float_as_uint(c + kRound), __float_as_uint(d + kRound), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
+  }
 };
+// Codes of v[0 .. N) * inv; `careful`: some may be out of range or not finite (infinities count as NaN, which neither
+// type tells apart).
+template <typename F, int N>
+__device__ __forceinline__ Bits<uint8_t, N> codes_of(const float* v, float inv, bool careful) {
+  uint32_t w[(N + 3) / 4];
+  if (careful) {
+#pragma unroll
+    for (int i = 0; i < (N + 3) / 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 4 && 4 * i + e < N; ++e)
+        w[i] |= (uint32_t)F::code(fabsf(v[4 * i + e]) <= FLT_MAX ? v[4 * i + e] * inv : NAN) << (8 * e);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < (N + 3) / 4; ++i) {
+      auto at = [&](int e) { return 4 * i + e < N ? v[4 * i + e] * inv : 0.f; };
+      w[i] = F::code4(at(0), at(1), at(2), at(3));
+    }
+  }
+  Bits<uint8_t, N> out;
+  memcpy(&out, w, sizeof(out));
+  return out;
+}
 
 // The scale's exponent for the largest finite magnitude `amax`.
 template <typename F>
@@ -287,126 +391,190 @@ __device__ __forceinline__ int scale_exp(float amax) {
 }
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }  // |k| <= 126
 
-// Of the rows that go into one page for one kv head: the items' values.
-template <typename TI, int NP>
-__device__ __forceinline__ void page_item(const AppendArgs& a, const Rows& r, bool key, int s, int h, int i, int c,
-                                          long long pos, float (&v)[2 * NP]) {
-  const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
-  load_item<TI, NP>(reinterpret_cast<const TI*>(r.x) + s * r.xs[0] + h * r.xs[1] + i * r.xs[2], it, v);
-  if (key && it.turned) {
-    float cs[NP], sn[NP];
-    item_angles<NP>(a.sp, pos, c, cs, sn);
-    turn<NP>(v, cs, sn, a.sp.interleaved);
-  }
-}
-
-// CTA = one page of one sequence that gets new tokens, one kv head, keys or
-// values; CTAs behind them turn the query.  All tokens of the page are one
-// CTA's, so its scale has one writer.
-template <typename TI, typename F, int NP>
-__global__ void __launch_bounds__(128) append8_kernel(const __grid_constant__ AppendArgs a) {
-  if (blockIdx.x < a.q_ctas) {
-    const long long w = blockIdx.x * 128ll + threadIdx.x;
-    const long long tok = w / a.items;
-    const int group = blockIdx.y;  // (gridDim.y groups of head_group heads)
-    if (tok >= (long long)a.num_seqs * a.num_new) return;
-    const int c = (int)(w % a.items), s = (int)(tok / a.num_new), i = (int)(tok % a.num_new);
+// The query's CTAs of append8_kernel (small calls): cta_tokens tokens and head_group heads.
+template <typename T, int NP>
+__device__ __forceinline__ void turn_query(const AppendArgs& a, int cta) {
+  const int in_cta = threadIdx.x / a.items;
+  const int tok = cta % a.q_ctas * a.cta_tokens + in_cta, h0 = cta / a.q_ctas * a.head_group;
+  if (in_cta >= a.cta_tokens || tok >= a.num_seqs * a.num_new) return;
+  const int s = tok / a.num_new, i = tok % a.num_new, h1 = min(h0 + a.head_group, a.q.heads);
+  const T* x = reinterpret_cast<const T*>(a.q.x) + s * a.q.xs[0] + i * a.q.xs[2];
+  T* y = reinterpret_cast<T*>(a.q.out) + s * a.q.os[0] + i * a.q.os[2];
+  for (int c = threadIdx.x % a.items; c < a.items; c += blockDim.x) {
     const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
     float cs[NP], sn[NP];
     if (it.turned) item_angles<NP>(a.sp, (long long)a.lens[s] + i, c, cs, sn);
-    for (int h = group * a.head_group; h < min((group + 1) * a.head_group, a.q.heads); ++h) {
+    for (int h = h0; h < h1; ++h) {
       float v[2 * NP];
-      load_item<TI, NP>(reinterpret_cast<const TI*>(a.q.x) + s * a.q.xs[0] + h * a.q.xs[1] + i * a.q.xs[2], it, v);
+      widen<T, NP>(load_raw<T, NP>(x + h * a.q.xs[1], it), v);
       if (it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
-      store_item<TI, NP>(reinterpret_cast<TI*>(a.q.out) + s * a.q.os[0] + h * a.q.os[1] + i * a.q.os[2], it, v);
+      store_item<T, NP>(y + h * a.q.os[1], it, v);
     }
+  }
+}
+
+constexpr int kPageThreads = 256;
+constexpr int kAngleBytes = 40960;  // of shared memory, at most
+
+// CTAs [0, page_ctas): one page of one sequence that gets new tokens, keys or values, and page_heads kv heads one
+// after another.  All tokens of a page and head are one CTA's, so a scale has one writer.  The sines of the page's
+// tokens are kept in shared memory for all of its heads (`angles` items of them, 0: formed again where they are
+// needed).  CTAs behind them turn the query.  A thread keeps its first item between the pass for the largest
+// magnitude and the one for the codes; a larger page's others are read twice.
+template <typename TI, typename F, int NP>
+__global__ void __launch_bounds__(kPageThreads, 3) append8_kernel(const __grid_constant__ AppendArgs a) {
+  if (blockIdx.x >= a.page_ctas) {
+    turn_query<TI, NP>(a, blockIdx.x - a.page_ctas);
     return;
   }
-  if (blockIdx.y) return;
-  const int hk = a.k.heads;
-  int x = blockIdx.x - a.q_ctas;
-  const int h = x % hk;
-  x /= hk;
+  extern __shared__ float2 table[];  // [pair of the item][item]
+  const int hk = a.k.heads, tid = threadIdx.x, threads = blockDim.x, lane = tid % 32;
+  const int groups = (hk + a.page_heads - 1) / a.page_heads;
+  int x = blockIdx.x;
+  const int h0 = x % groups * a.page_heads, h1 = min(h0 + a.page_heads, hk);
+  x /= groups;
   const bool key = x & 1;
   x >>= 1;
   const int j = x % a.page_slots, s = x / a.page_slots;
-  if (s >= a.num_seqs) return;
-  if (j == 0 && h == 0 && key && threadIdx.x == 0) write_length(a, s);
-  const int n = new_tokens(a, s);
   const long long len = a.lens[s];
+  const int n = new_tokens(a, s);
+  if (j == 0 && h0 == 0 && key && tid == 0) write_length(a, s);
   if (n == 0 || len < 0) {
-    if (n && j == 0 && threadIdx.x == 0) skip_notice();
+    if (n && j == 0 && tid == 0) skip_notice();
     return;
   }
   const long long p0 = (len / a.bs + j) * a.bs;  // the page's first position
   if (p0 >= len + n) return;
   const int page = write_page(a, s, p0);
   if (page < 0) {
-    if (threadIdx.x == 0) skip_notice();
+    if (tid == 0) skip_notice();
     return;
   }
-  const int old = (int)ll_max(len - p0, 0);                    // tokens that were there
+  const int old = (int)ll_max(len - p0, 0);                        // tokens that were there
   const int count = (int)(ll_min(len + n, p0 + a.bs) - p0) - old;  // new ones, in front of them i0 of the call's
   const int i0 = (int)(p0 + old - len);
   const Rows& r = key ? a.k : a.v;
-  const int total = count * a.items;
-  float v0[2 * NP];
-  float amax = 0.f;
-  bool odd = false;
-  for (int w = threadIdx.x; w < total; w += 128) {
-    float v[2 * NP];
-    const int i = i0 + w / a.items;
-    page_item<TI, NP>(a, r, key, s, h, i, w % a.items, len + i, v);
+  float* const scales = (key ? a.ks : a.vs) + (long long)page * hk;
+  const int pool_row = hk * a.dim;
+  uint8_t* const pool = reinterpret_cast<uint8_t*>(r.out) + (long long)page * a.bs * pool_row;
+  const TI* const rows = reinterpret_cast<const TI*>(r.x) + s * r.xs[0] + i0 * r.xs[2];
+  // Thread (i, c) has item c of the tokens i, i + step, ..
+  const int c = tid % a.items, step = threads / a.items, i = tid / a.items < step ? tid / a.items : count;
+  const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
+  const bool turns = key && it.turned;
+  if (key && a.angles) {
+    if (turns)
+      for (int w = i; w < count; w += step) {
+        float cs[NP], sn[NP];
+        item_angles<NP>(a.sp, len + i0 + w, c, cs, sn);
 #pragma unroll
-    for (int e = 0; e < 2 * NP; ++e) {
-      const float m = fabsf(v[e]);
-      const bool fin = m <= FLT_MAX;
-      amax = fin ? fmaxf(amax, m) : amax;
-      odd = odd || !fin;
-      if (w == threadIdx.x) v0[e] = v[e];
-    }
+        for (int e = 0; e < NP; ++e) table[e * a.angles + w * a.items + c] = make_float2(cs[e], sn[e]);
+      }
+    __syncthreads();
   }
-  float* scales = key ? a.ks : a.vs;
-  const float s_old = old ? scales[(long long)page * hk + h] : 0.f;  // (read by all before one of them writes it)
-  __shared__ float part[4];
-  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = amax;
-  odd = __syncthreads_or(odd);
-  amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-  uint8_t* pool = reinterpret_cast<uint8_t*>(r.out);
-  const long long row0 = (long long)page * a.bs * hk + h;
-  const float need = pow2(scale_exp<F>(amax));
-  float s_new = s_old > need ? s_old : need;
-  const float inv = 1.f / s_new;
-  // int8 has no NaN: a page that was given one has a NaN scale, until it is begun anew
-  if (!F::kHasNan && (odd || isnan(s_old))) s_new = NAN;
-  for (int w = threadIdx.x; w < total; w += 128) {
-    float v[2 * NP];
-    const int i = i0 + w / a.items;
-    if (w != threadIdx.x) {
-      page_item<TI, NP>(a, r, key, s, h, i, w % a.items, len + i, v);
+  auto load = [&](int h, int w) { return load_raw<TI, NP>(rows + h * r.xs[1] + w * r.xs[2], it); };
+  auto values = [&](const Raw<TI, NP>& raw, int w, float (&v)[2 * NP]) {
+    widen<TI, NP>(raw, v);
+    if (!turns) return;
+    float cs[NP], sn[NP];
+    if (a.angles) {
+#pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        const float2 x = table[e * a.angles + w * a.items + c];
+        cs[e] = x.x;
+        sn[e] = x.y;
+      }
     } else {
-#pragma unroll
-      for (int e = 0; e < 2 * NP; ++e) v[e] = v0[e];
+      item_angles<NP>(a.sp, len + i0 + w, c, cs, sn);
     }
-    const Item it = item_at<NP>(w % a.items, a.sp.rot, a.dim, a.sp.interleaved);
-    Vec<uint8_t, NP> c1, c2;
+    turn<NP>(v, cs, sn, a.sp.interleaved);
+  };
+  const bool any = i < count;
+  Raw<TI, NP> raw{};
+  if (any) raw = load(h0, i);
+  __shared__ uint32_t part[3][kPageThreads / 32];
+  const bool wide = a.dim % 16 == 0 && reinterpret_cast<uintptr_t>(r.out) % 16 == 0;
+  const int vecs = a.dim / 16;
+  const bool early = wide && old * vecs <= threads;
+  for (int h = h0; h < h1; ++h) {
+    uint8_t* const head = pool + h * a.dim;
+    const float s_old = old ? scales[h] : 0.f;  // (read by all before one of them writes it)
+    // Old codes are asked for before it is known whether they are needed: a decode step would wait for them otherwise.
+    uint4 codes = make_uint4(0, 0, 0, 0);
+    if (early && tid < old * vecs)
+      codes = *reinterpret_cast<const uint4*>(head + tid / vecs * pool_row + tid % vecs * 16);
+    float v[2 * NP];
+    values(raw, any ? i : 0, v);
+    if (h + 1 < h1 && any) raw = load(h + 1, i);
+    uint32_t amax = 0;  // magnitudes as integers order like the floats; infinities and NaN are above them
+    if (any) {
 #pragma unroll
-    for (int e = 0; e < NP; ++e) {
-      // (infinities count as NaN: neither type has them)
-      c1.e[e] = F::code(fabsf(v[e]) <= FLT_MAX ? v[e] * inv : NAN);
-      c2.e[e] = F::code(fabsf(v[NP + e]) <= FLT_MAX ? v[NP + e] * inv : NAN);
+      for (int e = 0; e < 2 * NP; ++e) amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
     }
-    uint8_t* row = pool + (row0 + (long long)(old + w / a.items) * hk) * a.dim;
-    *reinterpret_cast<Vec<uint8_t, NP>*>(row + it.o1) = c1;
-    if (it.second) *reinterpret_cast<Vec<uint8_t, NP>*>(row + it.o2) = c2;
-  }
-  if (threadIdx.x == 0 && !(old && s_new == s_old)) scales[(long long)page * hk + h] = s_new;
-  if (old && s_new > s_old) {  // (never with a NaN)
+    for (int w = i + step; w < count; w += step) {
+      float o[2 * NP];
+      values(load(h, w), w, o);
+#pragma unroll
+      for (int e = 0; e < 2 * NP; ++e) amax = max(amax, __float_as_uint(o[e]) & 0x7fffffffu);
+    }
+    auto block_max = [&](uint32_t m, uint32_t* at) {
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (lane == 0) at[tid / 32] = m;
+      __syncthreads();
+      return __reduce_max_sync(0xffffffffu, lane < threads / 32 ? at[lane] : 0u);
+    };
+    amax = block_max(amax, part[(h - h0) & 1]);  // (two places in turn: one barrier a head)
+    const bool odd = amax >= 0x7f800000u;
+    if (odd) {  // the scale goes by the finite ones
+      uint32_t m = 0;
+      auto finite = [&](float f) { m = fabsf(f) <= FLT_MAX ? max(m, __float_as_uint(f) & 0x7fffffffu) : m; };
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < 2 * NP; ++e) finite(v[e]);
+      }
+      for (int w = i + step; w < count; w += step) {
+        float o[2 * NP];
+        values(load(h, w), w, o);
+#pragma unroll
+        for (int e = 0; e < 2 * NP; ++e) finite(o[e]);
+      }
+      amax = block_max(m, part[2]);
+      __syncthreads();
+    }
+    const int k = scale_exp<F>(__uint_as_float(amax));
+    const float need = pow2(k);
+    float s_new = s_old > need ? s_old : need;
+    const float inv = 1.f / s_new;
+    // int8 has no NaN: a page that was given one has a NaN scale, until it is begun anew
+    if (!F::kHasNan && (odd || isnan(s_old))) s_new = NAN;
+    const bool careful = odd || k == F::kTop;
+    auto write = [&](int w, const float* f) {
+      uint8_t* row = head + (old + w) * pool_row;
+      *reinterpret_cast<Bits<uint8_t, NP>*>(row + it.o1) = codes_of<F, NP>(f, inv, careful);
+      if (it.second) *reinterpret_cast<Bits<uint8_t, NP>*>(row + it.o2) = codes_of<F, NP>(f + NP, inv, careful);
+    };
+    if (any) write(i, v);
+    for (int w = i + step; w < count; w += step) {
+      float o[2 * NP];
+      values(load(h, w), w, o);
+      write(w, o);
+    }
+    if (tid == 0 && !(old && s_new == s_old)) scales[h] = s_new;
+    if (!(old && s_new > s_old)) continue;  // (a NaN: the old codes stay)
     const float ratio = s_old / s_new;
-    for (int w = threadIdx.x; w < old * a.dim; w += 128) {
-      uint8_t* at = pool + (row0 + (long long)(w / a.dim) * hk) * a.dim + w % a.dim;
-      *at = F::code(F::value(*at) * ratio);
+    if (wide) {
+      for (int w = tid; w < old * vecs; w += threads) {
+        uint8_t* at = head + w / vecs * pool_row + w % vecs * 16;
+        Vec<uint8_t, 16> c = unpack<uint8_t, 16>(early ? codes : *reinterpret_cast<const uint4*>(at));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) c.e[e] = F::code(F::value(c.e[e]) * ratio);
+        store_vec<uint8_t, 16>(at, c);
+      }
+    } else {
+      for (int w = tid; w < old * a.dim; w += threads) {
+        uint8_t* at = head + w / a.dim * pool_row + w % a.dim;
+        *at = F::code(F::value(*at) * ratio);
+      }
     }
   }
 }
@@ -420,46 +588,57 @@ struct GatherArgs {
   int num_seqs, max_blocks, num_blocks, bs, hk, dim, count, vecs;
 };
 
-template <typename F, typename TO>
-__device__ __forceinline__ TO gather_value(const void* pool, long long at, float scale) {
-  if constexpr (std::is_same<F, E4m3>::value || std::is_same<F, Int8>::value)
-    return from_f32<TO>(F::value(reinterpret_cast<const uint8_t*>(pool)[at]) * scale);
-  else
-    return from_f32<TO>(to_f32(reinterpret_cast<const F*>(pool)[at]));
-}
+template <typename F>
+struct Stored {
+  using T = F;
+  static constexpr bool kCode = false;
+  __device__ static float value(F x, float) { return to_f32(x); }
+};
+template <>
+struct Stored<E4m3> {
+  using T = uint8_t;
+  static constexpr bool kCode = true;
+  __device__ static float value(uint8_t x, float scale) { return E4m3::value(x) * scale; }
+};
+template <>
+struct Stored<Int8> {
+  using T = uint8_t;
+  static constexpr bool kCode = true;
+  __device__ static float value(uint8_t x, float scale) { return Int8::value(x) * scale; }
+};
 
-// Thread = NV elements of one token's kv head, of keys (blockIdx.y 0) or
-// values; positions outside the sequence give zeros.
+// Thread = NV elements of one token's kv head of sequence blockIdx.y, of keys (blockIdx.z 0) or values; positions
+// outside the sequence give zeros.
 template <typename F, typename TO, int NV>
 __global__ void __launch_bounds__(256) gather_tokens_kernel(const __grid_constant__ GatherArgs a) {
-  const long long w = blockIdx.x * 256ll + threadIdx.x;
-  const long long per_tok = (long long)a.hk * a.vecs;
-  const long long t = w / per_tok;
-  if (t >= (long long)a.num_seqs * a.count) return;
-  const int x = (int)(w % per_tok), h = x / a.vecs, e = x % a.vecs * NV;
-  const int s = (int)(t / a.count);
-  const long long pos = (a.starts ? a.starts[s] : 0ll) + t % a.count;
+  using S = typename Stored<F>::T;
+  const int s = blockIdx.y, len = a.lens[s];
+  const long long start = a.starts ? a.starts[s] : 0ll;
+  const unsigned per_tok = (unsigned)a.hk * a.vecs;
+  const unsigned w = blockIdx.x * 256u + threadIdx.x;  // (the launch has less than 2^32 of a sequence)
+  const unsigned i = w / per_tok, x = w % per_tok;
+  const long long pos = start + i;
+  if (i >= (unsigned)a.count) return;
+  const int h = (int)(x / a.vecs), e = (int)(x % a.vecs) * NV;
   Vec<TO, NV> o;
 #pragma unroll
   for (int j = 0; j < NV; ++j) o.e[j] = from_f32<TO>(0.f);
-  if (pos >= 0 && pos < a.lens[s]) {
+  if (pos >= 0 && pos < len) {
     if (pos / a.bs >= a.max_blocks) {
       atomicCAS(&g_notice, 0, kNoticeTableOverrun);
     } else {
-      const long long page = paged_phys_page(a.table[(long long)s * a.max_blocks + pos / a.bs], a.num_blocks);
-      const long long at = ((page * a.bs + pos % a.bs) * a.hk + h) * a.dim + e;
-      const void* pool = blockIdx.y ? a.v : a.k;
-      float scale = 1.f;
-      constexpr bool bits8 = std::is_same<F, E4m3>::value || std::is_same<F, Int8>::value;
-      if (bits8) scale = (blockIdx.y ? a.vs : a.ks)[page * a.hk + h];
-      using S = typename std::conditional<bits8, uint8_t, F>::type;
-      const Vec<S, NV> in = *reinterpret_cast<const Vec<S, NV>*>(reinterpret_cast<const S*>(pool) + at);
+      const int p = (int)pos;
+      const long long page = paged_phys_page(a.table[(long long)s * a.max_blocks + p / a.bs], a.num_blocks);
+      const S* pool = reinterpret_cast<const S*>(blockIdx.z ? a.v : a.k);
+      const Vec<S, NV> in = unpack<S, NV>(
+          *reinterpret_cast<const Bits<S, NV>*>(pool + ((page * a.bs + p % a.bs) * a.hk + h) * a.dim + e));
+      const float scale = Stored<F>::kCode ? (blockIdx.z ? a.vs : a.ks)[page * a.hk + h] : 1.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) o.e[j] = gather_value<F, TO>(&in, j, scale);
+      for (int j = 0; j < NV; ++j) o.e[j] = from_f32<TO>(Stored<F>::value(in.e[j], scale));
     }
   }
-  TO* out = reinterpret_cast<TO*>(blockIdx.y ? a.vo : a.ko);
-  *reinterpret_cast<Vec<TO, NV>*>(out + (t * a.hk + h) * a.dim + e) = o;
+  TO* out = reinterpret_cast<TO*>(blockIdx.z ? a.vo : a.ko) + (((long long)s * a.count + i) * a.hk + h) * a.dim + e;
+  store_vec<TO, NV>(out, o);
 }
 
 // -------------------------------------------------------------------- host --
@@ -493,12 +672,43 @@ static Rows make_rows(const void* x, const int64_t* xs, void* out, const int64_t
   return r;
 }
 
-// Heads per thread: as many as leave about two waves of threads, so that the sines are shared but no SM is idle.
-static int head_group(long long threads, int heads) {
-  const long long want = 148ll * 2048 * 2;
-  long long groups = ll_min(heads, ll_max(1, (want + threads - 1) / threads));
-  groups = ll_min(groups, 65535);
-  return (int)((heads + groups - 1) / groups);
+// Items of a CTA of `threads` threads: whole tokens (one where a token has more items than that).
+static int cta_tokens(int items, int threads) { return items >= threads ? 1 : threads / items; }
+
+// Head lanes of a tensor with these strides (rotary_kernel).
+static int head_lanes(const Rows& r, int heads, int items) {
+  return heads >= 4 && items * 4 <= 256 && r.xs[1] < r.xs[2] ? 4 : 1;
+}
+
+// Heads per CTA, for `ctas` CTAs of 256 threads that three of an SM hold at a time: one group of all heads (the sines
+// are shared) unless that leaves SMs idle; above a wave, few enough groups that the last wave is nearly full (B4 S8192
+// Hq32 Hkv8, tokens of a head side by side: 114 us in 2.3 waves, 109 in 6.9; where heads lie side by side, their groups
+// would come to the same memory at different times: 112 us in one, 130 in two).  A head for each lane at least.
+static int head_group(int ctas, int heads, int lanes) {
+  const int wave = 148 * 3, most = heads / lanes > 1 ? heads / lanes : 1;
+  int groups = wave / ctas < most ? (wave / ctas > 1 ? wave / ctas : 1) : most;
+  for (int g = groups; g <= most && g < groups + 4 && lanes == 1 && ctas > wave / 2; ++g) {
+    const double waves = (double)ctas * g / wave;
+    if (waves > 1 && (long long)waves + 1 <= 1.06 * waves) {
+      groups = g;
+      break;
+    }
+  }
+  const int group = (heads + groups - 1) / groups;
+  const int least = (heads + 65534) / 65535;  // (a grid dimension)
+  return (group + lanes - 1) / lanes * lanes > least ? (group + lanes - 1) / lanes * lanes : least;
+}
+
+template <typename T, int NP>
+static void launch_rotary(Args& a, cudaStream_t st) {
+  const int heads = a.t[0].heads + a.t[1].heads;
+  a.items = items_of(NP, a.sp.rot, a.dim);
+  a.head_lanes = head_lanes(a.t[a.t[0].heads ? 0 : 1], heads, a.items);
+  a.cta_tokens = cta_tokens(a.items * a.head_lanes, 256);
+  const int ctas = (a.tokens - 1) / a.cta_tokens + 1;
+  a.head_group = head_group(ctas, heads, a.head_lanes);
+  const dim3 grid(ctas, (heads + a.head_group - 1) / a.head_group);
+  rotary_kernel<T, NP><<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace rotary
@@ -541,7 +751,8 @@ int attn_rotary(const attn_rotary_params_t* p, void* stream) {
   a.positions = p->positions;
   a.positions_64 = p->positions_64;
   a.ps[0] = p->position_strides[0]; a.ps[1] = p->position_strides[1];
-  a.batch = p->batch; a.seq = p->seq; a.dim = p->head_dim;
+  if (tokens > INT_MAX) return ATTN_ERR_UNSUPPORTED;
+  a.tokens = (int)tokens; a.seq = p->seq; a.dim = p->head_dim;
   const int es = (int)dtype_size(p->dtype);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto ok = [&](int np) {
@@ -550,15 +761,7 @@ int attn_rotary(const attn_rotary_params_t* p, void* stream) {
       if (r.heads && !(fits(r.x, r.xs, es, np * es) && fits(r.out, r.os, es, np * es))) return false;
     return true;
   };
-#define LAUNCH(T, NP)                                                                  \
-  do {                                                                                 \
-    a.items = items_of(NP, a.sp.rot, a.dim);                                           \
-    const long long threads = tokens * a.items;                                        \
-    if ((threads + 255) / 256 > INT_MAX) return ATTN_ERR_UNSUPPORTED;                  \
-    a.head_group = head_group(threads, heads);                                         \
-    const dim3 grid((unsigned)((threads + 255) / 256), (heads + a.head_group - 1) / a.head_group); \
-    rotary_kernel<T, NP><<<grid, 256, 0, st>>>(a);                                     \
-  } while (0)
+#define LAUNCH(T, NP) launch_rotary<T, NP>(a, st)
 #define CALL(NP)                                              \
   do {                                                        \
     if (p->dtype == ATTN_F32) LAUNCH(float, (NP > 4 ? 4 : NP)); \
@@ -605,27 +808,48 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
     return !a.q.heads || (fits(a.q.x, a.q.xs, es, np * es) && fits(a.q.out, a.q.os, es, np * es));
   };
   const long long tokens = (long long)a.num_seqs * a.num_new;
+  if (tokens > INT_MAX) return ATTN_ERR_UNSUPPORTED;
+  int launches = 1;
 #define WIDE(TI, TO, NP)                                                               \
   do {                                                                                 \
     a.items = items_of(NP, a.sp.rot, a.dim);                                           \
-    const long long threads = tokens * a.items;                                        \
     const int heads = a.q.heads + 2 * a.k.heads;                                       \
-    if ((threads + 255) / 256 > INT_MAX) return ATTN_ERR_UNSUPPORTED;                  \
-    a.head_group = head_group(threads, heads);                                         \
-    const dim3 grid((unsigned)((threads + 255) / 256), (heads + a.head_group - 1) / a.head_group); \
+    a.head_lanes = head_lanes(a.k, heads, a.items);                                    \
+    a.cta_tokens = cta_tokens(a.items * a.head_lanes, 256);                            \
+    const int ctas = (int)((tokens - 1) / a.cta_tokens + 1);                           \
+    a.head_group = head_group(ctas, heads, a.head_lanes);                              \
+    const dim3 grid(ctas, (heads + a.head_group - 1) / a.head_group); \
     append_kernel<TI, TO, NP><<<grid, 256, 0, st>>>(a);                                \
   } while (0)
 #define BITS8(TI, F, NP)                                                               \
   do {                                                                                 \
     a.items = items_of(NP, a.sp.rot, a.dim);                                           \
     a.page_slots = (int)(((long long)a.num_new + a.bs - 1) / a.bs) + 1;                \
-    const long long pages = (long long)a.num_seqs * a.page_slots * 2 * a.k.heads;      \
-    const long long qc = a.q.heads ? (tokens * a.items + 127) / 128 : 0;               \
-    if (pages + qc > INT_MAX) return ATTN_ERR_UNSUPPORTED;                             \
-    a.q_ctas = (int)qc;                                                                \
-    a.head_group = a.q.heads ? head_group(tokens * a.items, a.q.heads) : 1;            \
-    const dim3 grid((unsigned)(pages + qc), a.q.heads ? (a.q.heads + a.head_group - 1) / a.head_group : 1); \
-    append8_kernel<TI, F, NP><<<grid, 128, 0, st>>>(a);                                \
+    if (a.items > kPageThreads) return ATTN_ERR_UNSUPPORTED;                           \
+    const long long most = ll_min(a.num_new, a.bs) * (long long)a.items;               \
+    const int threads = (int)ll_min(kPageThreads, ll_max(128, (most + 31) / 32 * 32)); \
+    a.angles = a.sp.rot && most * NP * 8 <= kAngleBytes ? (int)most : 0;               \
+    a.cta_tokens = cta_tokens(a.items, threads);                                       \
+    /* a large query has a launch of its own, whose threads hold more loads in flight */ \
+    if (a.q.heads && tokens * a.q.heads >= (1 << 15)) {                                \
+      Args r{};                                                                        \
+      r.t[0] = a.q; r.t[1] = a.q; r.t[1].heads = 0;                                    \
+      r.sp = a.sp; r.first = a.lens;                                                   \
+      r.tokens = (int)tokens; r.seq = a.num_new; r.dim = a.dim;                        \
+      launch_rotary<TI, NP>(r, st);                                                    \
+      a.q.heads = 0;                                                                   \
+      ++launches;                                                                      \
+    }                                                                                  \
+    a.q_ctas = (int)((tokens + a.cta_tokens - 1) / a.cta_tokens);                      \
+    a.head_group = a.q.heads ? head_group(a.q_ctas, a.q.heads, 1) : 1;                 \
+    const long long groups = (a.q.heads + a.head_group - 1) / a.head_group;            \
+    const long long slots = (long long)a.num_seqs * a.page_slots * 2;                  \
+    /* heads of a CTA: as many as leave about 16 CTAs per SM */                        \
+    a.page_heads = (int)ll_max(1, ll_min(a.k.heads, slots * a.k.heads / (148 * 16)));   \
+    const long long pages = slots * ((a.k.heads + a.page_heads - 1) / a.page_heads);   \
+    if (pages + a.q_ctas * groups > INT_MAX) return ATTN_ERR_UNSUPPORTED;              \
+    a.page_ctas = (int)pages;                                                          \
+    append8_kernel<TI, F, NP><<<(unsigned)(pages + a.q_ctas * groups), threads, a.angles * NP * 8, st>>>(a); \
   } while (0)
 #define POOL(TI, NP)                                                    \
   do {                                                                  \
@@ -648,7 +872,7 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
 #undef POOL
 #undef BITS8
 #undef WIDE
-  return launch_status();
+  return launch_status(launches);
 }
 
 int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream) {
@@ -669,13 +893,14 @@ int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream) 
   const uintptr_t in = addr(a.k) | addr(a.v), out = addr(a.ko) | addr(a.vo);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = a.dim % 4 == 0 && in % (4 * pi) == 0 && out % (4 * po) == 0;
-  const bool wider = bits8 && po == 2 && a.dim % 8 == 0 && in % 8 == 0 && out % 16 == 0;
+  const bool wider = bits8 && a.dim % 16 == 0 && (in | out) % 16 == 0;
+  if (a.num_seqs > 65535) return ATTN_ERR_UNSUPPORTED;  // (a grid dimension)
 #define RUN(F, TO, NV)                                                                 \
   do {                                                                                 \
     a.vecs = a.dim / NV;                                                               \
-    const long long n = ((long long)a.num_seqs * a.count * a.hk * a.vecs + 255) / 256; \
-    if (n > INT_MAX) return ATTN_ERR_UNSUPPORTED;                                      \
-    gather_tokens_kernel<F, TO, NV><<<dim3((unsigned)n, 2), 256, 0, st>>>(a);          \
+    const long long n = ((long long)a.count * a.hk * a.vecs + 255) / 256;              \
+    if (n > (1 << 24) - 1) return ATTN_ERR_UNSUPPORTED;                                \
+    gather_tokens_kernel<F, TO, NV><<<dim3((unsigned)n, a.num_seqs, 2), 256, 0, st>>>(a); \
   } while (0)
 #define TO_(F, NV)                                             \
   do {                                                         \
@@ -688,11 +913,10 @@ int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream) 
     if (wide) TO_(F, 4); \
     else TO_(F, 1);     \
   } while (0)
-#define W8(F)                                                    \
-  do {                                                           \
-    if (wider && p->dtype == ATTN_BF16) RUN(F, __nv_bfloat16, 8); \
-    else if (wider) RUN(F, __half, 8);                           \
-    else W(F);                                                   \
+#define W8(F)               \
+  do {                      \
+    if (wider) TO_(F, 16);  \
+    else W(F);              \
   } while (0)
   switch (p->pool_format) {
     case ATTN_F32: W(float); break;

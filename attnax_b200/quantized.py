@@ -21,9 +21,8 @@ import torch
 
 from . import _lib
 from ._spec import dtype_code
-from .flash import softmax_scale
 from .paged import PagedKVCache
-from .paged_rows import _bound, check_tables, on_device, paged_window_attention
+from .paged_rows import _bound, _scale, check_tables, on_device, paged_window_attention
 from .rotary import RotaryPlan, check_plan, plan_spec, unit_stride
 
 _FORMATS = {torch.float8_e4m3fn: _lib.POOL_E4M3, torch.int8: _lib.POOL_INT8}
@@ -105,7 +104,48 @@ def _need_cuda(cache):
 def _scales(cache):
     if isinstance(cache, QuantizedPagedKVCache):
         return cache.key_scales.data_ptr(), cache.value_scales.data_ptr()
-    return None, None
+    return 0, 0
+
+
+def _with_lengths(cache, lengths: torch.Tensor):
+    """The cache with other lengths (dataclasses.replace without its host time)."""
+    new = object.__new__(type(cache))
+    new.__dict__.update(cache.__dict__, seq_lengths=lengths)
+    return new
+
+
+_append_params = _lib.packer(_lib.PagedAppendParams)
+_gather_params = _lib.packer(_lib.PagedGatherParams)
+_attend_params = _lib.packer(_lib.PagedAttend8Params)
+_NO_QUERY = (0, 0, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _check_append(cache, n: int, hk: int, d: int, keys, values, query, rotary):
+    dev = cache.key_pool.device
+    for name, x in (("keys", keys), ("values", values)):
+        if not isinstance(x, torch.Tensor) or x.dim() != 4 or x.shape[0] != n or x.shape[1] != hk or x.shape[3] != d:
+            raise ValueError(f"{name} must have shape ({n}, {hk}, T, {d}), got {tuple(getattr(x, 'shape', ()))}")
+        if x.device != dev:
+            raise RuntimeError(f"{name} must be on the cache's device")
+    if keys.shape != values.shape:
+        raise ValueError(f"keys shape {tuple(keys.shape)} != values shape {tuple(values.shape)}")
+    if keys.dtype != values.dtype:
+        raise ValueError(f"keys are {keys.dtype}, values {values.dtype}")
+    dtype_code(keys.dtype)
+    t = keys.shape[2]
+    if query is not None:
+        if not isinstance(query, torch.Tensor) or query.dim() != 4 or query.shape[0] != n or query.shape[2] != t \
+                or query.shape[3] != d:
+            raise ValueError(f"query must have shape ({n}, Hq, {t}, {d}), got {tuple(getattr(query, 'shape', ()))}")
+        if query.dtype != keys.dtype:
+            raise ValueError(f"query is {query.dtype}, keys {keys.dtype}")
+        if query.device != dev:
+            raise RuntimeError("query must be on the cache's device")
+        if rotary is None:
+            raise ValueError("query needs a rotary plan")
+    if rotary is not None:
+        check_plan(rotary, d, dev)
+    _need_cuda(cache)
 
 
 def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_lengths=None,
@@ -130,52 +170,28 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     ``_lib.device_status()`` (``NOTICE_PAGE_LIST``; lengths still count them).
     """
     pool, (n, width), fmt = _checked(cache)
-    dev = cache.key_pool.device
-    hk, d = pool[2], pool[3]
-    for name, x in (("keys", keys), ("values", values)):
-        if not isinstance(x, torch.Tensor) or x.dim() != 4 or x.shape[0] != n or x.shape[1] != hk or x.shape[3] != d:
-            raise ValueError(f"{name} must have shape ({n}, {hk}, T, {d}), got {tuple(getattr(x, 'shape', ()))}")
-        if x.device != dev:
-            raise RuntimeError(f"{name} must be on the cache's device")
-    if keys.shape != values.shape:
-        raise ValueError(f"keys shape {tuple(keys.shape)} != values shape {tuple(values.shape)}")
-    if keys.dtype != values.dtype:
-        raise ValueError(f"keys are {keys.dtype}, values {values.dtype}")
-    code, t = dtype_code(keys.dtype), keys.shape[2]
-    if query is not None:
-        if not isinstance(query, torch.Tensor) or query.dim() != 4 or query.shape[0] != n or query.shape[2] != t \
-                or query.shape[3] != d:
-            raise ValueError(f"query must have shape ({n}, Hq, {t}, {d}), got {tuple(getattr(query, 'shape', ()))}")
-        if query.dtype != keys.dtype:
-            raise ValueError(f"query is {query.dtype}, keys {keys.dtype}")
-        if query.device != dev:
-            raise RuntimeError("query must be on the cache's device")
-        if rotary is None:
-            raise ValueError("query needs a rotary plan")
-    if rotary is not None:
-        check_plan(rotary, d, dev)
-    _need_cuda(cache)
+    kp, vp = cache.key_pool, cache.value_pool
+    dev = kp.device
+    _check_append(cache, n, pool[2], pool[3], keys, values, query, rotary)
     if new_lengths is not None:
         new_lengths = on_device(new_lengths, dev)
         if new_lengths.shape != (n,):
             raise ValueError(f"new_lengths must have shape ({n},), got {tuple(new_lengths.shape)}")
+    t = keys.shape[2]
     if n == 0 or t == 0:
         if check and n and new_lengths is not None and bool((new_lengths != 0).any()):
             raise ValueError("new_lengths counts tokens that are not there")
         return cache if query is None else (cache, torch.empty_like(query))
     k, v = unit_stride(keys), unit_stride(values)
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    ks, vs = _scales(cache)
-    p = _lib.PagedAppendParams(code, fmt, *pool, cache.key_pool.data_ptr(), cache.value_pool.data_ptr(), ks, vs, n,
-                               width, bt.data_ptr(), sl.data_ptr(), k.data_ptr(), v.data_ptr(), k.stride()[:3],
-                               v.stride()[:3], t, None if new_lengths is None else new_lengths.data_ptr(),
-                               plan_spec(rotary))
-    q = q_out = None
-    if query is not None and query.shape[1]:
+    q_out, q_args = None, _NO_QUERY
+    if query is not None:
         q = unit_stride(query)
         q_out = torch.empty_like(q)
-        p.num_heads_q, p.q, p.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
-        p.q_strides, p.q_out_strides = q.stride()[:3], q_out.stride()[:3]
+        q_args = (q.shape[1], q.data_ptr(), q_out.data_ptr(), *q.stride()[:3], *q_out.stride()[:3])
+    p = _append_params(dtype_code(keys.dtype), fmt, *pool, kp.data_ptr(), vp.data_ptr(), *_scales(cache), n, width,
+                       bt.data_ptr(), sl.data_ptr(), k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], t,
+                       0 if new_lengths is None else new_lengths.data_ptr(), *plan_spec(rotary), *q_args, 0, 0)
     if check:
         bad = torch.full((), 2**31 - 1, dtype=torch.int32, device=dev)
         p.bad = bad.data_ptr()
@@ -188,14 +204,8 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     p.lengths_out = out.data_ptr()
     _lib.run("attn_paged_append_tokens", dev, C.byref(p))
     del bt, sl, k, v
-    if isinstance(cache, QuantizedPagedKVCache):
-        new = QuantizedPagedKVCache(cache.key_pool, cache.value_pool, cache.key_scales, cache.value_scales,
-                                    cache.block_table, out)
-    else:
-        new = PagedKVCache(cache.key_pool, cache.value_pool, cache.block_table, out)
-    if query is None:
-        return new
-    return new, (q_out if q is not None else torch.empty_like(query))
+    new = _with_lengths(cache, out)
+    return new if query is None else (new, q_out)
 
 
 def _gather(cache, pool, rows, fmt, starts, count: int, dtype):
@@ -204,10 +214,9 @@ def _gather(cache, pool, rows, fmt, starts, count: int, dtype):
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
     k = torch.empty((n, count, pool[2], pool[3]), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    ks, vs = _scales(cache)
-    p = _lib.PagedGatherParams(dtype_code(dtype), fmt, *pool, cache.key_pool.data_ptr(), cache.value_pool.data_ptr(),
-                               ks, vs, n, width, bt.data_ptr(), sl.data_ptr(),
-                               None if starts is None else starts.data_ptr(), count, k.data_ptr(), v.data_ptr())
+    p = _gather_params(dtype_code(dtype), fmt, *pool, cache.key_pool.data_ptr(), cache.value_pool.data_ptr(),
+                       *_scales(cache), n, width, bt.data_ptr(), sl.data_ptr(),
+                       0 if starts is None else starts.data_ptr(), count, k.data_ptr(), v.data_ptr())
     _lib.run("attn_paged_gather_tokens", dev, C.byref(p))
     del bt, sl
     return k, v
@@ -279,9 +288,9 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
     out = torch.empty_like(q)
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
     ctx = min(_bound(cache, max_context), rows[1] * bs)
-    p = _lib.PagedAttend8Params(code, fmt, n, hq, hk, d, t, nb, bs, rows[1], ctx, q.data_ptr(), kp.data_ptr(),
-                                vp.data_ptr(), cache.key_scales.data_ptr(), cache.value_scales.data_ptr(),
-                                bt.data_ptr(), sl.data_ptr(), out.data_ptr(), softmax_scale(d))
+    p = _attend_params(code, fmt, n, hq, hk, d, t, nb, bs, rows[1], ctx, q.data_ptr(), kp.data_ptr(), vp.data_ptr(),
+                       cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), bt.data_ptr(), sl.data_ptr(),
+                       out.data_ptr(), _scale(d), 0, 0)
     nbytes = _lib.load().attn_paged_attend8_workspace_size(C.byref(p))
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -124,13 +124,18 @@ def check_plan(plan: RotaryPlan, head_dim: int, device):
 
 
 def plan_spec(plan: RotaryPlan | None):
+    """The flattened ``attn_rotary_spec_t``."""
     if plan is None:
-        return _lib.RotarySpec(None, 0, 0, 1.0)
-    return _lib.RotarySpec(plan.turns.data_ptr(), plan.rotary_dim, int(plan.interleaved), plan.magnitude)
+        return 0, 0, 0, 1.0
+    return plan.turns.data_ptr(), 2 * plan.turns.shape[0], plan.interleaved, plan.magnitude
 
 
 def unit_stride(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
+
+
+_params = _lib.packer(_lib.RotaryParams)
+_NO_STRIDES = (0, 0, 0)
 
 
 def _launch(q, k, turns, interleaved, magnitude, positions, inverse):
@@ -139,23 +144,19 @@ def _launch(q, k, turns, interleaved, magnitude, positions, inverse):
     q_out = torch.empty_like(q)
     b, hq, s, d = q.shape
     if k is None:
-        key, hk = (None, None), 0
-        ks = kos = (0, 0, 0)
-        k_out = None
+        k_out, hk, kp, kop, ks, kos = None, 0, 0, 0, _NO_STRIDES, _NO_STRIDES
     else:
         k = unit_stride(k)
         k_out = torch.empty_like(k)
-        key, hk = (k.data_ptr(), k_out.data_ptr()), k.shape[1]
-        ks, kos = k.stride()[:3], k_out.stride()[:3]
+        hk, kp, kop, ks, kos = k.shape[1], k.data_ptr(), k_out.data_ptr(), k.stride()[:3], k_out.stride()[:3]
     if positions is None:
-        pos, wide, ps = None, 0, (0, 0)
+        pos, wide, ps = 0, 0, (0, 0)
     else:
-        pos, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
-        ps = (positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1))
-    p = _lib.RotaryParams(dtype_code(q.dtype), b, s, d, hq, hk, q.data_ptr(), q_out.data_ptr(), *key, q.stride()[:3],
-                          q_out.stride()[:3], ks, kos,
-                          _lib.RotarySpec(turns.data_ptr(), 2 * turns.shape[0], interleaved, magnitude), inverse, pos,
-                          wide, ps)
+        pos, wide = positions.data_ptr(), positions.dtype is torch.int64
+        ps = positions.stride() if positions.shape[0] > 1 else (0, positions.stride(1))
+    p = _params(dtype_code(q.dtype), b, s, d, hq, hk, q.data_ptr(), q_out.data_ptr(), kp, kop, *q.stride()[:3],
+                *q_out.stride()[:3], *ks, *kos, turns.data_ptr(), 2 * turns.shape[0], interleaved, magnitude, inverse,
+                pos, wide, *ps)
     _lib.run("attn_rotary", q.device, C.byref(p))
     return q_out, k_out
 
@@ -177,11 +178,11 @@ class _Rotary(torch.autograd.Function):
         interleaved, magnitude, inverse = ctx.how
         gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
         if gq is not None and gk is not None:
-            gq, gk = _turned(gq, gk, turns, positions, interleaved, magnitude, 1 - inverse)
+            gq, gk = _turned(gq, gk, turns, positions, interleaved, magnitude, not inverse)
         elif gq is not None:
-            gq = _turned(gq, None, turns, positions, interleaved, magnitude, 1 - inverse)
+            gq = _turned(gq, None, turns, positions, interleaved, magnitude, not inverse)
         elif gk is not None:
-            gk = _turned(gk, None, turns, positions, interleaved, magnitude, 1 - inverse)
+            gk = _turned(gk, None, turns, positions, interleaved, magnitude, not inverse)
         return gq, gk, None, None, None, None, None
 
 
@@ -193,15 +194,22 @@ def _turned(q, k, *how):
     return out if k is not None else out[0]
 
 
-def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, plan: RotaryPlan, *, positions=None,
-                 inverse: bool = False):
-    """Turns ``query (B, Hq, S, D)`` and ``key (B, Hkv, S, D)`` by their positions: ``(query', key')``; with ``key``
-    ``None`` only ``query'``.  Differentiable (also twice).
+_POSITIONS = (torch.int32, torch.int64)
 
-    ``positions``: integers ``(S,)``, ``(1, S)`` or ``(B, S)`` on the tensors' device (default ``0 .. S-1``); they
-    may be negative or of any size.  ``inverse=True`` turns backwards.  bf16, fp16 or fp32, any strides; each value
-    is rounded once.  Results keep the inputs' dense layout (a transposed projection stays transposed).
-    """
+
+def _fits(query, key, plan) -> bool:
+    dev, dt, shape = query.device, query.dtype, query.shape
+    if not (isinstance(plan, RotaryPlan) and plan.turns.device == dev and 2 * plan.turns.shape[0] <= shape[3]
+            and plan.turns.dtype is torch.int64 and plan.turns.is_contiguous()):
+        return False
+    if key is None:
+        return True
+    return (isinstance(key, torch.Tensor) and key.dtype is dt and key.device == dev and key.dim() == 4
+            and key.shape[0] == shape[0] and key.shape[2:] == shape[2:])
+
+
+def _check(query, key, plan, positions):
+    """Refuses what cannot be turned; the positions as the kernel reads them."""
     for name, x in (("query", query), ("key", key)):
         if x is None and name == "key":
             continue
@@ -232,5 +240,24 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, plan: RotaryPlan
             positions = positions.to(torch.int64)
     if not query.is_cuda:
         raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
-    how = (plan.turns, positions, int(plan.interleaved), plan.magnitude, int(bool(inverse)))
+    return positions
+
+
+def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, plan: RotaryPlan, *, positions=None,
+                 inverse: bool = False):
+    """Turns ``query (B, Hq, S, D)`` and ``key (B, Hkv, S, D)`` by their positions: ``(query', key')``; with ``key``
+    ``None`` only ``query'``.  Differentiable (also twice).
+
+    ``positions``: integers ``(S,)``, ``(1, S)`` or ``(B, S)`` on the tensors' device (default ``0 .. S-1``); they
+    may be negative or of any size.  ``inverse=True`` turns backwards.  bf16, fp16 or fp32, any strides; each value
+    is rounded once.  Results keep the inputs' dense layout (a transposed projection stays transposed).
+    """
+    # (one pass where all is well: the checks are a good part of a small call's host time)
+    if not (isinstance(query, torch.Tensor) and query.is_cuda and query.dim() == 4 and _fits(query, key, plan)
+            and (positions is None or (isinstance(positions, torch.Tensor) and positions.dim() == 2
+                                       and positions.dtype in _POSITIONS and positions.device == query.device
+                                       and positions.shape[0] in (1, query.shape[0])
+                                       and positions.shape[1] == query.shape[2]))):
+        positions = _check(query, key, plan, positions)
+    how = (plan.turns, positions, plan.interleaved, plan.magnitude, bool(inverse))
     return _turned(query, key, *how)
