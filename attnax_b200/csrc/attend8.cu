@@ -80,6 +80,37 @@ struct E4m3 {
         : "=r"(*lo), "=r"(*hi)
         : "r"(w));
   }
+  // 16 codes times 2^kShift as fp16, two 16-byte pieces: the bits of a code are those of an fp16 whose exponent is
+  // biased by eight more, subnormal ones too.  Three integer steps a pair instead of a conversion on the unit that the
+  // exponentials need.  NaN is put in where there is one.
+  static constexpr float kShift = -8.f, kUnshift = 256.f;
+  __device__ static void pairs(uint32_t w, uint32_t* lo, uint32_t* hi) {
+    // (bytes with their signs spread above them, then seven up; what spills over and the second sign bit are masked)
+    uint32_t a, b;
+    asm("prmt.b32 %0, %1, 0, 0x9180;" : "=r"(a) : "r"(w));
+    asm("prmt.b32 %0, %1, 0, 0xb3a2;" : "=r"(b) : "r"(w));
+    *lo = (a << 7) & 0xbf80bf80u;
+    *hi = (b << 7) & 0xbf80bf80u;
+  }
+  __device__ static void wide16(const uint4& w, uint4& lo, uint4& hi) {
+    pairs(w.x, &lo.x, &lo.y);
+    pairs(w.y, &lo.z, &lo.w);
+    pairs(w.z, &hi.x, &hi.y);
+    pairs(w.w, &hi.z, &hi.w);
+    const uint32_t full = 0x7f7f7f7fu, one = 0x01010101u;
+    if ((((w.x & full) + one) | ((w.y & full) + one) | ((w.z & full) + one) | ((w.w & full) + one)) & 0x80808080u) {
+      const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y), n2 = nan_bytes(w.z), n3 = nan_bytes(w.w);
+      nan_pair(n0, &lo.x, &lo.y);
+      nan_pair(n1, &lo.z, &lo.w);
+      nan_pair(n2, &hi.x, &hi.y);
+      nan_pair(n3, &hi.z, &hi.w);
+    }
+  }
+  // fp16 NaN where a code's byte of `bad` is set
+  __device__ static void nan_pair(uint32_t bad, uint32_t* lo, uint32_t* hi) {
+    *lo |= __byte_perm(bad, 0, 0x1100) & 0x7fff7fffu;
+    *hi |= __byte_perm(bad, 0, 0x3322) & 0x7fff7fffu;
+  }
   // 0xff in the place of each code that is NaN (0x7f or 0xff)
   __device__ static uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 };
@@ -93,6 +124,13 @@ struct Int8 {
     const __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
     *lo = *reinterpret_cast<const uint32_t*>(&ha);
     *hi = *reinterpret_cast<const uint32_t*>(&hb);
+  }
+  static constexpr float kShift = 0.f, kUnshift = 1.f;
+  __device__ static void wide16(const uint4& w, uint4& lo, uint4& hi) {
+    halves(w.x, &lo.x, &lo.y);
+    halves(w.y, &lo.z, &lo.w);
+    halves(w.z, &hi.x, &hi.y);
+    halves(w.w, &hi.z, &hi.w);
   }
   __device__ static uint32_t nan_bytes(uint32_t) { return 0; }
 };
@@ -110,32 +148,42 @@ __device__ __forceinline__ uint32_t place(int token, int c) {
   return D == 128 ? token * 128 + ((c ^ (token & 7)) << 4) : token * 64 + ((c ^ ((token >> 1) & 3)) << 4);
 }
 
-// 16 channels of the query as floats (zeros where `there` is false); rows start on 32 bytes.
-__device__ __forceinline__ void load_q16(const Args& a, long long at, bool there, float (&x)[16]) {
-  if (a.dtype == ATTN_F32) {
+// 16 channels of the query as floats; rows start on 32 bytes.  (The loads are behind no branch: what it would move
+// behind itself waits for them one by one.)
+__device__ __forceinline__ void load_q16(const Args& a, long long at, float (&x)[16]) {
+  const int elem = a.dtype == ATTN_F32 ? 4 : 2;
+  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.q) + at * elem);
+  const uint4 w[4] = {p[0], p[1], p[elem == 4 ? 2 : 0], p[elem == 4 ? 3 : 1]};
+  if (elem == 4) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float4 w = there ? reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + at)[c] : make_float4(0.f, 0.f, 0.f, 0.f);
-      x[4 * c] = w.x; x[4 * c + 1] = w.y; x[4 * c + 2] = w.z; x[4 * c + 3] = w.w;
+      x[4 * c] = __uint_as_float(w[c].x);
+      x[4 * c + 1] = __uint_as_float(w[c].y);
+      x[4 * c + 2] = __uint_as_float(w[c].z);
+      x[4 * c + 3] = __uint_as_float(w[c].w);
     }
     return;
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const uint4 w = there ? reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + at)[c] : make_uint4(0, 0, 0, 0);
-    const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t h[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (a.dtype == ATTN_BF16) {
-        x[8 * c + 2 * e] = __uint_as_float(p[e] << 16);
-        x[8 * c + 2 * e + 1] = __uint_as_float(p[e] & 0xffff0000u);
+        x[8 * c + 2 * e] = __uint_as_float(h[e] << 16);
+        x[8 * c + 2 * e + 1] = __uint_as_float(h[e] & 0xffff0000u);
       } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[e]));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
         x[8 * c + 2 * e] = f.x;
         x[8 * c + 2 * e + 1] = f.y;
       }
     }
   }
+}
+// The power of two that is taken out of a row whose largest channel is `big`: that goes to [2^14, 2^15); rows with
+// infinities stay as they are.
+__device__ __forceinline__ int query_exponent(float big) {
+  return big <= FLT_MAX ? max((int)(__float_as_uint(big) >> 23) - 127, -100) - 14 : 0;
 }
 __device__ __forceinline__ void store_out(void* out, int dtype, long long at, float x) {
   if (dtype == ATTN_BF16) reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(x);
@@ -146,6 +194,14 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+}  // namespace attend8
+}  // namespace attnb200
+
+#include "attend8_tc.cuh"
+
+namespace attnb200 {
+namespace attend8 {
 
 // CTA = (kv head x group of 8 NT rows, split, sequence); its warps take the split's units in turn.
 template <class F, int D, int NT>
@@ -228,26 +284,28 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
   constexpr bool QS = NT > 1;
   __shared__ uint2 qs[QS ? NT : 1][KH][4][QS ? 32 : 1];
   uint32_t qf[QS ? 1 : NT][KH][4][2];
+  const long long row0 = ((long long)seq * a.hq + hk * a.group) * a.t;  // the kv head's rows follow one another
   float cq[NT][2];   // rows 2t, 2t + 1 of each tile: softmax scale * log2 e / that power
   int last[NT][2];   // their last visible position of this split + 1
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int row = rg * R + 8 * n + g;
     const bool there = row < a.rows;
-    const int head = hk * a.group + (there ? row % a.group : 0), pos = there ? row / a.group : 0;
-    const long long at = (((long long)seq * a.hq + head) * a.t + pos) * D;
+    const int pos = there ? row % a.t : 0;
+    const long long at = (row0 + (there ? row : 0)) * D;
     float x[KH][16], big = 0.f;
 #pragma unroll
     for (int h = 0; h < KH; ++h) {
-      load_q16(a, at + 64 * h + 16 * t, there, x[h]);
+      load_q16(a, at + 64 * h + 16 * t, x[h]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) big = fmaxf(big, fabsf(x[h][e]));
+      for (int e = 0; e < 16; ++e) {
+        x[h][e] = there ? x[h][e] : 0.f;
+        big = fmaxf(big, fabsf(x[h][e]));
+      }
     }
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // the largest goes to [2^14, 2^15); infinite rows stay as they are
-    int e2 = (int)(__float_as_uint(big) >> 23) - 127;
-    e2 = big <= FLT_MAX ? max(e2, -100) - 14 : 0;
+    const int e2 = query_exponent(big);
     const float mul = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
     for (int h = 0; h < KH; ++h)
@@ -325,7 +383,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
     const bool edge = tok0 + 16 > free_until;
     // scores in log2; a maximum that one of them passes by kSlack moves
     bool move = false;
-    const float lv = fmaxf(lg2(fabsf(vs)), -100.f);
+    const float lv = fmaxf(lg2(vs), -100.f);
     const int ta = tok0 + tk, tb = ta + 8;  // tokens of s[.][0, 1] and s[.][2, 3]
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -473,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
       for (int e = 0; e < D / 32; ++e) acc[e] += f * ow[(w * R + row) * D + lane + 32 * e];
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;  // (nothing visible: zeros)
-    const long long orow = ((long long)seq * a.hq + hk * a.group + gr % a.group) * a.t + gr / a.group;
+    const long long orow = row0 + gr;
     if (a.splits == 1) {
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) store_out(a.out, a.dtype, orow * D + lane + 32 * e, acc[e] * inv);
@@ -565,28 +623,55 @@ static bool shape_ok(const attn_paged_attend8_params_t* p) {
 }
 
 struct Plan {
+  bool tc;
   int nt, row_groups, splits, chunk;
 };
+
+// From this many rows per kv head on the tcgen05 kernel runs: it converts the codes once for 256 rows, the other one
+// for every 32 (8 sequences of 1000 to 16384 tokens, 8 kv heads: 32 rows 65 us against 69, 64 rows 89 against 74, 128
+// rows 135 against 84, 256 rows 226 against 120; 48 sequences: 64 rows 317 against 331).
+constexpr int kManyRows = 49;
 
 static Plan make_plan(const attn_paged_attend8_params_t* p) {
   Plan pl;
   const long long rows = (long long)p->num_heads_q / p->num_heads_kv * p->seq_q;
+  pl.tc = rows >= kManyRows;
   pl.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  pl.row_groups = (int)((rows + 8 * pl.nt - 1) / (8 * pl.nt));
+  const int group = pl.tc ? 256 : 8 * pl.nt;
+  pl.row_groups = (int)((rows + group - 1) / group);
   const long long ctx = ll_max(1, ll_min(p->max_context, (long long)p->max_blocks_per_seq * p->block_size));
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * pl.row_groups;
-  // Lengths are ragged more often than not: four waves if all were as long as the longest (13 sequences of 300 to 20011
-  // tokens, 15 rows: 37 us with one wave, 28 us with four).
-  const long long step = kWarps * 16, want = 148 * 3 * 4;
-  long long chunk = step * kBatch;
-  if (ctas * ((ctx + chunk - 1) / chunk) < want) chunk = ll_max(1, ctx * ctas / want / step) * step;
+  long long step, chunk, want;  // tokens that splits come in, at most (but for what follows), CTAs that are wanted
+  if (pl.tc) {
+    // A CTA costs 14 us beside its tiles (4 us each) and writes 128 KB of partials: splits no shorter than fill the GPU
+    // once, and longer ones (64 rows, 48 sequences: 368 -> 331 us) where there are many waves.
+    step = 128;
+    want = 148;
+    chunk = ctas * ctx >= 148ll * 4 * 2048 ? 2048 : 1024;
+  } else {
+    // Lengths are ragged more often than not: four waves if all were as long as the longest (13 sequences of 300 to
+    // 20011 tokens, 15 rows: 37 us with one wave, 28 us with four).
+    step = kWarps * 16;
+    want = 148 * 3 * 4;
+    chunk = step * kBatch;
+  }
   // the partials stay within 1 GiB
+  if (ctas * ((ctx + chunk - 1) / chunk) < want) chunk = ll_max(1, ctx * ctas / want / step) * step;
   const long long row_bytes = (p->head_dim + 1) * 4ll * p->num_seqs * p->num_heads_q * p->seq_q;
   while (chunk < ctx && row_bytes * ((ctx + chunk - 1) / chunk) > (1ll << 30)) chunk *= 2;
   if (chunk >= ctx) chunk = (ctx + step - 1) / step * step;
-  pl.chunk = (int)chunk;
-  pl.splits = (int)((ctx + chunk - 1) / chunk);
+  pl.chunk = (int)ll_min(chunk, INT_MAX / step * step);
+  pl.splits = (int)((ctx + pl.chunk - 1) / pl.chunk);
   return pl;
+}
+
+template <class F, int D>
+static int launch_tc(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, dim3 grid, cudaStream_t st) {
+  auto* kern = &attend8_tc_kernel<F, D>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<D>::SMEM) != cudaSuccess)
+    return ATTN_ERR_CUDA;
+  kern<<<grid, Tc<D>::THREADS, Tc<D>::SMEM, st>>>(tk, tv, a);
+  return ATTN_OK;
 }
 
 }  // namespace attend8
@@ -655,7 +740,10 @@ int attn_paged_attend8(const attn_paged_attend8_params_t* p, void* stream) {
   } while (0)
 #define BY_ROWS(F, D)            \
   do {                           \
-    if (pl.nt == 1) RUN(F, D, 1); \
+    if (pl.tc) {                 \
+      const int rc = launch_tc<F, D>(tk, tv, a, grid, st); \
+      if (rc != ATTN_OK) return rc; \
+    } else if (pl.nt == 1) RUN(F, D, 1); \
     else if (pl.nt == 2) RUN(F, D, 2); \
     else RUN(F, D, 4);           \
   } while (0)
