@@ -89,7 +89,7 @@ class PagedCacheParams(C.Structure):
     _fields_ = [
         ("dtype", C.c_int), ("num_blocks", i32), ("block_size", i32), ("num_heads_kv", i32), ("head_dim", i32),
         ("key_pool", vp), ("value_pool", vp), ("num_seqs", i32), ("max_blocks_per_seq", i32),
-        ("block_table", vp), ("seq_lengths", vp),
+        ("block_table", vp), ("seq_lengths", vp), ("key_scales", vp), ("value_scales", vp),
     ]
 
 

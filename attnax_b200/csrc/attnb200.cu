@@ -397,7 +397,8 @@ using namespace attnb200;
 
 extern "C" {
 
-int attn_version(void) { return 2; }  // 2: attn_mask_t, attn_fwd_params_t, attn_bwd_params_t grew (sinks)
+// 2: attn_mask_t, attn_fwd_params_t, attn_bwd_params_t grew (sinks); 3: attn_paged_cache_t (scales)
+int attn_version(void) { return 3; }
 
 uint64_t attn_launch_count(void) { return g_launches.load(); }
 

@@ -38,12 +38,22 @@ struct Pool {
   void *k, *v;
   int num_blocks;
   long long vecs;  // vectors per page
+  float *ks, *vs;  // pools of 8-bit codes: heads scales per page, or null
+  int heads;
 };
+
+__device__ __forceinline__ void copy_scales(const Pool& p, float* scales, int src, int dst) {
+  if (!scales) return;
+  for (int h = threadIdx.x; h < p.heads; h += blockDim.x)
+    scales[(long long)dst * p.heads + h] = scales[(long long)src * p.heads + h];
+}
 
 template <typename V>
 __device__ __forceinline__ void copy_page(const Pool& p, int src, int dst) {
   copy_vecs(reinterpret_cast<const V*>(p.k) + src * p.vecs, reinterpret_cast<V*>(p.k) + dst * p.vecs, p.vecs);
   copy_vecs(reinterpret_cast<const V*>(p.v) + src * p.vecs, reinterpret_cast<V*>(p.v) + dst * p.vecs, p.vecs);
+  copy_scales(p, p.ks, src, dst);
+  copy_scales(p, p.vs, src, dst);
 }
 
 // ------------------------------------------------------------------- copy --
@@ -77,6 +87,7 @@ __global__ void __launch_bounds__(256) copy_kernel(Pool p, const int32_t* src, c
       if (threadIdx.x == 0) skip_notice();
     } else {
       copy_vecs(pool + s[e] * p.vecs, pool + d[e] * p.vecs, p.vecs);
+      copy_scales(p, blockIdx.y ? p.vs : p.ks, s[e], d[e]);
     }
   }
 }
@@ -504,26 +515,33 @@ __global__ void __launch_bounds__(256) accept_kernel(AcceptArgs a) {
 }
 
 // ------------------------------------------------------------------- host --
+// Whether the pools hold 8-bit codes.
+static bool codes(const attn_paged_cache_t* c) {
+  return (int)c->dtype == ATTN_POOL_E4M3 || (int)c->dtype == ATTN_POOL_INT8;
+}
+
 static bool cache_ok(const attn_paged_cache_t* c, bool pools, bool table) {
   if (!c || c->num_blocks <= 0 || c->block_size <= 0 || c->num_heads_kv <= 0 || c->head_dim <= 0) return false;
-  if (c->dtype != ATTN_F32 && c->dtype != ATTN_BF16 && c->dtype != ATTN_F16) return false;
-  if (pools && (!c->key_pool || !c->value_pool)) return false;
+  if (c->dtype != ATTN_F32 && c->dtype != ATTN_BF16 && c->dtype != ATTN_F16 && !codes(c)) return false;
+  if (pools && (!c->key_pool || !c->value_pool || (codes(c) && (!c->key_scales || !c->value_scales)))) return false;
   return !table || (c->num_seqs > 0 && c->max_blocks_per_seq > 0 && c->block_table && c->seq_lengths);
 }
 
 // Widest vector that divides `bytes` and fits the alignment of the addresses in `bits`.
 static int vec_bytes(long long bytes, uintptr_t bits) {
   int v = 16;
-  while (v > 2 && (bytes % v || bits % v)) v /= 2;
+  while (v > 1 && (bytes % v || bits % v)) v /= 2;
   return v;
 }
 
 static uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 static Pool make_pool(const attn_paged_cache_t* c, int* vec) {
-  const long long bytes = (long long)c->block_size * c->num_heads_kv * c->head_dim * dtype_size(c->dtype);
+  const long long bytes =
+      (long long)c->block_size * c->num_heads_kv * c->head_dim * (codes(c) ? 1 : dtype_size(c->dtype));
   *vec = vec_bytes(bytes, addr(c->key_pool) | addr(c->value_pool));
-  return Pool{c->key_pool, c->value_pool, c->num_blocks, bytes / *vec};
+  return Pool{c->key_pool, c->value_pool, c->num_blocks, bytes / *vec,
+              codes(c) ? c->key_scales : nullptr, codes(c) ? c->value_scales : nullptr, c->num_heads_kv};
 }
 
 #define PAGES_BY_VEC(vec, CALL) \
@@ -531,7 +549,8 @@ static Pool make_pool(const attn_paged_cache_t* c, int* vec) {
     if (vec == 16) CALL(uint4); \
     else if (vec == 8) CALL(uint2); \
     else if (vec == 4) CALL(uint32_t); \
-    else CALL(uint16_t);        \
+    else if (vec == 2) CALL(uint16_t); \
+    else CALL(uint8_t);         \
   } while (0)
 
 static size_t map_bytes(const attn_paged_cache_t* c) { return align256((size_t)(c->num_blocks + 31) / 32 * 4); }
@@ -690,6 +709,7 @@ int attn_paged_accept(const attn_paged_cache_t* c, const void* draft_keys, const
   if (!pages::cache_ok(c, true, true) || !draft_keys || !draft_values || !k_strides || !v_strides || num_drafts <= 0 ||
       max_accepted < 0 || (max_accepted > 0 && !accepted) || !accepted_lengths || (!lengths_out && !bad))
     return ATTN_ERR_INVALID;
+  if (pages::codes(c)) return ATTN_ERR_UNSUPPORTED;      // (their scales: attn_paged_append_tokens)
   if (c->num_seqs > 65535) return ATTN_ERR_UNSUPPORTED;  // (a grid dimension)
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const long long es = dtype_size(c->dtype), row = c->head_dim * es;

@@ -20,6 +20,7 @@ from ._api import compose_score_mods
 from .flash import flash_attention
 from .kv_cache import KVLayerCache, kv_cache_attention, update_kv_layer_cache
 from .rope import apply_rope_table, rope_cos_sin_table
+from .rotary import RotaryPlan, apply_rotary
 from .score_mods import sink_window_mod, sliding_window_mod
 
 
@@ -30,7 +31,8 @@ def _split_heads(x: torch.Tensor, heads: int) -> torch.Tensor:
 
 def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, num_heads: int,
                    num_kv_heads: int, use_rope: bool = False, rope_base: float = 10000.0,
-                   rope_max_positions: int = 4096, position_ids_q=None, position_ids_kv=None,
+                   rope_max_positions: int = 4096, rotary: RotaryPlan | None = None, position_ids_q=None,
+                   position_ids_kv=None,
                    kv_cache: KVLayerCache | None = None, attention_window: int | None = None,
                    attention_sinks: int = 0,
                    self_attention: bool = True, mask=None, score_mod=None, base_score_mod=None,
@@ -46,6 +48,10 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     than Q (every function of this package does).  ``attention_sinks`` keeps
     the first tokens of the sequence visible beside ``attention_window`` (no
     counterpart in the reference).
+
+    ``rotary`` (a plan of ``rotary_plan``; no counterpart in the reference)
+    turns Q and K in place of ``use_rope``, with gradients; position ids that
+    are not given go on behind the cached tokens.
     """
     if attention_sinks < 0 or (attention_sinks and attention_window is None):
         raise ValueError("attention_sinks must not be negative and needs an attention_window")
@@ -53,6 +59,8 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
         raise ValueError("kv_cache is only supported for self-attention (context must be None).")
     if num_heads % num_kv_heads:
         raise ValueError(f"num_heads ({num_heads}) must be divisible by num_kv_heads ({num_kv_heads})")
+    if rotary is not None and use_rope:
+        raise ValueError("rotary takes the place of use_rope")
     q = _split_heads(query, num_heads)
     k = _split_heads(key, num_kv_heads)
     v = _split_heads(value, num_kv_heads).contiguous()
@@ -61,6 +69,19 @@ def attention_core(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
         cos_t, sin_t = rope_cos_sin_table(rope_max_positions, head_dim, rope_base, q.dtype, q.device)
         q = apply_rope_table(q, cos_t, sin_t, position_ids_q)
         k = apply_rope_table(k, cos_t, sin_t, position_ids_kv)
+    elif rotary is not None:
+        if kv_cache is not None and kv_cache.length:
+            first = int(kv_cache.length)
+            if position_ids_q is None:
+                position_ids_q = torch.arange(first, first + seq_q, device=q.device)
+                position_ids_kv = position_ids_q if position_ids_kv is None and k.shape[2] == seq_q else position_ids_kv
+            if position_ids_kv is None:
+                position_ids_kv = torch.arange(first, first + k.shape[2], device=k.device)
+        if position_ids_q is position_ids_kv and k.shape[2] == seq_q:
+            q, k = apply_rotary(q, k, rotary, positions=position_ids_q)
+        else:
+            q = apply_rotary(q, None, rotary, positions=position_ids_q)
+            k = apply_rotary(k, None, rotary, positions=position_ids_kv)
     else:
         q, k = q.contiguous(), k.contiguous()
 

@@ -1,6 +1,7 @@
 """Operators on the pages of a :class:`PagedKVCache`: accept, copy, fork, free and compact.
 
-They take whole batches and return new ``PagedKVCache`` objects like the rest
+All but ``append_accepted`` take a :class:`QuantizedPagedKVCache` too, whose
+scales go where their pages go.  They take whole batches and return new cache objects like the rest
 of the paged API (``allocate_blocks``, ``append_kv``); tables and lengths are
 new tensors, the pools are written in place and shared.  Nothing here waits
 for the GPU unless it says so: counts come back as 0-d int32 tensors on the
@@ -24,22 +25,29 @@ from . import _lib
 from ._spec import dtype_code
 from .paged import PagedKVCache
 from .paged_rows import cast, check_tables, narrow, on_device
+from .quantized import QuantizedPagedKVCache, check_cache, with_table
 
 
 _Strides = C.c_int64 * 3
 
 
-def _params(cache: PagedKVCache):
-    """(PagedCacheParams, tensors it points into)."""
-    pool, rows = check_tables(cache)
+def _params(cache):
+    """(PagedCacheParams, tensors it points into) of either kind of cache."""
+    scales = (None, None)
+    if isinstance(cache, QuantizedPagedKVCache):
+        pool, rows, code = check_cache(cache)
+        scales = cache.key_scales.data_ptr(), cache.value_scales.data_ptr()
+    else:
+        pool, rows = check_tables(cache)
+        code = dtype_code(cache.key_pool.dtype)
     kp, vpool = cache.key_pool, cache.value_pool
     if not kp.is_cuda:
         raise RuntimeError("attnax_b200 kernels need CUDA tensors; there is no CPU path")
     if not (kp.is_contiguous() and vpool.is_contiguous()):
         raise ValueError("page operators write the pools in place and need them contiguous")
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    p = _lib.PagedCacheParams(dtype_code(kp.dtype), *pool, kp.data_ptr(), vpool.data_ptr(), *rows,
-                              bt.data_ptr(), sl.data_ptr())
+    p = _lib.PagedCacheParams(code, *pool, kp.data_ptr(), vpool.data_ptr(), *rows, bt.data_ptr(), sl.data_ptr(),
+                              *scales)
     return p, (bt, sl)
 
 
@@ -121,7 +129,7 @@ def fork_sequences(cache: PagedKVCache, src_sequences, dst_sequences, free_block
     _lib.run("attn_paged_fork", dev, C.byref(p), src.data_ptr(), dst.data_ptr(), src.numel(),
           free.data_ptr() if free.numel() else None, free.numel(), table.data_ptr(), lens.data_ptr(), used.data_ptr())
     del keep
-    return PagedKVCache(cache.key_pool, cache.value_pool, table, lens), used
+    return with_table(cache, table, lens), used
 
 
 def _scratch(ws):
@@ -152,7 +160,7 @@ def free_sequences(cache: PagedKVCache, sequences):
     _lib.run("attn_paged_free", dev, C.byref(p), seqs.data_ptr() if seqs.numel() else None, seqs.numel(),
           table.data_ptr(), lens.data_ptr(), freed.data_ptr(), count.data_ptr(), *_scratch(ws))
     del keep
-    return PagedKVCache(cache.key_pool, cache.value_pool, table, lens), freed, count
+    return with_table(cache, table, lens), freed, count
 
 
 def free_window(cache: PagedKVCache, *, window_size: int, num_sinks: int = 0):
@@ -174,7 +182,7 @@ def free_window(cache: PagedKVCache, *, window_size: int, num_sinks: int = 0):
     _lib.run("attn_paged_free_window", dev, C.byref(p), min(int(window_size), 1 << 40), min(int(num_sinks), 1 << 40),
           table.data_ptr(), freed.data_ptr(), count.data_ptr(), *_scratch(ws))
     del keep
-    return PagedKVCache(cache.key_pool, cache.value_pool, table, cache.seq_lengths), freed, count
+    return with_table(cache, table, cache.seq_lengths), freed, count
 
 
 def compact_blocks(cache: PagedKVCache):
@@ -192,7 +200,7 @@ def compact_blocks(cache: PagedKVCache):
     ws = torch.empty(_lib.load().attn_paged_compact_workspace_size(C.byref(p)), dtype=torch.uint8, device=dev)
     _lib.run("attn_paged_compact", dev, C.byref(p), table.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel())
     del keep
-    return PagedKVCache(cache.key_pool, cache.value_pool, table, cache.seq_lengths), live
+    return with_table(cache, table, cache.seq_lengths), live
 
 
 def append_accepted(cache: PagedKVCache, draft_keys, draft_values, accepted, accepted_lengths, *,
@@ -210,6 +218,8 @@ def append_accepted(cache: PagedKVCache, draft_keys, draft_values, accepted, acc
     with ``check=False`` there is no wait, and such tokens are skipped and
     noted (lengths still count them).
     """
+    if not isinstance(cache, PagedKVCache):
+        raise ValueError("append_accepted takes a PagedKVCache; append_tokens puts tokens into 8-bit pages")
     dev = cache.key_pool.device
     n = cache.block_table.shape[0]
     for name, x in (("draft_keys", draft_keys), ("draft_values", draft_values)):

@@ -71,7 +71,7 @@ def init_quantized_paged_kv_cache(*, num_blocks: int, block_size: int, num_kv_he
                                  torch.zeros(batch_size, dtype=torch.int32, device=device))
 
 
-def _checked(cache):
+def check_cache(cache):
     """(pool shape, table shape, pool format) of either kind of cache, its tensors checked."""
     if not isinstance(cache, (PagedKVCache, QuantizedPagedKVCache)):
         raise ValueError("cache must be a PagedKVCache or a QuantizedPagedKVCache")
@@ -107,10 +107,10 @@ def _scales(cache):
     return 0, 0
 
 
-def _with_lengths(cache, lengths: torch.Tensor):
-    """The cache with other lengths (dataclasses.replace without its host time)."""
+def with_table(cache, table: torch.Tensor, lengths: torch.Tensor):
+    """The cache with another table and lengths (dataclasses.replace without its host time)."""
     new = object.__new__(type(cache))
-    new.__dict__.update(cache.__dict__, seq_lengths=lengths)
+    new.__dict__.update(cache.__dict__, block_table=table, seq_lengths=lengths)
     return new
 
 
@@ -169,7 +169,7 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     missing or out of range; with ``check=False`` there is no wait, and such tokens are skipped and noted in
     ``_lib.device_status()`` (``NOTICE_PAGE_LIST``; lengths still count them).
     """
-    pool, (n, width), fmt = _checked(cache)
+    pool, (n, width), fmt = check_cache(cache)
     kp, vp = cache.key_pool, cache.value_pool
     dev = kp.device
     _check_append(cache, n, pool[2], pool[3], keys, values, query, rotary)
@@ -204,7 +204,7 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     p.lengths_out = out.data_ptr()
     _lib.run("attn_paged_append_tokens", dev, C.byref(p))
     del bt, sl, k, v
-    new = _with_lengths(cache, out)
+    new = with_table(cache, cache.block_table, out)
     return new if query is None else (new, q_out)
 
 
@@ -230,7 +230,7 @@ def gather_tokens(cache, starts, count: int, *, dtype=None):
     come back as the values that they stand for, rounded to ``dtype`` (default: the pools' type; bfloat16 for 8-bit
     pools, which holds every code times a power of two exactly).  Nothing waits for the GPU.
     """
-    pool, rows, fmt = _checked(cache)
+    pool, rows, fmt = check_cache(cache)
     if dtype is None:
         dtype = torch.bfloat16 if isinstance(cache, QuantizedPagedKVCache) else cache.key_pool.dtype
     dtype_code(dtype)
@@ -267,7 +267,7 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
     if not isinstance(query, torch.Tensor) or query.dim() != 4:
         raise ValueError("query must be (num_seqs, num_heads, seq_q, head_dim)")
     n, hq, t, d = query.shape
-    pool, rows, fmt = _checked(cache)
+    pool, rows, fmt = check_cache(cache)
     if n != rows[0]:
         raise ValueError(f"query has {n} sequences, the cache {rows[0]}")
     if hq % pool[2] != 0:

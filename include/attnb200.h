@@ -206,6 +206,10 @@ int attn_paged_append(attn_dtype_t dtype, void* key_pool, void* value_pool, int3
                       const int32_t* block_table_row, int32_t max_blocks, int32_t start, int32_t chunk,
                       const void* keys_new, const void* values_new, int32_t* bad_slot, void* stream);
 /* ---- pages of the cache ------------------------------------------------- */
+/* What a pool holds: an attn_dtype_t, or 8-bit codes.  The codes of one page
+ * and kv head stand for code * scale, scales float32 [num_blocks, heads_kv],
+ * not negative, powers of two where attn_paged_append_tokens wrote them. */
+enum { ATTN_POOL_E4M3 = 16, ATTN_POOL_INT8 = 17 };
 /* A paged cache as the page operators see it.  They work on whole batches
  * without a host round trip; index lists live on the device.  An index that
  * cannot be used (out of range, not allocated, given twice where that is
@@ -213,13 +217,15 @@ int attn_paged_append(attn_dtype_t dtype, void* key_pool, void* value_pool, int3
  * notice 0x204 is left.  No counterparts in the reference, which allocates
  * and appends one sequence at a time (attnax/paged_cache.py:92-198). */
 typedef struct {
-  attn_dtype_t dtype;
+  attn_dtype_t dtype;            /* or ATTN_POOL_E4M3, ATTN_POOL_INT8 (not attn_paged_accept) */
   int32_t num_blocks, block_size, num_heads_kv, head_dim;
   void* key_pool;                /* [num_blocks, block_size, heads_kv, head_dim] */
   void* value_pool;
   int32_t num_seqs, max_blocks_per_seq;
   const int32_t* block_table;    /* [num_seqs, max_blocks_per_seq], -1 unused */
   const int32_t* seq_lengths;    /* [num_seqs] */
+  float* key_scales;             /* 8-bit pools: [num_blocks, heads_kv], they move with the pages */
+  float* value_scales;
 } attn_paged_cache_t;
 /* Copies page src[i] over page dst[i], keys and values, i < n.  A dst given
  * twice takes the first; a page that is a source of another entry is not
@@ -419,10 +425,6 @@ typedef struct {
 int attn_rotary(const attn_rotary_params_t* p, void* stream);
 
 /* ---- tokens into and out of a paged cache ---------------------------------- */
-/* What a pool holds: an attn_dtype_t, or 8-bit codes.  The codes of one page
- * and kv head stand for code * scale, scales float32 [num_blocks, heads_kv],
- * powers of two where attn_paged_append_tokens wrote them. */
-enum { ATTN_POOL_E4M3 = 16, ATTN_POOL_INT8 = 17 };
 /* Appends the tokens [0, new_lengths[s]) of every sequence s to its pages at
  * positions seq_lengths[s].., keys turned by their position on the way (turns
  * NULL: not turned), and turns the query rows: row i by seq_lengths[s] + i,
