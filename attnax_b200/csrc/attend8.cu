@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
   const int t0 = split * a.chunk;
   if (t0 >= ctx && split) return;
   const int t1 = (int)ll_min(ctx, (long long)t0 + a.chunk);
+  if (split == a.splits - 1 && t1 < ctx && threadIdx.x == 0) atomicCAS(&g_notice, 0, kNoticeContextOverrun);
   const int units = (t1 - t0 + 15) / 16;
 
   extern __shared__ uint8_t smem_raw[];
@@ -558,9 +559,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   int n = 0;
   if (row < rows) {
     const int ctx = (int)ll_min(max(a.lens[row / (a.hq * a.t)], 0), (long long)a.max_blocks * a.bs);
-    const int need = (int)(((long long)ctx + a.chunk - 1) / a.chunk);
-    n = min(need, a.splits);
-    if (need > a.splits && lane == 0) atomicCAS(&g_notice, 0, kNoticeContextOverrun);
+    n = (int)ll_min(((long long)ctx + a.chunk - 1) / a.chunk, a.splits);
   }
   const float* lse = a.part_lse + (long long)row * a.splits;
   float mx = -FLT_MAX;
@@ -655,8 +654,8 @@ static Plan make_plan(const attn_paged_attend8_params_t* p) {
     want = 148 * 3 * 4;
     chunk = step * kBatch;
   }
-  // the partials stay within 1 GiB
   if (ctas * ((ctx + chunk - 1) / chunk) < want) chunk = ll_max(1, ctx * ctas / want / step) * step;
+  // the partials stay within 1 GiB
   const long long row_bytes = (p->head_dim + 1) * 4ll * p->num_seqs * p->num_heads_q * p->seq_q;
   while (chunk < ctx && row_bytes * ((ctx + chunk - 1) / chunk) > (1ll << 30)) chunk *= 2;
   if (chunk >= ctx) chunk = (ctx + step - 1) / step * step;

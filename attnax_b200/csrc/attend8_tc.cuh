@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
   const int t0 = split * a.chunk;
   if (t0 >= ctx && split) return;
   const int t1 = (int)ll_min(ctx, (long long)t0 + a.chunk);
+  if (split == a.splits - 1 && t1 < ctx && threadIdx.x == 0) atomicCAS(&g_notice, 0, kNoticeContextOverrun);
   const int n = (t1 - t0 + BN - 1) / BN;                                     // tiles
   const int row_tiles = min(2, (a.rows - rg * 2 * BM + BM - 1) / BM);
   const int free_until = min(ctx - a.t + 1, t1);  // tokens of this split in front of it are visible to every row

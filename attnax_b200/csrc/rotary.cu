@@ -545,8 +545,8 @@ __global__ void __launch_bounds__(kPageThreads, 3) append8_kernel(const __grid_c
     const float need = pow2(k);
     float s_new = s_old > need ? s_old : need;
     const float inv = 1.f / s_new;
-    // int8 has no NaN: a page that was given one has a NaN scale, until it is begun anew
-    if (!F::kHasNan && (odd || isnan(s_old))) s_new = NAN;
+    // int8 has no NaN: a page that was given one has a NaN scale; it stays until the page is begun anew
+    if ((!F::kHasNan && odd) || isnan(s_old)) s_new = NAN;
     const bool careful = odd || k == F::kTop;
     auto write = [&](int w, const float* f) {
       uint8_t* row = head + (old + w) * pool_row;
@@ -751,7 +751,7 @@ int attn_rotary(const attn_rotary_params_t* p, void* stream) {
   a.positions = p->positions;
   a.positions_64 = p->positions_64;
   a.ps[0] = p->position_strides[0]; a.ps[1] = p->position_strides[1];
-  if (tokens > INT_MAX) return ATTN_ERR_UNSUPPORTED;
+  if (tokens > INT_MAX - 256) return ATTN_ERR_UNSUPPORTED;
   a.tokens = (int)tokens; a.seq = p->seq; a.dim = p->head_dim;
   const int es = (int)dtype_size(p->dtype);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -808,7 +808,7 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
     return !a.q.heads || (fits(a.q.x, a.q.xs, es, np * es) && fits(a.q.out, a.q.os, es, np * es));
   };
   const long long tokens = (long long)a.num_seqs * a.num_new;
-  if (tokens > INT_MAX) return ATTN_ERR_UNSUPPORTED;
+  if (tokens > INT_MAX - 256) return ATTN_ERR_UNSUPPORTED;
   int launches = 1;
 #define WIDE(TI, TO, NP)                                                               \
   do {                                                                                 \

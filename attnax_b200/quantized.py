@@ -31,7 +31,7 @@ _FORMATS = {torch.float8_e4m3fn: _lib.POOL_E4M3, torch.int8: _lib.POOL_INT8}
 @dataclass(frozen=True)
 class QuantizedPagedKVCache:
     """Pools of 8-bit codes ``(num_blocks, block_size, num_kv_heads, head_dim)``, float32 scales
-    ``(num_blocks, num_kv_heads)``, block table and lengths as :class:`PagedKVCache` has them."""
+    ``(num_blocks, num_kv_heads)`` (not negative), block table and lengths as :class:`PagedKVCache` has them."""
 
     key_pool: torch.Tensor
     value_pool: torch.Tensor

@@ -247,6 +247,18 @@ def test_not_finite(bad):
     assert bool((k == 1).all())
 
 
+@pytest.mark.parametrize("pool", BITS8)
+def test_a_nan_scale_stays_until_the_page_is_begun_anew(pool):
+    cache = make_cache(pool, [5], 16)
+    page = int(cache.block_table[0, 0])
+    cache.value_scales[page, 1] = math.nan
+    one = torch.ones(1, 2, 1, 64, device=DEV)
+    out = ax.append_tokens(cache, one, one)
+    assert bool(torch.isnan(out.value_scales[page, 1])) and bool(torch.isfinite(out.value_scales[page, 0]))
+    new = dataclasses.replace(out, seq_lengths=torch.zeros_like(out.seq_lengths))
+    assert bool(torch.isfinite(ax.append_tokens(new, one, one).value_scales[page]).all())
+
+
 @pytest.mark.parametrize("pool", [BF16, E4M3, INT8])
 def test_bad_pages_and_counts(pool):
     torch.manual_seed(10)

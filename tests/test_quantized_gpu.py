@@ -97,6 +97,72 @@ def test_against_64_bits(pool, lens, hq, hk, d, bs, t):
     check(ax.paged_quantized_attention(q, cache, max_context=max(lens) + 1000), want, "bounded")
 
 
+MANY = [  # many rows per kv head: the tcgen05 kernel
+    ([700, 130, 5], 8, 2, 128, 16, 13), ([129, 128, 127, 0], 12, 4, 64, 32, 20), ([2500], 7, 1, 128, 64, 7),
+    ([1100, 3], 40, 2, 64, 16, 9), ([300], 8, 1, 128, 16, 45), ([3000, 600], 16, 2, 128, 128, 70), ([64], 64, 1, 64, 16, 1),
+]
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("pool", [E4M3, INT8])
+@pytest.mark.parametrize("lens,hq,hk,d,bs,t", MANY)
+def test_many_rows(pool, lens, hq, hk, d, bs, t, dt):
+    assert hq // hk * t >= 49
+    cache = make_cache(pool, lens, 0, hk, d, bs, seed=sum(lens) + t)
+    q = query(cache, hq, t, dt)
+    check(ax.paged_quantized_attention(q, cache, max_context=max(lens)), attention64(q, cache))
+
+
+@pytest.mark.parametrize("pool", [E4M3, INT8])
+@pytest.mark.parametrize("spread", [8, 40])
+def test_many_rows_with_scales_that_differ(pool, spread):
+    cache = make_cache(pool, [260, 40], 0, 2, 64, 16)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(4)
+    cache.value_scales.copy_(2.0 ** torch.randint(-spread, spread, cache.value_scales.shape, generator=g, device=DEV).float())
+    cache.value_scales[int(cache.block_table[0, 3])] = 0
+    cache.key_scales[int(cache.block_table[0, 4])] = 0
+    cache.key_scales.mul_(1.37)
+    q = query(cache, 8, 30) * 2
+    check(ax.paged_quantized_attention(q, cache), attention64(q, cache))
+
+
+def test_many_rows_with_growing_scores():
+    cache = make_cache(INT8, [3000], 0, 1, 64, 16)
+    table = cache.block_table[0].long()
+    cache.key_scales[table, 0] = torch.linspace(2.0 ** -9, 2.0 ** -2, table.numel(), device=DEV)
+    q = query(cache, 8, 9) * 3
+    check(ax.paged_quantized_attention(q, cache), attention64(q, cache))
+
+
+def test_many_rows_and_small_codes():
+    """Subnormal codes are values as well."""
+    cache = make_cache(E4M3, [200], 0, 1, 128, 16)
+    for x in (cache.key_pool, cache.value_pool):
+        x.copy_((torch.randint(-15, 16, x.shape, device=DEV) * 2.0 ** -9).to(E4M3))
+    cache.key_scales.fill_(64.0)
+    for t in (1, 64):
+        q = query(cache, 2, t)
+        check(ax.paged_quantized_attention(q, cache), attention64(q, cache))
+
+
+@pytest.mark.parametrize("t", [60, 130])
+def test_many_rows_and_nan(t):
+    for which in ("key", "value"):
+        for back in (1, 50, 129, 140):
+            cache = make_cache(E4M3, [150], 0, 2, 64, 16, seed=back)
+            pos = 150 - back
+            as_bytes(getattr(cache, f"{which}_pool"))[int(cache.block_table[0, pos // 16]), pos % 16, 1, 7] = 0x7F
+            got = ax.paged_quantized_attention(query(cache, 4, t), cache)
+            rows = 150 - t + torch.arange(t, device=DEV) >= pos
+            nan = torch.isnan(got)
+            assert not bool(nan[:, :2].any()) and not bool(nan[:, 2:, ~rows].any())
+            assert bool((nan[:, 2:] if which == "key" else nan[:, 2:, :, 7])[:, :, rows].all())
+            if which == "value":
+                nan[..., 7] = False
+                assert not bool(nan.any())
+
+
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("size", [2.0 ** -14, 1.0, 30.0])
 def test_query_types_and_sizes(dt, size):
@@ -230,6 +296,13 @@ def test_lengths_past_the_bound_and_the_table():
     got = ax.paged_quantized_attention(q, cache, max_context=2500)
     assert _lib.device_status() == _lib.NOTICE_CONTEXT_OVERRUN
     check(got[1:], tuple(x[1:] for x in attention64(q, cache)))
+    got = ax.paged_quantized_attention(q, cache, max_context=40)  # one split, of 64 tokens
+    assert _lib.device_status() == _lib.NOTICE_CONTEXT_OVERRUN
+    many = query(cache, 64, 1)
+    ax.paged_quantized_attention(many, cache, max_context=40)
+    assert _lib.device_status() == _lib.NOTICE_CONTEXT_OVERRUN
+    ax.paged_quantized_attention(many, cache, max_context=5000)
+    assert _lib.device_status() == 0
     longer = dataclasses.replace(cache, seq_lengths=torch.tensor([6000, 100], dtype=torch.int32, device=DEV))
     with pytest.raises(ValueError):
         ax.paged_quantized_attention(q, longer)
