@@ -627,8 +627,8 @@ struct Plan {
 };
 
 // From this many rows per kv head on the tcgen05 kernel runs: it converts the codes once for 256 rows, the other one
-// for every 32 (8 sequences of 1000 to 16384 tokens, 8 kv heads: 32 rows 65 us against 69, 64 rows 89 against 74, 128
-// rows 135 against 84, 256 rows 226 against 120; 48 sequences: 64 rows 317 against 331).
+// for every 32.  Over the batches of make_plan's comment its time is 1.29 of the other one's at 32 rows, 0.99 at 48
+// and 0.98 at 64; 8 sequences of 1000 to 16384 tokens, 8 kv heads: 128 rows 137 us against 86, 256 rows 229 against 125.
 constexpr int kManyRows = 49;
 
 static Plan make_plan(const attn_paged_attend8_params_t* p) {
@@ -640,21 +640,27 @@ static Plan make_plan(const attn_paged_attend8_params_t* p) {
   pl.row_groups = (int)((rows + group - 1) / group);
   const long long ctx = ll_max(1, ll_min(p->max_context, (long long)p->max_blocks_per_seq * p->block_size));
   const long long ctas = (long long)p->num_seqs * p->num_heads_kv * pl.row_groups;
-  long long step, chunk, want;  // tokens that splits come in, at most (but for what follows), CTAs that are wanted
+  // tokens that splits come in, at most (but for what follows), CTAs that are wanted, steps of a split at least
+  long long step, chunk, want, least;
   if (pl.tc) {
     // A CTA costs 14 us beside its tiles (4 us each) and writes 128 KB of partials: splits no shorter than fill the GPU
     // once, and longer ones (64 rows, 48 sequences: 368 -> 331 us) where there are many waves.
     step = 128;
+    least = 1;
     want = 148;
     chunk = ctas * ctx >= 148ll * 4 * 2048 ? 2048 : 1024;
   } else {
-    // Lengths are ragged more often than not: four waves if all were as long as the longest (13 sequences of 300 to
-    // 20011 tokens, 15 rows: 37 us with one wave, 28 us with four).
+    // Lengths are ragged more often than not, so two waves if all were as long as the longest; and at least 256 tokens
+    // (four units a warp), for a shorter split costs more at its start and in the join than it brings.  Over 14 batches
+    // (1 to 64 sequences of 100 to 100000 tokens, 2 to 8 kv heads), on average above the best choice of each batch at
+    // 4, 8, 16 and 32 rows: 3, 5, 7 and 9%; four waves and 64 tokens 16, 19, 27 and 38%, one wave and 256 tokens 8, 10,
+    // 13 and 8%, three waves 5, 6, 9 and 12%, two waves and 128 or 512 tokens 6 to 15% and 8 to 10%.
     step = kWarps * 16;
-    want = 148 * 3 * 4;
+    least = 4;
+    want = 148 * 3 * 2;
     chunk = step * kBatch;
   }
-  if (ctas * ((ctx + chunk - 1) / chunk) < want) chunk = ll_max(1, ctx * ctas / want / step) * step;
+  if (ctas * ((ctx + chunk - 1) / chunk) < want) chunk = ll_max(least, ctx * ctas / want / step) * step;
   // the partials stay within 1 GiB
   const long long row_bytes = (p->head_dim + 1) * 4ll * p->num_seqs * p->num_heads_q * p->seq_q;
   while (chunk < ctx && row_bytes * ((ctx + chunk - 1) / chunk) > (1ll << 30)) chunk *= 2;
