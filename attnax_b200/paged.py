@@ -53,13 +53,19 @@ def check_pools(cache: PagedKVCache):
     k, v = cache.key_pool, cache.value_pool
     shape = k.shape
     if len(shape) == 4 and v.shape == shape and v.dtype == k.dtype and v.device == k.device:
-        dtype_code(k.dtype)  # (8-bit pools have scales, which the operators of this class would not read)
         return
     if len(shape) != 4:
         raise ValueError(f"key_pool must be (num_blocks, block_size, num_kv_heads, head_dim), got {tuple(shape)}")
     if v.device != k.device:
         raise RuntimeError(f"value_pool is on {v.device}, key_pool on {k.device}")
     raise ValueError(f"value_pool {tuple(v.shape)} {v.dtype} != key_pool {tuple(shape)} {k.dtype}")
+
+
+def refuse_codes(cache):
+    """The operators of :class:`PagedKVCache` would take the codes of a quantized cache for values."""
+    if hasattr(cache, "key_scales"):
+        raise ValueError(f"the pools hold codes ({cache.key_pool.dtype}), which have scales; use append_tokens, "
+                         "gather_tokens and paged_quantized_attention")
 
 
 def pools_contiguous(cache: PagedKVCache) -> bool:
@@ -125,6 +131,7 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
     if keys_new.shape != values_new.shape:
         raise ValueError(f"keys_new shape {tuple(keys_new.shape)} != values_new shape "
                          f"{tuple(values_new.shape)}")
+    refuse_codes(cache)
     check_pools(cache)
     check_rows(cache.block_table, cache.seq_lengths)
     if not pools_contiguous(cache):
@@ -156,6 +163,7 @@ def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,
 
 def gather_kv(cache: PagedKVCache, sequence_idx: int):
     """Contiguous ``(seq_len, Hkv, D)`` keys/values of one sequence (paged_cache.py:201-231)."""
+    refuse_codes(cache)
     check_pools(cache)
     check_rows(cache.block_table, cache.seq_lengths)
     seq_len = int(cache.seq_lengths[sequence_idx])
@@ -189,6 +197,7 @@ def paged_decode_raw(query, cache: PagedKVCache, *, block_table=None, seq_length
     and reported by ``_lib.device_status()`` (``NOTICE_CONTEXT_OVERRUN`` /
     ``NOTICE_TABLE_OVERRUN``) instead of raising.
     """
+    refuse_codes(cache)
     check_pools(cache)
     if not pools_contiguous(cache):
         raise ValueError("paged_decode_raw reads the pools where they are and needs them contiguous")

@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from ._spec import dtype_code
 from .flash import attention, softmax_scale
-from .paged import PagedKVCache, check_pools, check_rows, gather_kv, gather_positions, pools_by_tma
+from .paged import PagedKVCache, check_pools, check_rows, gather_kv, gather_positions, pools_by_tma, refuse_codes
 
 
 def _check_query(query, cache: PagedKVCache):
@@ -157,7 +157,7 @@ def paged_window_attention(query, cache: PagedKVCache, *, window_size: int, num_
     if n == 0 or t == 0:
         return torch.zeros_like(query)
     if not _fused(cache, pool):
-        dtype_code(cache.key_pool.dtype)  # (8-bit pools have scales, which this operator would not read)
+        refuse_codes(cache)
         _bound(cache, None)
         return _window_by_sequence(query, cache, int(window_size), int(num_sinks))
     lib = _lib.load()
@@ -246,7 +246,7 @@ def paged_tree_attention(query, draft_keys, draft_values, cache: PagedKVCache, p
     if n == 0 or t == 0:
         return torch.zeros_like(query)
     if not _fused(cache, pool):
-        dtype_code(cache.key_pool.dtype)
+        refuse_codes(cache)
         _bound(cache, None)
         return _tree_by_sequence(query, draft_keys, draft_values, cache, parents, tree_lengths)
     lib = _lib.load()

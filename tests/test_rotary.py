@@ -1,5 +1,6 @@
 """Rotary plans and the refusals of the rotary and 8-bit page operators (no GPU)."""
 
+import dataclasses
 import math
 from fractions import Fraction
 
@@ -211,3 +212,29 @@ def test_struct_layouts_match_the_c_compiler(tmp_path):
         assert int(got[cname]) == ctypes.sizeof(py), cname
         for fname, _ in py._fields_:
             assert int(got[f"{cname}.{fname}"]) == getattr(py, fname).offset, f"{cname}.{fname}"
+
+
+def test_strided_pools_of_other_types_are_still_gathered():
+    """gather_kv reads pools that no kernel can address through torch, whatever their type."""
+    for dt in (torch.float64, torch.int8):
+        pool = torch.arange(4 * 16 * 2 * 8, dtype=torch.int64).remainder(100).to(dt).view(4, 2, 16, 8).transpose(1, 2)
+        cache = ax.PagedKVCache(pool, pool, torch.tensor([[2, 1]], dtype=torch.int32),
+                                torch.tensor([20], dtype=torch.int32))
+        k, v, n = ax.gather_kv(cache, 0)
+        want = torch.cat([pool[2], pool[1]])[:20]
+        assert n == 20 and torch.equal(k, want) and torch.equal(v, want)
+
+
+def test_codes_are_not_taken_for_values():
+    cache = ax.init_quantized_paged_kv_cache(num_blocks=4, block_size=16, num_kv_heads=2, head_dim=8, batch_size=1,
+                                             max_blocks_per_seq=2, device="cpu")
+    for c in (cache, dataclasses.replace(cache, key_pool=cache.key_pool.transpose(1, 2).contiguous().transpose(1, 2),
+                                         value_pool=cache.value_pool.transpose(1, 2).contiguous().transpose(1, 2))):
+        for call in (lambda: ax.gather_kv(c, 0),
+                     lambda: ax.append_kv(c, 0, torch.zeros(1, 2, 8), torch.zeros(1, 2, 8)),
+                     lambda: ax.paged_attention(torch.zeros(2, 1, 8), c, 0)):
+            with pytest.raises(ValueError, match="codes"):
+                call()
+    wide = dataclasses.replace(cache, block_table=cache.block_table.long())
+    with pytest.raises(ValueError, match="block_table"):
+        ax.append_tokens(wide, torch.zeros(1, 2, 1, 8), torch.zeros(1, 2, 1, 8))
