@@ -285,6 +285,8 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
     if d not in (64, 128) or bs % 16 or (kp.data_ptr() | vp.data_ptr()) % 16:
         return _attend_gathered(query, cache, pool, rows, fmt)
     q = query.contiguous()
+    if q.data_ptr() % 16:  # (vector loads)
+        q = q.clone()
     out = torch.empty_like(q)
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
     ctx = min(_bound(cache, max_context), rows[1] * bs)

@@ -394,3 +394,17 @@ def test_prompt_then_decode():
         wide, qb = ax.append_tokens(wide, k, v, rotary=plan, query=q)
         assert torch.equal(qa, qb)
         check(ax.paged_quantized_attention(qa, q8), attention64(qa, q8))
+
+
+@pytest.mark.parametrize("t", [1, 30])
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_query_off_sixteen_bytes(t, dt):
+    cache = make_cache(E4M3, [50, 33], 0, 2, 64, 16)
+    q = query(cache, 4, t, dt)
+    room = torch.empty(q.numel() + 1, dtype=dt, device=DEV)[1:]
+    room.copy_(q.reshape(-1))
+    odd = room.view(q.shape)
+    assert odd.is_contiguous() and odd.data_ptr() % 16
+    got = ax.paged_quantized_attention(odd, cache)
+    assert torch.equal(got, ax.paged_quantized_attention(q, cache))
+    check(got, attention64(q, cache))
