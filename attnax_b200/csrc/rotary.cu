@@ -784,6 +784,8 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
   const bool bits8 = p->pool_format == ATTN_POOL_E4M3 || p->pool_format == ATTN_POOL_INT8;
   if (!bits8 && !dtype_ok(p->pool_format)) return ATTN_ERR_INVALID;
   if (bits8 && (!p->key_scales || !p->value_scales)) return ATTN_ERR_INVALID;
+  if (bits8 && (long long)p->block_size * p->num_heads_kv > INT_MAX / p->head_dim)
+    return ATTN_ERR_UNSUPPORTED;  // (a page's offsets are 32 bits)
   AppendArgs a{};
   a.q = make_rows(p->q, p->q_strides, p->q_out, p->q_out_strides, p->num_heads_q);
   a.k = make_rows(p->keys, p->k_strides, p->key_pool, nullptr, p->num_heads_kv);

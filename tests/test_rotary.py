@@ -1,5 +1,6 @@
 """Rotary plans and the refusals of the rotary and 8-bit page operators (no GPU)."""
 
+import ctypes
 import dataclasses
 import math
 from fractions import Fraction
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 import attnax_b200 as ax
-from attnax_b200 import rotary
+from attnax_b200 import _lib, rotary
 
 
 def test_frequencies_follow_their_formulas():
@@ -238,3 +239,18 @@ def test_codes_are_not_taken_for_values():
     wide = dataclasses.replace(cache, block_table=cache.block_table.long())
     with pytest.raises(ValueError, match="block_table"):
         ax.append_tokens(wide, torch.zeros(1, 2, 1, 8), torch.zeros(1, 2, 1, 8))
+
+
+def test_pages_whose_offsets_pass_32_bits_are_refused():
+    """Refused on the host, before anything is read through the pointers (which are never followed)."""
+    x = torch.zeros(64, dtype=torch.int64)
+    p = _lib.PagedAppendParams()
+    p.dtype, p.pool_format, p.num_blocks = _lib.ATTN_BF16, _lib.POOL_E4M3, 1
+    p.block_size, p.num_heads_kv, p.head_dim = 1 << 20, 64, 64
+    p.num_seqs, p.max_blocks_per_seq, p.num_new = 1, 1, 1
+    for name in ("key_pool", "value_pool", "key_scales", "value_scales", "block_table", "seq_lengths", "keys", "values",
+                 "lengths_out"):
+        setattr(p, name, x.data_ptr())
+    status = _lib.load().attn_paged_append_tokens(ctypes.byref(p), None)
+    with pytest.raises(NotImplementedError):
+        _lib.check(status, "attn_paged_append_tokens")
