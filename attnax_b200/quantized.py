@@ -163,7 +163,7 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     are restated where it grows (e4m3 codes keep their values unless they become subnormal, int8 codes round once
     more).  Infinities and NaN are stored as NaN; in an int8 page, which has none, the whole page reads as NaN
     until it is begun anew.  A page that gets tokens must belong to one sequence (``fork_sequences`` shares full
-    pages only).
+    pages only).  What is written and returned carries no gradient.
 
     ``check=True`` waits for the GPU and raises ``ValueError`` before anything is written if a length or a page is
     missing or out of range; with ``check=False`` there is no wait, and such tokens are skipped and noted in
@@ -260,7 +260,8 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
     the planned splits and noted in ``_lib.device_status()``, as in ``paged_attention_batched``.  head_dim 64 or
     128, a block size that is a multiple of 16 and pools that start on 16 bytes take the fused kernel; other caches
     are brought to bf16 or fp32 (``gather_tokens``), then attended as ``paged_window_attention`` does, waiting for the
-    lengths (``NotImplementedError`` for head dims that the flash kernels do not have).  For inference: what it returns carries no gradient.
+    lengths (``NotImplementedError`` for head dims that the flash kernels do not have).  For inference: what it
+    returns carries no gradient.
     """
     if not isinstance(cache, QuantizedPagedKVCache):
         raise ValueError("cache must be a QuantizedPagedKVCache (paged_attention_batched takes the other one)")
@@ -289,7 +290,7 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
         q = q.clone()
     out = torch.empty_like(q)
     bt, sl = cache.block_table.contiguous(), cache.seq_lengths.contiguous()
-    ctx = min(_bound(cache, max_context), rows[1] * bs)
+    ctx = min(max(_bound(cache, max_context), 0), rows[1] * bs, 2**31 - 1)
     p = _attend_params(code, fmt, n, hq, hk, d, t, nb, bs, rows[1], ctx, q.data_ptr(), kp.data_ptr(), vp.data_ptr(),
                        cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), bt.data_ptr(), sl.data_ptr(),
                        out.data_ptr(), _scale(d), 0, 0)

@@ -408,3 +408,14 @@ def test_query_off_sixteen_bytes(t, dt):
     got = ax.paged_quantized_attention(odd, cache)
     assert torch.equal(got, ax.paged_quantized_attention(q, cache))
     check(got, attention64(q, cache))
+
+
+def test_bounds_of_any_size():
+    cache = make_cache(E4M3, [50, 0], 0, 2, 64, 16)
+    q = query(cache, 4, 2)
+    want = ax.paged_quantized_attention(q, cache)
+    for bound in (50, 2**31, 2**40):
+        assert torch.equal(ax.paged_quantized_attention(q, cache, max_context=bound), want)
+    assert _lib.device_status() == 0
+    zero = dataclasses.replace(cache, seq_lengths=torch.zeros_like(cache.seq_lengths))
+    assert not ax.paged_quantized_attention(q, zero, max_context=0).any()
