@@ -195,6 +195,14 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// After a wait that ran out: what is in flight gets its time, with a limit, before its memory is given up.  (mbar_wait
+// does not wait once a failure is recorded.)
+__device__ __noinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < ATTN_WAIT_NS) {
+  }
+}
+
 }  // namespace attend8
 }  // namespace attnb200
 
@@ -333,7 +341,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
   if (QS) __syncthreads();
 
   bool ok = true;
-  for (int j = 0; j < mine; ++j) {
+  int j = 0;
+  for (; j < mine; ++j) {
     if (j % kBatch == 0) {
       lks = nks;
       lvs = nvs;
@@ -488,10 +497,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
     }
   }
 
-  if (!ok)  // (a load that did not come: those in flight get their time before the slots are given up)
-    for (int i = 0; i < S; ++i)
-      for (int n = 0; n < 4096 && !mbar_try_wait(bars + 8 * i, 0) && !mbar_try_wait(bars + 8 * i, 1); ++n) {
-      }
+  if (!ok)  // (a load that did not come: units j and on are in flight and get their time before the slots are given up)
+    for (int u = j; u < min(j + S, mine); ++u) mbar_drain(bars + 8 * (u % S), (u / S) & 1);
   // ---- the warps' states into one ----
   if (!__syncthreads_and(ok)) return;
   float* ow = reinterpret_cast<float*>(smem);  // [warp][R][D]

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
   auto codes_free = [&](int s) { return bar0 + 8u * (6 + s); };
   auto scales_full = [&](int s) { return bar0 + 8u * (8 + s); };
   const uint32_t q_full = bar0 + 80, k_full = bar0 + 88, v_full = bar0 + 96, k_free = bar0 + 104, v_free = bar0 + 112,
-                 o_done = bar0 + 120;
+                 o_done = bar0 + 120, given_up = bar0 + 128;
   if (threadIdx.x == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_full(x), 1);
@@ -105,6 +105,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
     mbar_init(k_free, 1);
     mbar_init(v_free, 1);
     mbar_init(o_done, 1);
+    mbar_init(given_up, 1);
     fence_mbar_init();
     any_nan = 0;
   }
@@ -132,8 +133,8 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
         const long long page = paged_phys_page(a.table[(long long)seq * a.max_blocks + tok / a.bs], a.num_blocks);
         return (int)(page * a.bs + tok % a.bs);
       };
-      int row = n > 0 ? row_of(0) : -1;
-      for (int i = 0; i < n; ++i) {
+      int row = n > 0 ? row_of(0) : -1, i = 0;
+      for (; i < n; ++i) {
         const int s = i % C::STAGES;
         const int next = i + 1 < n ? row_of(i + 1) : -1;
         if (!wait_warp(codes_free(s), ((i / C::STAGES) & 1) ^ 1, kStatusTimeoutLoad)) break;
@@ -147,6 +148,8 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
         }
         row = next;
       }
+      // (every tile's codes are in place before the block ends; where a role gave up nobody else waits for them)
+      for (int u = max(i - C::STAGES, 0); u < i; ++u) mbar_drain(codes_full(u % C::STAGES), (u / C::STAGES) & 1);
     } else if (warp == 13 && lane == 0 && n > 0) {
       constexpr uint32_t ID_S = idesc_f16(BM, BN, 0, 0, 0);
       constexpr uint32_t ID_O = idesc_f16(BM, D, 0, 0, 1);
@@ -193,7 +196,12 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
           umma_commit(k_free);
         }
       }
-      if (ok) umma_commit(o_done);
+      if (ok) {
+        umma_commit(o_done);
+      } else {  // (products in flight end before their memory is given up)
+        umma_commit(given_up);
+        mbar_drain(given_up, 0);
+      }
     }
   } else if (warp >= 8) {
     const int r = threadIdx.x - 256;  // this thread's token of a tile
