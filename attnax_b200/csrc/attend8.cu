@@ -6,9 +6,10 @@
 //
 // HBM bounds it: every visible code is read once per kv head (D bytes per
 // token each for K and V, half of a 16-bit cache), and all query rows of the
-// head share it.  A warp streams units of 16 tokens through a private ring in
-// shared memory by 16-byte asynchronous copies, several units ahead, and needs
-// no barrier: lanes copy what they read themselves.
+// head share it.  A warp streams units of 16 tokens by TMA through a private
+// ring in shared memory, several units ahead, and shares no barrier with the
+// other warps (64 sequences of 512 to 32768 tokens: 181 us, 5.7 TB/s; 16-byte
+// copies by the lanes took 225).
 //
 // The products run transposed, S^T = K Q^T and O^T = V^T P^T, as mma.sync
 // m16n8k16: tokens (channels) are the 16 rows and 8 query rows the columns,

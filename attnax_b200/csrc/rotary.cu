@@ -4,7 +4,7 @@
 //   a' = m (a cos - b sin), b' = m (a sin + b cos);
 // the gradient turns by -p w.  Frequencies come as fixed point: w / 2 pi as a
 // fraction of 2^64, so p times it modulo 2^64 is the angle's fraction of a
-// turn, exact to p 2^-65 turns at any position, and 32 bits of it are enough
+// turn, exact to p 2^-64 turns at any position, and 32 bits of it are enough
 // for fp32 sines.  No cos/sin tables are read: the tensors' own bytes are all
 // that moves (x once in, once out; 3 flops per element), so HBM bounds the
 // large calls and launch latency the small ones.  A thread computes the sines
