@@ -185,7 +185,6 @@ struct Args {
   Spec sp;
   const void* positions;
   long long ps[2];
-  const int32_t* first;  // [batch] added to the positions, or null
   int positions_64, seq, dim, items, head_group, head_lanes, cta_tokens;
   int tokens;
 };
@@ -209,7 +208,6 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
     pos = a.positions_64 ? reinterpret_cast<const long long*>(a.positions)[at]
                          : reinterpret_cast<const int*>(a.positions)[at];
   }
-  if (a.first) pos += a.first[b];
   const int hq = a.t[0].heads, hl = a.head_lanes;
   const int h0 = blockIdx.y * a.head_group, h1 = min(h0 + a.head_group, hq + a.t[1].heads);
   const T* x0 = reinterpret_cast<const T*>(a.t[0].x) + b * a.t[0].xs[0] + s * a.t[0].xs[2];
@@ -391,10 +389,11 @@ __device__ __forceinline__ int scale_exp(float amax) {
 }
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }  // |k| <= 126
 
-// The query's CTAs of append8_kernel (small calls): cta_tokens tokens and head_group heads.
+// The query's CTAs of append8_kernel: cta_tokens tokens and head_group heads, threads as in rotary_kernel.
 template <typename T, int NP>
 __device__ __forceinline__ void turn_query(const AppendArgs& a, int cta) {
-  const int in_cta = threadIdx.x / a.items;
+  const int hl = a.head_lanes;
+  const int in_cta = threadIdx.x / a.items / hl, sub = threadIdx.x / a.items % hl;
   const int tok = cta % a.q_ctas * a.cta_tokens + in_cta, h0 = cta / a.q_ctas * a.head_group;
   if (in_cta >= a.cta_tokens || tok >= a.num_seqs * a.num_new) return;
   const int s = tok / a.num_new, i = tok % a.num_new, h1 = min(h0 + a.head_group, a.q.heads);
@@ -404,11 +403,19 @@ __device__ __forceinline__ void turn_query(const AppendArgs& a, int cta) {
     const Item it = item_at<NP>(c, a.sp.rot, a.dim, a.sp.interleaved);
     float cs[NP], sn[NP];
     if (it.turned) item_angles<NP>(a.sp, (long long)a.lens[s] + i, c, cs, sn);
-    for (int h = h0; h < h1; ++h) {
-      float v[2 * NP];
-      widen<T, NP>(load_raw<T, NP>(x + h * a.q.xs[1], it), v);
-      if (it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
-      store_item<T, NP>(y + h * a.q.os[1], it, v);
+    for (int h = h0 + sub; h < h1; h += kHeads * hl) {
+      Raw<T, NP> raw[kHeads];
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u)
+        if (h + u * hl < h1) raw[u] = load_raw<T, NP>(x + (h + u * hl) * a.q.xs[1], it);
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        if (h + u * hl >= h1) break;
+        float v[2 * NP];
+        widen<T, NP>(raw[u], v);
+        if (it.turned) turn<NP>(v, cs, sn, a.sp.interleaved);
+        store_item<T, NP>(y + (h + u * hl) * a.q.os[1], it, v);
+      }
     }
   }
 }
@@ -416,21 +423,24 @@ __device__ __forceinline__ void turn_query(const AppendArgs& a, int cta) {
 constexpr int kPageThreads = 256;
 constexpr int kAngleBytes = 40960;  // of shared memory, at most
 
-// CTAs [0, page_ctas): one page of one sequence that gets new tokens, keys or values, and page_heads kv heads one
+// page_ctas CTAs: one page of one sequence that gets new tokens, keys or values, and page_heads kv heads one
 // after another.  All tokens of a page and head are one CTA's, so a scale has one writer.  The sines of the page's
 // tokens are kept in shared memory for all of its heads (`angles` items of them, 0: formed again where they are
-// needed).  CTAs behind them turn the query.  A thread keeps its first item between the pass for the largest
+// needed).  The others turn the query and lie evenly among them: pages wait for instructions, the query for HBM
+// (8 prompts of 4096, 32 heads over 8, e4m3: 181 us, 193 with the query in a launch in front; 16 of 128: 27 against
+// 31; four CTAs per SM at 64 registers spill: 209).  A thread keeps its first item between the pass for the largest
 // magnitude and the one for the codes; a larger page's others are read twice.
 template <typename TI, typename F, int NP>
 __global__ void __launch_bounds__(kPageThreads, 3) append8_kernel(const __grid_constant__ AppendArgs a) {
-  if (blockIdx.x >= a.page_ctas) {
-    turn_query<TI, NP>(a, blockIdx.x - a.page_ctas);
+  const int query_ctas = gridDim.x - a.page_ctas, before = (int)((long long)blockIdx.x * query_ctas / gridDim.x);
+  if ((long long)(blockIdx.x + 1) * query_ctas / gridDim.x > before) {
+    turn_query<TI, NP>(a, before);
     return;
   }
   extern __shared__ float2 table[];  // [pair of the item][item]
   const int hk = a.k.heads, tid = threadIdx.x, threads = blockDim.x, lane = tid % 32;
   const int groups = (hk + a.page_heads - 1) / a.page_heads;
-  int x = blockIdx.x;
+  int x = blockIdx.x - before;
   const int h0 = x % groups * a.page_heads, h1 = min(h0 + a.page_heads, hk);
   x /= groups;
   const bool key = x & 1;
@@ -675,9 +685,9 @@ static Rows make_rows(const void* x, const int64_t* xs, void* out, const int64_t
 // Items of a CTA of `threads` threads: whole tokens (one where a token has more items than that).
 static int cta_tokens(int items, int threads) { return items >= threads ? 1 : threads / items; }
 
-// Head lanes of a tensor with these strides (rotary_kernel).
-static int head_lanes(const Rows& r, int heads, int items) {
-  return heads >= 4 && items * 4 <= 256 && r.xs[1] < r.xs[2] ? 4 : 1;
+// Head lanes of a tensor with these strides in a CTA of `threads` (rotary_kernel).
+static int head_lanes(const Rows& r, int heads, int items, int threads = 256) {
+  return heads >= 4 && items * 4 <= threads && r.xs[1] < r.xs[2] ? 4 : 1;
 }
 
 // Heads per CTA, for `ctas` CTAs of 256 threads that three of an SM hold at a time: one group of all heads (the sines
@@ -811,7 +821,6 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
   };
   const long long tokens = (long long)a.num_seqs * a.num_new;
   if (tokens > INT_MAX - 256) return ATTN_ERR_UNSUPPORTED;
-  int launches = 1;
 #define WIDE(TI, TO, NP)                                                               \
   do {                                                                                 \
     a.items = items_of(NP, a.sp.rot, a.dim);                                           \
@@ -831,19 +840,10 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
     const long long most = ll_min(a.num_new, a.bs) * (long long)a.items;               \
     const int threads = (int)ll_min(kPageThreads, ll_max(128, (most + 31) / 32 * 32)); \
     a.angles = a.sp.rot && most * NP * 8 <= kAngleBytes ? (int)most : 0;               \
-    a.cta_tokens = cta_tokens(a.items, threads);                                       \
-    /* a large query has a launch of its own, whose threads hold more loads in flight */ \
-    if (a.q.heads && tokens * a.q.heads >= (1 << 15)) {                                \
-      Args r{};                                                                        \
-      r.t[0] = a.q; r.t[1] = a.q; r.t[1].heads = 0;                                    \
-      r.sp = a.sp; r.first = a.lens;                                                   \
-      r.tokens = (int)tokens; r.seq = a.num_new; r.dim = a.dim;                        \
-      launch_rotary<TI, NP>(r, st);                                                    \
-      a.q.heads = 0;                                                                   \
-      ++launches;                                                                      \
-    }                                                                                  \
+    a.head_lanes = head_lanes(a.q, a.q.heads, a.items, threads);                       \
+    a.cta_tokens = cta_tokens(a.items * a.head_lanes, threads);                        \
     a.q_ctas = (int)((tokens + a.cta_tokens - 1) / a.cta_tokens);                      \
-    a.head_group = a.q.heads ? head_group(a.q_ctas, a.q.heads, 1) : 1;                 \
+    a.head_group = a.q.heads ? head_group(a.q_ctas, a.q.heads, a.head_lanes) : 1;                 \
     const long long groups = (a.q.heads + a.head_group - 1) / a.head_group;            \
     const long long slots = (long long)a.num_seqs * a.page_slots * 2;                  \
     /* heads of a CTA: as many as leave about 16 CTAs per SM */                        \
@@ -874,7 +874,7 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream) 
 #undef POOL
 #undef BITS8
 #undef WIDE
-  return launch_status(launches);
+  return launch_status();
 }
 
 int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream) {
