@@ -5,9 +5,11 @@
 // rows of the CTA; S = Q K^T and O += P V run in TMEM as in the 16-bit kernels, and a thread per row keeps the same two
 // maxima and carries the value scales in P as the kernel for few rows does (see there).
 //
-// What bounds it: a tile takes 4.1 us with two row tiles (2.9 with one), of which the products need 1.8 at the
-// sustained rate; the softmax of a row tile takes 2.3 (S is read from TMEM twice, since half of 512 threads cannot hold
-// 128 columns each), the hand-offs the rest.  A CTA's start and end take 14 us (7 until the query is in place).
+// What bounds it: a tile takes 3.7 us with two row tiles (3.0 with one), of which the products need 1.8 at the
+// sustained rate; the softmax of a row tile takes 2.1 to 2.7 (S is read from TMEM twice, since half of 512 threads
+// cannot hold 128 columns each; reading it once took as long), the products in its chain 0.8, the conversion of K and V
+// 1.2 to 1.5 each beside it.  V has two places, so that the conversion does not wait for P V (4.1 us with one).  A CTA's
+// start and end take 14 us (7 until the query is in place).
 #pragma once
 
 namespace attnb200 {
@@ -17,11 +19,11 @@ template <int D>
 struct Tc {
   static constexpr int BM = 128, BN = 128;
   static constexpr int KCH = D / 64;
-  static constexpr int THREADS = 512;  // warps 0-7 softmax (two row tiles), 8-11 conversion, 12 TMA, 13 MMA, 14-15 idle
+  static constexpr int THREADS = 512;  // warps 0-7 softmax (two row tiles), 8-11 conversion, 12 TMA, 13 MMA, 14 scales, 15 idle
   static constexpr int TILE = KCH * BN * 128;  // 128 rows of fp16
   static constexpr int CODES = BN * D;         // 128 tokens of codes
   static constexpr int STAGES = 2;
-  static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + TILE, OFF_CODES = OFF_V + TILE;
+  static constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + TILE, OFF_CODES = OFF_V + 2 * TILE;
   static constexpr int SMEM = OFF_CODES + STAGES * 2 * CODES + 1024;
 };
 
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sb = (raw + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (sb - raw);
-  __shared__ uint64_t bars[17];
+  __shared__ uint64_t bars[21];
   __shared__ uint32_t tmem_slot;
   __shared__ float scales[2][16];  // of a tile's eight units: keys, then values
   __shared__ int nan_from[D];      // first token whose value is NaN in a channel, among those not all rows see
@@ -89,21 +91,25 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
   auto codes_full = [&](int s) { return bar0 + 8u * (4 + s); };
   auto codes_free = [&](int s) { return bar0 + 8u * (6 + s); };
   auto scales_full = [&](int s) { return bar0 + 8u * (8 + s); };
-  const uint32_t q_full = bar0 + 80, k_full = bar0 + 88, v_full = bar0 + 96, k_free = bar0 + 104, v_free = bar0 + 112,
+  auto scales_free = [&](int s) { return bar0 + 8u * (17 + s); };
+  auto v_full = [&](int s) { return bar0 + 8u * (s ? 19 : 12); };
+  auto v_free = [&](int s) { return bar0 + 8u * (s ? 20 : 14); };
+  const uint32_t q_full = bar0 + 80, k_full = bar0 + 88, k_free = bar0 + 104,
                  o_done = bar0 + 120, given_up = bar0 + 128;
   if (threadIdx.x == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_full(x), 1);
       mbar_init(p_full(x), 4);  // (one arrival per warp)
+      mbar_init(v_full(x), 4);
+      mbar_init(v_free(x), 1);
       mbar_init(codes_full(x), 1);
       mbar_init(codes_free(x), 4);
       mbar_init(scales_full(x), 1);
+      mbar_init(scales_free(x), 4 * row_tiles);  // (the softmax warps of the tiles that are there)
     }
     mbar_init(q_full, 8);
     mbar_init(k_full, 4);
-    mbar_init(v_full, 4);
     mbar_init(k_free, 1);
-    mbar_init(v_free, 1);
     mbar_init(o_done, 1);
     mbar_init(given_up, 1);
     fence_mbar_init();
@@ -168,7 +174,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < BN / 16; ++k)
-          umma_f16_ts(tmem + 256 + x * D, tmem + x * 128 + k * 8, sdesc_add(dV, k * 16 * 128), ID_O,
+          umma_f16_ts(tmem + 256 + x * D, tmem + x * 128 + k * 8, sdesc_add(dV, (i & 1) * C::TILE + k * 16 * 128), ID_O,
                       (i > 0 || k > 0) ? 1u : 0u);
         return true;
       };
@@ -176,9 +182,9 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       bool ok = mbar_wait(q_full, 0, kStatusTimeoutMma);
       for (int i = 0; ok && i <= n; ++i) {
         if (i > 0) {
-          ok = mbar_wait(v_full, (i - 1) & 1, kStatusTimeoutMma) && issue_pv(0, i - 1);
+          ok = mbar_wait(v_full((i - 1) & 1), ((i - 1) >> 1) & 1, kStatusTimeoutMma) && issue_pv(0, i - 1);
           if (!ok) break;
-          if (row_tiles == 1) umma_commit(v_free);
+          if (row_tiles == 1) umma_commit(v_free((i - 1) & 1));
         }
         if (i < n) {
           ok = mbar_wait(k_full, i & 1, kStatusTimeoutMma);
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
         if (row_tiles == 2 && i > 0) {
           ok = issue_pv(1, i - 1);
           if (!ok) break;
-          umma_commit(v_free);
+          umma_commit(v_free((i - 1) & 1));
         }
         if (i < n) {
           if (row_tiles == 2) issue_s(1);
@@ -202,33 +208,35 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
         umma_commit(given_up);
         mbar_drain(given_up, 0);
       }
-    }
-  } else if (warp >= 8) {
-    const int r = threadIdx.x - 256;  // this thread's token of a tile
-    // warp 8, lane u or 8 + u: the key or value scale of unit u
-    auto scale_of = [&](int i) {
-      const int tok = t0 + i * BN + 16 * (lane & 7);
-      if (warp != 8 || lane >= 16 || i >= n || tok >= t1) return 0.f;
-      const long long page = paged_phys_page(a.table[(long long)seq * a.max_blocks + tok / a.bs], a.num_blocks);
-      return (lane < 8 ? a.ks : a.vs)[page * a.hkv + hk];
-    };
-    float sc = scale_of(0);
-    for (int i = 0; i < n; ++i) {
-      const int s = i % C::STAGES, tok = t0 + i * BN + r;
-      if (warp == 8) {
-        // (the softmax warps are done with the place: P V of tile i - 2 was waited for below)
+    } else if (warp == 14) {
+      // Lane u or 8 + u: the key or value scale of unit u.  (A warp of its own: its loads follow one another, page and
+      // then scale, and held the conversion up for 0.6 us a tile when one of those warps did this.)
+      auto scale_of = [&](int i) {
+        const int tok = t0 + i * BN + 16 * (lane & 7);
+        if (lane >= 16 || i >= n || tok >= t1) return 0.f;
+        const long long page = paged_phys_page(a.table[(long long)seq * a.max_blocks + tok / a.bs], a.num_blocks);
+        return (lane < 8 ? a.ks : a.vs)[page * a.hkv + hk];
+      };
+      float sc = scale_of(0);
+      for (int i = 0; i < n; ++i) {
+        if (!wait_warp(scales_free(i & 1), ((i >> 1) & 1) ^ 1, kStatusTimeoutLoad)) break;
         if (lane < 16) scales[i & 1][lane] = sc;
         mbar_arrive_warp(scales_full(i & 1));
         sc = scale_of(i + 1);
       }
+    }
+  } else if (warp >= 8) {
+    const int r = threadIdx.x - 256;  // this thread's token of a tile
+    for (int i = 0; i < n; ++i) {
+      const int s = i % C::STAGES, tok = t0 + i * BN + r;
       if (!wait_warp(codes_full(s), (i / C::STAGES) & 1, kStatusTimeoutLoad)) break;
       const uint32_t codes = sb + C::OFF_CODES + s * 2 * C::CODES;
       bool ok = true;
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
-        ok = wait_warp(kv ? v_free : k_free, (i & 1) ^ 1, kStatusTimeoutLoad);
+        ok = wait_warp(kv ? v_free(i & 1) : k_free, ((kv ? i >> 1 : i) & 1) ^ 1, kStatusTimeoutLoad);
         if (!ok) break;
-        uint8_t* const tile = smem + (kv ? C::OFF_V : C::OFF_K) + r * 128;
+        uint8_t* const tile = smem + (kv ? C::OFF_V + (i & 1) * C::TILE : C::OFF_K) + r * 128;
         const bool there = tok < t1;  // (K behind the split is masked; V there is zero: P is, but 0 * NaN is not)
         if (there || kv) {
           const bool edge = kv && there && tok >= free_until;
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
           }
         }
         fence_proxy_async_smem();
-        mbar_arrive_warp(kv ? v_full : k_full);
+        mbar_arrive_warp(kv ? v_full(i & 1) : k_full);
       }
       if (!ok) break;
       mbar_arrive_warp(codes_free(s));
@@ -310,6 +318,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       tc_fence_after();
       if (idle) {
         tc_fence_before();
+        mbar_arrive_warp(scales_free(i & 1));
         mbar_arrive_warp(p_full(x_tile));
         continue;
       }
@@ -408,10 +417,11 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive_warp(p_full(x_tile));
+      mbar_arrive_warp(scales_free(i & 1));
     }
     // (the last V tile's barrier too: what its makers noted about NaN is then seen)
     if (ok && n > 0)
-      ok = wait_warp(v_full, (n - 1) & 1, kStatusTimeoutSoftmax) && wait_warp(o_done, 0, kStatusTimeoutSoftmax);
+      ok = wait_warp(v_full((n - 1) & 1), ((n - 1) >> 1) & 1, kStatusTimeoutSoftmax) && wait_warp(o_done, 0, kStatusTimeoutSoftmax);
     if (ok) {
       tc_fence_after();
       if (!there) l = 0.f;

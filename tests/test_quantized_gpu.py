@@ -419,3 +419,22 @@ def test_bounds_of_any_size():
     assert _lib.device_status() == 0
     zero = dataclasses.replace(cache, seq_lengths=torch.zeros_like(cache.seq_lengths))
     assert not ax.paged_quantized_attention(q, zero, max_context=0).any()
+
+
+@pytest.mark.parametrize("pool", [E4M3, INT8])
+@pytest.mark.parametrize("where", ["keys", "values", "both"])
+@pytest.mark.parametrize("step", [4, 10])
+def test_many_rows_whose_maxima_grow_within_a_tile(pool, where, step):
+    """Of every 128 tokens the later 64 bring larger scores, larger values or both, more with every tile."""
+    cache = make_cache(pool, [500, 300], 0, 2, 128, 16, seed=step)
+    q = query(cache, 8, 40)
+    for b in range(2):
+        for i, page in enumerate(cache.block_table[b].tolist()):
+            if page < 0:
+                continue
+            grow = 2.0 ** (step * (i // 8 + (i // 4) % 2))
+            if where != "values":
+                cache.key_scales[page] *= grow ** 0.25
+            if where != "keys":
+                cache.value_scales[page] *= grow
+    check(ax.paged_quantized_attention(q, cache), attention64(q, cache))
