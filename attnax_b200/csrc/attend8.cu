@@ -636,7 +636,7 @@ struct Plan {
 
 // From this many rows per kv head on the tcgen05 kernel runs: it converts the codes once for 256 rows, the other one
 // for every 32.  Over the batches of make_plan's comment its time is 1.29 of the other one's at 32 rows, 0.99 at 48
-// and 0.98 at 64; 8 sequences of 1000 to 16384 tokens, 8 kv heads: 128 rows 137 us against 86, 256 rows 229 against 125.
+// and 0.98 at 64; 8 sequences of 1000 to 16384 tokens, 8 kv heads: 128 rows 137 us against 86, 256 rows 229 against 119.
 constexpr int kManyRows = 49;
 
 static Plan make_plan(const attn_paged_attend8_params_t* p) {
@@ -651,7 +651,7 @@ static Plan make_plan(const attn_paged_attend8_params_t* p) {
   // tokens that splits come in, at most (but for what follows), CTAs that are wanted, steps of a split at least
   long long step, chunk, want, least;
   if (pl.tc) {
-    // A CTA costs 14 us beside its tiles (4 us each) and writes 128 KB of partials: splits no shorter than fill the GPU
+    // A CTA costs 14 us beside its tiles (3 to 3.7 us each) and writes 128 KB of partials: splits no shorter than fill the GPU
     // once, and longer ones (64 rows, 48 sequences: 368 -> 331 us) where there are many waves.
     step = 128;
     least = 1;
