@@ -23,7 +23,7 @@ from . import _lib
 from ._spec import dtype_code
 from .paged import PagedKVCache
 from .paged_rows import _bound, _scale, check_tables, on_device, paged_window_attention
-from .rotary import RotaryPlan, check_plan, plan_spec, unit_stride
+from .rotary import RotaryPlan, check_plan, plan_spec, rows_like, unit_stride
 
 _FORMATS = {torch.float8_e4m3fn: _lib.POOL_E4M3, torch.int8: _lib.POOL_INT8}
 
@@ -187,7 +187,7 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     q_out, q_args = None, _NO_QUERY
     if query is not None:
         q = unit_stride(query)
-        q_out = torch.empty_like(q)
+        q_out = rows_like(q)
         q_args = (q.shape[1], q.data_ptr(), q_out.data_ptr(), *q.stride()[:3], *q_out.stride()[:3])
     p = _append_params(dtype_code(keys.dtype), fmt, *pool, kp.data_ptr(), vp.data_ptr(), *_scales(cache), n, width,
                        bt.data_ptr(), sl.data_ptr(), k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], t,

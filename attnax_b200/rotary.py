@@ -134,6 +134,13 @@ def unit_stride(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
+def rows_like(x: torch.Tensor) -> torch.Tensor:
+    """An output for ``x``, in its layout where that is dense.  (Views whose rows overlap have no such layout:
+    ``empty_like`` may then put other axes inside the channels, which the kernels take for neighbours.)"""
+    out = torch.empty_like(x)
+    return out if out.stride(3) == 1 or x.shape[3] == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 _params = _lib.packer(_lib.RotaryParams)
 _NO_STRIDES = (0, 0, 0)
 
@@ -141,13 +148,13 @@ _NO_STRIDES = (0, 0, 0)
 def _launch(q, k, turns, interleaved, magnitude, positions, inverse):
     """Turned copies of ``q`` and ``k`` (or ``None``), laid out like them."""
     q = unit_stride(q)
-    q_out = torch.empty_like(q)
+    q_out = rows_like(q)
     b, hq, s, d = q.shape
     if k is None:
         k_out, hk, kp, kop, ks, kos = None, 0, 0, 0, _NO_STRIDES, _NO_STRIDES
     else:
         k = unit_stride(k)
-        k_out = torch.empty_like(k)
+        k_out = rows_like(k)
         hk, kp, kop, ks, kos = k.shape[1], k.data_ptr(), k_out.data_ptr(), k.stride()[:3], k_out.stride()[:3]
     if positions is None:
         pos, wide, ps = 0, 0, (0, 0)
