@@ -17,6 +17,7 @@ import torch
 
 from . import _lib
 from ._spec import dtype_code
+from .rotary import rows_like
 
 
 def rope_inv_freq(head_dim: int, base: float, dtype: torch.dtype, device="cuda") -> torch.Tensor:
@@ -65,6 +66,16 @@ def _as_table(t: torch.Tensor, batch: int, seq: int, half: int, dtype: torch.dty
     return t.to(dtype).reshape(-1, half).contiguous()
 
 
+def _out_for(x: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    """The kernel takes a row's channels as neighbours and steps by the other strides."""
+    if out is None:
+        return rows_like(x)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+        raise ValueError(f"out must be {tuple(x.shape)} {x.dtype} on {x.device} with unit stride on the channels, got "
+                         f"{tuple(out.shape)} {out.dtype} on {out.device}, strides {out.stride()}")
+    return out
+
+
 def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, out=None) -> torch.Tensor:
     """Split-half RoPE of ``x (batch, heads, seq, head_dim)`` (embeddings.py:126-159):
     ``(x1 cos - x2 sin, x1 sin + x2 cos)``.  ``cos``/``sin``: ``(seq, half)``,
@@ -80,7 +91,7 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, out=Non
     ct, st = _as_table(cos, B, S, half, x.dtype), _as_table(sin, B, S, half, x.dtype)
     per_batch = ct.shape[0] == B * S and B > 1
     xx = x if x.stride(-1) == 1 else x.contiguous()
-    out = torch.empty_like(xx) if out is None else out
+    out = _out_for(xx, out)
     p = _lib.RopeParams()
     p.dtype = dtype_code(x.dtype)
     p.batch, p.heads, p.seq, p.head_dim = B, H, S, D
@@ -108,7 +119,7 @@ def apply_rope_table(x: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.
         raise ValueError("tables must be (table_len, head_dim // 2) for an even head_dim")
     ct, st = cos_table.to(x.dtype).contiguous(), sin_table.to(x.dtype).contiguous()
     xx = x if x.stride(-1) == 1 else x.contiguous()
-    out = torch.empty_like(xx) if out is None else out
+    out = _out_for(xx, out)
     pos = None
     if position_ids is not None:
         pos = position_ids.to(device=x.device, dtype=torch.int32).expand(B, S).contiguous()
