@@ -511,7 +511,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      const float f = ex2(mo[n][r] - m[n][r] - kHead);
+      // means, not sums: those of values near fp32's largest pass it
+      const float f = sum == 0.f ? 0.f : ex2(mo[n][r] - m[n][r] - kHead) / sum;
       const int row = 8 * n + 2 * t + r;
       float* at = ow + (warp * R + row) * D + g * (D / 8);
 #pragma unroll
@@ -531,29 +532,33 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w][row][0]);
     float tot = 0.f, acc[D / 32];
 #pragma unroll
+    for (int w = 0; w < kWarps; ++w) tot += ex2(ml[w][row][0] - mx) * ml[w][row][1];
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;  // (nothing visible: zeros)
+#pragma unroll
     for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+    // A share is 2^(m_w - mx) sum_w / tot of the warp's mean.  That power meets the mean in two halves: alone it passes
+    // the lower end of fp32 where the mean is large enough to count still.
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(ml[w][row][0] - mx);
-      tot += f * ml[w][row][1];
+      const float half = ex2(0.5f * (ml[w][row][0] - mx)), c = half * ml[w][row][1] * inv;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] += f * ow[(w * R + row) * D + lane + 32 * e];
+      for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(ow[(w * R + row) * D + lane + 32 * e] * half, c, acc[e]);
     }
-    const float inv = tot == 0.f ? 0.f : 1.f / tot;  // (nothing visible: zeros)
     const long long orow = row0 + gr;
     if (a.splits == 1) {
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) store_out(a.out, a.dtype, orow * D + lane + 32 * e, acc[e] * inv);
+      for (int e = 0; e < D / 32; ++e) store_out(a.out, a.dtype, orow * D + lane + 32 * e, acc[e]);
     } else {
       const long long at = orow * a.splits + split;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) a.part_o[at * D + lane + 32 * e] = acc[e] * inv;
+      for (int e = 0; e < D / 32; ++e) a.part_o[at * D + lane + 32 * e] = acc[e];
       if (lane == 0) a.part_lse[at] = tot == 0.f ? -INFINITY : mx + lg2(tot);
     }
   }
 }
 
-// Splits of a row: o = sum 2^(lse_i - M) o_i / sum 2^(lse_i - M).  `per_row` warps share a row's splits, each with a
+// Splits of a row: o = sum 2^(lse_i - M) o_i / sum 2^(lse_i - M), the terms times a power of two that keeps sums of the
+// largest values in range, and in two halves as the warps' shares above.  `per_row` warps share a row's splits, each with a
 // few in flight, and join through shared memory: one thread per channel that walks 40 splits took 9.3 us.
 constexpr int kJoinWarps = 8;
 template <int D>
@@ -577,16 +582,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   float tot = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  const float least = __uint_as_float((uint32_t)(127 - 32 + __clz(n)) << 23);  // 2^-k with 2^k > n
   const V* po = reinterpret_cast<const V*>(a.part_o + (long long)row * a.splits * D) + lane;
 #pragma unroll 4
   for (int i = part; i < n; i += per_row) {
-    const float f = ex2(lse[i] - mx);
+    const float half = ex2(0.5f * (lse[i] - mx)), c = half * least;
     const V x = po[(long long)i * 32];
-    tot += f;
+    tot = fmaf(half, c, tot);
+    acc[0] = fmaf(x.x * half, c, acc[0]);
+    acc[1] = fmaf(x.y * half, c, acc[1]);
     if constexpr (E == 4) {
-      acc[0] += f * x.x; acc[1] += f * x.y; acc[2] += f * x.z; acc[3] += f * x.w;
-    } else {
-      acc[0] += f * x.x; acc[1] += f * x.y;
+      acc[2] = fmaf(x.z * half, c, acc[2]);
+      acc[3] = fmaf(x.w * half, c, acc[3]);
     }
   }
   if (per_row > 1) {
