@@ -27,7 +27,10 @@
 // scales are and is rounded relative to the largest contribution, not to the
 // largest probability.  Both maxima move only when a value passes them by 2^7
 // (exact: everything is divided by sums of the same terms), which leaves one
-// vote per unit instead of shuffles and rescaling.
+// vote per unit instead of shuffles and rescaling.  w is p times one factor
+// sv 2^(8 + m - M); where that passes 2^(8 + kFar), w comes from an exponential
+// of its own (the factor would pass fp32 in the end, and p its lower end).
+// Such a p is below 2^(7 - kFar), which a sum of at least one does not hold.
 #include <cuda_fp16.h>
 
 #include <climits>
@@ -47,6 +50,7 @@ constexpr int kSmem = kRing + 1024;  // (aligned by hand for the swizzle)
 constexpr int kBatch = 32;         // units of a warp whose pages and scales its lanes hold
 constexpr float kSlack = 7.f;      // a maximum moves when it is passed by this much (log2)
 constexpr float kHead = 8.f;       // w <= 2^(kHead + kSlack) < 65504
+constexpr float kFar = 64.f;       // log2(sv) + m - M from which w is formed without p
 
 struct Args {
   const float *ks, *vs;
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
     up[n][0] = up[n][1] = 256.f;
     l[n][0] = l[n][1] = 0.f;
   }
-  static_assert(kHead == 8.f, "up starts at 2^kHead");
+  static_assert(kHead == 8.f, "up starts at 2^kHead, w of far pages has it as a factor");
   const int free_until = min(ctx - a.t + 1, t1);  // tokens of this split in front of it are visible to every row
   // This warp's units are warp + kWarps * j, j < mine.  Lane i holds the pool row and the scales of unit i of the
   // batch that is being loaded, and the scales of the batch that is being worked on.
@@ -433,11 +437,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float f = vs * up[n][r];
+        const bool far = lv + (m[n][r] - mo[n][r]) > kFar;
+        const float f = far ? 256.f : vs * up[n][r], from = far ? mo[n][r] - lv : m[n][r], in_sum = far ? 0.f : 1.f;
 #pragma unroll
         for (int e = r; e < 4; e += 2) {
-          const float p = ex2(s[n][e] - m[n][r]);
-          l[n][r] += p;
+          const float p = ex2(s[n][e] - from);
+          l[n][r] = fmaf(p, in_sum, l[n][r]);
           s[n][e] = p * f;  // w
           if (edge && (e < 2 ? ta : tb) >= last[n][r]) s[n][e] = 0.f;  // (f may be NaN)
         }

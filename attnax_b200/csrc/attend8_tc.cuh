@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       const bool whole = tok0 + BN <= free_until;
       // the maximum of the scores in log2, and that of score + log2 of the value scale
       // (64 columns at a time, here and below, in loops that stay rolled: all 128 do not fit a thread's registers.)
-      float mx = -FLT_MAX, mxo = -FLT_MAX;
+      float mx = -FLT_MAX, mxo = -FLT_MAX, lvx = -100.f;
 #pragma unroll 1
       for (int c0 = 0; c0 < BN; c0 += 64) {
         float x[64];
@@ -347,7 +347,9 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
           const float top = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
           const float p = top == -INFINITY ? top : top * (ks[c0 / 16 + u] * cq);  // (scales are not negative)
           mx = fmaxf(mx, p);
-          mxo = fmaxf(mxo, p + fmaxf(lg2(vs[c0 / 16 + u]), -100.f));
+          const float lv = fmaxf(lg2(vs[c0 / 16 + u]), -100.f);
+          mxo = fmaxf(mxo, p + lv);
+          lvx = fmaxf(lvx, lv);
         }
       }
       float fo = 1.f;
@@ -359,45 +361,59 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
         mo = mo_new;
         up = ex2(m - mo + kHead);
       }
-      const unsigned long long nm2 = f2_pack(-m, -m);
       unsigned long long sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-      // (S is read again; P, half as wide, stays behind what has been read.)
+      auto weights = [&](auto far_units) {
+        constexpr bool FAR = decltype(far_units)::value;
+        constexpr int W = FAR ? 32 : 64;
+        // (S is read again; P, half as wide, stays behind what has been read.)
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 64) {
-        float x[64];
+        for (int c0 = 0; c0 < BN; c0 += W) {
+          float x[W];
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) tmem_ld32(s_addr + c0 + c, *reinterpret_cast<uint32_t(*)[32]>(&x[c]));
-        tmem_wait_ld();
-        uint32_t pk[32];
+          for (int c = 0; c < W; c += 32) tmem_ld32(s_addr + c0 + c, *reinterpret_cast<uint32_t(*)[32]>(&x[c]));
+          tmem_wait_ld();
+          uint32_t pk[W / 2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float f = ks[c0 / 16 + u] * cq, g = vs[c0 / 16 + u] * up;
-          const unsigned long long f2 = f2_pack(f, f), g2 = f2_pack(g, g);
-#pragma unroll
-          for (int c = 16 * u; c < 16 * u + 16; c += 2) {
-            float y0, y1;
-            f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), f2, nm2), y0, y1);
-            y0 = ex2(y0);
-            y1 = ex2(y1);
-            if (!whole) {  // (f may be 0, g NaN)
-              if (tok0 + c0 + c >= last) y0 = 0.f;
-              if (tok0 + c0 + c + 1 >= last) y1 = 0.f;
+          for (int u = 0; u < W / 16; ++u) {
+            const float f = ks[c0 / 16 + u] * cq;
+            float g = vs[c0 / 16 + u] * up, from = -m, in_sum = 1.f;
+            if (FAR) {  // (w without p, as in the kernel for few rows)
+              const float lv = fmaxf(lg2(vs[c0 / 16 + u]), -100.f);
+              const bool far = lv + (m - mo) > kFar;
+              g = far ? 256.f : g;
+              from = far ? lv - mo : from;
+              in_sum = far ? 0.f : 1.f;
             }
-            const unsigned long long p = f2_pack(y0, y1);
-            sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], p);
-            f2_unpack(f2_mul(p, g2), y0, y1);
-            pk[c / 2] = half_pair(y0, y1);
-          }
-        }
-        if (!whole) {
+            const unsigned long long f2 = f2_pack(f, f), g2 = f2_pack(g, g), nm2 = f2_pack(from, from);
 #pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            if (tok0 + c0 + c >= last) pk[c / 2] = 0u;
-            else if (tok0 + c0 + c + 1 >= last) pk[c / 2] &= 0xffffu;
+            for (int c = 16 * u; c < 16 * u + 16; c += 2) {
+              float y0, y1;
+              f2_unpack(f2_fma(f2_pack(x[c], x[c + 1]), f2, nm2), y0, y1);
+              y0 = ex2(y0);
+              y1 = ex2(y1);
+              if (!whole) {  // (f may be 0, g NaN)
+                if (tok0 + c0 + c >= last) y0 = 0.f;
+                if (tok0 + c0 + c + 1 >= last) y1 = 0.f;
+              }
+              const unsigned long long p = f2_pack(y0, y1);
+              sum[(c >> 1) & 1] = FAR ? f2_fma(p, f2_pack(in_sum, in_sum), sum[(c >> 1) & 1]) : f2_add(sum[(c >> 1) & 1], p);
+              f2_unpack(f2_mul(p, g2), y0, y1);
+              pk[c / 2] = half_pair(y0, y1);
+            }
           }
+          if (!whole) {
+#pragma unroll
+            for (int c = 0; c < W; c += 2) {
+              if (tok0 + c0 + c >= last) pk[c / 2] = 0u;
+              else if (tok0 + c0 + c + 1 >= last) pk[c / 2] &= 0xffffu;
+            }
+          }
+          tmem_st_cols<W / 2>(s_addr + c0 / 2, pk);
         }
-        tmem_st32(s_addr + c0 / 2, pk);
-      }
+      };
+      // (a copy of its own: its factors of every unit would not fit the registers of the usual case)
+      if (__any_sync(0xffffffffu, lvx + (m - mo) > kFar)) weights(std::true_type{});
+      else weights(std::false_type{});
       float s0, s1, s2, s3;
       f2_unpack(sum[0], s0, s1);
       f2_unpack(sum[1], s2, s3);
