@@ -724,8 +724,8 @@ int attn_paged_attend8(const attn_paged_attend8_params_t* p, void* stream) {
       !p->block_table || !p->seq_lengths || p->max_context < 0)
     return ATTN_ERR_INVALID;
   if ((p->head_dim != 64 && p->head_dim != 128) || p->block_size % 16 ||
-      (addr(p->key_pool) | addr(p->value_pool) | addr(p->q)) % 16)
-    return ATTN_ERR_UNSUPPORTED;
+      (addr(p->key_pool) | addr(p->value_pool) | addr(p->q) | addr(p->out)) % 16)
+    return ATTN_ERR_UNSUPPORTED;  // (TMA and vector accesses)
   const Plan pl = make_plan(p);
   const long long rows = (long long)p->num_heads_q / p->num_heads_kv * p->seq_q;
   if (rows > INT_MAX / 2 || p->num_seqs > 65535 || pl.splits > 65535 ||

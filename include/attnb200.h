@@ -476,10 +476,11 @@ typedef struct {
 int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream);
 /* Attention over 8-bit pages: query row i of sequence s stands at position
  * seq_lengths[s] - seq_q + i and sees the keys up to it; rows in front of the
- * sequence give zeros.  head_dim 64 or 128, block_size a multiple of 16, pools
- * on 16 bytes; others are ATTN_ERR_UNSUPPORTED.  max_context bounds the
- * lengths: a longer sequence is cut to the planned splits (notice 0x201), one
- * longer than its table row ends with the row (0x202). */
+ * sequence give zeros.  head_dim 64 or 128, block_size a multiple of 16, pools,
+ * q and out on 16 bytes; others are ATTN_ERR_UNSUPPORTED.  (The workspace too
+ * starts on 16 bytes.)  max_context bounds the lengths: a longer sequence is
+ * cut to the planned splits (notice 0x201), one longer than its table row ends
+ * with the row (0x202). */
 typedef struct {
   attn_dtype_t dtype;                /* q and out */
   int32_t pool_format;
