@@ -618,7 +618,7 @@ struct Stored<Int8> {
 };
 
 // Thread = NV elements of one token's kv head of sequence blockIdx.y, of keys (blockIdx.z 0) or values; positions
-// outside the sequence give zeros.
+// outside the sequence give zeros, and so do those without a page.
 template <typename F, typename TO, int NV>
 __global__ void __launch_bounds__(256) gather_tokens_kernel(const __grid_constant__ GatherArgs a) {
   using S = typename Stored<F>::T;
@@ -638,13 +638,17 @@ __global__ void __launch_bounds__(256) gather_tokens_kernel(const __grid_constan
       atomicCAS(&g_notice, 0, kNoticeTableOverrun);
     } else {
       const int p = (int)pos;
-      const long long page = paged_phys_page(a.table[(long long)s * a.max_blocks + p / a.bs], a.num_blocks);
-      const S* pool = reinterpret_cast<const S*>(blockIdx.z ? a.v : a.k);
-      const Vec<S, NV> in = unpack<S, NV>(
-          *reinterpret_cast<const Bits<S, NV>*>(pool + ((page * a.bs + p % a.bs) * a.hk + h) * a.dim + e));
-      const float scale = Stored<F>::kCode ? (blockIdx.z ? a.vs : a.ks)[page * a.hk + h] : 1.f;
+      const long long page = a.table[(long long)s * a.max_blocks + p / a.bs];
+      if (page < 0 || page >= a.num_blocks) {  // (freed by a window, or out of range: nothing of the sequence's is there)
+        skip_notice();
+      } else {
+        const S* pool = reinterpret_cast<const S*>(blockIdx.z ? a.v : a.k);
+        const Vec<S, NV> in = unpack<S, NV>(
+            *reinterpret_cast<const Bits<S, NV>*>(pool + ((page * a.bs + p % a.bs) * a.hk + h) * a.dim + e));
+        const float scale = Stored<F>::kCode ? (blockIdx.z ? a.vs : a.ks)[page * a.hk + h] : 1.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) o.e[j] = from_f32<TO>(Stored<F>::value(in.e[j], scale));
+        for (int j = 0; j < NV; ++j) o.e[j] = from_f32<TO>(Stored<F>::value(in.e[j], scale));
+      }
     }
   }
   TO* out = reinterpret_cast<TO*>(blockIdx.z ? a.vo : a.ko) + (((long long)s * a.count + i) * a.hk + h) * a.dim + e;

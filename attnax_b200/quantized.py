@@ -226,7 +226,8 @@ def gather_tokens(cache, starts, count: int, *, dtype=None):
     """``(keys, values)``, each ``(B, Hkv, count, D)``: positions ``starts[b] .. starts[b] + count - 1`` of every
     sequence, the batched form of ``gather_kv`` for both kinds of cache.
 
-    ``starts (B,)`` integers, or ``None`` for the beginning; positions outside a sequence give zeros.  8-bit codes
+    ``starts (B,)`` integers, or ``None`` for the beginning; positions outside a sequence give zeros, and so do those
+    whose page is missing (``free_window``), noted in ``_lib.device_status()`` (``NOTICE_PAGE_LIST``).  8-bit codes
     come back as the values that they stand for, rounded to ``dtype`` (default: the pools' type; bfloat16 for 8-bit
     pools, which holds every code times a power of two exactly).  Nothing waits for the GPU.
     """

@@ -458,8 +458,8 @@ int attn_paged_append_tokens(const attn_paged_append_params_t* p, void* stream);
 /* keys_out/values_out [num_seqs, count, heads_kv, head_dim] in `dtype`: the
  * tokens at positions starts[s] .. starts[s] + count (starts NULL: from 0) of
  * every sequence, 8-bit codes as the values that they stand for; zeros in
- * front of a sequence and from its length on.  Table entries are read as
- * attn_paged_gather reads them; positions past the table row give zeros and
+ * front of a sequence and from its length on.  Tokens whose table entry is no
+ * page give zeros and the notice 0x204, positions past the table row zeros and
  * the notice 0x202. */
 typedef struct {
   attn_dtype_t dtype;
