@@ -72,6 +72,15 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
+// The page of sequence `seq`'s token `tok`.  An entry that is no page (freed by a window, or out
+// of range) has nothing to read: `there` turns false, a notice is left, and the caller takes NaN for the scales, so that
+// the rows which see such a token are NaN instead of another sequence's.
+__device__ __forceinline__ long long page_of(const Args& a, int seq, int tok, bool* there) {
+  const int e = a.table[(long long)seq * a.max_blocks + tok / a.bs];
+  *there = e >= 0 && e < a.num_blocks;
+  if (!*there) atomicCAS(&g_notice, 0, kNoticePageList);
+  return *there ? e : 0;
+}
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -277,10 +286,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
     if (j >= mine) return;
     if (j % kBatch == 0 && j + lane < mine) {
       const int tok = t0 + 16 * (warp + kWarps * (j + lane));
-      const long long page = paged_phys_page(a.table[(long long)seq * a.max_blocks + tok / a.bs], a.num_blocks);
+      bool there;
+      const long long page = page_of(a, seq, tok, &there);
       first = (int)(page * a.bs + tok % a.bs);
-      nks = a.ks[page * a.hkv + hk];
-      nvs = a.vs[page * a.hkv + hk];
+      nks = there ? a.ks[page * a.hkv + hk] : NAN;
+      nvs = there ? a.vs[page * a.hkv + hk] : NAN;
     }
     const int row = __shfl_sync(0xffffffffu, first, j % kBatch);
     if (lane == 0) {

@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       auto row_of = [&](int i) {
         const int tok = t0 + i * BN + 16 * lane;
         if (lane >= BN / 16 || tok >= t1) return -1;
-        const long long page = paged_phys_page(a.table[(long long)seq * a.max_blocks + tok / a.bs], a.num_blocks);
+        bool there;
+        const long long page = page_of(a, seq, tok, &there);
         return (int)(page * a.bs + tok % a.bs);
       };
       int row = n > 0 ? row_of(0) : -1, i = 0;
@@ -214,8 +215,9 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       auto scale_of = [&](int i) {
         const int tok = t0 + i * BN + 16 * (lane & 7);
         if (lane >= 16 || i >= n || tok >= t1) return 0.f;
-        const long long page = paged_phys_page(a.table[(long long)seq * a.max_blocks + tok / a.bs], a.num_blocks);
-        return (lane < 8 ? a.ks : a.vs)[page * a.hkv + hk];
+        bool there;
+        const long long page = page_of(a, seq, tok, &there);
+        return there ? (lane < 8 ? a.ks : a.vs)[page * a.hkv + hk] : NAN;
       };
       float sc = scale_of(0);
       for (int i = 0; i < n; ++i) {

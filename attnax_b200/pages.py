@@ -170,7 +170,8 @@ def free_window(cache: PagedKVCache, *, window_size: int, num_sinks: int = 0):
     front of the window of the next token (position ``seq_lengths``); its entry
     becomes -1 and the lengths stay.  Whatever reads the whole context
     (``paged_attention``, ``paged_tree_attention``, ``gather_kv``) must not be
-    used on such rows.
+    used on such rows.  Over 8-bit pages there is no attention with a window yet:
+    ``paged_quantized_attention`` answers such rows with NaN.
     """
     if window_size <= 0:
         raise ValueError(f"window_size must be positive, got {window_size}")

@@ -257,6 +257,9 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
     is scaled by a power of two per row and held in fp16: exact for 16-bit types down to 2^-29 of the row's largest
     channel, and off by at most 2^-39 of that below.
 
+    Rows that stand behind a page which is missing (taken by ``free_window``, or out of range) are NaN, noted in
+    ``_lib.device_status()`` (``NOTICE_PAGE_LIST``): there is no window here that would leave such pages out.
+
     With ``max_context`` (an upper bound of the lengths) there is no host sync; a longer sequence is then cut to
     the planned splits and noted in ``_lib.device_status()``, as in ``paged_attention_batched``.  head_dim 64 or
     128, a block size that is a multiple of 16 and pools that start on 16 bytes take the fused kernel; other caches
@@ -311,6 +314,10 @@ def _attend_gathered(query, cache, pool, rows, fmt):
     dtype = torch.bfloat16 if query.dtype == torch.bfloat16 else torch.float32  # (fp16 does not hold every scale)
     size = -(-longest // 16) * 16
     k, v = _gather(cache, pool, rows, fmt, None, size, dtype)
+    pos = torch.arange(size, dtype=torch.int32, device=query.device)
+    entry = cache.block_table[:, (pos // pool[1]).clamp(max=rows[1] - 1).long()]
+    missing = ((entry < 0) | (entry >= pool[0])) & (pos < cache.seq_lengths[:, None])
+    k[..., 0].masked_fill_(missing[:, :, None], float("nan"))  # (such tokens came back as zeros)
     table = torch.arange(n * (size // 16), dtype=torch.int32, device=query.device).view(n, size // 16)
     wide = PagedKVCache(k.view(-1, 16, hk, d), v.view(-1, 16, hk, d), table, cache.seq_lengths)
     return paged_window_attention(query, wide, window_size=size + t, max_context=longest)
