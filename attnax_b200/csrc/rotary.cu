@@ -252,9 +252,9 @@ __device__ __forceinline__ int new_tokens(const AppendArgs& a, int s) {
   return a.new_lens ? min(max(a.new_lens[s], 0), a.num_new) : a.num_new;
 }
 
-// The page that position `pos` of sequence s is written to, or -1.
+// The page that position `pos` of sequence s is written to, or -1 (a sequence whose length is negative has none).
 __device__ __forceinline__ int write_page(const AppendArgs& a, int s, long long pos) {
-  if (pos < 0 || pos / a.bs >= a.max_blocks) return -1;
+  if (a.lens[s] < 0 || pos / a.bs >= a.max_blocks) return -1;
   const int page = a.table[(long long)s * a.max_blocks + pos / a.bs];
   return page >= 0 && page < a.num_blocks ? page : -1;
 }

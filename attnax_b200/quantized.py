@@ -166,8 +166,8 @@ def append_tokens(cache, keys: torch.Tensor, values: torch.Tensor, *, new_length
     pages only).  What is written and returned carries no gradient.
 
     ``check=True`` waits for the GPU and raises ``ValueError`` before anything is written if a length or a page is
-    missing or out of range; with ``check=False`` there is no wait, and such tokens are skipped and noted in
-    ``_lib.device_status()`` (``NOTICE_PAGE_LIST``; lengths still count them).
+    missing or out of range; with ``check=False`` there is no wait, and such tokens (all of a sequence whose length is
+    negative) are skipped and noted in ``_lib.device_status()`` (``NOTICE_PAGE_LIST``; lengths still count them).
     """
     pool, (n, width), fmt = check_cache(cache)
     kp, vp = cache.key_pool, cache.value_pool

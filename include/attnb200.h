@@ -432,10 +432,11 @@ int attn_rotary(const attn_rotary_params_t* p, void* stream);
  * keeps the larger of its old scale and the one that the new tokens need; its
  * old codes are restated if it grows.  Infinities and NaN become NaN codes;
  * int8 has none, so the page's scale becomes NaN until it is begun anew.  A
- * page that gets tokens must belong to one sequence.  Tokens without a page,
- * and new_lengths outside [0, num_new], are skipped or cut and leave the
- * notice 0x204.  With bad non-NULL (pre-set to INT32_MAX) only checks: the
- * lowest such sequence is stored there and nothing is written. */
+ * page that gets tokens must belong to one sequence.  Tokens without a page
+ * (all of a sequence whose length is negative), and new_lengths outside
+ * [0, num_new], are skipped or cut and leave the notice 0x204.  With bad
+ * non-NULL (pre-set to INT32_MAX) only checks: the lowest such sequence is
+ * stored there and nothing is written. */
 typedef struct {
   attn_dtype_t dtype;                /* keys, values, q, q_out */
   int32_t pool_format;
