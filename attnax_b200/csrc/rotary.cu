@@ -39,9 +39,8 @@ struct Spec {
 // cosine end below 2^-25 after the terms x^9 and x^10.
 __device__ __forceinline__ void cos_sin(long long p, unsigned long long turn, float* c, float* s) {
   const unsigned long long f = (unsigned long long)p * turn + 0x80000000ull;
-  const int t = (int)(f >> 32);
-  const int q = (int)(((unsigned)t + 0x20000000u) >> 30);
-  const float x = (float)(t - (int)((unsigned)q << 30)) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const unsigned t = (unsigned)(f >> 32), q = (t + 0x20000000u) >> 30;
+  const float x = (float)(int)(t - (q << 30)) * 1.4629180792671596e-9f;  // 2 pi / 2^32
   const float z = x * x;
   float sn = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
   sn = fmaf(z, sn, 8.3333333e-3f);
