@@ -44,7 +44,7 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
     * ``"ntk"``: the base becomes ``base * factor ** (rotary_dim / (rotary_dim - 2))``;
     * ``"yarn"``: pairs that turn more than ``beta_fast`` times within ``original_length`` keep their frequency,
       those below ``beta_slow`` turns get ``w / factor``, a linear ramp over the pair index between them;
-      magnitude ``0.1 ln(factor) + 1``;
+      magnitude ``0.1 ln(factor) + 1`` (1 for factors up to 1);
     * ``"wavelength"``: by ``original_length`` over the wavelength: at or above ``high_factor`` the frequency stays,
       at or below ``low_factor`` it is ``w / factor``, linear in that quotient between them.
     """
@@ -80,7 +80,7 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
 
         lo, hi = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
         ramp = ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
-        return w * (1 - ramp) + w / factor * ramp, 0.1 * math.log(factor) + 1.0
+        return w * (1 - ramp) + w / factor * ramp, 0.1 * math.log(max(factor, 1.0)) + 1.0
     if not high_factor > low_factor:
         raise ValueError("'wavelength' needs high_factor > low_factor")
     keep = ((original_length * w / (2 * math.pi) - low_factor) / (high_factor - low_factor)).clamp(0, 1)
