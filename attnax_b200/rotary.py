@@ -43,7 +43,8 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
     * ``"linear"``: ``w / factor`` (positions interpolated);
     * ``"ntk"``: the base becomes ``base * factor ** (rotary_dim / (rotary_dim - 2))``;
     * ``"yarn"``: pairs that turn more than ``beta_fast`` times within ``original_length`` keep their frequency,
-      those below ``beta_slow`` turns get ``w / factor``, a linear ramp over the pair index between them;
+      those below ``beta_slow`` turns get ``w / factor``, a linear ramp over the pair index between them (its ends
+      rounded outwards and kept within ``0 .. rotary_dim - 1``);
       magnitude ``0.1 ln(factor) + 1`` (1 for factors up to 1);
     * ``"wavelength"``: by ``original_length`` over the wavelength: at or above ``high_factor`` the frequency stays,
       at or below ``low_factor`` it is ``w / factor``, linear in that quotient between them.
@@ -72,14 +73,14 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
     if original_length is None or original_length <= 0:
         raise ValueError(f"{scaling!r} needs the original_length that the frequencies were trained for")
     if scaling == "yarn":
-        if base == 1.0 or not beta_fast > beta_slow > 0:
-            raise ValueError("'yarn' needs a base other than 1 and beta_fast > beta_slow > 0")
+        if base <= 1.0 or not beta_fast > beta_slow > 0:
+            raise ValueError("'yarn' needs a base above 1 and beta_fast > beta_slow > 0")
 
-        def pair_of(turns):  # 2 x the (real) pair index whose frequency turns that often within original_length
+        def pair_of(turns):  # the (real) index of the pair that turns that often within original_length
             return rotary_dim * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(base))
 
         lo, hi = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
-        ramp = ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+        ramp = ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1) if pair_of(beta_slow) > 0 else torch.ones_like(i)
         return w * (1 - ramp) + w / factor * ramp, 0.1 * math.log(max(factor, 1.0)) + 1.0
     if not high_factor > low_factor:
         raise ValueError("'wavelength' needs high_factor > low_factor")
