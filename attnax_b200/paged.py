@@ -122,7 +122,9 @@ def allocate_blocks(cache: PagedKVCache, *, sequence_idx: int, num_new_tokens: i
     table = cache.block_table.clone()
     if new > 0:
         table[sequence_idx, have:have + new] = free[:new].to(device=table.device, dtype=torch.int32)
-    return replace(cache, block_table=table), new
+    if hasattr(cache, "key_scales"):
+        return replace(cache, block_table=table), new
+    return PagedKVCache(cache.key_pool, cache.value_pool, table, cache.seq_lengths), new
 
 
 def append_kv(cache: PagedKVCache, sequence_idx: int, keys_new: torch.Tensor,

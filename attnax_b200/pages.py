@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from ._spec import dtype_code
-from .paged import PagedKVCache
+from .paged import PagedKVCache, refuse_codes
 from .paged_rows import cast, check_tables, narrow, on_device
 from .quantized import QuantizedPagedKVCache, check_cache, with_table
 
@@ -219,8 +219,7 @@ def append_accepted(cache: PagedKVCache, draft_keys, draft_values, accepted, acc
     with ``check=False`` there is no wait, and such tokens are skipped and
     noted (lengths still count them).
     """
-    if not isinstance(cache, PagedKVCache):
-        raise ValueError("append_accepted takes a PagedKVCache; append_tokens puts tokens into 8-bit pages")
+    refuse_codes(cache)
     dev = cache.key_pool.device
     n = cache.block_table.shape[0]
     for name, x in (("draft_keys", draft_keys), ("draft_values", draft_values)):

@@ -108,9 +108,15 @@ def _scales(cache):
 
 
 def with_table(cache, table: torch.Tensor, lengths: torch.Tensor):
-    """The cache with another table and lengths (dataclasses.replace without its host time)."""
-    new = object.__new__(type(cache))
-    new.__dict__.update(cache.__dict__, block_table=table, seq_lengths=lengths)
+    """The cache with another table and lengths: a QuantizedPagedKVCache, or a PagedKVCache of whatever has the fields
+    of one (without the host time of dataclasses.replace and of a frozen constructor)."""
+    if isinstance(cache, QuantizedPagedKVCache):
+        new = object.__new__(type(cache))
+        new.__dict__.update(cache.__dict__, block_table=table, seq_lengths=lengths)
+    else:
+        new = object.__new__(PagedKVCache)
+        new.__dict__.update(key_pool=cache.key_pool, value_pool=cache.value_pool, block_table=table,
+                            seq_lengths=lengths)
     return new
 
 
