@@ -14,6 +14,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._api import ComposedScoreMod, position_indices
@@ -30,6 +31,17 @@ def dtype_code(dt: torch.dtype) -> int:
         return _DTYPE_CODE[dt]
     except KeyError:
         raise ValueError(f"unsupported dtype {dt}; expected float32, bfloat16 or float16") from None
+
+
+def differentiated(*tensors) -> bool:
+    """Whether a call on these tensors goes through its autograd function: one of them needs a gradient, or has a
+    forward-mode tangent (which the function refuses; a bare launch would drop it)."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                return True
+    return _forward_ad._current_level >= 0 and any(
+        x is not None and _forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
 def flatten_mods(score_mod):

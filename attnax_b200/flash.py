@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._spec import build_spec, dtype_code
+from ._spec import build_spec, differentiated, dtype_code
 
 
 def _stream_ptr(device) -> int:
@@ -165,7 +165,7 @@ def attention(query, key, value, *, mask=None, score_mod=None):
     B, Hq, Hkv, Sq, Skv, D = check_qkv(query, key, value)
     spec = build_spec(score_mod, mask, batch=B, heads_q=Hq, seq_q=Sq, seq_kv=Skv, device=query.device)
     q, k, v = _prep(query), _prep(key), _prep(value)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if differentiated(q, k, v):
         return _FlashAttnFn.apply(q, k, v, spec)
     out, _ = fwd_raw(q, k, v, spec, want_lse=False)
     return out

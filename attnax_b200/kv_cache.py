@@ -24,6 +24,7 @@ from dataclasses import dataclass
 
 import torch
 
+from ._spec import differentiated
 from .paged import PagedKVCache, paged_decode_raw
 
 _BLOCK_SIZES = (256, 128, 64, 32, 16)  # tensor-core decode units; the largest dividing max_len
@@ -108,7 +109,7 @@ def _window_attention(query, cache: KVLayerCache, n: int, mask, score_mod, windo
     hkv = k.shape[1]
     bs = next((x for x in _BLOCK_SIZES if cache.max_len % x == 0), None)
     # (the page kernels have no backward; the flash kernel below has)
-    grads = torch.is_grad_enabled() and (query.requires_grad or k.requires_grad or v.requires_grad)
+    grads = differentiated(query, k, v)
     if (not grads and mask is None and score_mod is None and bs is not None and d in (64, 128) and k.is_contiguous()
             and v.is_contiguous() and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float16)):
         nseq, nblk = b * hkv, cache.max_len // bs

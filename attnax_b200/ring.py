@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _ring_capi
+from ._spec import differentiated
 from .flash import _output_dropout, attention
 
 _AXES = {}
@@ -59,7 +60,7 @@ def ring_forward(query, key, value, *, mask=None, score_mod=None, group=None, zi
     B, Hq, Hkv, S, Skv, D = check_qkv(query, key, value)
     if S != Skv:
         raise ValueError("ring_attention needs equal local query and key/value shard lengths")
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+    if differentiated(query, key, value):
         return _RingFn.apply(query, key, value, score_mod, mask, group, zigzag)
     return _ring_run(query, key, value, score_mod, mask, group, zigzag, None)
 

@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._spec import dtype_code
+from ._spec import differentiated, dtype_code
 
 
 @dataclass(frozen=True)
@@ -195,7 +195,7 @@ class _Rotary(torch.autograd.Function):
 
 
 def _turned(q, k, *how):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if differentiated(q, k):
         return _Rotary.apply(q, k, *how)
     turns, positions, interleaved, magnitude, inverse = how
     out = _launch(q, k, turns, interleaved, magnitude, positions, inverse)
