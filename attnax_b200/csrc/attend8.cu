@@ -199,6 +199,11 @@ __device__ __forceinline__ void load_q16(const Args& a, long long at, float (&x)
 __device__ __forceinline__ int query_exponent(float big) {
   return big <= FLT_MAX ? max((int)(__float_as_uint(big) >> 23) - 127, -100) - 14 : 0;
 }
+// What turns products with such a row into scores in log2, but for the key scale.  With an infinity in it they are
+// infinite or NaN for every key, and so the softmax is NaN; all of them -inf would pass for a row without keys.
+__device__ __forceinline__ float query_factor(const Args& a, float big, int e2) {
+  return big <= FLT_MAX ? a.scale_log2 * __uint_as_float((uint32_t)(127 + e2) << 23) : NAN;
+}
 __device__ __forceinline__ void store_out(void* out, int dtype, long long at, float x) {
   if (dtype == ATTN_BF16) reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(x);
   else if (dtype == ATTN_F16) reinterpret_cast<__half*>(out)[at] = __float2half_rn(x);
@@ -344,7 +349,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT <= 2 ? 3 : 2) attend8_kernel(
           qf[n][h][j][1] = b1;
         }
       }
-    const float c = a.scale_log2 * __uint_as_float((uint32_t)(127 + e2) << 23);
+    const float c = query_factor(a, big, e2);
     const int lim = there ? min(ctx - a.t + pos + 1, t1) : 0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {

@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(512, 1) attend8_tc_kernel(
       }
       const int e2 = query_exponent(big);
       const float mul = there ? __uint_as_float((uint32_t)(127 - e2) << 23) : 0.f;
-      cq = a.scale_log2 * __uint_as_float((uint32_t)(127 + e2) << 23) * F::kUnshift;
+      cq = query_factor(a, big, e2) * F::kUnshift;
 #pragma unroll
       for (int p = 0; p < D / 8; ++p) {
         float q[8];
