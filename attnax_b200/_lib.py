@@ -25,7 +25,7 @@ STATUS_TIMEOUTS = (0x101, 0x102, 0x103, 0x104)
 NOTICE_CONTEXT_OVERRUN = 0x201   # a paged decode met a length above max_context
 NOTICE_TABLE_OVERRUN = 0x202     # a paged decode met a length past its block-table row
 NOTICE_TREE_ORDER = 0x203        # a drafted token's parent was not in front of it
-NOTICE_PAGE_LIST = 0x204         # a page operator skipped an entry that it could not use
+NOTICE_PAGE_LIST = 0x204         # an entry that a page operator could not use, or a page that was not there
 
 i32, i64, f32, vp, szt = C.c_int32, C.c_int64, C.c_float, C.c_void_p, C.c_size_t
 

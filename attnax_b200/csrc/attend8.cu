@@ -8,7 +8,7 @@
 // token each for K and V, half of a 16-bit cache), and all query rows of the
 // head share it.  A warp streams units of 16 tokens by TMA through a private
 // ring in shared memory, several units ahead, and shares no barrier with the
-// other warps (64 sequences of 512 to 32768 tokens: 181 us, 5.7 TB/s; 16-byte
+// other warps (64 sequences of 512 to 32768 tokens: 186 us, 5.5 TB/s; 16-byte
 // copies by the lanes took 225).
 //
 // The products run transposed, S^T = K Q^T and O^T = V^T P^T, as mma.sync
@@ -19,8 +19,9 @@
 // V bytes are A fragments after one byte permutation, and P^T is a B fragment
 // after one 8 x 8 transposition.  Codes become fp16 exactly (e4m3 and int8
 // both fit).  The query is scaled by a power of two per row and rounded to
-// fp16 (exact for bf16 and fp16 down to 2^-29 of the row's largest channel,
-// below that off by at most 2^-39 of it).
+// fp16 (exact for bf16 and fp16 down to 2^-28 of the row's largest channel,
+// below that off by at most 2^-39 of it; fp32 channels keep 11 bits, which is
+// what P keeps too: a second product for their rest would leave P's rounding).
 //
 // P carries sv: w_rj = p_rj sv_j 2^(8 - M_r), with M_r a running maximum of
 // log2(p sv) beside the softmax maximum m_r, so w fits fp16 whatever the
@@ -693,14 +694,17 @@ static Plan make_plan(const attn_paged_attend8_params_t* p) {
   // tokens that splits come in, at most (but for what follows), CTAs that are wanted, steps of a split at least
   long long step, chunk, want, least;
   if (pl.tc) {
-    // A CTA costs 14 us beside its tiles (3 to 3.7 us each) and writes 128 KB of partials: splits no shorter than fill the GPU
-    // once, and longer ones (64 rows, 48 sequences: 368 -> 331 us) where there are many waves.
+    // A CTA costs 14 us beside its tiles (3 to 3.7 us each) and writes 128 KB of partials: where one wave is not full,
+    // splits of about what fills it, and longer ones (64 rows, 48 sequences: 368 -> 331 us) where there are many waves.
+    // (The chunk is rounded down to tiles, so a few CTAs can be left to a second wave: one sequence of 16384 with 8 kv
+    // heads and 256 rows has 176, and 72 us by these costs where splits of 1024 would have 44.)
     step = 128;
     least = 1;
     want = 148;
     chunk = ctas * ctx >= 148ll * 4 * 2048 ? 2048 : 1024;
   } else {
-    // Lengths are ragged more often than not, so two waves if all were as long as the longest; and at least 256 tokens
+    // Lengths are ragged more often than not, so two waves if all were as long as the longest (of three CTAs an SM; with
+    // 17 to 48 rows an SM holds two, and it is three); and at least 256 tokens
     // (four units a warp), for a shorter split costs more at its start and in the join than it brings.  Over 14 batches
     // (1 to 64 sequences of 100 to 100000 tokens, 2 to 8 kv heads), on average above the best choice of each batch at
     // 4, 8, 16 and 32 rows: 3, 5, 7 and 9%; four waves and 64 tokens 16, 19, 27 and 38%, one wave and 256 tokens 8, 10,

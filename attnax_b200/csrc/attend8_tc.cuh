@@ -9,7 +9,9 @@
 // sustained rate; the softmax of a row tile takes 2.1 to 2.7 (S is read from TMEM twice, since half of 512 threads
 // cannot hold 128 columns each; reading it once took as long), the products in its chain 0.8, the conversion of K and V
 // 1.2 to 1.5 each beside it.  V has two places, so that the conversion does not wait for P V (4.1 us with one).  A CTA's
-// start and end take 14 us (7 until the query is in place).
+// start and end take 14 us (7 until the query is in place; a row is read, and its partials are stored, by one thread).
+// Every row group walks to the end of its split and masks: a chunk of a prompt with nothing in front of it does up to
+// twice the work that its rows see.
 #pragma once
 
 namespace attnb200 {

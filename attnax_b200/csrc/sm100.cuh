@@ -33,7 +33,7 @@ enum : int {
   kNoticeContextOverrun = 0x201,  // a seq_lengths entry above max_context: cut to the planned splits
   kNoticeTableOverrun = 0x202,    // a sequence longer than its block-table row: last entry reused
   kNoticeTreeOrder = 0x203,       // a drafted token whose parent is not in front of it: taken as a root
-  kNoticePageList = 0x204         // a page operator met an index it could not use: that entry was skipped
+  kNoticePageList = 0x204         // an index of a page operator, or a page of the 8-bit attention or of gather_tokens, that is none
 };
 
 // Host: reads and clears this unit's words.

@@ -260,8 +260,9 @@ def paged_quantized_attention(query: torch.Tensor, cache: QuantizedPagedKVCache,
     Row ``t`` of sequence ``b`` stands at position ``seq_lengths[b] - T + t`` (append the T tokens first) and sees
     the keys up to it.  Rows in front of the sequence (T > its length) and empty sequences give zeros.  bf16, fp16
     or fp32 queries; products in fp16 on codes that fp16 holds exactly, with scales and softmax in fp32.  The query
-    is scaled by a power of two per row and held in fp16: exact for 16-bit types down to 2^-29 of the row's largest
-    channel, and off by at most 2^-39 of that below.
+    is scaled by a power of two per row and held in fp16: exact for 16-bit types down to 2^-28 of the row's largest
+    channel, and off by at most 2^-39 of that below; the channels of an fp32 query are rounded to 11 bits.  So are
+    the weights that meet the values.  An fp32 result is therefore good to about 11 bits (other caches, below: all).
 
     Rows that stand behind a page which is missing (taken by ``free_window``, or out of range) are NaN, noted in
     ``_lib.device_status()`` (``NOTICE_PAGE_LIST``): there is no window here that would leave such pages out.

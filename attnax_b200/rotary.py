@@ -257,7 +257,8 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor | None, plan: RotaryPlan
     ``None`` only ``query'``.  Differentiable (also twice).
 
     ``positions``: integers ``(S,)``, ``(1, S)`` or ``(B, S)`` on the tensors' device (default ``0 .. S-1``); they
-    may be negative or of any size.  ``inverse=True`` turns backwards.  bf16, fp16 or fp32, any strides; each value
+    may be negative or of any size.  ``inverse=True`` turns backwards, which is the gradient (the plan's magnitude is
+    a factor in both directions).  bf16, fp16 or fp32, any strides; each value
     is rounded once.  Results keep the inputs' dense layout (a transposed projection stays transposed).
     """
     # (one pass where all is well: the checks are a good part of a small call's host time)

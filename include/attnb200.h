@@ -481,7 +481,8 @@ int attn_paged_gather_tokens(const attn_paged_gather_params_t* p, void* stream);
  * q and out on 16 bytes; others are ATTN_ERR_UNSUPPORTED.  (The workspace too
  * starts on 16 bytes.)  max_context bounds the lengths: a longer sequence is
  * cut to the planned splits (notice 0x201), one longer than its table row ends
- * with the row (0x202). */
+ * with the row (0x202).  Rows that see a token whose table entry is no page are
+ * NaN (0x204).  fp32 rows of q are rounded to 11 bits. */
 typedef struct {
   attn_dtype_t dtype;                /* q and out */
   int32_t pool_format;
@@ -507,7 +508,9 @@ int attn_paged_attend8(const attn_paged_attend8_params_t* p, void* stream);
  * and reused the row's last entry for the pages past it (attn_paged_window and
  * attn_paged_tree read such a sequence as if it ended with its row).  0x203: a drafted
  * token's parent was not in front of it.  0x204: a page operator skipped an
- * entry that it could not use.  A timeout code takes precedence over a notice. */
+ * entry that it could not use, or attn_paged_attend8 (rows become NaN) or
+ * attn_paged_gather_tokens (zeros) met a table entry that is no page.  A
+ * timeout code takes precedence over a notice. */
 int attn_device_status(int32_t* status);
 const char* attn_status_string(int status);
 int attn_version(void);
